@@ -16,11 +16,13 @@ computed by hand-written HIP kernels behind a C ABI (include/gfa.h, libgfa.so):
     segments.from_padding_mask / from_lengths / from_cu_seqlens / from_position_ids
                                                                          ragged-batch tables
                                                                          (``segments=`` keyword)
+    kv4.plan / write / read / attention                                  serving: a key/value cache
+                                                                         in 4 bits (kv4.py)
 
 q: (B, N_Q_HEADS, N, D), k/v: (B, N_KV_HEADS, N, D), fp16/bf16, D in {64, 128, 256, 512}.
 """
 from .attention import FlashAttnGQAFunction, attention_flash_gqa, flash_attn_gqa_train
-from . import segments
+from . import kv4, segments
 from .ops import flash_attn_gqa_op
 from .hf_integration import (
     patch_gemma4_shared_kv_states_for_fsdp2,
@@ -50,5 +52,6 @@ __all__ = [
     "KernelConfig",
     "get_config",
     "segments",
+    "kv4",
     "__version__",
 ]

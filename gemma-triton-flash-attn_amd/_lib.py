@@ -38,11 +38,12 @@ STATUS_NAMES = {
 # GFA_VERSION of include/gfa.h whose struct layouts FwdArgs / BwdArgs below mirror. A library
 # built from other sources reads another prefix of the argument structs (an older one ignores the
 # segment, soft-cap and dropout fields), so load() refuses it instead of computing wrong results.
-ABI_VERSION = 107
+ABI_VERSION = 108
 
 EXPORTED = ("gfa_fwd", "gfa_bwd", "gfa_bwd_noalloc", "gfa_bwd_workspace_size", "gfa_bwd_workspace_bytes",
             "gfa_bwd_ds_limit", "gfa_config", "gfa_last_error", "gfa_version", "gfa_set_runtime_scheduling",
-            "gfa_segments_from_positions", "gfa_segments_from_mask")
+            "gfa_segments_from_positions", "gfa_segments_from_mask", "gfa_kv4_write", "gfa_kv4_read", "gfa_kv4_plan",
+            "gfa_kv4_attn", "gfa_kv4_attn_workspace_bytes")
 NOALLOC_SCRATCH_BYTES = 64 << 20  # GFA_NOALLOC_SCRATCH_BYTES
 
 
@@ -100,6 +101,37 @@ class ConfigInfo(ctypes.Structure):
         return {name: int(getattr(self, name)) for name, _ in self._fields_}
 
 
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("num_blocks", ctypes.c_int32),
+                ("heads_kv", ctypes.c_int32), ("block_size", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
+class Kv4RowsArgs(ctypes.Structure):
+    _fields_ = [("cache", Kv4Cache), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_strides", Strides),
+                ("v_strides", Strides), ("batch", ctypes.c_int32), ("seq_len", ctypes.c_int32),
+                ("slots", ctypes.c_void_p), ("stream", ctypes.c_void_p)]
+
+
+class Kv4PlanArgs(ctypes.Structure):
+    _fields_ = [("lens", ctypes.c_void_p), ("fresh", ctypes.c_void_p), ("table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("free_ids", ctypes.c_void_p), ("used", ctypes.c_void_p),
+                ("requests", ctypes.c_int32), ("table_width", ctypes.c_int32), ("free_count", ctypes.c_int32),
+                ("block_size", ctypes.c_int32), ("tokens", ctypes.c_int32), ("slots", ctypes.c_void_p),
+                ("positions", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("lens_out", ctypes.c_void_p),
+                ("used_out", ctypes.c_void_p), ("stream", ctypes.c_void_p)]
+
+
+class Kv4AttnArgs(ctypes.Structure):
+    _fields_ = [("cache", Kv4Cache), ("q", ctypes.c_void_p), ("o", ctypes.c_void_p), ("q_strides", Strides),
+                ("o_strides", Strides), ("batch", ctypes.c_int32), ("heads_q", ctypes.c_int32),
+                ("seq_len", ctypes.c_int32), ("requests", ctypes.c_int32), ("table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p),
+                ("table_width", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
+                ("max_new", ctypes.c_int32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p)]
+
+
 _lib = None
 _lock = threading.Lock()
 
@@ -142,6 +174,12 @@ def load() -> ctypes.CDLL:
         lib.gfa_segments_from_positions.restype = ctypes.c_int
         lib.gfa_segments_from_mask.argtypes = [ptr, i64, i32, i32, ptr, ptr, ptr, ptr]
         lib.gfa_segments_from_mask.restype = ctypes.c_int
+        for name, args in (("gfa_kv4_write", Kv4RowsArgs), ("gfa_kv4_read", Kv4RowsArgs), ("gfa_kv4_plan", Kv4PlanArgs),
+                           ("gfa_kv4_attn", Kv4AttnArgs)):
+            getattr(lib, name).argtypes = [ctypes.POINTER(args)]
+            getattr(lib, name).restype = ctypes.c_int
+        lib.gfa_kv4_attn_workspace_bytes.argtypes = [ctypes.POINTER(Kv4AttnArgs)]
+        lib.gfa_kv4_attn_workspace_bytes.restype = ctypes.c_size_t
         built = int(lib.gfa_version())
         if built != ABI_VERSION:
             raise RuntimeError(

@@ -32,6 +32,22 @@ int ok() {
   return GFA_OK;
 }
 
+}  // namespace
+
+// The thread's error message for the other files of the ABI.
+namespace gfa {
+int api_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int api_ok() { return ok(); }
+}  // namespace gfa
+
+namespace {
+
 // ---------------------------------------------------------------------------------
 // HEAD_DIM-keyed registry (mirrors registry.py). Replaces the reference's if/else tile
 // tables (/root/reference/flash_attn/attention.py:561-579, 1445-1451, 1498-1504,

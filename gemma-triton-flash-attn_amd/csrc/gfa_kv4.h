@@ -1,0 +1,130 @@
+// The key/value cache in 4 bits: format, byte order and the device helpers its kernels share.
+//
+// Format (OCP Microscaling, MXFP4): 32 neighbouring channels of one token and KV head share a power
+// of two 2^e, held as the byte e + 127; an element is a sign and one of {0, .5, 1, 1.5, 2, 3, 4, 6},
+// channel 2i in the low half of a byte, 2i + 1 in the high half. gfx950 decodes two elements,
+// scale included, in one instruction (v_cvt_scalef32_pk_{bf16,f16}_fp4).
+//
+// Byte order. A block holds `block_size` tokens of every KV head, its bytes as (head, K | V, tiles of
+// 32 tokens). Inside a tile the order is the one in which the lanes of a wave take 16-byte pieces
+// as operands of v_mfma_f32_16x16x32, so that the attention kernel reads whole 1 KB runs and
+// decodes in registers. With token t of the tile, channel d, PP = D / 16:
+//   K (operand row = token, lane 16 g + t % 16 holds 32 channels of token t): 128 channels a chunk,
+//     byte (d / 128) * 2048 + t * 64 + (d % 128) / 2; D = 64: t * 32 + d / 2
+//   V (operand row p = channels p PP .. p PP + PP - 1, lane 16 g + p holds tokens 4 g + r and
+//     16 + 4 g + r): byte (d % PP / 8) * 2048 + (t / 16) * 1024 + (16 g + p) * 16 + r * 4 + (d % 8) / 2 with
+//     p = d / PP, g = t % 16 / 4, r = t % 4; D = 64: (16 g + p) * 16 + (t / 16) * 8 + r * 2 + (d % 4) / 2
+//   scales, D bytes a tile, block c = d / 32: K t * (D / 32) + (c % 4) * (D / 128) + c / 4 (D = 64: t * 2 + c);
+//     V (g * (D / 32) + c) * 8 + (t / 16) * 4 + r
+// A token's bytes are its own: tokens of one tile are stored by different waves without a race.
+#pragma once
+#include "gfa_common.h"
+
+namespace gfa {
+
+// 2^e a written block can have, as the byte: 0.5 * 2^e and 6 * 2^e are finite in the 16-bit type, and
+// the smallest is no subnormal of bf16.
+template <bool IS_BF16>
+struct Kv4Range {
+  static constexpr int lo = IS_BF16 ? 127 - 125 : 127 - 23;
+  static constexpr int hi = IS_BF16 ? 127 + 125 : 127 + 13;
+};
+constexpr int kKv4Nan = 255;  // scale byte of a block that holds an infinity or a NaN
+
+struct Kv4Cache {
+  uint8_t* codes;   // (num_blocks, Hkv, 2, block_size, D / 2)
+  uint8_t* scales;  // (num_blocks, Hkv, 2, block_size, D / 32)
+  int num_blocks, Hkv, bs_log2;  // block_size = 1 << bs_log2 >= 32
+};
+
+template <int D>
+struct Kv4Layout {
+  static constexpr int PP = D / 16;              // channels of a V operand row
+  static constexpr int KW = D < 128 ? D : 128;   // channels of a K chunk
+  static constexpr int SC = D / 32;              // scale blocks of a token
+  static constexpr int TILE_CODES = 16 * D, TILE_SCALES = D;
+  // Byte of the 16-byte piece that holds channels 32 c .. 32 c + 31 of token t.
+  static __device__ __forceinline__ int k_code(int t, int c) {
+    return c / (KW / 32) * (16 * KW) + t * (KW / 2) + c % (KW / 32) * 16;
+  }
+  // Byte of the piece (4 bytes, 8 channels; D = 64: 2 bytes, 4 channels) of operand row p, piece x8.
+  static __device__ __forceinline__ int v_code(int t, int p, int x8) {
+    const int lane = (t & 12) * 4 + p;
+    if constexpr (D == 64) return lane * 16 + (t >> 4) * 8 + (t & 3) * 2;
+    return x8 * 2048 + (t >> 4) * 1024 + lane * 16 + (t & 3) * 4;
+  }
+  static __device__ __forceinline__ int k_scale(int t, int c) {
+    if constexpr (D == 64) return t * 2 + c;
+    return t * SC + (c & 3) * (D / 128) + (c >> 2);
+  }
+  static __device__ __forceinline__ int v_scale(int t, int c) {
+    return (((t >> 2) & 3) * SC + c) * 8 + (t >> 4) * 4 + (t & 3);
+  }
+};
+
+// First byte of the codes (scales) of side 0 (K) or 1 (V) of a block and head; 64-bit, a cache may pass 4 GiB.
+template <int D>
+__device__ __forceinline__ int64_t kv4_codes_at(const Kv4Cache& c, int block, int head, int side) {
+  return ((((int64_t)block * c.Hkv + head) * 2 + side) << c.bs_log2) * (D / 2);
+}
+template <int D>
+__device__ __forceinline__ int64_t kv4_scales_at(const Kv4Cache& c, int block, int head, int side) {
+  return ((((int64_t)block * c.Hkv + head) * 2 + side) << c.bs_log2) * (D / 32);
+}
+
+// Elements 2 SEL and 2 SEL + 1 of the 8 in a dword, times the power of two in `scale`, as a pair of
+// 16-bit values. Exact: a 2-bit significand.
+template <bool IS_BF16, int SEL>
+__device__ __forceinline__ unsigned kv4_pair(unsigned codes, float scale) {
+  if constexpr (IS_BF16) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, SEL));
+  } else {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, SEL));
+  }
+}
+
+// Power of two of byte I of a dword of scale bytes, as a float's bits.
+template <int I>
+__device__ __forceinline__ unsigned kv4_scale_bits(unsigned bytes) {
+  if constexpr (I == 3) return (bytes >> 1) & 0x7f800000u;
+  return (bytes << (23 - 8 * I)) & 0x7f800000u;
+}
+
+struct Kv4RowsParams {
+  Kv4Cache cache;
+  const uint16_t *k, *v;  // write: (rows, Hkv, N, D)
+  uint16_t *ko, *vo;      // read
+  int64_t ksb, ksh, ksn, vsb, vsh, vsn;
+  const int64_t* slots;   // (T,), T = rows * N
+  int N, T;
+};
+
+struct Kv4PlanParams {
+  const int *lens, *fresh, *free_ids, *used;
+  int* table;
+  int64_t table_stride;
+  int B, M, F, bs_log2, T;
+  int64_t* slots;
+  int *positions, *cu, *lens_out, *used_out;
+};
+
+struct Kv4AttnParams {
+  Kv4Cache cache;
+  const uint16_t* q;
+  uint16_t* o;
+  int64_t qsb, qsh, qsn, osb, osh, osn;
+  int N, T;  // tokens per batch row of q and o, and altogether
+  const int *table, *lens, *cu;
+  int64_t table_stride;
+  int B, M, Hq, G;
+  int causal, window;
+  float xs;     // multiplier of a score ahead of exp2: scale log2(e), or with soft-capping cap log2(e)
+  float cap_a;  // scale / cap, 0: no soft-capping
+  int min_tiles, target;  // work split, see Kv4Split
+  int nblocks;            // workgroups of the split grid
+  int row_limit;          // requests with more query rows than this belong to the chunk kernel
+  float* part;            // (nblocks, rows, D) sums and (nblocks, rows, 2) row maxima and sums
+  float* part_ml;
+};
+
+}  // namespace gfa

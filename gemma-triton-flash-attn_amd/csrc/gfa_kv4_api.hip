@@ -1,0 +1,237 @@
+// C ABI of the key/value cache in 4 bits: argument checks, work split, launches. Nothing here
+// allocates, frees or synchronises.
+#include <algorithm>
+#include <cmath>
+
+#include "gfa.h"
+#include "gfa_kv4.h"
+#include "gfa_launch.h"
+
+namespace gfa {
+int api_fail(int code, const char* fmt, ...);  // gfa_api.hip
+int api_ok();
+}  // namespace gfa
+
+namespace {
+
+using gfa::api_fail;
+
+bool aligned(const void* p, unsigned n) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int check_cache(const gfa_kv4_cache& c) {
+  if (!aligned(c.codes, 16) || !aligned(c.scales, 16))
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "codes and scales must be 16-byte aligned pointers");
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256 && c.head_dim != 512)
+    return api_fail(GFA_ERR_UNSUPPORTED, "head_dim=%d not built (64, 128, 256, 512)", c.head_dim);
+  if (c.block_size < 32 || c.block_size > 1024 || (c.block_size & (c.block_size - 1)) != 0)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block_size=%d must be a power of two, 32 to 1024", c.block_size);
+  if (c.num_blocks < 1 || c.heads_kv < 1 || c.heads_kv > 65535)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "num_blocks=%d and heads_kv=%d must be positive", c.num_blocks, c.heads_kv);
+  if (c.dtype != GFA_DTYPE_FP16 && c.dtype != GFA_DTYPE_BF16)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "dtype=%d is not a gfa_dtype", c.dtype);
+  return GFA_OK;
+}
+
+gfa::Kv4Cache cache_of(const gfa_kv4_cache& c) {
+  int log2 = 5;
+  while ((1 << log2) < c.block_size) ++log2;
+  return gfa::Kv4Cache{static_cast<uint8_t*>(c.codes), static_cast<uint8_t*>(c.scales), c.num_blocks, c.heads_kv, log2};
+}
+
+int check_rows(const char* name, const void* p, const gfa_strides& s) {
+  if (!aligned(p, 16)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "%s must be a 16-byte aligned pointer", name);
+  if (s.batch % 8 != 0 || s.head % 8 != 0 || s.row % 8 != 0 || s.batch < 0 || s.head < 0 || s.row < 0)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "%s strides must be non-negative multiples of 8 elements", name);
+  return GFA_OK;
+}
+
+int launched(hipError_t err, const char* what) {
+  if (err != hipSuccess) return api_fail(GFA_ERR_LAUNCH, "%s launch failed: %s", what, hipGetErrorString(err));
+  return gfa::api_ok();
+}
+
+int rows_call(const gfa_kv4_rows_args* a, bool write) {
+  if (a == nullptr) return api_fail(GFA_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (int rc = check_cache(a->cache)) return rc;
+  if (a->batch < 1 || a->seq_len < 1) return api_fail(GFA_ERR_INVALID_ARGUMENT, "batch=%d and seq_len=%d must be positive", a->batch, a->seq_len);
+  if (int rc = check_rows("k", a->k, a->k_strides)) return rc;
+  if (int rc = check_rows("v", a->v, a->v_strides)) return rc;
+  if (!aligned(a->slots, 8)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "slots must be an 8-byte aligned pointer");
+  const int64_t tokens = (int64_t)a->batch * a->seq_len;
+  // a wave per 2048 / head_dim tokens and head, four waves a workgroup
+  if (tokens > 0x7fffffff || (tokens + 3) * a->cache.heads_kv / 4 >= 0x7fffffff)
+    return api_fail(GFA_ERR_UNSUPPORTED, "%lld tokens of %d heads exceed one launch", (long long)tokens, a->cache.heads_kv);
+  gfa::Kv4RowsParams p{};
+  p.cache = cache_of(a->cache);
+  p.k = p.ko = static_cast<uint16_t*>(a->k);
+  p.v = p.vo = static_cast<uint16_t*>(a->v);
+  p.ksb = a->k_strides.batch;
+  p.ksh = a->k_strides.head;
+  p.ksn = a->k_strides.row;
+  p.vsb = a->v_strides.batch;
+  p.vsh = a->v_strides.head;
+  p.vsn = a->v_strides.row;
+  p.slots = a->slots;
+  p.N = a->seq_len;
+  p.T = (int)tokens;
+  const auto stream = static_cast<hipStream_t>(a->stream);
+  const bool bf16 = a->cache.dtype == GFA_DTYPE_BF16;
+  return launched(write ? gfa::launch_kv4_write(p, a->cache.head_dim, bf16, stream)
+                        : gfa::launch_kv4_read(p, a->cache.head_dim, bf16, stream),
+                  write ? "cache write" : "cache read");
+}
+
+// Work split of one attention call. The lengths live on the device, so the host sizes the grid for any
+// lengths the block tables can hold and the kernels divide what there is (gfa_kv4_attn.hip).
+struct Split {
+  int min_tiles, target;
+  int64_t nblocks;
+  bool join;  // some request may take more than one chunk
+  size_t part_bytes, ml_bytes;
+};
+
+constexpr int kRows = 16;
+
+Split split_of(const gfa_kv4_attn_args* a) {
+  Split s{};
+  const int64_t G = a->heads_q / a->cache.heads_kv;
+  const int64_t T = (int64_t)a->batch * a->seq_len;
+  s.min_tiles = 8;
+  s.target = 512;
+  int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
+  if (a->causal && a->window > 0) tiles = std::min<int64_t>(tiles, ((int64_t)a->window + T + 31) / 32 + 1);
+  const int64_t row_blocks = a->cu ? (T * G + (kRows - 1) * (int64_t)a->requests) / kRows
+                                   : a->requests * ((T / a->requests * G + kRows - 1) / kRows);
+  // chunks: one per row block, and as many more as there are full ones
+  const int64_t chunks = std::max<int64_t>(1, (tiles + s.min_tiles - 1) / s.min_tiles);
+  s.join = chunks > 1;
+  if (!s.join) s.min_tiles = 0x3fffffff;
+  const int64_t items = std::min(row_blocks * chunks, row_blocks + (s.target + a->cache.heads_kv - 1) / a->cache.heads_kv);
+  s.nblocks = items * a->cache.heads_kv + (a->cu ? 64 : 0);
+  if (s.join) {
+    s.part_bytes = (size_t)s.nblocks * kRows * a->cache.head_dim * sizeof(float);
+    s.ml_bytes = (size_t)s.nblocks * kRows * 2 * sizeof(float);
+  }
+  return s;
+}
+
+int check_attn(const gfa_kv4_attn_args* a) {
+  if (a == nullptr) return api_fail(GFA_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (int rc = check_cache(a->cache)) return rc;
+  if (a->batch < 1 || a->seq_len < 1 || a->requests < 1 || a->table_width < 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "batch=%d, seq_len=%d, requests=%d and table_width=%d must be positive", a->batch,
+                    a->seq_len, a->requests, a->table_width);
+  if (a->heads_q < 1 || a->heads_q % a->cache.heads_kv != 0)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "heads_q=%d must be a multiple of heads_kv=%d", a->heads_q, a->cache.heads_kv);
+  const int64_t T = (int64_t)a->batch * a->seq_len;
+  if (T * a->heads_q > 0x7fffffff) return api_fail(GFA_ERR_UNSUPPORTED, "%lld query rows exceed one launch", (long long)(T * a->heads_q));
+  if ((int64_t)a->table_width * a->cache.block_size > 0x40000000)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block tables of %lld tokens (most 2^30)", (long long)a->table_width * a->cache.block_size);
+  if (a->cu == nullptr && T % a->requests != 0)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "%lld tokens do not divide among %d requests (pass cu)", (long long)T, a->requests);
+  if (!std::isfinite(a->scale) || a->scale <= 0.f) return api_fail(GFA_ERR_INVALID_ARGUMENT, "scale=%g must be finite and > 0", (double)a->scale);
+  if (!std::isfinite(a->softcap) || a->softcap < 0.f)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "softcap=%g must be finite and >= 0 (0 = off)", (double)a->softcap);
+  if (a->window < 0 || a->max_new < 0) return api_fail(GFA_ERR_INVALID_ARGUMENT, "window=%d and max_new=%d must be >= 0", a->window, a->max_new);
+  if (a->table_stride < a->table_width && a->requests > 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "table_stride=%lld below table_width=%d", (long long)a->table_stride, a->table_width);
+  return GFA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gfa_kv4_write(const gfa_kv4_rows_args* args) { return rows_call(args, true); }
+int gfa_kv4_read(const gfa_kv4_rows_args* args) { return rows_call(args, false); }
+
+int gfa_kv4_plan(const gfa_kv4_plan_args* a) {
+  if (a == nullptr) return api_fail(GFA_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->block_size < 32 || a->block_size > 1024 || (a->block_size & (a->block_size - 1)) != 0)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block_size=%d must be a power of two, 32 to 1024", a->block_size);
+  if (a->requests < 1 || a->table_width < 1 || a->free_count < 0 || a->tokens < 0)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "requests=%d and table_width=%d must be positive, free_count=%d and tokens=%d not negative",
+                    a->requests, a->table_width, a->free_count, a->tokens);
+  if (a->table_stride < a->table_width && a->requests > 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "table_stride=%lld below table_width=%d", (long long)a->table_stride, a->table_width);
+  const void* ptrs[] = {a->lens, a->fresh, a->table, a->used, a->cu, a->lens_out, a->used_out};
+  for (const void* p : ptrs)
+    if (!aligned(p, 4)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "plan arrays must be 4-byte aligned pointers");
+  if ((a->free_count > 0 && !aligned(a->free_ids, 4)) ||
+      (a->tokens > 0 && (!aligned(a->slots, 8) || !aligned(a->positions, 4))))
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "plan arrays must be aligned pointers");
+  gfa::Kv4PlanParams p{};
+  p.lens = a->lens;
+  p.fresh = a->fresh;
+  p.free_ids = a->free_ids;
+  p.used = a->used;
+  p.table = a->table;
+  p.table_stride = a->table_stride;
+  p.B = a->requests;
+  p.M = a->table_width;
+  p.F = a->free_count;
+  p.T = a->tokens;
+  p.bs_log2 = 5;
+  while ((1 << p.bs_log2) < a->block_size) ++p.bs_log2;
+  p.slots = a->slots;
+  p.positions = a->positions;
+  p.cu = a->cu;
+  p.lens_out = a->lens_out;
+  p.used_out = a->used_out;
+  return launched(gfa::launch_kv4_plan(p, static_cast<hipStream_t>(a->stream)), "plan");
+}
+
+size_t gfa_kv4_attn_workspace_bytes(const gfa_kv4_attn_args* a) {
+  if (check_attn(a) != GFA_OK) return 0;
+  const Split s = split_of(a);
+  return s.part_bytes + s.ml_bytes;
+}
+
+int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
+  if (int rc = check_attn(a)) return rc;
+  if (int rc = check_rows("q", a->q, a->q_strides)) return rc;
+  if (int rc = check_rows("o", a->o, a->o_strides)) return rc;
+  if (!aligned(a->table, 4) || !aligned(a->lens, 4) || (a->cu != nullptr && !aligned(a->cu, 4)))
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "table, lens and cu must be 4-byte aligned pointers");
+  const Split s = split_of(a);
+  if (s.nblocks > 0x7fffffff) return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)s.nblocks);
+  const size_t need = s.part_bytes + s.ml_bytes;
+  if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
+    return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, a->workspace_bytes);
+  gfa::Kv4AttnParams p{};
+  p.cache = cache_of(a->cache);
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.o = static_cast<uint16_t*>(a->o);
+  p.qsb = a->q_strides.batch;
+  p.qsh = a->q_strides.head;
+  p.qsn = a->q_strides.row;
+  p.osb = a->o_strides.batch;
+  p.osh = a->o_strides.head;
+  p.osn = a->o_strides.row;
+  p.N = a->seq_len;
+  p.T = a->batch * a->seq_len;
+  p.table = a->table;
+  p.lens = a->lens;
+  p.cu = a->cu;
+  p.table_stride = a->table_stride;
+  p.B = a->requests;
+  p.M = a->table_width;
+  p.Hq = a->heads_q;
+  p.G = a->heads_q / a->cache.heads_kv;
+  p.causal = a->causal != 0;
+  p.window = a->causal ? a->window : 0;
+  const bool cap = a->softcap > 0.f;
+  p.xs = (cap ? a->softcap : a->scale) * 1.4426950408889634f;
+  p.cap_a = cap ? a->scale / a->softcap : 0.f;
+  p.min_tiles = s.min_tiles;
+  p.target = s.target;
+  p.nblocks = (int)s.nblocks;
+  p.row_limit = 0x7fffffff;
+  p.part = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + s.part_bytes);
+  return launched(gfa::launch_kv4_split(p, a->cache.head_dim, a->cache.dtype == GFA_DTYPE_BF16, cap, s.join,
+                                        static_cast<hipStream_t>(a->stream)),
+                  "cache attention");
+}
+
+}  // extern "C"

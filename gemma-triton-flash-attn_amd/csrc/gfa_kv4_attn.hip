@@ -1,0 +1,487 @@
+// Attention of a step's new tokens over the key/value cache in 4 bits (gfa_kv4.h), gfx950: few query rows
+// per request (single tokens, drafted tokens), split over the keys.
+//
+// Rows: the G query heads of a KV head for every new token of a request, row r = token r / G, head r % G;
+// ROWS = 16 of them are a row block. Work item: (request, row block, chunk of the request's key tiles); a
+// workgroup takes one item of one KV head, its waves take the chunk's 32-token tiles in turn.
+//  * S^T = K Q^T (v_mfma_f32_16x16x32): A = 16 tokens of K decoded in registers from the 16 bytes a lane
+//    loads, B = the wave's resident Q rows. Rows sit on lanes, so softmax statistics are per-lane
+//    values, and a lane's scores are in the B layout of O^T += V^T P^T for the token order
+//    4 g + r, 16 + 4 g + r, in which V is stored. No LDS and no barrier until the end.
+//  * Every wave keeps its own running maximum m, row sum l and O^T; they are joined once through LDS,
+//    and the chunks' results by the join kernel below from fp32 partial sums, in a fixed order.
+#include "gfa_kv4.h"
+#include "gfa_launch.h"
+
+namespace gfa {
+
+namespace {
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+template <bool IS_BF16>
+__device__ __forceinline__ f32x4 mma16(i16x8 a, i16x8 b, f32x4 c) {
+  if constexpr (IS_BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+// Over the four lanes that hold one column of a 16 x 16 result (16 apart).
+__device__ __forceinline__ float quad_max(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+constexpr int kRows = 16;
+constexpr int kWaves = 4;
+constexpr int kTile = 32;  // tokens
+
+// What a request asks for.
+struct Request {
+  int t0, fresh, len;  // first new token, new tokens, tokens with the new ones
+  int row_blocks;      // 0: not this kernel's
+  int first, tiles;    // key tiles that some row sees
+};
+__device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
+  Request r{};
+  if (b >= p.B) return r;
+  if (p.cu != nullptr) {
+    r.t0 = p.cu[b];
+    r.fresh = max(p.cu[b + 1] - r.t0, 0);
+  } else {
+    r.fresh = p.T / p.B;
+    r.t0 = b * r.fresh;
+  }
+  r.len = max(p.lens[b], 0);
+  const int64_t rows = (int64_t)r.fresh * p.G;
+  r.row_blocks = rows > p.row_limit ? 0 : (int)((rows + kRows - 1) / kRows);
+  const int held = (int)min((int64_t)r.len, (int64_t)p.M << p.cache.bs_log2);
+  const int lo = p.causal && p.window > 0 ? max(r.len - r.fresh - p.window + 1, 0) : 0;
+  r.first = lo / kTile;
+  r.tiles = held > lo ? (held + kTile - 1) / kTile - r.first : 0;
+  return r;
+}
+
+__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
+  return x;
+}
+
+// Key tiles per chunk: the whole grid's tiles spread over about `target` workgroups, at least min_tiles
+// each. The lengths are the device's, so every wave derives the split from them, the same in every
+// workgroup and in the join kernel.
+__device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, int lane) {
+  int64_t total = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Request r = request_of(p, b0 + lane);
+    total += (int64_t)r.row_blocks * r.tiles;
+  }
+  total = wave_sum64(total) * p.cache.Hkv;
+  const int64_t each = (total + p.target - 1) / p.target;
+  return (int)min(max(each, (int64_t)p.min_tiles), (int64_t)0x3fffffff);
+}
+__device__ __forceinline__ int chunks_of(const Request& r, int per) { return max((r.tiles + per - 1) / per, 1); }
+
+// 1 / l of a finished row. Without weight l is a mark, not a sum: the row is 0 / 0 where it saw keys.
+__device__ __forceinline__ float row_inv(float m, float l) { return m == -INFINITY ? 1.0f / (0.f * l) : 1.0f / l; }
+
+}  // namespace
+
+template <int D, bool IS_BF16, bool CAP>
+__global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4AttnParams p) {
+  using L = Kv4Layout<D>;
+  constexpr int KT = D / 32;   // products of a score block
+  constexpr int XB = D / 16;   // 16-row blocks of O^T, one per channel of an operand row
+  constexpr int NJ = D == 64 ? 1 : D / 128;
+  __shared__ __attribute__((aligned(16))) float o_lds[2][kRows * D];
+  __shared__ float ml_lds[kWaves][kRows][2];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, c16 = lane & 15;
+  const int head = (int)blockIdx.x % p.cache.Hkv;
+  const int64_t item = (int)blockIdx.x / p.cache.Hkv;
+
+  // ---- the item: its request, row block and chunk ----
+  const int per = chunk_tiles(p, lane);
+  Request rq{};
+  int b = -1, rb = 0, ch = 0, nch = 1;
+  int64_t items = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Request r = request_of(p, b0 + lane);
+    const int64_t mine = (int64_t)r.row_blocks * chunks_of(r, per);
+    int64_t s = mine;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int64_t y = __shfl_up(s, m);
+      if (lane >= m) s += y;
+    }
+    const int64_t before = items + s - mine;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
+    if (hit != 0) {
+      const int src = __builtin_ctzll(hit);
+      b = __builtin_amdgcn_readfirstlane(b0 + src);
+      rq = request_of(p, b);
+      nch = chunks_of(rq, per);
+      const int i = (int)(item - __shfl(before, src));
+      rb = __builtin_amdgcn_readfirstlane(i / nch);
+      ch = __builtin_amdgcn_readfirstlane(i % nch);
+    }
+    items += __shfl(s, 63);
+  }
+  if (b < 0) {
+    // No item: tokens behind the last request's are zeros, the workgroups without an item take them in turn.
+    if (p.cu == nullptr) return;
+    const int64_t n0 = max(p.cu[p.B], 0);
+    const int64_t extra = (int)blockIdx.x - items * p.cache.Hkv, n_extra = p.nblocks - items * p.cache.Hkv;
+    const int64_t chunks = (p.T - n0) * p.Hq * (D / 8);
+    for (int64_t i = extra * blockDim.x + threadIdx.x; i < chunks; i += n_extra * blockDim.x) {
+      const int64_t hd = i / (D / 8);
+      const int t = (int)(n0 + hd / p.Hq);
+      uint16_t* at = p.o + (t / p.N) * p.osb + hd % p.Hq * p.osh + (t % p.N) * p.osn + i % (D / 8) * 8;
+      *reinterpret_cast<i16x8*>(at) = i16x8{};
+    }
+    return;
+  }
+
+  // ---- this lane's row: token, head, visible keys [lo, hi] ----
+  const int row = rb * kRows + c16;
+  const int i = row / p.G;
+  const int qh = head * p.G + row % p.G;
+  const int t = rq.t0 + i;
+  const bool live = i < rq.fresh && t >= 0 && t < p.T;
+  const int pos = rq.len - rq.fresh + i;
+  const int hi = live ? min(p.causal ? pos : rq.len - 1, (int)min(((int64_t)p.M << p.cache.bs_log2) - 1, (int64_t)0x7fffffff)) : -1;
+  const int lo = p.causal && p.window > 0 ? max(pos - p.window + 1, 0) : 0;
+  const VisRange vis = make_range(lo, hi);
+
+  i16x8 qf[KT];
+  {
+    const int tc = live ? t : 0;
+    const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)qh * p.qsh + (tc % p.N) * p.qsn;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int k = 0; k < KT / NJ; ++k) {
+        // k-step (j, k): lane group g holds channels 128 j + 32 g + 8 k .. (D = 64: 16 g + 8 k ..)
+        const int d = D == 64 ? 16 * g + 8 * k : 128 * j + 32 * g + 8 * k;
+        qf[j * (KT / NJ) + k] = live ? *reinterpret_cast<const i16x8*>(qp + d) : i16x8{};
+      }
+    }
+  }
+
+  f32x4 acc[XB];
+#pragma unroll
+  for (int x = 0; x < XB; ++x) acc[x] = f32x4{};
+  float m_run = -INFINITY, l_run = 0.f;
+  bool seen = false;  // the row sees a token of a tile this wave took
+
+  const int t_first = rq.first + ch * per;
+  const int t_end = min(rq.first + rq.tiles, t_first + per);
+  const int tpb_log2 = p.cache.bs_log2 - 5;  // tiles per block
+  const int* table = p.table + (int64_t)b * p.table_stride;
+  const unsigned nan2 = IS_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+
+  for (int tile = t_first + wave; tile < t_end; tile += kWaves) {
+    const int block = __builtin_amdgcn_readfirstlane(table[tile >> tpb_log2]);
+    if ((unsigned)block >= (unsigned)p.cache.num_blocks) continue;  // no block: nothing there to see
+    const int sub = tile & ((1 << tpb_log2) - 1);
+    const uint8_t* kc = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 0) + sub * L::TILE_CODES;
+    const uint8_t* vc = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 1) + sub * L::TILE_CODES;
+    const uint8_t* ks = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 0) + sub * L::TILE_SCALES;
+    const uint8_t* vs = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 1) + sub * L::TILE_SCALES;
+
+    // ---- S^T, 16 tokens at a time ----
+    f32x4 s[2];
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      s[hh] = f32x4{};
+      const int tok = hh * 16 + c16;
+      if constexpr (D == 64) {
+        const uint2 w = *reinterpret_cast<const uint2*>(kc + tok * 32 + g * 8);
+        const unsigned sb = ks[tok * 2 + (g >> 1)];
+        const float sc = __uint_as_float(sb << 23);
+        const unsigned cw[2] = {w.x, w.y};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          unsigned a[4] = {kv4_pair<IS_BF16, 0>(cw[k], sc), kv4_pair<IS_BF16, 1>(cw[k], sc),
+                           kv4_pair<IS_BF16, 2>(cw[k], sc), kv4_pair<IS_BF16, 3>(cw[k], sc)};
+          if (k == 0) a[0] = sb == kKv4Nan ? nan2 : a[0];
+          s[hh] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, a), qf[k], s[hh]);
+        }
+      } else {
+        unsigned sb;  // NJ scale bytes
+        const uint8_t* sp = ks + tok * L::SC + g * NJ;
+        if constexpr (NJ == 4) {
+          sb = *reinterpret_cast<const unsigned*>(sp);
+        } else if constexpr (NJ == 2) {
+          sb = *reinterpret_cast<const uint16_t*>(sp);
+        } else {
+          sb = *sp;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const uint4 w = *reinterpret_cast<const uint4*>(kc + j * 2048 + tok * 64 + g * 16);
+          const unsigned bits = j == 0 ? kv4_scale_bits<0>(sb) : j == 1 ? kv4_scale_bits<1>(sb) : j == 2 ? kv4_scale_bits<2>(sb) : kv4_scale_bits<3>(sb);
+          const float sc = __uint_as_float(bits);
+          const unsigned cw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            unsigned a[4] = {kv4_pair<IS_BF16, 0>(cw[k], sc), kv4_pair<IS_BF16, 1>(cw[k], sc),
+                             kv4_pair<IS_BF16, 2>(cw[k], sc), kv4_pair<IS_BF16, 3>(cw[k], sc)};
+            if (k == 0) a[0] = bits == 0x7f800000u ? nan2 : a[0];
+            s[hh] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, a), qf[4 * j + k], s[hh]);
+          }
+        }
+      }
+    }
+
+    seen = seen || (lo < (tile + 1) * kTile && hi >= tile * kTile);
+
+    // ---- softmax: this lane's row, tokens 4 g + r and 16 + 4 g + r ----
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float v = s[e >> 2][e & 3];
+      if constexpr (CAP) v = cap_tanh(v * p.cap_a);
+      x[e] = vis.has(tile * kTile + (e >> 2) * 16 + 4 * g + (e & 3)) ? v * p.xs : -INFINITY;
+    }
+    float mt = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
+    const float m_new = fmaxf(m_run, quad_max(mt));
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
+      const float a = fast_exp2(m_run - m_use);
+      l_run *= a;
+#pragma unroll
+      for (int xb = 0; xb < XB; ++xb) acc[xb] *= a;
+      m_run = m_new;
+    }
+    i16x8 pb;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float pv = fast_exp2(x[e] - m_use);
+      l_run += pv;
+      pb[e] = to16<IS_BF16>(pv);
+    }
+
+    // ---- O^T += V^T P^T ----
+    const uint2 vsb = *reinterpret_cast<const uint2*>(vs + (g * L::SC + c16 * L::PP / 32) * 8);
+    float sc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned w = e < 4 ? vsb.x : vsb.y;
+      const unsigned bits = (e & 3) == 0 ? kv4_scale_bits<0>(w) : (e & 3) == 1 ? kv4_scale_bits<1>(w) : (e & 3) == 2 ? kv4_scale_bits<2>(w) : kv4_scale_bits<3>(w);
+      // finite whatever the byte: P is 0 where a row does not see the token, and 0 times that stays 0
+      sc[e] = __uint_as_float(min(bits, (unsigned)Kv4Range<IS_BF16>::hi << 23));
+    }
+    auto products = [&](auto sel, int x0, const unsigned (&cw)[8]) __attribute__((always_inline)) {
+      constexpr int SEL = decltype(sel)::value;
+      unsigned q[8], even[4], odd[4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = kv4_pair<IS_BF16, SEL>(cw[e], sc[e]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        even[e] = __builtin_amdgcn_perm(q[2 * e + 1], q[2 * e], 0x05040100u);
+        odd[e] = __builtin_amdgcn_perm(q[2 * e + 1], q[2 * e], 0x07060302u);
+      }
+      acc[x0] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, even), pb, acc[x0]);
+      acc[x0 + 1] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, odd), pb, acc[x0 + 1]);
+    };
+    if constexpr (D == 64) {
+      const uint4 w = *reinterpret_cast<const uint4*>(vc + lane * 16);
+      const unsigned cw[8] = {w.x, w.x >> 16, w.y, w.y >> 16, w.z, w.z >> 16, w.w, w.w >> 16};
+      products(std::integral_constant<int, 0>{}, 0, cw);
+      products(std::integral_constant<int, 1>{}, 2, cw);
+    } else {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint4 a = *reinterpret_cast<const uint4*>(vc + j * 2048 + lane * 16);
+        const uint4 c = *reinterpret_cast<const uint4*>(vc + j * 2048 + 1024 + lane * 16);
+        const unsigned cw[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
+        products(std::integral_constant<int, 0>{}, 8 * j, cw);
+        products(std::integral_constant<int, 1>{}, 8 * j + 2, cw);
+        products(std::integral_constant<int, 2>{}, 8 * j + 4, cw);
+        products(std::integral_constant<int, 3>{}, 8 * j + 6, cw);
+      }
+    }
+  }
+
+  // ---- join the waves ----
+  // A row without weight (m = -inf) keeps in l whether it saw a key: none is a zero row, keys whose scores
+  // are all -inf are 0 / 0 as in the formula. Against a finite maximum either weighs nothing.
+  float l_row = quad_sum(l_run);
+  if (m_run == -INFINITY && l_row == 0.f && seen) l_row = 1.f;
+  if (g == 0) {
+    ml_lds[wave][c16][0] = m_run;
+    ml_lds[wave][c16][1] = l_row;
+  }
+  __syncthreads();
+  float m_all = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, ml_lds[w][c16][0]);
+  const float m_use = m_all == -INFINITY ? 0.f : m_all;
+  float l_all = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w)
+    l_all += ml_lds[w][c16][1] * (m_all == -INFINITY ? 1.f : fast_exp2(ml_lds[w][c16][0] - m_use));
+  const float mine = fast_exp2(m_run - m_use);
+#pragma unroll
+  for (int x = 0; x < XB; ++x) acc[x] *= mine;
+  // Rows of O^T: lane (g, row) holds channels (4 g + r) PP + x.
+  auto at = [&](int r, int x) { return (x * 4 + r) * 64 + lane; };
+#pragma unroll
+  for (int step = 2; step >= 1; step >>= 1) {
+    if (wave >= step && wave < 2 * step) {
+#pragma unroll
+      for (int x = 0; x < XB; ++x) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o_lds[wave - step][at(r, x)] = acc[x][r];
+      }
+    }
+    __syncthreads();
+    if (wave < step) {
+#pragma unroll
+      for (int x = 0; x < XB; ++x) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[x][r] += o_lds[wave][at(r, x)];
+      }
+    }
+    __syncthreads();
+  }
+  if (wave != 0) return;
+
+  if (nch > 1) {
+    float* part = p.part + ((int64_t)blockIdx.x * kRows + c16) * D;
+    if (live) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int x = 0; x < XB; x += 4)
+          *reinterpret_cast<f32x4*>(part + (4 * g + r) * L::PP + x) = f32x4{acc[x][r], acc[x + 1][r], acc[x + 2][r], acc[x + 3][r]};
+      }
+    }
+    if (g == 0) {
+      float* ml = p.part_ml + ((int64_t)blockIdx.x * kRows + c16) * 2;
+      ml[0] = m_all;
+      ml[1] = l_all;
+    }
+    return;
+  }
+  if (!live) return;
+  const bool none = m_all == -INFINITY && l_all == 0.f;
+  const float inv = row_inv(m_all, l_all);
+  uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int x = 0; x < XB; x += 4) {
+      i16x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = to16<IS_BF16>(none ? 0.f : acc[x + e][r] * inv);
+      *reinterpret_cast<i16x4*>(op + (4 * g + r) * L::PP + x) = v;
+    }
+  }
+}
+
+// Joins the chunks of a row: one workgroup per token and query head.
+template <int D, bool IS_BF16>
+__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnParams p) {
+  constexpr int LPR = D / 4;         // lanes per row, four channels each
+  constexpr int GR = 256 / LPR;      // chunks at a time
+  __shared__ f32x4 o_lds[256];
+  const int lane = threadIdx.x & 63;
+  const int t = (int)(blockIdx.x / p.Hq), qh = (int)(blockIdx.x % p.Hq);
+  const int head = qh / p.G;
+  // the token's request
+  const int per = chunk_tiles(p, lane);
+  int64_t items = 0, base = -1;
+  Request rq{};
+  for (int b0 = 0; b0 < p.B; b0 += 64) {
+    const Request r = request_of(p, b0 + lane);
+    const int64_t mine = (int64_t)r.row_blocks * chunks_of(r, per);
+    int64_t s = mine;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+      const int64_t y = __shfl_up(s, m);
+      if (lane >= m) s += y;
+    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(t >= r.t0 && t < r.t0 + r.fresh);
+    if (hit != 0) {
+      const int src = __builtin_ctzll(hit);
+      base = items + __shfl(s - mine, src);
+      rq = request_of(p, __builtin_amdgcn_readfirstlane(b0 + src));
+      break;
+    }
+    items += __shfl(s, 63);
+  }
+  if (base < 0 || rq.row_blocks == 0) return;
+  const int nch = chunks_of(rq, per);
+  if (nch == 1) return;
+  const int i = t - rq.t0;
+  const int row = i * p.G + qh % p.G;
+  const int64_t first = base + (int64_t)(row / kRows) * nch;  // item of chunk 0
+  if ((first + nch) * p.cache.Hkv > p.nblocks) return;       // lengths that do not fit the grid: see gfa.h
+  const int rr = row % kRows;
+  auto slot = [&](int c) { return ((first + c) * p.cache.Hkv + head) * kRows + rr; };
+  float m = -INFINITY;
+  for (int c = lane; c < nch; c += 64) m = fmaxf(m, p.part_ml[slot(c) * 2]);
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+  const float m_use = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int c = lane; c < nch; c += 64)
+    l += p.part_ml[slot(c) * 2 + 1] * (m == -INFINITY ? 1.f : fast_exp2(p.part_ml[slot(c) * 2] - m_use));
+#pragma unroll
+  for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
+  f32x4 o{};
+  const int part = threadIdx.x / LPR, d = threadIdx.x % LPR * 4;
+  for (int c = part; c < nch; c += GR) {
+    const float w = fast_exp2(p.part_ml[slot(c) * 2] - m_use);
+    o += *reinterpret_cast<const f32x4*>(p.part + slot(c) * D + d) * w;
+  }
+  o_lds[threadIdx.x] = o;
+  __syncthreads();
+  if (part != 0) return;
+#pragma unroll
+  for (int k = 1; k < GR; ++k) o += o_lds[k * LPR + threadIdx.x];
+  const bool none = m == -INFINITY && l == 0.f;
+  const float inv = row_inv(m, l);
+  uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn + d;
+  i16x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = to16<IS_BF16>(none ? 0.f : o[e] * inv);
+  *reinterpret_cast<i16x4*>(op) = v;
+}
+
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, bool join, hipStream_t stream) {
+  auto go = [&](auto d, auto b, auto c) {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;
+    hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC>), dim3((unsigned)p.nblocks), dim3(kWaves * 64), 0, stream, p);
+    if (join) hipLaunchKernelGGL((kv4_join_kernel<DD, BB>), dim3((unsigned)(p.T * p.Hq)), dim3(256), 0, stream, p);
+  };
+  auto by_type = [&](auto d) {
+    if (bf16 && cap) go(d, std::true_type{}, std::true_type{});
+    if (bf16 && !cap) go(d, std::true_type{}, std::false_type{});
+    if (!bf16 && cap) go(d, std::false_type{}, std::true_type{});
+    if (!bf16 && !cap) go(d, std::false_type{}, std::false_type{});
+  };
+  switch (D) {
+    case 64: by_type(std::integral_constant<int, 64>{}); break;
+    case 128: by_type(std::integral_constant<int, 128>{}); break;
+    case 256: by_type(std::integral_constant<int, 256>{}); break;
+    default: by_type(std::integral_constant<int, 512>{}); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace gfa

@@ -5,6 +5,10 @@
 
 namespace gfa {
 
+struct Kv4RowsParams;
+struct Kv4PlanParams;
+struct Kv4AttnParams;
+
 hipError_t launch_fwd(const FwdParams& p, int head_dim, int block_kv, int nwaves, bool bf16, bool cap, bool drop,
                       hipStream_t stream);
 hipError_t launch_fwd_rows(const FwdParams& p, int head_dim, bool bf16, bool cap, bool drop, hipStream_t stream);
@@ -20,5 +24,9 @@ hipError_t launch_seg_mask(const uint8_t* mask, int64_t row_stride, int B, int N
                            hipStream_t stream);
 hipError_t launch_bwd_dq_rows(const BwdDqDsParams& p, int head_dim, bool bf16, hipStream_t stream);
 hipError_t launch_bwd_dq_ds(const BwdDqDsParams& p, int head_dim, bool bf16, hipStream_t stream);
+hipError_t launch_kv4_write(const Kv4RowsParams& p, int head_dim, bool bf16, hipStream_t stream);
+hipError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, bool bf16, hipStream_t stream);
+hipError_t launch_kv4_plan(const Kv4PlanParams& p, hipStream_t stream);
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, bool join, hipStream_t stream);
 
 }  // namespace gfa

@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define GFA_VERSION 107 /* 1.0.7: segment tables from position ids and masks (1.0.6: materialised backward, 1.0.5: run-time work distribution, 1.0.4: attention dropout, 1.0.3: soft-capping) */
+#define GFA_VERSION 108 /* 1.0.8: key/value cache in 4 bits (1.0.7: segment tables from position ids and masks, 1.0.6: materialised backward, 1.0.5: run-time work distribution, 1.0.4: attention dropout, 1.0.3: soft-capping) */
 
 typedef enum {
   GFA_DTYPE_FP16 = 0,
@@ -246,6 +246,102 @@ int gfa_segments_from_positions(const void* pos, int32_t pos_bits, int64_t row_s
                                 int32_t* seg_lo, int32_t* seg_hi, void* stream);
 int gfa_segments_from_mask(const uint8_t* mask, int64_t row_stride, int32_t batch, int32_t seq_len, int32_t* seg_lo,
                            int32_t* seg_hi, int32_t* bad, void* stream);
+
+/* ---- Serving: a key/value cache held in 4 bits (no counterpart in the reference) ----
+ *
+ * A cache is two device arrays. `codes` (num_blocks, heads_kv, 2, block_size, head_dim / 2) bytes and
+ * `scales` (num_blocks, heads_kv, 2, block_size, head_dim / 32) bytes hold blocks of block_size tokens
+ * (a power of two, 32 to 1024) of K (side 0) and V (side 1). Format: MXFP4, 4.25 bits per
+ * element: 32 neighbouring channels of a token and head share a power of two 2^e (its byte is
+ * e + 127), an element is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6. With amax the largest
+ * magnitude of the 32, e = floor(log2 amax) - 2, one more where amax > 7 * 2^e, within [-125, 125] for
+ * bf16 and [-23, 13] for fp16; elements round to the nearest value, ties to the even code, and
+ * saturate at 6. A block that holds an infinity or a NaN has the byte 255 and reads as NaN; where it
+ * is one of V, the token's first block of K has it too. The order of the bytes inside a head's block
+ * is the kernels' own (csrc/gfa_kv4.h). `dtype` is the type of the rows written, read and
+ * attended with.
+ *
+ * A token's place is its slot, block * block_size + offset. A request's blocks stand in its row of a
+ * block table, position p of it in block table[p / block_size]; entries outside [0, num_blocks) are
+ * no block. Token rows are (batch, heads, seq_len, head_dim) tensors with a unit-stride head dim, 16-byte
+ * aligned rows and strides that are multiples of 8 elements; token t of a call is row t % seq_len of
+ * batch entry t / seq_len (a packed step has batch 1, a step of single tokens may have seq_len 1). */
+typedef struct {
+  void* codes;
+  void* scales;
+  int32_t num_blocks, heads_kv, block_size, head_dim;
+  int32_t dtype; /* gfa_dtype */
+} gfa_kv4_cache;
+
+/* Rows to the cache (gfa_kv4_write: k and v are read) or from it (gfa_kv4_read: k and v are written). */
+typedef struct {
+  gfa_kv4_cache cache;
+  void* k; /* (batch, heads_kv, seq_len, head_dim) */
+  void* v;
+  gfa_strides k_strides, v_strides;
+  int32_t batch, seq_len;
+  const int64_t* slots; /* (batch * seq_len); outside [0, num_blocks * block_size): writes nothing, reads zeros.
+                           Slots of one write must differ: a slot given twice ends with bytes of both rows. */
+  void* stream;
+} gfa_kv4_rows_args;
+
+int gfa_kv4_write(const gfa_kv4_rows_args* args);
+int gfa_kv4_read(const gfa_kv4_rows_args* args);
+
+/* A step's plan: request b holds lens[b] tokens and gets fresh[b] more (negative counts are 0), packed
+ * in the order of the requests. It holds ceil(lens / block_size) blocks; further ones it needs are the
+ * next entries of free_ids behind the *used that are taken, handed out in the order of the requests
+ * and entered in its row of the table. Where the free list ends, -1 is entered: *used_out above
+ * free_count tells of it. One launch; the inputs other than the table are only read, the outputs must not
+ * overlap them. */
+typedef struct {
+  const int32_t* lens;  /* (requests) */
+  const int32_t* fresh; /* (requests) */
+  int32_t* table;       /* (requests, table_width), rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* free_ids; /* (free_count) */
+  const int32_t* used;     /* (1) */
+  int32_t requests, table_width, free_count, block_size;
+  int32_t tokens;     /* length of slots and positions */
+  int64_t* slots;     /* (tokens): the new tokens' slots; -1 where there is no block, behind the last token or
+                         past the table's width */
+  int32_t* positions; /* (tokens): their positions in their requests (0 behind the last) */
+  int32_t* cu;        /* (requests + 1): first token of each request, at most `tokens` */
+  int32_t* lens_out;  /* (requests): lens + fresh */
+  int32_t* used_out;  /* (1) */
+  void* stream;
+} gfa_kv4_plan_args;
+
+int gfa_kv4_plan(const gfa_kv4_plan_args* args);
+
+/* Attention of a step's new tokens over the cache, the new tokens' own keys and values in it. Request b has
+ * lens[b] tokens altogether, its new ones are the last cu[b + 1] - cu[b] of them and stand in q from
+ * token cu[b] on (cu NULL: every request has batch * seq_len / requests). New token i, at position
+ * p = lens - fresh + i, attends to positions <= p, with a window W > 0 only to those > p - W; without
+ * causal to all lens positions. Positions without a block are not attended to; a row that attends to
+ * nothing is zero, and so are rows behind the last request's. max_new, when not 0, is the most new tokens
+ * of any request and only chooses the kernel. Values in the tables, lens and cu cannot make the call
+ * address memory outside its arrays. */
+typedef struct {
+  gfa_kv4_cache cache;
+  const void* q; /* (batch, heads_q, seq_len, head_dim) */
+  void* o;
+  gfa_strides q_strides, o_strides;
+  int32_t batch, heads_q, seq_len, requests;
+  const int32_t* table; /* (requests, table_width), rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* lens; /* (requests) */
+  const int32_t* cu;   /* (requests + 1) or NULL */
+  int32_t table_width, causal, window, max_new;
+  float scale, softcap; /* softcap 0 = off */
+  void* workspace;      /* >= gfa_kv4_attn_workspace_bytes(args), 16-byte aligned */
+  size_t workspace_bytes;
+  void* stream;
+} gfa_kv4_attn_args;
+
+int gfa_kv4_attn(const gfa_kv4_attn_args* args);
+/* Workspace of gfa_kv4_attn(args) in bytes; pointers are not read, but for whether cu is NULL. */
+size_t gfa_kv4_attn_workspace_bytes(const gfa_kv4_attn_args* args);
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* gfa_last_error(void);
