@@ -108,6 +108,9 @@ struct Kv4PlanParams {
   int *positions, *cu, *lens_out, *used_out;
 };
 
+// Query rows of a workgroup of the chunk kernel.
+constexpr int kv4_chunk_rows(int D) { return D == 512 ? 128 : 256; }
+
 struct Kv4AttnParams {
   Kv4Cache cache;
   const uint16_t* q;

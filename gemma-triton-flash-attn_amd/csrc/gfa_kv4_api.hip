@@ -81,37 +81,66 @@ int rows_call(const gfa_kv4_rows_args* a, bool write) {
                   write ? "cache write" : "cache read");
 }
 
-// Work split of one attention call. The lengths live on the device, so the host sizes the grid for any
-// lengths the block tables can hold and the kernels divide what there is (gfa_kv4_attn.hip).
-struct Split {
+// One kernel's part of an attention call. The lengths live on the device, so the host sizes the grid for any
+// lengths the block tables can hold and the kernels divide what there is (gfa_kv4_sched.h).
+struct Part {
+  bool runs;
   int min_tiles, target;
   int64_t nblocks;
-  bool join;  // some request may take more than one chunk
+  bool join;  // some row block may take more than one chunk
   size_t part_bytes, ml_bytes;
+  size_t bytes() const { return part_bytes + ml_bytes; }
+};
+struct Split {
+  int row_limit;  // requests of more query rows (new tokens times heads of a KV head) take the chunk kernel
+  Part few, many;
 };
 
-constexpr int kRows = 16;
+constexpr int kRows = 16;  // of a workgroup of the split kernel
+constexpr int kRowLimit = 32;
+
+void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int min_tiles, int target, int spare) {
+  int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
+  if (a->causal && a->window > 0)
+    tiles = std::min<int64_t>(tiles, ((int64_t)a->window + (int64_t)a->batch * a->seq_len + 31) / 32 + 1);
+  const int64_t chunks = std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles);
+  s.runs = row_blocks > 0;
+  s.join = chunks > 1;
+  s.min_tiles = s.join ? min_tiles : 0x3fffffff;
+  s.target = target;
+  // items: one per row block, and as many more as there are full chunks
+  const int64_t hkv = a->cache.heads_kv;
+  const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
+  s.nblocks = items * hkv + spare;
+  if (s.join) {
+    s.part_bytes = (size_t)s.nblocks * rows * a->cache.head_dim * sizeof(float);
+    s.ml_bytes = (size_t)s.nblocks * rows * 2 * sizeof(float);
+  }
+}
 
 Split split_of(const gfa_kv4_attn_args* a) {
   Split s{};
-  const int64_t G = a->heads_q / a->cache.heads_kv;
+  const int64_t G = a->heads_q / a->cache.heads_kv, R = a->requests;
   const int64_t T = (int64_t)a->batch * a->seq_len;
-  s.min_tiles = 8;
-  s.target = 512;
-  int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
-  if (a->causal && a->window > 0) tiles = std::min<int64_t>(tiles, ((int64_t)a->window + T + 31) / 32 + 1);
-  const int64_t row_blocks = a->cu ? (T * G + (kRows - 1) * (int64_t)a->requests) / kRows
-                                   : a->requests * ((T / a->requests * G + kRows - 1) / kRows);
-  // chunks: one per row block, and as many more as there are full ones
-  const int64_t chunks = std::max<int64_t>(1, (tiles + s.min_tiles - 1) / s.min_tiles);
-  s.join = chunks > 1;
-  if (!s.join) s.min_tiles = 0x3fffffff;
-  const int64_t items = std::min(row_blocks * chunks, row_blocks + (s.target + a->cache.heads_kv - 1) / a->cache.heads_kv);
-  s.nblocks = items * a->cache.heads_kv + (a->cu ? 64 : 0);
-  if (s.join) {
-    s.part_bytes = (size_t)s.nblocks * kRows * a->cache.head_dim * sizeof(float);
-    s.ml_bytes = (size_t)s.nblocks * kRows * 2 * sizeof(float);
+  const int64_t most = a->cu == nullptr ? T / R : a->max_new > 0 ? std::min<int64_t>(a->max_new, T) : T;
+  // No request can have more rows than the limit: then all are the split kernel's, whatever max_new promised.
+  s.row_limit = most * G <= kRowLimit ? 0x7fffffff : kRowLimit;
+  const int D = a->cache.head_dim, big = gfa::kv4_chunk_rows(D);
+  int64_t few, many = 0;
+  if (a->cu == nullptr) {
+    const bool large = most * G > s.row_limit;
+    few = large ? 0 : R * ((most * G + kRows - 1) / kRows);
+    many = large ? R * ((most * G + big - 1) / big) : 0;
+  } else {
+    few = (T * G + (kRows - 1) * R) / kRows;
+    if (s.row_limit == kRowLimit) {
+      few = std::min<int64_t>(few, R * ((kRowLimit + kRows - 1) / kRows));
+      many = T * G / big + std::min<int64_t>(R, T * G / (kRowLimit + 1));
+    }
   }
+  // with cu, workgroups to spare: rows behind the last request's
+  size_part(s.few, a, few, kRows, 8, 512, a->cu ? 64 : 0);
+  size_part(s.many, a, many, big, 32, 512, 0);
   return s;
 }
 
@@ -184,7 +213,7 @@ int gfa_kv4_plan(const gfa_kv4_plan_args* a) {
 size_t gfa_kv4_attn_workspace_bytes(const gfa_kv4_attn_args* a) {
   if (check_attn(a) != GFA_OK) return 0;
   const Split s = split_of(a);
-  return s.part_bytes + s.ml_bytes;
+  return s.few.bytes() + s.many.bytes();
 }
 
 int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
@@ -194,8 +223,9 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   if (!aligned(a->table, 4) || !aligned(a->lens, 4) || (a->cu != nullptr && !aligned(a->cu, 4)))
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "table, lens and cu must be 4-byte aligned pointers");
   const Split s = split_of(a);
-  if (s.nblocks > 0x7fffffff) return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)s.nblocks);
-  const size_t need = s.part_bytes + s.ml_bytes;
+  for (const Part* part : {&s.few, &s.many})
+    if (part->nblocks > 0x7fffffff) return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)part->nblocks);
+  const size_t need = s.few.bytes() + s.many.bytes();
   if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
     return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, a->workspace_bytes);
   gfa::Kv4AttnParams p{};
@@ -223,15 +253,25 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   const bool cap = a->softcap > 0.f;
   p.xs = (cap ? a->softcap : a->scale) * 1.4426950408889634f;
   p.cap_a = cap ? a->scale / a->softcap : 0.f;
-  p.min_tiles = s.min_tiles;
-  p.target = s.target;
-  p.nblocks = (int)s.nblocks;
-  p.row_limit = 0x7fffffff;
-  p.part = static_cast<float*>(a->workspace);
-  p.part_ml = reinterpret_cast<float*>(static_cast<char*>(a->workspace) + s.part_bytes);
-  return launched(gfa::launch_kv4_split(p, a->cache.head_dim, a->cache.dtype == GFA_DTYPE_BF16, cap, s.join,
-                                        static_cast<hipStream_t>(a->stream)),
-                  "cache attention");
+  p.row_limit = s.row_limit;
+  const auto stream = static_cast<hipStream_t>(a->stream);
+  const int D = a->cache.head_dim;
+  const bool bf16 = a->cache.dtype == GFA_DTYPE_BF16;
+  char* ws = static_cast<char*>(a->workspace);
+  for (const bool large : {true, false}) {
+    const Part& part = large ? s.many : s.few;
+    if (!part.runs) continue;
+    p.min_tiles = part.min_tiles;
+    p.target = part.target;
+    p.nblocks = (int)part.nblocks;
+    p.part = reinterpret_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);
+    ws += part.bytes();
+    hipError_t err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, stream) : gfa::launch_kv4_split(p, D, bf16, cap, stream);
+    if (err == hipSuccess && part.join) err = gfa::launch_kv4_join(p, D, bf16, large, stream);
+    if (err != hipSuccess) return launched(err, "cache attention");
+  }
+  return gfa::api_ok();
 }
 
 }  // extern "C"

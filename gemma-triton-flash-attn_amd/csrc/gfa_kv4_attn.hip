@@ -10,14 +10,12 @@
 //    4 g + r, 16 + 4 g + r, in which V is stored. No LDS and no barrier until the end.
 //  * Every wave keeps its own running maximum m, row sum l and O^T; they are joined once through LDS,
 //    and the chunks' results by the join kernel below from fp32 partial sums, in a fixed order.
-#include "gfa_kv4.h"
+#include "gfa_kv4_sched.h"
 #include "gfa_launch.h"
 
 namespace gfa {
 
 namespace {
-
-typedef float f32x4v __attribute__((ext_vector_type(4)));
 
 template <bool IS_BF16>
 __device__ __forceinline__ f32x4 mma16(i16x8 a, i16x8 b, f32x4 c) {
@@ -40,57 +38,6 @@ __device__ __forceinline__ float quad_sum(float x) {
 
 constexpr int kRows = 16;
 constexpr int kWaves = 4;
-constexpr int kTile = 32;  // tokens
-
-// What a request asks for.
-struct Request {
-  int t0, fresh, len;  // first new token, new tokens, tokens with the new ones
-  int row_blocks;      // 0: not this kernel's
-  int first, tiles;    // key tiles that some row sees
-};
-__device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
-  Request r{};
-  if (b >= p.B) return r;
-  if (p.cu != nullptr) {
-    r.t0 = p.cu[b];
-    r.fresh = max(p.cu[b + 1] - r.t0, 0);
-  } else {
-    r.fresh = p.T / p.B;
-    r.t0 = b * r.fresh;
-  }
-  r.len = max(p.lens[b], 0);
-  const int64_t rows = (int64_t)r.fresh * p.G;
-  r.row_blocks = rows > p.row_limit ? 0 : (int)((rows + kRows - 1) / kRows);
-  const int held = (int)min((int64_t)r.len, (int64_t)p.M << p.cache.bs_log2);
-  const int lo = p.causal && p.window > 0 ? max(r.len - r.fresh - p.window + 1, 0) : 0;
-  r.first = lo / kTile;
-  r.tiles = held > lo ? (held + kTile - 1) / kTile - r.first : 0;
-  return r;
-}
-
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-  return x;
-}
-
-// Key tiles per chunk: the whole grid's tiles spread over about `target` workgroups, at least min_tiles
-// each. The lengths are the device's, so every wave derives the split from them, the same in every
-// workgroup and in the join kernel.
-__device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, int lane) {
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Request r = request_of(p, b0 + lane);
-    total += (int64_t)r.row_blocks * r.tiles;
-  }
-  total = wave_sum64(total) * p.cache.Hkv;
-  const int64_t each = (total + p.target - 1) / p.target;
-  return (int)min(max(each, (int64_t)p.min_tiles), (int64_t)0x3fffffff);
-}
-__device__ __forceinline__ int chunks_of(const Request& r, int per) { return max((r.tiles + per - 1) / per, 1); }
-
-// 1 / l of a finished row. Without weight l is a mark, not a sum: the row is 0 / 0 where it saw keys.
-__device__ __forceinline__ float row_inv(float m, float l) { return m == -INFINITY ? 1.0f / (0.f * l) : 1.0f / l; }
 
 }  // namespace
 
@@ -109,33 +56,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
   const int head = (int)blockIdx.x % p.cache.Hkv;
   const int64_t item = (int)blockIdx.x / p.cache.Hkv;
 
-  // ---- the item: its request, row block and chunk ----
-  const int per = chunk_tiles(p, lane);
-  Request rq{};
-  int b = -1, rb = 0, ch = 0, nch = 1;
-  int64_t items = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Request r = request_of(p, b0 + lane);
-    const int64_t mine = (int64_t)r.row_blocks * chunks_of(r, per);
-    int64_t s = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int64_t y = __shfl_up(s, m);
-      if (lane >= m) s += y;
-    }
-    const int64_t before = items + s - mine;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
-    if (hit != 0) {
-      const int src = __builtin_ctzll(hit);
-      b = __builtin_amdgcn_readfirstlane(b0 + src);
-      rq = request_of(p, b);
-      nch = chunks_of(rq, per);
-      const int i = (int)(item - __shfl(before, src));
-      rb = __builtin_amdgcn_readfirstlane(i / nch);
-      ch = __builtin_amdgcn_readfirstlane(i % nch);
-    }
-    items += __shfl(s, 63);
-  }
+  const Item it = find_item<kRows, false>(p, item, lane);
+  const Request& rq = it.rq;
+  const int b = it.b, rb = it.rb, ch = it.ch, nch = it.nch, per = it.per;
+  const int64_t items = it.items;
   if (b < 0) {
     // No item: tokens behind the last request's are zeros, the workgroups without an item take them in turn.
     if (p.cu == nullptr) return;
@@ -392,82 +316,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
   }
 }
 
-// Joins the chunks of a row: one workgroup per token and query head.
-template <int D, bool IS_BF16>
-__global__ __launch_bounds__(256) void kv4_join_kernel(const Kv4AttnParams p) {
-  constexpr int LPR = D / 4;         // lanes per row, four channels each
-  constexpr int GR = 256 / LPR;      // chunks at a time
-  __shared__ f32x4 o_lds[256];
-  const int lane = threadIdx.x & 63;
-  const int t = (int)(blockIdx.x / p.Hq), qh = (int)(blockIdx.x % p.Hq);
-  const int head = qh / p.G;
-  // the token's request
-  const int per = chunk_tiles(p, lane);
-  int64_t items = 0, base = -1;
-  Request rq{};
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Request r = request_of(p, b0 + lane);
-    const int64_t mine = (int64_t)r.row_blocks * chunks_of(r, per);
-    int64_t s = mine;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-      const int64_t y = __shfl_up(s, m);
-      if (lane >= m) s += y;
-    }
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(t >= r.t0 && t < r.t0 + r.fresh);
-    if (hit != 0) {
-      const int src = __builtin_ctzll(hit);
-      base = items + __shfl(s - mine, src);
-      rq = request_of(p, __builtin_amdgcn_readfirstlane(b0 + src));
-      break;
-    }
-    items += __shfl(s, 63);
-  }
-  if (base < 0 || rq.row_blocks == 0) return;
-  const int nch = chunks_of(rq, per);
-  if (nch == 1) return;
-  const int i = t - rq.t0;
-  const int row = i * p.G + qh % p.G;
-  const int64_t first = base + (int64_t)(row / kRows) * nch;  // item of chunk 0
-  if ((first + nch) * p.cache.Hkv > p.nblocks) return;       // lengths that do not fit the grid: see gfa.h
-  const int rr = row % kRows;
-  auto slot = [&](int c) { return ((first + c) * p.cache.Hkv + head) * kRows + rr; };
-  float m = -INFINITY;
-  for (int c = lane; c < nch; c += 64) m = fmaxf(m, p.part_ml[slot(c) * 2]);
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-  const float m_use = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-  for (int c = lane; c < nch; c += 64)
-    l += p.part_ml[slot(c) * 2 + 1] * (m == -INFINITY ? 1.f : fast_exp2(p.part_ml[slot(c) * 2] - m_use));
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) l += __shfl_xor(l, x);
-  f32x4 o{};
-  const int part = threadIdx.x / LPR, d = threadIdx.x % LPR * 4;
-  for (int c = part; c < nch; c += GR) {
-    const float w = fast_exp2(p.part_ml[slot(c) * 2] - m_use);
-    o += *reinterpret_cast<const f32x4*>(p.part + slot(c) * D + d) * w;
-  }
-  o_lds[threadIdx.x] = o;
-  __syncthreads();
-  if (part != 0) return;
-#pragma unroll
-  for (int k = 1; k < GR; ++k) o += o_lds[k * LPR + threadIdx.x];
-  const bool none = m == -INFINITY && l == 0.f;
-  const float inv = row_inv(m, l);
-  uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn + d;
-  i16x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = to16<IS_BF16>(none ? 0.f : o[e] * inv);
-  *reinterpret_cast<i16x4*>(op) = v;
-}
-
-hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, bool join, hipStream_t stream) {
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, hipStream_t stream) {
   auto go = [&](auto d, auto b, auto c) {
     constexpr int DD = decltype(d)::value;
     constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;
     hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC>), dim3((unsigned)p.nblocks), dim3(kWaves * 64), 0, stream, p);
-    if (join) hipLaunchKernelGGL((kv4_join_kernel<DD, BB>), dim3((unsigned)(p.T * p.Hq)), dim3(256), 0, stream, p);
   };
   auto by_type = [&](auto d) {
     if (bf16 && cap) go(d, std::true_type{}, std::true_type{});

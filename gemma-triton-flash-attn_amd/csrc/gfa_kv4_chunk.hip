@@ -1,0 +1,498 @@
+// Attention of a step's new tokens over the key/value cache in 4 bits (gfa_kv4.h), gfx950: many query rows per
+// request (chunks of a prompt).
+//
+// A workgroup takes ROWS query rows of one request and KV head (all query heads of neighbouring tokens, so
+// that causal row blocks end close together) and one chunk of the key tiles they see (gfa_kv4_sched.h; one
+// chunk where the row blocks fill the GPU). Its four waves hold MT x 32 rows each:
+//  * A tile's codes and scales (34 D bytes for 32 tokens; K swizzled) are copied global -> LDS once per
+//    workgroup, one tile ahead, and every wave decodes what it multiplies in registers: S^T = K Q^T
+//    and O^T += V^T P^T with v_mfma_f32_32x32x16, rows on lanes, P in registers in the B layout of the
+//    second product. A tile kept decoded in LDS would cost four times the LDS reads (64 D bytes per
+//    wave and product), which then take as long as the products; the codes cost a quarter, and the
+//    decoding (one instruction per two elements, two for V) issues in the products' shadow.
+//  * Softmax against a fixed reference per row, the maximum of the first tile it sees a key of, so that the
+//    loop never rescales O^T (which stays in AGPRs). A row whose scores pass the reference by more than
+//    2^kMargin (P ends at 2^16 in fp16) makes the workgroup redo its rows once against the exact maxima, seen
+//    along the way. Ordinary inputs never do. Row sums are held in 32 bits.
+#include "gfa_kv4_sched.h"
+#include "gfa_launch.h"
+
+namespace gfa {
+
+namespace {
+
+// Tile copies of one wave: 1 KB runs of codes (K, then V) and the scales, dealt to the four waves in turn.
+template <int D>
+struct Kv4Copies {
+  using L = Kv4Layout<D>;
+  static constexpr int RUNS = L::TILE_CODES / 1024;  // per side
+  unsigned k_off;                                    // this lane's byte of a K run, swizzled
+  int lane, wave;
+  __device__ __forceinline__ void init(int wave_, int lane_) {
+    lane = lane_;
+    wave = wave_;
+    if constexpr (D == 64) {
+      const int t = lane >> 1;  // 32 tokens of 2 pieces
+      k_off = t * 32 + (((lane & 1) ^ ((t >> 3) & 1)) << 4);
+    } else {
+      const int t = lane >> 2;  // 16 tokens of 4 pieces
+      k_off = t * 64 + (((lane & 3) ^ ((t >> 2) & 3)) << 4);
+    }
+  }
+  __device__ __forceinline__ void load(const Kv4Cache& c, int block, int head, int sub, char GFA_LDS* kt, char GFA_LDS* vt,
+                                       char GFA_LDS* st) const {
+    // one (block, head): K side, then V side
+    const int side = (D / 2) << c.bs_log2, sside = (D / 32) << c.bs_log2;
+    const auto rc = __builtin_amdgcn_make_buffer_rsrc(c.codes + kv4_codes_at<D>(c, block, head, 0), 0, 2 * side, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 2 * RUNS; i += 4) {
+      const int run = i + wave;
+      if (2 * RUNS >= 4 || run < 2 * RUNS) {
+        const bool v = run >= RUNS;
+        const int r = v ? run - RUNS : run;
+        const unsigned soff = (unsigned)((v ? side : 0) + sub * L::TILE_CODES + r * 1024);
+        char GFA_LDS* dst = (v ? vt : kt) + r * 1024;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (void GFA_LDS*)dst, 16, v ? (unsigned)lane * 16 : k_off, soff, 0, 0);
+      }
+    }
+    if (wave == (2 * RUNS) % 4) {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(c.scales + kv4_scales_at<D>(c, block, head, 0), 0, 2 * sside, 0x00020000);
+      constexpr int LS = D / 16;  // lanes per side
+      const unsigned off = (unsigned)(lane < LS ? lane * 16 : sside + (lane - LS) * 16);
+      if (lane < 2 * LS) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (void GFA_LDS*)st, 16, off, sub * L::TILE_SCALES, 0, 0);
+    }
+  }
+};
+
+// A product of the S^T chain kept in VGPRs (O^T fills the AGPRs, and built from the builtin the chain would
+// run there too), whose operand the vector unit has just decoded: two wait states until a product may
+// read it. The chain's result is read behind mfma_result_fence.
+template <bool IS_BF16, bool FIRST>
+__device__ __forceinline__ void mma32_decoded(f32x16& c, const i16x8& a, const i16x8& b) {
+  if constexpr (FIRST) {
+    if constexpr (IS_BF16) {
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+    } else {
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, 0" : "=&v"(c) : "v"(a), "v"(b));
+    }
+  } else {
+    if constexpr (IS_BF16) {
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    } else {
+      asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(c) : "v"(a), "v"(b));
+    }
+  }
+}
+
+}  // namespace
+
+template <int D, bool IS_BF16, bool CAP>
+__global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p) {
+  using L = Kv4Layout<D>;
+  constexpr int ROWS = kv4_chunk_rows(D);
+  constexpr int MT = ROWS / 128;                 // 32-row blocks per wave
+  constexpr int KT = D / 16;                     // products of a score block
+  constexpr int CPL = D / 32;                    // channels of an O^T operand row: 32-row blocks of O^T
+  constexpr int NJ = D == 64 ? 1 : D / 128;
+  constexpr bool PIN = D >= 256;                 // O^T fills the AGPRs
+  constexpr float kMargin = IS_BF16 ? 64.0f : 15.0f;          // log2
+  __shared__ int redo_flag;
+  __shared__ __attribute__((aligned(1024))) char k_lds0[L::TILE_CODES], k_lds1[L::TILE_CODES];
+  __shared__ __attribute__((aligned(1024))) char v_lds0[L::TILE_CODES], v_lds1[L::TILE_CODES];
+  __shared__ __attribute__((aligned(1024))) char s_lds0[1024], s_lds1[1024];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int h = lane >> 5, l32 = lane & 31, p16 = lane & 15, hi = (lane >> 4) & 1;
+  const int head = (int)blockIdx.x % p.cache.Hkv;
+
+  const Item it = find_item<ROWS, true>(p, (int)blockIdx.x / p.cache.Hkv, lane);
+  if (it.b < 0) return;
+  const Request& rq = it.rq;
+  const int rb = rq.row_blocks - 1 - it.rb;  // the rows that see most keys first
+  const int row0 = rb * ROWS;
+
+  // ---- key tiles of this row block's chunk ----
+  const int held = (int)min((int64_t)rq.len, (int64_t)p.M << p.cache.bs_log2);
+  const int i_lo = row0 / p.G, i_hi = min((row0 + ROWS - 1) / p.G, rq.fresh - 1);
+  const int pos0 = rq.len - rq.fresh;  // position of new token 0
+  int k_lo = 0, k_hi = held;
+  if (p.causal) {
+    k_hi = min(held, pos0 + i_hi + 1);
+    if (p.window > 0) k_lo = max(0, pos0 + i_lo - p.window + 1);
+  }
+  const int t_first = k_lo / kTile + it.ch * it.per;
+  const int t_end = k_hi > k_lo ? min((k_hi + kTile - 1) / kTile, t_first + it.per) : t_first;
+
+  // ---- this lane's rows ----
+  int qt[MT], qh[MT];
+  bool live[MT];
+  VisRange vis[MT];
+  int all_lo = 0, all_hi = held;  // keys that every row of the wave sees
+  i16x8 qf[MT][KT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    const int row = row0 + (wave * MT + m) * 32 + l32;
+    const int i = row / p.G;
+    qt[m] = rq.t0 + i;
+    qh[m] = head * p.G + row % p.G;
+    live[m] = i < rq.fresh && qt[m] >= 0 && qt[m] < p.T;
+    const int pos = pos0 + i;
+    const int last = live[m] ? min(p.causal ? pos : rq.len - 1, held - 1) : -1;
+    vis[m] = make_range(p.causal && p.window > 0 ? max(pos - p.window + 1, 0) : 0, last);
+    const int tc = live[m] ? qt[m] : 0;  // rows past the last read another's query; nothing of theirs goes out
+    const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)qh[m] * p.qsh + (tc % p.N) * p.qsn;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+      for (int u = 0; u < (D == 64 ? 1 : 2); ++u) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          qf[m][(j * 2 + u) * 4 + k] = *reinterpret_cast<const i16x8*>(qp + 128 * j + 32 * (2 * u + h) + 8 * k);
+      }
+    }
+  }
+  if (p.causal) {
+    const int first = row0 + wave * MT * 32;
+    all_hi = min(all_hi, pos0 + first / p.G + 1);
+    if (p.window > 0) all_lo = pos0 + (first + MT * 32 - 1) / p.G - p.window + 1;
+  }
+
+  f32x16 acc[MT][CPL];
+  float m_ref[MT], m_seen[MT], l_run[MT];
+  bool seen[MT], ovf = false;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    m_ref[m] = m_seen[m] = -INFINITY;
+    seen[m] = false;
+  }
+  if (threadIdx.x == 0) redo_flag = 0;  // read behind a later barrier
+
+  // ---- the blocks of the tiles, 64 at a time in the lanes ----
+  const int tpb_log2 = p.cache.bs_log2 - 5;
+  const int* table = p.table + (int64_t)it.b * p.table_stride;
+  int ids = 0, ids_at = -1;
+  auto block_of = [&](int tile) __attribute__((always_inline)) {
+    const int col = tile >> tpb_log2;
+    if (ids_at < 0 || col - ids_at >= 64) {
+      ids_at = col;
+      ids = table[min(col + lane, p.M - 1)];
+    }
+    return __builtin_amdgcn_readlane(ids, col - ids_at);
+  };
+  Kv4Copies<D> copies;
+  copies.init(wave, lane);
+  const unsigned n_blocks = (unsigned)p.cache.num_blocks;
+  bool held_next = false;
+  auto fetch = [&](int tile, char GFA_LDS* kt, char GFA_LDS* vt, char GFA_LDS* st) __attribute__((always_inline)) {
+    const int block = block_of(tile);
+    const bool there = (unsigned)block < n_blocks;
+    held_next = there && tile < t_end;
+    copies.load(p.cache, there ? block : 0, head, tile & ((1 << tpb_log2) - 1), kt, vt, st);
+  };
+
+  const unsigned nan2 = IS_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
+  // LDS bytes of this lane: its K pieces (pair u of a chunk), K scales, V pieces, V scales
+  const int k_row = D == 64 ? l32 * 32 : l32 * 64;
+  const int k_swz = D == 64 ? (l32 >> 3) & 1 : (l32 >> 2) & 3;
+  const int v_piece = p16 * 16;
+  const int v_blk = p16 * L::PP / 32;
+
+  auto step = [&](int tile, const char GFA_LDS* kt, const char GFA_LDS* vt, const char GFA_LDS* st, char GFA_LDS* kn,
+                  char GFA_LDS* vn, char GFA_LDS* sn) __attribute__((always_inline)) {
+    barrier_tile();
+    const bool is_held = held_next;
+    fetch(tile + 1, kn, vn, sn);
+
+    // ---- S^T ----
+    f32x16 s[MT];
+    if constexpr (!PIN) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) s[m] = f32x16{};
+    }
+    // piece i = (u, j): 32 channels of a token a lane, four products; read one piece ahead
+    constexpr int NU = D == 64 ? 1 : 2, NP = NU * NJ;
+    auto k_piece = [&](int i) __attribute__((always_inline)) {
+      const int u = i / NJ, j = i % NJ;
+      return __builtin_bit_cast(uint4, lds_read16(kt, j * 2048 + k_row + (((D == 64 ? h : 2 * u + h) ^ k_swz) << 4)));
+    };
+    auto k_scales = [&](int u) __attribute__((always_inline)) -> unsigned {
+      if constexpr (D == 64) return *reinterpret_cast<const uint8_t GFA_LDS*>(st + l32 * 2 + h);
+      const char GFA_LDS* sp = st + l32 * L::SC + (2 * u + h) * NJ;
+      if constexpr (NJ == 4) return *reinterpret_cast<const unsigned GFA_LDS*>(sp);
+      if constexpr (NJ == 2) return *reinterpret_cast<const uint16_t GFA_LDS*>(sp);
+      return *reinterpret_cast<const uint8_t GFA_LDS*>(sp);
+    };
+    uint4 next = k_piece(0);
+    unsigned sbs[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) sbs[u] = k_scales(u);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int j = i % NJ;
+      const uint4 w = next;
+      if (i + 1 < NP) next = k_piece(i + 1);
+      const unsigned sb = sbs[i / NJ];
+      const unsigned bits = j == 0 ? kv4_scale_bits<0>(sb) : j == 1 ? kv4_scale_bits<1>(sb) : j == 2 ? kv4_scale_bits<2>(sb) : kv4_scale_bits<3>(sb);
+      const float sc = __uint_as_float(bits);
+      const unsigned cw[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        unsigned a[4] = {kv4_pair<IS_BF16, 0>(cw[k], sc), kv4_pair<IS_BF16, 1>(cw[k], sc),
+                         kv4_pair<IS_BF16, 2>(cw[k], sc), kv4_pair<IS_BF16, 3>(cw[k], sc)};
+        if (k == 0) a[0] = bits == 0x7f800000u ? nan2 : a[0];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const i16x8& q = qf[m][(j * 2 + i / NJ) * 4 + k];
+          if constexpr (!PIN) {
+            s[m] = mma32<IS_BF16>(__builtin_bit_cast(i16x8, a), q, s[m]);
+          } else if (i == 0 && k == 0) {
+            mma32_decoded<IS_BF16, true>(s[m], __builtin_bit_cast(i16x8, a), q);
+          } else {
+            mma32_decoded<IS_BF16, false>(s[m], __builtin_bit_cast(i16x8, a), q);
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (PIN) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) mfma_result_fence(s[m]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- softmax ----
+    const int k0 = tile * kTile;
+    const bool whole = is_held && k0 + kTile <= all_hi && k0 >= all_lo;
+    i16x8 pb[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      if constexpr (CAP) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[m][r] = cap_tanh(s[m][r] * p.cap_a);
+      }
+      if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[m][r] = is_held && vis[m].has(k0 + 8 * (r >> 2) + 4 * h + (r & 3)) ? s[m][r] : -INFINITY;
+      }
+      const int from = max(vis[m].base, k0);
+      seen[m] = seen[m] || (is_held && from < k0 + kTile && vis[m].has(from));
+      auto row_max = [&]() __attribute__((always_inline)) {
+        float mt = s[m][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[m][r]);
+        return halves_max(mt) * p.xs;
+      };
+      const float mt = row_max();
+      m_ref[m] = m_ref[m] == -INFINITY ? mt : m_ref[m];
+      ovf = ovf || mt > m_ref[m] + kMargin;
+      m_seen[m] = fmaxf(m_seen[m], mt);
+      const float m_use = m_ref[m] == -INFINITY ? 0.f : m_ref[m];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float pv = fast_exp2(s[m][r] * p.xs - m_use);
+        l_run[m] += pv;
+        pb[m][r >> 3][r & 7] = to16<IS_BF16>(pv);
+      }
+    }
+
+    __builtin_amdgcn_sched_barrier(0);
+    // ---- O^T += V^T P^T; step s2 over tokens 16 s2 .. 16 s2 + 15 ----
+    unsigned vsb[2][2];  // [token group h, 2 + h][half]
+#pragma unroll
+    for (int g2 = 0; g2 < 2; ++g2) {
+      const char GFA_LDS* sp = st + L::TILE_SCALES + ((2 * g2 + h) * L::SC + v_blk) * 8;
+      vsb[g2][0] = *reinterpret_cast<const unsigned GFA_LDS*>(sp);
+      vsb[g2][1] = *reinterpret_cast<const unsigned GFA_LDS*>(sp + 4);
+    }
+    // piece i = (s2, xx): 8 tokens of up to 8 channels a lane; read one piece ahead. Operand row (hi, p):
+    // channels p PP + CPL hi + x
+    constexpr int NX = D == 512 ? 2 : 1;
+    auto v_read = [&](int i, unsigned (&cw)[8]) __attribute__((always_inline)) {
+      const int s2 = i / NX, xx = i % NX;
+#pragma unroll
+      for (int g2 = 0; g2 < 2; ++g2) {
+        if constexpr (D == 64) {
+          const char GFA_LDS* vp = vt + (2 * g2 + h) * 256 + v_piece + s2 * 8;
+          const unsigned a = *reinterpret_cast<const unsigned GFA_LDS*>(vp), b = *reinterpret_cast<const unsigned GFA_LDS*>(vp + 4);
+          cw[4 * g2] = a >> (8 * hi);
+          cw[4 * g2 + 1] = a >> (16 + 8 * hi);
+          cw[4 * g2 + 2] = b >> (8 * hi);
+          cw[4 * g2 + 3] = b >> (16 + 8 * hi);
+        } else {
+          const int x8 = D == 512 ? 2 * hi + xx : D == 256 ? hi : 0;
+          const uint4 w = __builtin_bit_cast(uint4, lds_read16(vt, x8 * 2048 + s2 * 1024 + (2 * g2 + h) * 256 + v_piece));
+          cw[4 * g2] = w.x;
+          cw[4 * g2 + 1] = w.y;
+          cw[4 * g2 + 2] = w.z;
+          cw[4 * g2 + 3] = w.w;
+        }
+      }
+    };
+    float sc[8];
+    unsigned ahead[8];
+    v_read(0, ahead);
+#pragma unroll
+    for (int i = 0; i < 2 * NX; ++i) {
+      const int s2 = i / NX, xx = i % NX;
+      unsigned cw[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) cw[e] = D == 128 ? ahead[e] >> (16 * hi) : ahead[e];
+      if (i + 1 < 2 * NX) v_read(i + 1, ahead);
+      if (xx == 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const unsigned w = vsb[e >> 2][s2];
+          const unsigned bits = (e & 3) == 0 ? kv4_scale_bits<0>(w) : (e & 3) == 1 ? kv4_scale_bits<1>(w) : (e & 3) == 2 ? kv4_scale_bits<2>(w) : kv4_scale_bits<3>(w);
+          // finite whatever the byte: P is 0 where a row does not see the token, and 0 times that stays 0
+          sc[e] = __uint_as_float(min(bits, (unsigned)Kv4Range<IS_BF16>::hi << 23));
+        }
+      }
+      auto products = [&](auto sel, int x0) __attribute__((always_inline)) {
+        constexpr int SEL = decltype(sel)::value;
+        unsigned q[8], even[4], odd[4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = kv4_pair<IS_BF16, SEL>(cw[e], sc[e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          even[e] = __builtin_amdgcn_perm(q[2 * e + 1], q[2 * e], 0x05040100u);
+          odd[e] = __builtin_amdgcn_perm(q[2 * e + 1], q[2 * e], 0x07060302u);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          acc[m][x0] = mma32<IS_BF16>(__builtin_bit_cast(i16x8, even), pb[m][s2], acc[m][x0]);
+          acc[m][x0 + 1] = mma32<IS_BF16>(__builtin_bit_cast(i16x8, odd), pb[m][s2], acc[m][x0 + 1]);
+        }
+      };
+      products(std::integral_constant<int, 0>{}, 8 * xx);
+      if constexpr (D >= 128) products(std::integral_constant<int, 1>{}, 8 * xx + 2);
+      if constexpr (D >= 256) {
+        products(std::integral_constant<int, 2>{}, 8 * xx + 4);
+        products(std::integral_constant<int, 3>{}, 8 * xx + 6);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (PIN) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int x = 0; x < CPL; ++x) pin_agpr(acc[m][x]);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  char GFA_LDS* const K0 = (char GFA_LDS*)k_lds0;
+  char GFA_LDS* const K1 = (char GFA_LDS*)k_lds1;
+  char GFA_LDS* const V0 = (char GFA_LDS*)v_lds0;
+  char GFA_LDS* const V1 = (char GFA_LDS*)v_lds1;
+  char GFA_LDS* const S0 = (char GFA_LDS*)s_lds0;
+  char GFA_LDS* const S1 = (char GFA_LDS*)s_lds1;
+  // Two tiles a turn, straight-line: an odd number of tiles gets one that nothing sees, and the last step a copy that
+  // nothing reads. 
+  auto run_pass = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int x = 0; x < CPL; ++x) acc[m][x] = f32x16{};
+      l_run[m] = 0.f;
+    }
+    if (t_first < t_end) fetch(t_first, K0, V0, S0);
+    for (int t = t_first; t < t_end; t += 2) {
+      step(t, K0, V0, S0, K1, V1, S1);
+      step(t + 1, K1, V1, S1, K0, V0, S0);
+    }
+  };
+  for (int pass = 0;; ++pass) {
+    run_pass();
+    if (__builtin_amdgcn_ballot_w64(ovf) != 0 && lane == 0) redo_flag = 1;
+    barrier_tile();  // the last copy has landed too
+    if (pass == 1 || redo_flag == 0) break;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) m_ref[m] = m_seen[m];
+  }
+
+  // ---- rows out ----
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    float l = halves_sum(l_run[m]);
+    if (m_ref[m] == -INFINITY && l == 0.f && seen[m]) l = 1.f;  // a mark, see row_inv
+    if (it.nch > 1) {
+      const int64_t at = (int64_t)blockIdx.x * ROWS + (wave * MT + m) * 32 + l32;
+      if (h == 0) {
+        p.part_ml[at * 2] = m_ref[m];
+        p.part_ml[at * 2 + 1] = l;
+      }
+      if (live[m] && t_first < t_end) {
+        float* part = p.part + at * D;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int idx = 8 * (r >> 2) + 4 * h + (r & 3);
+          float* d = part + (idx & 15) * L::PP + CPL * (idx >> 4);
+          if constexpr (CPL >= 4) {
+#pragma unroll
+            for (int x = 0; x < CPL; x += 4)
+              *reinterpret_cast<f32x4*>(d + x) = f32x4{acc[m][x][r], acc[m][x + 1][r], acc[m][x + 2][r], acc[m][x + 3][r]};
+          } else {
+            d[0] = acc[m][0][r];
+            d[1] = acc[m][1][r];
+          }
+        }
+      }
+      continue;
+    }
+    if (!live[m]) continue;
+    const bool none = m_ref[m] == -INFINITY && l == 0.f;
+    const float inv = row_inv(m_ref[m], l);
+    uint16_t* op = p.o + (qt[m] / p.N) * p.osb + (int64_t)qh[m] * p.osh + (qt[m] % p.N) * p.osn;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int idx = 8 * (r >> 2) + 4 * h + (r & 3);
+      uint16_t* d = op + (idx & 15) * L::PP + CPL * (idx >> 4);
+      constexpr int W = CPL < 4 ? CPL : 4;
+#pragma unroll
+      for (int x = 0; x < CPL; x += W) {
+        typedef short vec __attribute__((ext_vector_type(W)));
+        vec v;
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] = to16<IS_BF16>(none ? 0.f : acc[m][x + e][r] * inv);
+        *reinterpret_cast<vec*>(d + x) = v;
+      }
+    }
+  }
+}
+
+// Explicit instantiations: the host launch stubs must exist for each variant.
+#define GFA_KV4_CHUNK_INST(DD)                                                      \
+  template __global__ void kv4_chunk_kernel<DD, true, true>(const Kv4AttnParams);   \
+  template __global__ void kv4_chunk_kernel<DD, true, false>(const Kv4AttnParams);  \
+  template __global__ void kv4_chunk_kernel<DD, false, true>(const Kv4AttnParams);  \
+  template __global__ void kv4_chunk_kernel<DD, false, false>(const Kv4AttnParams);
+GFA_KV4_CHUNK_INST(64)
+GFA_KV4_CHUNK_INST(128)
+GFA_KV4_CHUNK_INST(256)
+GFA_KV4_CHUNK_INST(512)
+#undef GFA_KV4_CHUNK_INST
+
+hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int D, bool bf16, bool cap, hipStream_t stream) {
+  auto go = [&](auto d, auto b, auto c) {
+    constexpr int DD = decltype(d)::value;
+    constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;
+    hipLaunchKernelGGL((kv4_chunk_kernel<DD, BB, CC>), dim3((unsigned)p.nblocks), dim3(256), 0, stream, p);
+  };
+  auto by_type = [&](auto d) {
+    if (bf16 && cap) go(d, std::true_type{}, std::true_type{});
+    if (bf16 && !cap) go(d, std::true_type{}, std::false_type{});
+    if (!bf16 && cap) go(d, std::false_type{}, std::true_type{});
+    if (!bf16 && !cap) go(d, std::false_type{}, std::false_type{});
+  };
+  switch (D) {
+    case 64: by_type(std::integral_constant<int, 64>{}); break;
+    case 128: by_type(std::integral_constant<int, 128>{}); break;
+    case 256: by_type(std::integral_constant<int, 256>{}); break;
+    default: by_type(std::integral_constant<int, 512>{}); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace gfa
