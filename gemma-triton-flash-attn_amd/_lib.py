@@ -230,6 +230,8 @@ def native():
 
         mod.bind(address("gfa_fwd"), address("gfa_bwd"), address("gfa_bwd_workspace_bytes"),
                  address("gfa_segments_from_positions"), address("gfa_last_error"), GfaError)
+        mod.bind_kv4(address("gfa_kv4_write"), address("gfa_kv4_read"), address("gfa_kv4_plan"), address("gfa_kv4_attn"),
+                     address("gfa_kv4_attn_workspace_bytes"))
         _native = mod
         return mod
 

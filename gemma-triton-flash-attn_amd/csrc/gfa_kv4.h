@@ -108,7 +108,8 @@ struct Kv4PlanParams {
   int *positions, *cu, *lens_out, *used_out;
 };
 
-// Query rows of a workgroup of the chunk kernel.
+// Query rows of a workgroup of the split and of the chunk kernel.
+constexpr int kSplitRows = 16;
 constexpr int kv4_chunk_rows(int D) { return D == 512 ? 128 : 256; }
 
 struct Kv4AttnParams {
@@ -123,10 +124,12 @@ struct Kv4AttnParams {
   int causal, window;
   float xs;     // multiplier of a score ahead of exp2: scale log2(e), or with soft-capping cap log2(e)
   float cap_a;  // scale / cap, 0: no soft-capping
-  int min_tiles, target;  // work split, see Kv4Split
-  int nblocks;            // workgroups of the split grid
-  int row_limit;          // requests with more query rows than this belong to the chunk kernel
-  float* part;            // (nblocks, rows, D) sums and (nblocks, rows, 2) row maxima and sums
+  int min_tiles;  // work split, see chunk_tiles in gfa_kv4_sched.h
+  float share;
+  int nblocks;    // workgroups of the split or chunk grid
+  int row_limit;  // requests with more query rows than this belong to the chunk kernel
+  int row_blocks, join_rows;  // the join grid: most row blocks, rows of one that workgroups take at a time
+  float* part;    // (nblocks, rows, D) sums and (nblocks, rows, 2) row maxima and sums
   float* part_ml;
 };
 

@@ -85,8 +85,10 @@ int rows_call(const gfa_kv4_rows_args* a, bool write) {
 // lengths the block tables can hold and the kernels divide what there is (gfa_kv4_sched.h).
 struct Part {
   bool runs;
-  int min_tiles, target;
-  int64_t nblocks;
+  int min_tiles;
+  float share;
+  int64_t nblocks, row_blocks;
+  int join_rows;
   bool join;  // some row block may take more than one chunk
   size_t part_bytes, ml_bytes;
   size_t bytes() const { return part_bytes + ml_bytes; }
@@ -96,10 +98,10 @@ struct Split {
   Part few, many;
 };
 
-constexpr int kRows = 16;  // of a workgroup of the split kernel
+constexpr int kRows = gfa::kSplitRows;
 constexpr int kRowLimit = 32;
 
-void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int min_tiles, int target, int spare) {
+void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
   if (a->causal && a->window > 0)
     tiles = std::min<int64_t>(tiles, ((int64_t)a->window + (int64_t)a->batch * a->seq_len + 31) / 32 + 1);
@@ -107,9 +109,11 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   s.runs = row_blocks > 0;
   s.join = chunks > 1;
   s.min_tiles = s.join ? min_tiles : 0x3fffffff;
-  s.target = target;
+  s.row_blocks = row_blocks;
+  s.join_rows = (int)std::min<int64_t>(rows, most_rows);
   // items: one per row block, and as many more as there are full chunks
   const int64_t hkv = a->cache.heads_kv;
+  s.share = (float)((double)hkv / target * (1.0 + 1.0 / 4096));  // see chunk_tiles
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
   s.nblocks = items * hkv + spare;
   if (s.join) {
@@ -139,8 +143,8 @@ Split split_of(const gfa_kv4_attn_args* a) {
     }
   }
   // with cu, workgroups to spare: rows behind the last request's
-  size_part(s.few, a, few, kRows, 8, 512, a->cu ? 64 : 0);
-  size_part(s.many, a, many, big, 32, 512, 0);
+  size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
+  size_part(s.many, a, many, big, most * G, 32, 512, 0);
   return s;
 }
 
@@ -150,6 +154,7 @@ int check_attn(const gfa_kv4_attn_args* a) {
   if (a->batch < 1 || a->seq_len < 1 || a->requests < 1 || a->table_width < 1)
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "batch=%d, seq_len=%d, requests=%d and table_width=%d must be positive", a->batch,
                     a->seq_len, a->requests, a->table_width);
+  if (a->requests > 65536) return api_fail(GFA_ERR_UNSUPPORTED, "%d requests (most 65536)", a->requests);
   if (a->heads_q < 1 || a->heads_q % a->cache.heads_kv != 0)
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "heads_q=%d must be a multiple of heads_kv=%d", a->heads_q, a->cache.heads_kv);
   const int64_t T = (int64_t)a->batch * a->seq_len;
@@ -224,7 +229,8 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "table, lens and cu must be 4-byte aligned pointers");
   const Split s = split_of(a);
   for (const Part* part : {&s.few, &s.many})
-    if (part->nblocks > 0x7fffffff) return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)part->nblocks);
+    if (part->nblocks > 0x7fffffff || part->row_blocks * part->join_rows * a->cache.heads_kv > 0x7fffffff)
+      return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)part->nblocks);
   const size_t need = s.few.bytes() + s.many.bytes();
   if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
     return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, a->workspace_bytes);
@@ -249,7 +255,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   p.Hq = a->heads_q;
   p.G = a->heads_q / a->cache.heads_kv;
   p.causal = a->causal != 0;
-  p.window = a->causal ? a->window : 0;
+  p.window = a->causal && a->window <= 0x40000000 ? a->window : 0;  // no table holds 2^30 tokens
   const bool cap = a->softcap > 0.f;
   p.xs = (cap ? a->softcap : a->scale) * 1.4426950408889634f;
   p.cap_a = cap ? a->scale / a->softcap : 0.f;
@@ -262,7 +268,9 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     const Part& part = large ? s.many : s.few;
     if (!part.runs) continue;
     p.min_tiles = part.min_tiles;
-    p.target = part.target;
+    p.share = part.share;
+    p.row_blocks = (int)part.row_blocks;
+    p.join_rows = part.join_rows;
     p.nblocks = (int)part.nblocks;
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);

@@ -5,8 +5,8 @@
 // ROWS = 16 of them are a row block. Work item: (request, row block, chunk of the request's key tiles); a
 // workgroup takes one item of one KV head, its waves take the chunk's 32-token tiles in turn.
 //  * S^T = K Q^T (v_mfma_f32_16x16x32): A = 16 tokens of K decoded in registers from the 16 bytes a lane
-//    loads, B = the wave's resident Q rows. Rows sit on lanes, so softmax statistics are per-lane
-//    values, and a lane's scores are in the B layout of O^T += V^T P^T for the token order
+//    loads (one tile ahead), B = the wave's resident Q rows. Rows sit on lanes, so softmax statistics are
+//    per-lane values, and a lane's scores are in the B layout of O^T += V^T P^T for the token order
 //    4 g + r, 16 + 4 g + r, in which V is stored. No LDS and no barrier until the end.
 //  * Every wave keeps its own running maximum m, row sum l and O^T; they are joined once through LDS,
 //    and the chunks' results by the join kernel below from fp32 partial sums, in a fixed order.
@@ -36,37 +36,45 @@ __device__ __forceinline__ float quad_sum(float x) {
   return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-constexpr int kRows = 16;
+constexpr int kRows = kSplitRows;
 constexpr int kWaves = 4;
+
+// What a lane holds of a 32-token tile.
+template <int D>
+struct TileRegs {
+  static constexpr int NJ = D == 64 ? 1 : D / 128;
+  uint4 k[D == 64 ? 1 : 2 * NJ], v[D == 64 ? 1 : 2 * NJ];  // D = 64: k holds both halves' 8 bytes
+  unsigned ks[2];
+  uint2 vs;
+  bool held;
+};
 
 }  // namespace
 
 template <int D, bool IS_BF16, bool CAP>
-__global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4AttnParams p) {
+__global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kernel(const Kv4AttnParams p) {
   using L = Kv4Layout<D>;
   constexpr int KT = D / 32;   // products of a score block
   constexpr int XB = D / 16;   // 16-row blocks of O^T, one per channel of an operand row
-  constexpr int NJ = D == 64 ? 1 : D / 128;
-  __shared__ __attribute__((aligned(16))) float o_lds[2][kRows * D];
+  constexpr int NJ = TileRegs<D>::NJ;
+  __shared__ __attribute__((aligned(16))) f32x4 o_lds[kWaves][XB * 64];
   __shared__ float ml_lds[kWaves][kRows][2];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
   const int head = (int)blockIdx.x % p.cache.Hkv;
-  const int64_t item = (int)blockIdx.x / p.cache.Hkv;
 
-  const Item it = find_item<kRows, false>(p, item, lane);
+  const Item it = find_item<kRows, false>(p, (int)blockIdx.x / p.cache.Hkv, lane);
   const Request& rq = it.rq;
-  const int b = it.b, rb = it.rb, ch = it.ch, nch = it.nch, per = it.per;
-  const int64_t items = it.items;
-  if (b < 0) {
+  if (it.b < 0) {
     // No item: tokens behind the last request's are zeros, the workgroups without an item take them in turn.
     if (p.cu == nullptr) return;
-    const int64_t n0 = max(p.cu[p.B], 0);
-    const int64_t extra = (int)blockIdx.x - items * p.cache.Hkv, n_extra = p.nblocks - items * p.cache.Hkv;
-    const int64_t chunks = (p.T - n0) * p.Hq * (D / 8);
-    for (int64_t i = extra * blockDim.x + threadIdx.x; i < chunks; i += n_extra * blockDim.x) {
+    const int n0 = max(p.cu[p.B], 0);
+    const int64_t taken = (int64_t)it.items * p.cache.Hkv;
+    const int64_t extra = (int)blockIdx.x - taken, n_extra = p.nblocks - taken;
+    const int64_t pieces = (int64_t)(p.T - n0) * p.Hq * (D / 8);
+    for (int64_t i = extra * blockDim.x + threadIdx.x; i < pieces; i += n_extra * blockDim.x) {
       const int64_t hd = i / (D / 8);
       const int t = (int)(n0 + hd / p.Hq);
       uint16_t* at = p.o + (t / p.N) * p.osb + hd % p.Hq * p.osh + (t % p.N) * p.osn + i % (D / 8) * 8;
@@ -75,28 +83,36 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
     return;
   }
 
-  // ---- this lane's row: token, head, visible keys [lo, hi] ----
-  const int row = rb * kRows + c16;
+  // ---- the chunk's tiles; their blocks, 64 at a time in the lanes ----
+  const int t_first = rq.first + it.ch * it.per;
+  const int t_end = min(rq.first + rq.tiles, t_first + it.per);
+  const int tpb_log2 = p.cache.bs_log2 - 5;
+  const int* table = p.table + (int64_t)it.b * p.table_stride;
+  int ids_at = t_first >> tpb_log2;
+  int ids = table[min(ids_at + lane, p.M - 1)];
+
+  // ---- this lane's row: token, head, visible keys ----
+  const int row = it.rb * kRows + c16;
   const int i = row / p.G;
   const int qh = head * p.G + row % p.G;
   const int t = rq.t0 + i;
   const bool live = i < rq.fresh && t >= 0 && t < p.T;
   const int pos = rq.len - rq.fresh + i;
-  const int hi = live ? min(p.causal ? pos : rq.len - 1, (int)min(((int64_t)p.M << p.cache.bs_log2) - 1, (int64_t)0x7fffffff)) : -1;
-  const int lo = p.causal && p.window > 0 ? max(pos - p.window + 1, 0) : 0;
+  const int hi = live ? min(p.causal ? pos : rq.len - 1, (p.M << p.cache.bs_log2) - 1) : -1;
+  const int lo = p.window > 0 ? max(pos - p.window + 1, 0) : 0;
   const VisRange vis = make_range(lo, hi);
 
   i16x8 qf[KT];
   {
-    const int tc = live ? t : 0;
+    const int tc = live ? t : 0;  // rows past the last read another's query; nothing of theirs goes out
     const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)qh * p.qsh + (tc % p.N) * p.qsn;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
 #pragma unroll
       for (int k = 0; k < KT / NJ; ++k) {
-        // k-step (j, k): lane group g holds channels 128 j + 32 g + 8 k .. (D = 64: 16 g + 8 k ..)
+        // product (j, k): lane group g holds channels 128 j + 32 g + 8 k .. (D = 64: 16 g + 8 k ..)
         const int d = D == 64 ? 16 * g + 8 * k : 128 * j + 32 * g + 8 * k;
-        qf[j * (KT / NJ) + k] = live ? *reinterpret_cast<const i16x8*>(qp + d) : i16x8{};
+        qf[j * (KT / NJ) + k] = *reinterpret_cast<const i16x8*>(qp + d);
       }
     }
   }
@@ -106,76 +122,97 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
   for (int x = 0; x < XB; ++x) acc[x] = f32x4{};
   float m_run = -INFINITY, l_run = 0.f;
   bool seen = false;  // the row sees a token of a tile this wave took
-
-  const int t_first = rq.first + ch * per;
-  const int t_end = min(rq.first + rq.tiles, t_first + per);
-  const int tpb_log2 = p.cache.bs_log2 - 5;  // tiles per block
-  const int* table = p.table + (int64_t)b * p.table_stride;
   const unsigned nan2 = IS_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
 
-  for (int tile = t_first + wave; tile < t_end; tile += kWaves) {
-    const int block = __builtin_amdgcn_readfirstlane(table[tile >> tpb_log2]);
-    if ((unsigned)block >= (unsigned)p.cache.num_blocks) continue;  // no block: nothing there to see
-    const int sub = tile & ((1 << tpb_log2) - 1);
+  auto load = [&](int tile, TileRegs<D>& r) __attribute__((always_inline)) {
+    const int tl = min(tile, t_end - 1);
+    const int col = tl >> tpb_log2;
+    if (col - ids_at >= 64) {
+      ids_at = col;
+      ids = table[min(col + lane, p.M - 1)];
+    }
+    int block = __builtin_amdgcn_readlane(ids, col - ids_at);
+    r.held = (unsigned)block < (unsigned)p.cache.num_blocks && tile < t_end;
+    block = r.held ? block : 0;
+    const int sub = tl & ((1 << tpb_log2) - 1);
     const uint8_t* kc = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 0) + sub * L::TILE_CODES;
     const uint8_t* vc = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 1) + sub * L::TILE_CODES;
     const uint8_t* ks = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 0) + sub * L::TILE_SCALES;
     const uint8_t* vs = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 1) + sub * L::TILE_SCALES;
+#pragma unroll
+    for (int hh = 0; hh < 2; ++hh) {
+      const int tok = hh * 16 + c16;
+      if constexpr (D == 64) {
+        const uint2 w = *reinterpret_cast<const uint2*>(kc + tok * 32 + g * 8);
+        if (hh == 0) {
+          r.k[0].x = w.x;
+          r.k[0].y = w.y;
+        } else {
+          r.k[0].z = w.x;
+          r.k[0].w = w.y;
+        }
+        r.ks[hh] = ks[tok * 2 + (g >> 1)];
+      } else {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) r.k[hh * NJ + j] = *reinterpret_cast<const uint4*>(kc + j * 2048 + tok * 64 + g * 16);
+        const uint8_t* sp = ks + tok * L::SC + g * NJ;
+        if constexpr (NJ == 4) {
+          r.ks[hh] = *reinterpret_cast<const unsigned*>(sp);
+        } else if constexpr (NJ == 2) {
+          r.ks[hh] = *reinterpret_cast<const uint16_t*>(sp);
+        } else {
+          r.ks[hh] = *sp;
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < (D == 64 ? 1 : 2 * NJ); ++j) r.v[j] = *reinterpret_cast<const uint4*>(vc + j * 1024 + lane * 16);
+    r.vs = *reinterpret_cast<const uint2*>(vs + (g * L::SC + c16 * L::PP / 32) * 8);
+  };
 
+  auto compute = [&](int tile, const TileRegs<D>& r) __attribute__((always_inline)) {
     // ---- S^T, 16 tokens at a time ----
     f32x4 s[2];
 #pragma unroll
     for (int hh = 0; hh < 2; ++hh) {
       s[hh] = f32x4{};
-      const int tok = hh * 16 + c16;
-      if constexpr (D == 64) {
-        const uint2 w = *reinterpret_cast<const uint2*>(kc + tok * 32 + g * 8);
-        const unsigned sb = ks[tok * 2 + (g >> 1)];
-        const float sc = __uint_as_float(sb << 23);
-        const unsigned cw[2] = {w.x, w.y};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
+      for (int j = 0; j < NJ; ++j) {
+        unsigned bits, cw[4];
+        if constexpr (D == 64) {
+          bits = r.ks[hh] << 23;
+          cw[0] = hh == 0 ? r.k[0].x : r.k[0].z;
+          cw[1] = hh == 0 ? r.k[0].y : r.k[0].w;
+        } else {
+          const unsigned sb = r.ks[hh];
+          bits = j == 0 ? kv4_scale_bits<0>(sb) : j == 1 ? kv4_scale_bits<1>(sb) : j == 2 ? kv4_scale_bits<2>(sb) : kv4_scale_bits<3>(sb);
+          const uint4 w = r.k[hh * NJ + j];
+          cw[0] = w.x;
+          cw[1] = w.y;
+          cw[2] = w.z;
+          cw[3] = w.w;
+        }
+        const float sc = __uint_as_float(bits);
+#pragma unroll
+        for (int k = 0; k < KT / NJ; ++k) {
           unsigned a[4] = {kv4_pair<IS_BF16, 0>(cw[k], sc), kv4_pair<IS_BF16, 1>(cw[k], sc),
                            kv4_pair<IS_BF16, 2>(cw[k], sc), kv4_pair<IS_BF16, 3>(cw[k], sc)};
-          if (k == 0) a[0] = sb == kKv4Nan ? nan2 : a[0];
-          s[hh] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, a), qf[k], s[hh]);
-        }
-      } else {
-        unsigned sb;  // NJ scale bytes
-        const uint8_t* sp = ks + tok * L::SC + g * NJ;
-        if constexpr (NJ == 4) {
-          sb = *reinterpret_cast<const unsigned*>(sp);
-        } else if constexpr (NJ == 2) {
-          sb = *reinterpret_cast<const uint16_t*>(sp);
-        } else {
-          sb = *sp;
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const uint4 w = *reinterpret_cast<const uint4*>(kc + j * 2048 + tok * 64 + g * 16);
-          const unsigned bits = j == 0 ? kv4_scale_bits<0>(sb) : j == 1 ? kv4_scale_bits<1>(sb) : j == 2 ? kv4_scale_bits<2>(sb) : kv4_scale_bits<3>(sb);
-          const float sc = __uint_as_float(bits);
-          const unsigned cw[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            unsigned a[4] = {kv4_pair<IS_BF16, 0>(cw[k], sc), kv4_pair<IS_BF16, 1>(cw[k], sc),
-                             kv4_pair<IS_BF16, 2>(cw[k], sc), kv4_pair<IS_BF16, 3>(cw[k], sc)};
-            if (k == 0) a[0] = bits == 0x7f800000u ? nan2 : a[0];
-            s[hh] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, a), qf[4 * j + k], s[hh]);
-          }
+          if (k == 0) a[0] = bits == 0x7f800000u ? nan2 : a[0];
+          s[hh] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, a), qf[j * (KT / NJ) + k], s[hh]);
         }
       }
     }
 
-    seen = seen || (lo < (tile + 1) * kTile && hi >= tile * kTile);
-
     // ---- softmax: this lane's row, tokens 4 g + r and 16 + 4 g + r ----
+    // a tile without a block: nothing there to see
+    const VisRange see = r.held ? vis : make_range(0, -1);
+    seen = seen || (r.held && lo < (tile + 1) * kTile && hi >= tile * kTile);
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       float v = s[e >> 2][e & 3];
       if constexpr (CAP) v = cap_tanh(v * p.cap_a);
-      x[e] = vis.has(tile * kTile + (e >> 2) * 16 + 4 * g + (e & 3)) ? v * p.xs : -INFINITY;
+      x[e] = see.has(tile * kTile + (e >> 2) * 16 + 4 * g + (e & 3)) ? v * p.xs : -INFINITY;
     }
     float mt = x[0];
 #pragma unroll
@@ -198,11 +235,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
     }
 
     // ---- O^T += V^T P^T ----
-    const uint2 vsb = *reinterpret_cast<const uint2*>(vs + (g * L::SC + c16 * L::PP / 32) * 8);
     float sc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const unsigned w = e < 4 ? vsb.x : vsb.y;
+      const unsigned w = e < 4 ? r.vs.x : r.vs.y;
       const unsigned bits = (e & 3) == 0 ? kv4_scale_bits<0>(w) : (e & 3) == 1 ? kv4_scale_bits<1>(w) : (e & 3) == 2 ? kv4_scale_bits<2>(w) : kv4_scale_bits<3>(w);
       // finite whatever the byte: P is 0 where a row does not see the token, and 0 times that stays 0
       sc[e] = __uint_as_float(min(bits, (unsigned)Kv4Range<IS_BF16>::hi << 23));
@@ -221,15 +257,14 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
       acc[x0 + 1] = mma16<IS_BF16>(__builtin_bit_cast(i16x8, odd), pb, acc[x0 + 1]);
     };
     if constexpr (D == 64) {
-      const uint4 w = *reinterpret_cast<const uint4*>(vc + lane * 16);
+      const uint4 w = r.v[0];
       const unsigned cw[8] = {w.x, w.x >> 16, w.y, w.y >> 16, w.z, w.z >> 16, w.w, w.w >> 16};
       products(std::integral_constant<int, 0>{}, 0, cw);
       products(std::integral_constant<int, 1>{}, 2, cw);
     } else {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
-        const uint4 a = *reinterpret_cast<const uint4*>(vc + j * 2048 + lane * 16);
-        const uint4 c = *reinterpret_cast<const uint4*>(vc + j * 2048 + 1024 + lane * 16);
+        const uint4 a = r.v[2 * j], c = r.v[2 * j + 1];
         const unsigned cw[8] = {a.x, a.y, a.z, a.w, c.x, c.y, c.z, c.w};
         products(std::integral_constant<int, 0>{}, 8 * j, cw);
         products(std::integral_constant<int, 1>{}, 8 * j + 2, cw);
@@ -237,9 +272,22 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
         products(std::integral_constant<int, 3>{}, 8 * j + 6, cw);
       }
     }
+  };
+
+  // The wave's tiles, one loaded ahead.
+  if (t_first + wave < t_end) {
+    TileRegs<D> r0, r1;
+    load(t_first + wave, r0);
+    for (int tile = t_first + wave; tile < t_end; tile += 2 * kWaves) {
+      load(tile + kWaves, r1);
+      compute(tile, r0);
+      if (tile + kWaves >= t_end) break;
+      load(tile + 2 * kWaves, r0);
+      compute(tile + kWaves, r1);
+    }
   }
 
-  // ---- join the waves ----
+  // ---- join the waves: each leaves its sums, each takes a quarter of the channels ----
   // A row without weight (m = -inf) keeps in l whether it saw a key: none is a zero row, keys whose scores
   // are all -inf are 0 / 0 as in the formula. Against a finite maximum either weighs nothing.
   float l_row = quad_sum(l_run);
@@ -248,71 +296,61 @@ __global__ __launch_bounds__(kWaves * 64, 1) void kv4_split_kernel(const Kv4Attn
     ml_lds[wave][c16][0] = m_run;
     ml_lds[wave][c16][1] = l_row;
   }
-  __syncthreads();
-  float m_all = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) m_all = fmaxf(m_all, ml_lds[w][c16][0]);
+  for (int x = 0; x < XB; ++x) o_lds[wave][x * 64 + lane] = acc[x];
+  __syncthreads();
+  float m_all = -INFINITY, m_w[kWaves];
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    m_w[w] = ml_lds[w][c16][0];
+    m_all = fmaxf(m_all, m_w[w]);
+  }
   const float m_use = m_all == -INFINITY ? 0.f : m_all;
   float l_all = 0.f;
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w)
-    l_all += ml_lds[w][c16][1] * (m_all == -INFINITY ? 1.f : fast_exp2(ml_lds[w][c16][0] - m_use));
-  const float mine = fast_exp2(m_run - m_use);
-#pragma unroll
-  for (int x = 0; x < XB; ++x) acc[x] *= mine;
-  // Rows of O^T: lane (g, row) holds channels (4 g + r) PP + x.
-  auto at = [&](int r, int x) { return (x * 4 + r) * 64 + lane; };
-#pragma unroll
-  for (int step = 2; step >= 1; step >>= 1) {
-    if (wave >= step && wave < 2 * step) {
-#pragma unroll
-      for (int x = 0; x < XB; ++x) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o_lds[wave - step][at(r, x)] = acc[x][r];
-      }
-    }
-    __syncthreads();
-    if (wave < step) {
-#pragma unroll
-      for (int x = 0; x < XB; ++x) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[x][r] += o_lds[wave][at(r, x)];
-      }
-    }
-    __syncthreads();
+  for (int w = 0; w < kWaves; ++w) {
+    m_w[w] = fast_exp2(m_w[w] - m_use);
+    l_all += ml_lds[w][c16][1] * (m_all == -INFINITY ? 1.f : m_w[w]);
   }
-  if (wave != 0) return;
+  constexpr int XW = XB / kWaves;  // this wave's: channels (4 g + r) PP + wave XW ..
+  f32x4 o[XW];
+#pragma unroll
+  for (int x = 0; x < XW; ++x) {
+    o[x] = f32x4{};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) o[x] += o_lds[w][(wave * XW + x) * 64 + lane] * m_w[w];
+  }
 
-  if (nch > 1) {
-    float* part = p.part + ((int64_t)blockIdx.x * kRows + c16) * D;
+  const int d0 = 4 * g * L::PP + wave * XW;
+  if (it.nch > 1) {
+    const int64_t at = (int64_t)blockIdx.x * kRows + c16;
     if (live) {
+      typedef float vec __attribute__((ext_vector_type(XW)));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        vec v;
 #pragma unroll
-        for (int x = 0; x < XB; x += 4)
-          *reinterpret_cast<f32x4*>(part + (4 * g + r) * L::PP + x) = f32x4{acc[x][r], acc[x + 1][r], acc[x + 2][r], acc[x + 3][r]};
+        for (int x = 0; x < XW; ++x) v[x] = o[x][r];
+        *reinterpret_cast<vec*>(p.part + at * D + d0 + r * L::PP) = v;
       }
     }
-    if (g == 0) {
-      float* ml = p.part_ml + ((int64_t)blockIdx.x * kRows + c16) * 2;
-      ml[0] = m_all;
-      ml[1] = l_all;
+    if (wave == 0 && g == 0) {
+      p.part_ml[at * 2] = m_all;
+      p.part_ml[at * 2 + 1] = l_all;
     }
     return;
   }
   if (!live) return;
   const bool none = m_all == -INFINITY && l_all == 0.f;
   const float inv = row_inv(m_all, l_all);
-  uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn;
+  uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn + d0;
+  typedef short vec __attribute__((ext_vector_type(XW)));
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
+    vec v;
 #pragma unroll
-    for (int x = 0; x < XB; x += 4) {
-      i16x4 v;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = to16<IS_BF16>(none ? 0.f : acc[x + e][r] * inv);
-      *reinterpret_cast<i16x4*>(op + (4 * g + r) * L::PP + x) = v;
-    }
+    for (int x = 0; x < XW; ++x) v[x] = to16<IS_BF16>(none ? 0.f : o[x][r] * inv);
+    *reinterpret_cast<vec*>(op + r * L::PP) = v;
   }
 }
 

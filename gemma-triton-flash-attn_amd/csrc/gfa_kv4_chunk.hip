@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
   const int row0 = rb * ROWS;
 
   // ---- key tiles of this row block's chunk ----
-  const int held = (int)min((int64_t)rq.len, (int64_t)p.M << p.cache.bs_log2);
+  const int held = min(rq.len, p.M << p.cache.bs_log2);
   const int i_lo = row0 / p.G, i_hi = min((row0 + ROWS - 1) / p.G, rq.fresh - 1);
   const int pos0 = rq.len - rq.fresh;  // position of new token 0
   int k_lo = 0, k_hi = held;

@@ -5,6 +5,8 @@
 // An item is a row block of ROWS of them and a chunk of the key tiles they see. Requests of up to
 // row_limit rows are the split kernel's, the others the chunk kernel's (LARGE).
 #pragma once
+#include <type_traits>
+
 #include "gfa_kv4.h"
 
 namespace gfa {
@@ -23,80 +25,131 @@ __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   if (b >= p.B) return r;
   if (p.cu != nullptr) {
     r.t0 = p.cu[b];
-    r.fresh = max(p.cu[b + 1] - r.t0, 0);
+    r.fresh = min(max((int)((unsigned)p.cu[b + 1] - (unsigned)r.t0), 0), p.T);
   } else {
     r.fresh = p.T / p.B;
     r.t0 = b * r.fresh;
   }
   r.len = max(p.lens[b], 0);
-  const int64_t rows = (int64_t)r.fresh * p.G;
-  r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)((rows + ROWS - 1) / ROWS);
-  const int held = (int)min((int64_t)r.len, (int64_t)p.M << p.cache.bs_log2);
-  const int lo = p.causal && p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : 0;
+  const int rows = r.fresh * p.G;
+  r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
+  const int held = min(r.len, p.M << p.cache.bs_log2);
+  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : 0;
   r.first = lo / kTile;
   r.tiles = held > lo ? (held + kTile - 1) / kTile - r.first : 0;
   return r;
 }
-
-__device__ __forceinline__ int64_t wave_sum64(int64_t x) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) x += __shfl_xor(x, m);
-  return x;
-}
-__device__ __forceinline__ int64_t wave_prefix64(int64_t x, int lane) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const int64_t y = __shfl_up(x, m);
-    if (lane >= m) x += y;
-  }
-  return x;
+// Lane src's request in every lane.
+__device__ __forceinline__ Request request_from(const Request& r, int src) {
+  auto at = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
+  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.first), at(r.tiles)};
 }
 
-// Key tiles per chunk: the whole grid's tiles spread over about `target` workgroups, at least min_tiles each.
+// Sum over the wave's lanes (the steps of wave_prefix_sum).
+__device__ __forceinline__ float wave_sum(float x) {
+  auto step = [&](auto ctrl, auto rows, auto bound) __attribute__((always_inline)) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, decltype(rows)::value, 0xf, decltype(bound)::value));
+  };
+  constexpr std::integral_constant<int, 0xf> all{};
+  constexpr std::true_type zero{};
+  constexpr std::false_type keep{};
+  step(std::integral_constant<int, 0x111>{}, all, zero);
+  step(std::integral_constant<int, 0x112>{}, all, zero);
+  step(std::integral_constant<int, 0x114>{}, all, zero);
+  step(std::integral_constant<int, 0x118>{}, all, zero);
+  step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}, keep);
+  step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}, keep);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+// Key tiles per chunk: the whole call's tiles spread over about `target` workgroups, at least min_tiles each. The
+// sum is a float's (a product of two counts can pass 32 bits); `share` = Hkv / target is rounded up by more than the
+// sum can be off, so that the grid the host sized holds every item. The same operations in the same order wherever
+// it is taken: contraction is off.
 template <int ROWS, bool LARGE>
-__device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, int lane) {
-  int64_t total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
+__device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, const Request& r0, int lane) {
+#pragma clang fp contract(off)
+  float total = (float)r0.row_blocks * (float)r0.tiles;
+  for (int b0 = 64; b0 < p.B; b0 += 64) {
     const Request r = request_of<ROWS, LARGE>(p, b0 + lane);
-    total += (int64_t)r.row_blocks * r.tiles;
+    const float x = (float)r.row_blocks * (float)r.tiles;
+    total += x;
   }
-  total = wave_sum64(total) * p.cache.Hkv;
-  const int64_t each = (total + p.target - 1) / p.target;
-  return (int)min(max(each, (int64_t)p.min_tiles), (int64_t)0x3fffffff);
+  const float each = ceilf(wave_sum(total) * p.share);
+  return max((int)fminf(each, 1.0e9f), p.min_tiles);
 }
 __device__ __forceinline__ int chunks_of(const Request& r, int per) { return max((r.tiles + per - 1) / per, 1); }
 
 struct Item {
   Request rq;
-  int b;             // -1: there is no such item
-  int rb, ch, nch;   // row block, chunk of nch
-  int per;           // tiles a chunk
-  int64_t items;     // of the whole call, where b < 0
+  int b;            // -1: there is no such item
+  int rb, ch, nch;  // row block, chunk of nch
+  int per;          // tiles a chunk
+  int items;        // of the whole call, where b < 0
 };
 template <int ROWS, bool LARGE>
-__device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int64_t item, int lane) {
+__device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int lane) {
   Item it{};
   it.b = -1;
-  it.per = chunk_tiles<ROWS, LARGE>(p, lane);
-  for (int b0 = 0; b0 < p.B; b0 += 64) {
-    const Request r = request_of<ROWS, LARGE>(p, b0 + lane);
-    const int64_t mine = (int64_t)r.row_blocks * chunks_of(r, it.per);
-    const int64_t s = wave_prefix64(mine, lane);
-    const int64_t before = it.items + s - mine;
+  Request r = request_of<ROWS, LARGE>(p, lane);
+  it.per = chunk_tiles<ROWS, LARGE>(p, r, lane);
+  for (int b0 = 0;;) {
+    const int mine = r.row_blocks * chunks_of(r, it.per);
+    const int s = wave_prefix_sum(mine);
+    const int before = it.items + s - mine;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
-      it.b = __builtin_amdgcn_readfirstlane(b0 + src);
-      it.rq = request_of<ROWS, LARGE>(p, it.b);
+      it.b = b0 + src;
+      it.rq = request_from(r, src);
       it.nch = chunks_of(it.rq, it.per);
-      const int i = (int)(item - __shfl(before, src));
-      it.rb = __builtin_amdgcn_readfirstlane(i / it.nch);
-      it.ch = __builtin_amdgcn_readfirstlane(i % it.nch);
+      const int i = item - __builtin_amdgcn_readlane(before, src);
+      it.rb = i / it.nch;
+      it.ch = i % it.nch;
       break;
     }
-    it.items += __shfl(s, 63);
+    it.items += __builtin_amdgcn_readlane(s, 63);
+    if ((b0 += 64) >= p.B) break;
+    r = request_of<ROWS, LARGE>(p, b0 + lane);
   }
   return it;
+}
+
+// Row block `block` of the call, counted through the requests: rq, b, rb, nch, and the first chunk's item.
+struct RowBlock {
+  Request rq;
+  int b;           // -1: there is no such row block
+  int rb, nch;
+  int item;
+};
+template <int ROWS, bool LARGE>
+__device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int block, int lane) {
+  RowBlock out{};
+  out.b = -1;
+  Request r = request_of<ROWS, LARGE>(p, lane);
+  const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
+  int blocks = 0, items = 0;
+  for (int b0 = 0;;) {
+    const int s = wave_prefix_sum(r.row_blocks);
+    const int mine = r.row_blocks * chunks_of(r, per);
+    const int t = wave_prefix_sum(mine);
+    const int before = blocks + s - r.row_blocks;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(block >= before && block < before + r.row_blocks);
+    if (hit != 0) {
+      const int src = __builtin_ctzll(hit);
+      out.b = b0 + src;
+      out.rq = request_from(r, src);
+      out.nch = chunks_of(out.rq, per);
+      out.rb = block - __builtin_amdgcn_readlane(before, src);
+      out.item = items + __builtin_amdgcn_readlane(t - mine, src) + out.rb * out.nch;
+      break;
+    }
+    blocks += __builtin_amdgcn_readlane(s, 63);
+    items += __builtin_amdgcn_readlane(t, 63);
+    if ((b0 += 64) >= p.B) break;
+    r = request_of<ROWS, LARGE>(p, b0 + lane);
+  }
+  return out;
 }
 
 // 1 / l of a finished row. Without weight l is a mark, not a sum: the row is 0 / 0 where it saw keys.

@@ -21,6 +21,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <optional>
 
 #include "gfa.h"
@@ -36,6 +37,11 @@ struct Api {
   decltype(&gfa_bwd) bwd = nullptr;
   decltype(&gfa_bwd_workspace_bytes) workspace_bytes = nullptr;
   decltype(&gfa_segments_from_positions) positions = nullptr;
+  decltype(&gfa_kv4_write) kv4_write = nullptr;
+  decltype(&gfa_kv4_read) kv4_read = nullptr;
+  decltype(&gfa_kv4_plan) kv4_plan = nullptr;
+  decltype(&gfa_kv4_attn) kv4_attn = nullptr;
+  decltype(&gfa_kv4_attn_workspace_bytes) kv4_attn_workspace_bytes = nullptr;
   decltype(&gfa_last_error) last_error = nullptr;
   PyObject* error_type = nullptr;  // GfaError(status, message); held for the process
 } api;
@@ -267,6 +273,218 @@ struct Attention : public torch::autograd::Function<Attention> {
   }
 };
 
+// ---- The key/value cache in 4 bits (kv4.py): argument checks, outputs, launches ----
+
+bool on_gpu(const Tensor& t, const c10::Device& device) { return t.is_cuda() && t.device() == device; }
+// A caller's array of one type on the call's GPU.
+void check_array(const char* name, const Tensor& t, at::ScalarType type, int64_t dim, const c10::Device& device) {
+  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " must be ", type, ", got ", t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == dim, name, " must be ", dim, "-D, got shape ", t.sizes());
+  TORCH_CHECK_VALUE(on_gpu(t, device), name, " must be on the call's GPU (", device, "; the engine has no CPU path), is on ",
+                    t.device());
+}
+Tensor dense(const Tensor& t) { return (t.is_neg() ? t.resolve_neg() : t).contiguous(); }
+
+bool block_size_ok(int64_t n) { return n >= 32 && n <= 1024 && (n & (n - 1)) == 0; }
+
+gfa_kv4_cache cache_of(const Tensor& codes, const Tensor& scales, bool bf16) {
+  gfa_kv4_cache c{};
+  c.codes = codes.data_ptr();
+  c.scales = scales.data_ptr();
+  c.num_blocks = (int32_t)codes.size(0);
+  c.heads_kv = (int32_t)codes.size(1);
+  c.block_size = (int32_t)codes.size(3);
+  c.head_dim = (int32_t)(2 * codes.size(4));
+  c.dtype = bf16 ? GFA_DTYPE_BF16 : GFA_DTYPE_FP16;
+  return c;
+}
+
+void check_cache(const Tensor& codes, const Tensor& scales) {
+  TORCH_CHECK_TYPE(codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte, "codes and scales must be uint8");
+  TORCH_CHECK_VALUE(codes.dim() == 5 && scales.dim() == 5,
+                    "codes and scales must be 5-D (num_blocks, heads_kv, 2, block_size, bytes)");
+  const auto c = codes.sizes(), s = scales.sizes();
+  const int64_t d = 2 * c[4];
+  TORCH_CHECK_VALUE(d == 64 || d == 128 || d == 256 || d == 512, "HEAD_DIM=", d, " not built (64, 128, 256, 512)");
+  TORCH_CHECK_VALUE(c[2] == 2 && s[0] == c[0] && s[1] == c[1] && s[2] == 2 && s[3] == c[3] && s[4] * 16 == c[4], "codes ", c,
+                    " and scales ", s, " do not belong together");
+  TORCH_CHECK_VALUE(block_size_ok(c[3]), "block_size=", c[3], " must be a power of two, 32 to 1024");
+  TORCH_CHECK_VALUE(c[0] > 0 && c[0] <= INT32_MAX && c[1] > 0 && c[1] <= 65535, "a cache of ", c[0], " blocks and ", c[1], " heads");
+  TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous() && !codes.is_neg() && !scales.is_neg(),
+                    "codes and scales must be contiguous");
+  TORCH_CHECK_VALUE(codes.is_cuda() && on_gpu(scales, codes.device()),
+                    "codes and scales must be on one GPU (the engine has no CPU path)");
+  TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(codes.const_data_ptr()) % 16 == 0 &&
+                        reinterpret_cast<uintptr_t>(scales.const_data_ptr()) % 16 == 0,
+                    "codes and scales must be 16-byte aligned");
+}
+
+void check_token_rows(const char* name, const Tensor& t, const Tensor& codes, bool bf16, bool kv) {
+  TORCH_CHECK_VALUE(t.dim() == 4, name, " must be 4-D (B, H, N, D), got shape ", t.sizes());
+  const auto type = bf16 ? at::kBFloat16 : at::kHalf;
+  TORCH_CHECK_TYPE(t.scalar_type() == type, name, " is ", t.scalar_type(), ", the cache is for ", type);
+  TORCH_CHECK_VALUE(t.size(3) == 2 * codes.size(4) && (!kv || t.size(1) == codes.size(1)), name, " ", t.sizes(),
+                    " does not fit a cache of ", codes.size(1), " heads of dim ", 2 * codes.size(4));
+  TORCH_CHECK_VALUE(on_gpu(t, codes.device()), name, " must be on the cache's GPU (", codes.device(), "), is on ", t.device());
+  TORCH_CHECK_VALUE(t.size(0) * t.size(2) <= INT32_MAX, name, " has more than 2^31 - 1 tokens");
+}
+
+// Rows apart of an int32 (requests, width) block table.
+int64_t check_table(const Tensor& table, int64_t requests, const c10::Device& device) {
+  check_array("table", table, at::kInt, 2, device);
+  TORCH_CHECK_VALUE(table.size(0) == requests, "table has ", table.size(0), " rows for ", requests, " requests");
+  TORCH_CHECK_VALUE(requests > 0 && table.size(1) > 0 && requests < INT32_MAX && table.size(1) <= INT32_MAX,
+                    "a block table of shape ", table.sizes());
+  TORCH_CHECK_VALUE((table.stride(1) == 1 || table.size(1) == 1) && (requests == 1 || table.stride(0) >= table.size(1)) && !table.is_neg(),
+                    "table rows must be contiguous and apart from each other");
+  return requests == 1 ? table.size(1) : table.stride(0);
+}
+
+gfa_kv4_rows_args rows_args(const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& k, const Tensor& v,
+                            const Tensor& slots) {
+  gfa_kv4_rows_args a{};
+  a.cache = cache_of(codes, scales, bf16);
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.k_strides = strides_of(k);
+  a.v_strides = strides_of(v);
+  a.batch = (int32_t)k.size(0);
+  a.seq_len = (int32_t)k.size(2);
+  a.slots = static_cast<const int64_t*>(slots.data_ptr());
+  a.stream = stream_of(codes);
+  return a;
+}
+
+void kv4_write(const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& k, const Tensor& v, const Tensor& slots) {
+  check_cache(codes, scales);
+  check_token_rows("k", k, codes, bf16, true);
+  check_token_rows("v", v, codes, bf16, true);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes(), "shape mismatch: k ", k.sizes(), ", v ", v.sizes());
+  check_array("slots", slots, at::kLong, 1, codes.device());
+  TORCH_CHECK_VALUE(slots.size(0) == k.size(0) * k.size(2), "slots holds ", slots.size(0), " entries for ",
+                    k.size(0) * k.size(2), " tokens");
+  if (slots.size(0) == 0) return;
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor kp = prep(k), vp = prep(v), sp = dense(slots);
+  const auto a = rows_args(codes, scales, bf16, kp, vp, sp);
+  check(api.kv4_write(&a));
+}
+
+std::tuple<Tensor, Tensor> kv4_read(const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& slots) {
+  check_cache(codes, scales);
+  check_array("slots", slots, at::kLong, 1, codes.device());
+  TORCH_CHECK_VALUE(slots.size(0) <= INT32_MAX, "slots holds more than 2^31 - 1 entries");
+  const c10::DeviceGuard guard(codes.device());
+  const auto options = codes.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
+  const int64_t T = slots.size(0), H = codes.size(1), D = 2 * codes.size(4);
+  // (1, H, T, D) views of token-major rows
+  const Tensor k = at::empty_strided({1, H, T, D}, {T * H * D, D, H * D, 1}, options);
+  const Tensor v = at::empty_strided({1, H, T, D}, {T * H * D, D, H * D, 1}, options);
+  if (T > 0) {
+    const Tensor sp = dense(slots);
+    const auto a = rows_args(codes, scales, bf16, k, v, sp);
+    check(api.kv4_read(&a));
+  }
+  return {k, v};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv4_plan(const Tensor& lens, const Tensor& fresh, const Tensor& table,
+                                                            const Tensor& free_ids, const Tensor& used, int64_t block_size,
+                                                            int64_t tokens) {
+  const auto device = lens.device();
+  check_array("lens", lens, at::kInt, 1, device);
+  const int64_t B = lens.size(0);
+  check_array("new", fresh, at::kInt, 1, device);
+  TORCH_CHECK_VALUE(fresh.size(0) == B, "new holds ", fresh.size(0), " entries for ", B, " requests");
+  const int64_t stride = check_table(table, B, device);
+  check_array("free", free_ids, at::kInt, 1, device);
+  check_array("used", used, at::kInt, 1, device);
+  TORCH_CHECK_VALUE(used.size(0) == 1 && free_ids.size(0) <= INT32_MAX, "used must hold one entry");
+  TORCH_CHECK_VALUE(block_size_ok(block_size), "block_size=", block_size, " must be a power of two, 32 to 1024");
+  TORCH_CHECK_VALUE(tokens >= 0 && tokens <= INT32_MAX, "tokens=", tokens, " must be in [0, 2^31)");
+  const c10::DeviceGuard guard(device);
+  const Tensor l = dense(lens), n = dense(fresh), f = dense(free_ids), u = dense(used);
+  const Tensor slots = at::empty({tokens}, lens.options().dtype(at::kLong)), positions = at::empty({tokens}, lens.options());
+  const Tensor cu = at::empty({B + 1}, lens.options()), lens_out = at::empty({B}, lens.options());
+  const Tensor used_out = at::empty({1}, lens.options());
+  const auto ints = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
+  gfa_kv4_plan_args a{};
+  a.lens = ints(l);
+  a.fresh = ints(n);
+  a.table = ints(table);
+  a.table_stride = stride;
+  a.free_ids = ints(f);
+  a.used = ints(u);
+  a.requests = (int32_t)B;
+  a.table_width = (int32_t)table.size(1);
+  a.free_count = (int32_t)f.size(0);
+  a.block_size = (int32_t)block_size;
+  a.tokens = (int32_t)tokens;
+  a.slots = static_cast<int64_t*>(slots.data_ptr());
+  a.positions = ints(positions);
+  a.cu = ints(cu);
+  a.lens_out = ints(lens_out);
+  a.used_out = ints(used_out);
+  a.stream = stream_of(lens);
+  check(api.kv4_plan(&a));
+  return {slots, positions, cu, lens_out, used_out};
+}
+
+Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& table,
+                     const Tensor& lens, const std::optional<Tensor>& cu, int64_t max_new, bool causal, int64_t window,
+                     double scale, double softcap) {
+  check_cache(codes, scales);
+  check_token_rows("q", q, codes, bf16, false);
+  const int64_t B = q.size(0), Hq = q.size(1), N = q.size(2), Hkv = codes.size(1);
+  TORCH_CHECK_VALUE(Hq > 0 && Hq % Hkv == 0, "N_Q_HEADS=", Hq, " must be a multiple of N_KV_HEADS=", Hkv);
+  TORCH_CHECK_VALUE(B > 0 && N > 0, "empty sequence or batch");
+  const auto device = codes.device();
+  check_array("lens", lens, at::kInt, 1, device);
+  const int64_t R = lens.size(0);
+  const int64_t stride = check_table(table, R, device);
+  if (cu) {
+    check_array("cu", *cu, at::kInt, 1, device);
+    TORCH_CHECK_VALUE(cu->size(0) == R + 1, "cu holds ", cu->size(0), " entries for ", R, " requests");
+  } else {
+    TORCH_CHECK_VALUE(B * N % R == 0, B * N, " tokens do not divide among ", R, " requests (pass cu)");
+  }
+  TORCH_CHECK_VALUE(window >= 0, "slide_size must be >= 0");
+  TORCH_CHECK_VALUE(max_new >= 0, "max_new must be at least 1");
+  const c10::DeviceGuard guard(device);
+  const Tensor qp = prep(q), lp = dense(lens), cp = cu ? dense(*cu) : Tensor();
+  const Tensor o = out_like(qp);
+  gfa_kv4_attn_args a{};
+  a.cache = cache_of(codes, scales, bf16);
+  a.q = qp.data_ptr();
+  a.o = o.data_ptr();
+  a.q_strides = strides_of(qp);
+  a.o_strides = strides_of(o);
+  a.batch = (int32_t)B;
+  a.heads_q = (int32_t)Hq;
+  a.seq_len = (int32_t)N;
+  a.requests = (int32_t)R;
+  a.table = static_cast<const int32_t*>(table.data_ptr());
+  a.table_stride = stride;
+  a.lens = static_cast<const int32_t*>(lp.data_ptr());
+  a.cu = cu ? static_cast<const int32_t*>(cp.data_ptr()) : nullptr;
+  a.table_width = (int32_t)table.size(1);
+  a.causal = causal;
+  a.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+  a.max_new = (int32_t)std::min<int64_t>(max_new, INT32_MAX);
+  a.scale = (float)scale;
+  a.softcap = (float)softcap;
+  a.stream = stream_of(q);
+  Tensor ws;
+  const size_t need = api.kv4_attn_workspace_bytes(&a);
+  if (need > 0) {
+    ws = at::empty({(int64_t)need}, codes.options());
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = need;
+  }
+  check(api.kv4_attn(&a));
+  return o;
+}
+
 template <typename F>
 F pointer(uintptr_t p) {
   return reinterpret_cast<F>(p);
@@ -285,6 +503,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     api.last_error = pointer<decltype(api.last_error)>(last_error);
     api.error_type = error_type.release().ptr();
   });
+  m.def("bind_kv4", [](uintptr_t write, uintptr_t read, uintptr_t plan, uintptr_t attn, uintptr_t workspace_bytes) {
+    api.kv4_write = pointer<decltype(api.kv4_write)>(write);
+    api.kv4_read = pointer<decltype(api.kv4_read)>(read);
+    api.kv4_plan = pointer<decltype(api.kv4_plan)>(plan);
+    api.kv4_attn = pointer<decltype(api.kv4_attn)>(attn);
+    api.kv4_attn_workspace_bytes = pointer<decltype(api.kv4_attn_workspace_bytes)>(workspace_bytes);
+  });
+  m.def("kv4_cache", torch::wrap_pybind_function_no_gil(check_cache));
+  m.def("kv4_write", torch::wrap_pybind_function_no_gil(kv4_write));
+  m.def("kv4_read", torch::wrap_pybind_function_no_gil(kv4_read));
+  m.def("kv4_plan", torch::wrap_pybind_function_no_gil(kv4_plan));
+  m.def("kv4_attention", torch::wrap_pybind_function_no_gil(kv4_attention));
   // Bodies run without the interpreter lock: an allocation or a launch that waits for the driver does
   // not hold up other Python threads (a data loader's, another stream's).
   const auto or_undefined = [](const std::optional<Tensor>& t) { return t ? *t : Tensor(); };
