@@ -128,7 +128,7 @@ struct Kv4AttnParams {
   float share;
   int nblocks;    // workgroups of the split or chunk grid
   int row_limit;  // requests with more query rows than this belong to the chunk kernel
-  int row_blocks, join_rows;  // the join grid: most row blocks, rows of one that workgroups take at a time
+  int row_blocks, join_rows, join_slice;  // the join grid: most row blocks, workgroups for the rows of one, channels of each
   float* part;    // (nblocks, rows, D) sums and (nblocks, rows, 2) row maxima and sums
   float* part_ml;
 };

@@ -88,7 +88,7 @@ struct Part {
   int min_tiles;
   float share;
   int64_t nblocks, row_blocks;
-  int join_rows;
+  int join_rows, join_slice;
   bool join;  // some row block may take more than one chunk
   size_t part_bytes, ml_bytes;
   size_t bytes() const { return part_bytes + ml_bytes; }
@@ -105,12 +105,18 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
   if (a->causal && a->window > 0)
     tiles = std::min<int64_t>(tiles, ((int64_t)a->window + (int64_t)a->batch * a->seq_len + 31) / 32 + 1);
-  const int64_t chunks = std::max<int64_t>(1, (tiles + min_tiles - 1) / min_tiles);
+  // Requests of 512 tokens or less are one chunk: one token of 333 at D = 256 takes 8.5 us, 10.9-11.6 us with a join.
+  const int64_t chunks = tiles <= 16 ? 1 : (tiles + min_tiles - 1) / min_tiles;
   s.runs = row_blocks > 0;
   s.join = chunks > 1;
   s.min_tiles = s.join ? min_tiles : 0x3fffffff;
   s.row_blocks = row_blocks;
-  s.join_rows = (int)std::min<int64_t>(rows, most_rows);
+  // The join: a large row block's rows sixteen to a workgroup (few chunks); a small one's each in a workgroup, and where
+  // there are few of them in one per 128 channels, so that many lanes share the chunks (8 rows of 64 chunks
+  // at D = 512: 6.7 us, one workgroup a row: 8 us; 256 rows of 8 chunks: the other way round).
+  s.join_rows = rows == kRows ? (int)std::min<int64_t>(rows, most_rows) : rows / 16;
+  const int D = a->cache.head_dim;
+  s.join_slice = rows == kRows && D > 128 && row_blocks * s.join_rows * a->cache.heads_kv * (D / 128) <= 1024 ? 128 : D;
   // items: one per row block, and as many more as there are full chunks
   const int64_t hkv = a->cache.heads_kv;
   s.share = (float)((double)hkv / target * (1.0 + 1.0 / 4096));  // see chunk_tiles
@@ -143,8 +149,12 @@ Split split_of(const gfa_kv4_attn_args* a) {
     }
   }
   // with cu, workgroups to spare: rows behind the last request's
+  // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 20.1 us; of 4: 21.8, of 2: 27.4). Twice the CUs' number
+  // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us). The
+  // chunk kernel fills a CU with one workgroup: as many as there are CUs, 16 tiles or more each
+  // (1000 tokens over a window of 1024 beside seven requests: 94 us, twice as many 118 us).
   size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
-  size_part(s.many, a, many, big, most * G, 32, 512, 0);
+  size_part(s.many, a, many, big, most * G, 16, 256, 0);
   return s;
 }
 
@@ -229,7 +239,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "table, lens and cu must be 4-byte aligned pointers");
   const Split s = split_of(a);
   for (const Part* part : {&s.few, &s.many})
-    if (part->nblocks > 0x7fffffff || part->row_blocks * part->join_rows * a->cache.heads_kv > 0x7fffffff)
+    if (part->nblocks > 0x7fffffff || part->row_blocks * part->join_rows * a->cache.heads_kv > 0x1fffffff)
       return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)part->nblocks);
   const size_t need = s.few.bytes() + s.many.bytes();
   if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
@@ -271,6 +281,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     p.share = part.share;
     p.row_blocks = (int)part.row_blocks;
     p.join_rows = part.join_rows;
+    p.join_slice = part.join_slice;
     p.nblocks = (int)part.nblocks;
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);

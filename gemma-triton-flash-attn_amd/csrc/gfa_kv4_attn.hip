@@ -38,6 +38,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 
 constexpr int kRows = kSplitRows;
 constexpr int kWaves = 4;
+constexpr float kMargin = 8.0f;  // log2
 
 // What a lane holds of a 32-token tile.
 template <int D>
@@ -84,8 +85,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   }
 
   // ---- the chunk's tiles; their blocks, 64 at a time in the lanes ----
-  const int t_first = rq.first + it.ch * it.per;
-  const int t_end = min(rq.first + rq.tiles, t_first + it.per);
+  const int per = chunk_len(rq, it.nch);
+  const int t_first = rq.first + it.ch * per;
+  const int t_end = min(rq.first + rq.tiles, t_first + per);
   const int tpb_log2 = p.cache.bs_log2 - 5;
   const int* table = p.table + (int64_t)it.b * p.table_stride;
   int ids_at = t_first >> tpb_log2;
@@ -171,6 +173,14 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   };
 
   auto compute = [&](int tile, const TileRegs<D>& r) __attribute__((always_inline)) {
+    // Two tiles' codes fill half the VGPRs at D = 512: Q and O^T live in AGPRs (left to the allocator some spill, and
+    // a reload waits for every load in flight).
+    if constexpr (D == 512) {
+#pragma unroll
+      for (int k = 0; k < KT; ++k) pin_agpr(qf[k]);
+#pragma unroll
+      for (int x = 0; x < XB; ++x) asm volatile("" : "+a"(acc[x]));
+    }
     // ---- S^T, 16 tokens at a time ----
     f32x4 s[2];
 #pragma unroll
@@ -217,15 +227,18 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
     float mt = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) mt = fmaxf(mt, x[e]);
-    const float m_new = fmaxf(m_run, quad_max(mt));
-    const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    if (__builtin_amdgcn_ballot_w64(m_new > m_run) != 0) {
-      const float a = fast_exp2(m_run - m_use);
+    // The maximum moves when a score passes it by more than 2^kMargin (or is the row's first): P stays within
+    // 2^kMargin, and O^T is rescaled once or twice per row instead of in most tiles.
+    mt = quad_max(mt);
+    if (__builtin_amdgcn_ballot_w64(mt > m_run + (m_run == -INFINITY ? 0.f : kMargin)) != 0) {
+      const float m_new = fmaxf(m_run, mt);
+      const float a = m_new == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
       l_run *= a;
 #pragma unroll
       for (int xb = 0; xb < XB; ++xb) acc[xb] *= a;
       m_run = m_new;
     }
+    const float m_use = m_run == -INFINITY ? 0.f : m_run;
     i16x8 pb;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {

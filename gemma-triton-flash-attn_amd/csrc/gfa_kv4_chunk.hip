@@ -121,8 +121,9 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
     k_hi = min(held, pos0 + i_hi + 1);
     if (p.window > 0) k_lo = max(0, pos0 + i_lo - p.window + 1);
   }
-  const int t_first = k_lo / kTile + it.ch * it.per;
-  const int t_end = k_hi > k_lo ? min((k_hi + kTile - 1) / kTile, t_first + it.per) : t_first;
+  const int per = chunk_len(rq, it.nch);
+  const int t_first = k_lo / kTile + it.ch * per;
+  const int t_end = k_hi > k_lo ? min((k_hi + kTile - 1) / kTile, t_first + per) : t_first;
 
   // ---- this lane's rows ----
   int qt[MT], qh[MT];

@@ -79,12 +79,13 @@ __device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, const Request
   return max((int)fminf(each, 1.0e9f), p.min_tiles);
 }
 __device__ __forceinline__ int chunks_of(const Request& r, int per) { return max((r.tiles + per - 1) / per, 1); }
+// Chunks of one length each, not full ones and a rest: the grid's last workgroups end closer together.
+__device__ __forceinline__ int chunk_len(const Request& r, int nch) { return (r.tiles + nch - 1) / nch; }
 
 struct Item {
   Request rq;
   int b;            // -1: there is no such item
   int rb, ch, nch;  // row block, chunk of nch
-  int per;          // tiles a chunk
   int items;        // of the whole call, where b < 0
 };
 template <int ROWS, bool LARGE>
@@ -92,9 +93,9 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
   Item it{};
   it.b = -1;
   Request r = request_of<ROWS, LARGE>(p, lane);
-  it.per = chunk_tiles<ROWS, LARGE>(p, r, lane);
+  const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
   for (int b0 = 0;;) {
-    const int mine = r.row_blocks * chunks_of(r, it.per);
+    const int mine = r.row_blocks * chunks_of(r, per);
     const int s = wave_prefix_sum(mine);
     const int before = it.items + s - mine;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
@@ -102,7 +103,7 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
       const int src = __builtin_ctzll(hit);
       it.b = b0 + src;
       it.rq = request_from(r, src);
-      it.nch = chunks_of(it.rq, it.per);
+      it.nch = chunks_of(it.rq, per);
       const int i = item - __builtin_amdgcn_readlane(before, src);
       it.rb = i / it.nch;
       it.ch = i % it.nch;
@@ -150,6 +151,17 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
     r = request_of<ROWS, LARGE>(p, b0 + lane);
   }
   return out;
+}
+
+// Adds a part's row (maximum mc, sum lc, O^T values v) to the row (m, l, o). Without a maximum on either side the
+// sums are marks and add up; a part without one has no values (they may never have been written).
+__device__ __forceinline__ void join_rows(float& m, float& l, f32x4& o, float mc, float lc, const f32x4& v) {
+  const float mn = fmaxf(m, mc);
+  const bool none = mn == -INFINITY;
+  const float a = none ? 1.f : fast_exp2(m - mn), b = none ? 1.f : fast_exp2(mc - mn);
+  l = l * a + lc * b;
+  o = mc == -INFINITY ? o * a : o * a + v * b;
+  m = mn;
 }
 
 // 1 / l of a finished row. Without weight l is a mark, not a sum: the row is 0 / 0 where it saw keys.
