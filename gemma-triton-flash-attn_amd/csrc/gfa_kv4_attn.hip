@@ -84,14 +84,17 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
     return;
   }
 
-  // ---- the chunk's tiles; their blocks, 64 at a time in the lanes ----
+  // ---- the chunk's tiles ----
   const int per = chunk_len(rq, it.nch);
   const int t_first = rq.first + it.ch * per;
   const int t_end = min(rq.first + rq.tiles, t_first + per);
   const int tpb_log2 = p.cache.bs_log2 - 5;
   const int* table = p.table + (int64_t)it.b * p.table_stride;
-  int ids_at = t_first >> tpb_log2;
-  int ids = table[min(ids_at + lane, p.M - 1)];
+  auto block_of = [&](int tile) __attribute__((always_inline)) { return table_entry(table, min(tile, t_end - 1) >> tpb_log2); };
+
+  const int t0 = t_first + wave;
+  const int b0 = t_first < t_end ? block_of(t0) : 0;
+  int b1 = t_first < t_end ? block_of(t0 + kWaves) : 0;
 
   // ---- this lane's row: token, head, visible keys ----
   const int row = it.rb * kRows + c16;
@@ -126,17 +129,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   bool seen = false;  // the row sees a token of a tile this wave took
   const unsigned nan2 = IS_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
 
-  auto load = [&](int tile, TileRegs<D>& r) __attribute__((always_inline)) {
-    const int tl = min(tile, t_end - 1);
-    const int col = tl >> tpb_log2;
-    if (col - ids_at >= 64) {
-      ids_at = col;
-      ids = table[min(col + lane, p.M - 1)];
-    }
-    int block = __builtin_amdgcn_readlane(ids, col - ids_at);
+  auto load = [&](int tile, int block, TileRegs<D>& r) __attribute__((always_inline)) {
+    const int sub = min(tile, t_end - 1) & ((1 << tpb_log2) - 1);
     r.held = (unsigned)block < (unsigned)p.cache.num_blocks && tile < t_end;
     block = r.held ? block : 0;
-    const int sub = tl & ((1 << tpb_log2) - 1);
     const uint8_t* kc = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 0) + sub * L::TILE_CODES;
     const uint8_t* vc = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 1) + sub * L::TILE_CODES;
     const uint8_t* ks = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 0) + sub * L::TILE_SCALES;
@@ -287,16 +283,17 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
     }
   };
 
-  // The wave's tiles, one loaded ahead.
-  if (t_first + wave < t_end) {
-    TileRegs<D> r0, r1;
-    load(t_first + wave, r0);
-    for (int tile = t_first + wave; tile < t_end; tile += 2 * kWaves) {
-      load(tile + kWaves, r1);
-      compute(tile, r0);
-      if (tile + kWaves >= t_end) break;
-      load(tile + 2 * kWaves, r0);
-      compute(tile + kWaves, r1);
+  // The wave's tiles, one loaded ahead. One copy of the body, the registers moved: few tiles a wave run it, and a
+  // second copy would have to come into the instruction cache.
+  if (t0 < t_end) {
+    TileRegs<D> now, next;
+    load(t0, b0, now);
+    for (int tile = t0;;) {
+      load(tile + kWaves, b1, next);
+      b1 = block_of(tile + 2 * kWaves);
+      compute(tile, now);
+      if ((tile += kWaves) >= t_end) break;
+      now = next;
     }
   }
 

@@ -169,24 +169,17 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
   }
   if (threadIdx.x == 0) redo_flag = 0;  // read behind a later barrier
 
-  // ---- the blocks of the tiles, 64 at a time in the lanes ----
   const int tpb_log2 = p.cache.bs_log2 - 5;
   const int* table = p.table + (int64_t)it.b * p.table_stride;
-  int ids = 0, ids_at = -1;
-  auto block_of = [&](int tile) __attribute__((always_inline)) {
-    const int col = tile >> tpb_log2;
-    if (ids_at < 0 || col - ids_at >= 64) {
-      ids_at = col;
-      ids = table[min(col + lane, p.M - 1)];
-    }
-    return __builtin_amdgcn_readlane(ids, col - ids_at);
-  };
+  auto block_of = [&](int tile) __attribute__((always_inline)) { return table_entry(table, min(tile, t_end - 1) >> tpb_log2); };
+  int block_next = 0;
   Kv4Copies<D> copies;
   copies.init(wave, lane);
   const unsigned n_blocks = (unsigned)p.cache.num_blocks;
   bool held_next = false;
   auto fetch = [&](int tile, char GFA_LDS* kt, char GFA_LDS* vt, char GFA_LDS* st) __attribute__((always_inline)) {
-    const int block = block_of(tile);
+    const int block = block_next;
+    block_next = block_of(tile + 1);
     const bool there = (unsigned)block < n_blocks;
     held_next = there && tile < t_end;
     copies.load(p.cache, there ? block : 0, head, tile & ((1 << tpb_log2) - 1), kt, vt, st);
@@ -398,7 +391,10 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
       for (int x = 0; x < CPL; ++x) acc[m][x] = f32x16{};
       l_run[m] = 0.f;
     }
-    if (t_first < t_end) fetch(t_first, K0, V0, S0);
+    if (t_first < t_end) {
+      block_next = block_of(t_first);
+      fetch(t_first, K0, V0, S0);
+    }
     for (int t = t_first; t < t_end; t += 2) {
       step(t, K0, V0, S0, K1, V1, S1);
       step(t + 1, K1, V1, S1, K0, V0, S0);

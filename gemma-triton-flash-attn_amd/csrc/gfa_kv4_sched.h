@@ -19,18 +19,18 @@ struct Request {
   int row_blocks;      // 0: not this kernel's
   int first, tiles;    // key tiles that some row sees
 };
+// Its three loads go out together (one wait: their latency is a good part of a short call).
 template <int ROWS, bool LARGE>
 __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   Request r{};
+  const int bc = min(b, p.B - 1);
+  const int* cu = p.cu != nullptr ? p.cu : p.lens;  // without cu read for nothing
+  const int t0 = cu[bc], t1 = cu[p.cu != nullptr ? bc + 1 : bc], len = p.lens[bc];
+  const int each = p.T / p.B;
   if (b >= p.B) return r;
-  if (p.cu != nullptr) {
-    r.t0 = p.cu[b];
-    r.fresh = min(max((int)((unsigned)p.cu[b + 1] - (unsigned)r.t0), 0), p.T);
-  } else {
-    r.fresh = p.T / p.B;
-    r.t0 = b * r.fresh;
-  }
-  r.len = max(p.lens[b], 0);
+  r.t0 = p.cu != nullptr ? t0 : b * each;
+  r.fresh = p.cu != nullptr ? min(max((int)((unsigned)t1 - (unsigned)t0), 0), p.T) : each;
+  r.len = max(len, 0);
   const int rows = r.fresh * p.G;
   r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
   const int held = min(r.len, p.M << p.cache.bs_log2);
@@ -151,6 +151,13 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
     r = request_of<ROWS, LARGE>(p, b0 + lane);
   }
   return out;
+}
+
+// Entry `col` of a block table row, through the scalar cache: the address is the wave's, and a scalar load's wait leaves
+// the tile loads in flight alone.
+__device__ __forceinline__ int table_entry(const int* row, int col) {
+  typedef const int __attribute__((address_space(4))) * Scalar;
+  return ((Scalar)(uintptr_t)row)[col];
 }
 
 // Adds a part's row (maximum mc, sum lc, O^T values v) to the row (m, l, o). Without a maximum on either side the
