@@ -110,7 +110,10 @@ struct Kv4PlanParams {
 
 // Query rows of a workgroup of the split and of the chunk kernel.
 constexpr int kSplitRows = 16;
-constexpr int kv4_chunk_rows(int D) { return D == 512 ? 128 : 256; }
+constexpr int kv4_chunk_rows(int D) { return D >= 128 ? 128 : 256; }
+
+// Workgroups of the chunk kernel that a CU holds (by their registers).
+constexpr int kv4_chunk_wgs(int D) { return D == 512 ? 1 : D == 128 ? 3 : 2; }
 
 struct Kv4AttnParams {
   Kv4Cache cache;
@@ -121,7 +124,8 @@ struct Kv4AttnParams {
   const int *table, *lens, *cu;
   int64_t table_stride;
   int B, M, Hq, G;
-  int causal, window;
+  int causal, window;  // window 0: none
+  int window_tiles;    // most key tiles a row block of this kernel sees through the window
   float xs;     // multiplier of a score ahead of exp2: scale log2(e), or with soft-capping cap log2(e)
   float cap_a;  // scale / cap, 0: no soft-capping
   int min_tiles;  // work split, see chunk_tiles in gfa_kv4_sched.h

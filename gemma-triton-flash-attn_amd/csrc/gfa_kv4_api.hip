@@ -88,7 +88,7 @@ struct Part {
   int min_tiles;
   float share;
   int64_t nblocks, row_blocks;
-  int join_rows, join_slice;
+  int join_rows, join_slice, window_tiles;
   bool join;  // some row block may take more than one chunk
   size_t part_bytes, ml_bytes;
   size_t bytes() const { return part_bytes + ml_bytes; }
@@ -103,8 +103,11 @@ constexpr int kRowLimit = 32;
 
 void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
-  if (a->causal && a->window > 0)
-    tiles = std::min<int64_t>(tiles, ((int64_t)a->window + (int64_t)a->batch * a->seq_len + 31) / 32 + 1);
+  if (a->causal && a->window > 0) {
+    const int64_t g = a->heads_q / a->cache.heads_kv, tokens = (rows + g - 2) / g + 1;  // a row block's, at most
+    s.window_tiles = (int)std::min<int64_t>((a->window + tokens + 29) / 32 + 1, 0x40000000);
+    tiles = std::min<int64_t>(tiles, s.window_tiles);
+  }
   // Requests of 512 tokens or less are one chunk: one token of 333 at D = 256 takes 8.5 us, 10.9-11.6 us with a join.
   const int64_t chunks = tiles <= 16 ? 1 : (tiles + min_tiles - 1) / min_tiles;
   s.runs = row_blocks > 0;
@@ -150,11 +153,11 @@ Split split_of(const gfa_kv4_attn_args* a) {
   }
   // with cu, workgroups to spare: rows behind the last request's
   // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 20.1 us; of 4: 21.8, of 2: 27.4). Twice the CUs' number
-  // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us). The
-  // chunk kernel fills a CU with one workgroup: as many as there are CUs, 16 tiles or more each
-  // (1000 tokens over a window of 1024 beside seven requests: 94 us, twice as many 118 us).
+  // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us); of the
+  // chunk kernel as many as the CUs hold at once (256 tokens at 16k, D = 512: 298 us, twice as many 327; 1024 tokens,
+  // D = 128: 256 482 us, 512 375, 768 354, 1024 360).
   size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
-  size_part(s.many, a, many, big, most * G, 16, 256, 0);
+  size_part(s.many, a, many, big, most * G, 8, 256 * gfa::kv4_chunk_wgs(D), 0);
   return s;
 }
 
@@ -279,6 +282,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     if (!part.runs) continue;
     p.min_tiles = part.min_tiles;
     p.share = part.share;
+    p.window_tiles = part.window_tiles;
     p.row_blocks = (int)part.row_blocks;
     p.join_rows = part.join_rows;
     p.join_slice = part.join_slice;

@@ -86,8 +86,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
 
   // ---- the chunk's tiles ----
   const int per = chunk_len(rq, it.nch);
-  const int t_first = rq.first + it.ch * per;
-  const int t_end = min(rq.first + rq.tiles, t_first + per);
+  const int2 tiles = tiles_of_rows(p, rq, it.rb * kRows, kRows);
+  const int t_first = tiles.x + it.ch * per;
+  const int t_end = min(tiles.y, t_first + per);
   const int tpb_log2 = p.cache.bs_log2 - 5;
   const int* table = p.table + (int64_t)it.b * p.table_stride;
   auto block_of = [&](int tile) __attribute__((always_inline)) { return table_entry(table, min(tile, t_end - 1) >> tpb_log2); };

@@ -21,48 +21,41 @@ namespace gfa {
 
 namespace {
 
-// Tile copies of one wave: 1 KB runs of codes (K, then V) and the scales, dealt to the four waves in turn.
+// Tile copies of one wave: 1 KB runs of codes (K, then V) and the scales, dealt to the four waves in turn. K pieces land
+// swizzled: a lane's 16-byte reads of a column of pieces then touch every bank once.
 template <int D>
-struct Kv4Copies {
+__device__ __forceinline__ void copy_tile(const Kv4Cache& c, int block, int head, int sub, int wave, int lane, char GFA_LDS* kt,
+                                          char GFA_LDS* vt, char GFA_LDS* st) {
   using L = Kv4Layout<D>;
-  static constexpr int RUNS = L::TILE_CODES / 1024;  // per side
-  unsigned k_off;                                    // this lane's byte of a K run, swizzled
-  int lane, wave;
-  __device__ __forceinline__ void init(int wave_, int lane_) {
-    lane = lane_;
-    wave = wave_;
-    if constexpr (D == 64) {
-      const int t = lane >> 1;  // 32 tokens of 2 pieces
-      k_off = t * 32 + (((lane & 1) ^ ((t >> 3) & 1)) << 4);
-    } else {
-      const int t = lane >> 2;  // 16 tokens of 4 pieces
-      k_off = t * 64 + (((lane & 3) ^ ((t >> 2) & 3)) << 4);
-    }
-  }
-  __device__ __forceinline__ void load(const Kv4Cache& c, int block, int head, int sub, char GFA_LDS* kt, char GFA_LDS* vt,
-                                       char GFA_LDS* st) const {
-    // one (block, head): K side, then V side
-    const int side = (D / 2) << c.bs_log2, sside = (D / 32) << c.bs_log2;
-    const auto rc = __builtin_amdgcn_make_buffer_rsrc(c.codes + kv4_codes_at<D>(c, block, head, 0), 0, 2 * side, 0x00020000);
+  constexpr int RUNS = L::TILE_CODES / 1024;  // per side
+  // 16 tokens of 4 pieces a run; D = 64: 32 of 2
+  const int t = D == 64 ? lane >> 1 : lane >> 2;
+  const unsigned k_off = D == 64 ? t * 32 + (((lane & 1) ^ ((t >> 3) & 1)) << 4) : t * 64 + (((lane & 3) ^ ((t >> 2) & 3)) << 4);
+  // one (block, head): K side, then V side
+  const int side = (D / 2) << c.bs_log2, sside = (D / 32) << c.bs_log2;
+  const auto rc = __builtin_amdgcn_make_buffer_rsrc(c.codes + kv4_codes_at<D>(c, block, head, 0), 0, 2 * side, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < 2 * RUNS; i += 4) {
-      const int run = i + wave;
-      if (2 * RUNS >= 4 || run < 2 * RUNS) {
-        const bool v = run >= RUNS;
-        const int r = v ? run - RUNS : run;
-        const unsigned soff = (unsigned)((v ? side : 0) + sub * L::TILE_CODES + r * 1024);
-        char GFA_LDS* dst = (v ? vt : kt) + r * 1024;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (void GFA_LDS*)dst, 16, v ? (unsigned)lane * 16 : k_off, soff, 0, 0);
-      }
-    }
-    if (wave == (2 * RUNS) % 4) {
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(c.scales + kv4_scales_at<D>(c, block, head, 0), 0, 2 * sside, 0x00020000);
-      constexpr int LS = D / 16;  // lanes per side
-      const unsigned off = (unsigned)(lane < LS ? lane * 16 : sside + (lane - LS) * 16);
-      if (lane < 2 * LS) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (void GFA_LDS*)st, 16, off, sub * L::TILE_SCALES, 0, 0);
+  for (int i = 0; i < 2 * RUNS; i += 4) {
+    const int run = i + wave;
+    if (2 * RUNS >= 4 || run < 2 * RUNS) {
+      const bool v = run >= RUNS;
+      const int r = v ? run - RUNS : run;
+      const unsigned soff = (unsigned)((v ? side : 0) + sub * L::TILE_CODES + r * 1024);
+      char GFA_LDS* dst = (v ? vt : kt) + r * 1024;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rc, (void GFA_LDS*)dst, 16, v ? (unsigned)lane * 16 : k_off, soff, 0, 0);
     }
   }
-};
+  if (wave == (2 * RUNS) % 4) {
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(c.scales + kv4_scales_at<D>(c, block, head, 0), 0, 2 * sside, 0x00020000);
+    constexpr int LS = D / 16;  // lanes per side
+    const unsigned off = (unsigned)(lane < LS ? lane * 16 : sside + (lane - LS) * 16);
+    if (lane < 2 * LS) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (void GFA_LDS*)st, 16, off, sub * L::TILE_SCALES, 0, 0);
+  }
+}
+
+// The lane's number, computed where it is needed (two instructions) rather than held with what derives from it: at D >=
+// 256 a register more in the loop is a reload, whose wait is one for the tile copies too.
+__device__ __forceinline__ int fresh_lane() { return opaque((int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u))); }
 
 // A product of the S^T chain kept in VGPRs (O^T fills the AGPRs, and built from the builtin the chain would
 // run there too), whose operand the vector unit has just decoded: two wait states until a product may
@@ -87,14 +80,14 @@ __device__ __forceinline__ void mma32_decoded(f32x16& c, const i16x8& a, const i
 }  // namespace
 
 template <int D, bool IS_BF16, bool CAP>
-__global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p) {
+__global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const Kv4AttnParams p) {
   using L = Kv4Layout<D>;
   constexpr int ROWS = kv4_chunk_rows(D);
   constexpr int MT = ROWS / 128;                 // 32-row blocks per wave
   constexpr int KT = D / 16;                     // products of a score block
   constexpr int CPL = D / 32;                    // channels of an O^T operand row: 32-row blocks of O^T
   constexpr int NJ = D == 64 ? 1 : D / 128;
-  constexpr bool PIN = D >= 256;                 // O^T fills the AGPRs
+  constexpr bool PIN = D == 512;                 // O^T fills the AGPRs
   constexpr float kMargin = IS_BF16 ? 64.0f : 15.0f;          // log2
   __shared__ int redo_flag;
   __shared__ __attribute__((aligned(1024))) char k_lds0[L::TILE_CODES], k_lds1[L::TILE_CODES];
@@ -103,7 +96,7 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int h = lane >> 5, l32 = lane & 31, p16 = lane & 15, hi = (lane >> 4) & 1;
+  const int h = lane >> 5;
   const int head = (int)blockIdx.x % p.cache.Hkv;
 
   const Item it = find_item<ROWS, true>(p, (int)blockIdx.x / p.cache.Hkv, lane);
@@ -114,35 +107,38 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
 
   // ---- key tiles of this row block's chunk ----
   const int held = min(rq.len, p.M << p.cache.bs_log2);
-  const int i_lo = row0 / p.G, i_hi = min((row0 + ROWS - 1) / p.G, rq.fresh - 1);
   const int pos0 = rq.len - rq.fresh;  // position of new token 0
-  int k_lo = 0, k_hi = held;
-  if (p.causal) {
-    k_hi = min(held, pos0 + i_hi + 1);
-    if (p.window > 0) k_lo = max(0, pos0 + i_lo - p.window + 1);
-  }
+  const int2 tiles = tiles_of_rows(p, rq, row0, ROWS);
   const int per = chunk_len(rq, it.nch);
-  const int t_first = k_lo / kTile + it.ch * per;
-  const int t_end = k_hi > k_lo ? min((k_hi + kTile - 1) / kTile, t_first + per) : t_first;
+  const int t_first = tiles.x + it.ch * per;
+  const int t_end = max(t_first, min(tiles.y, t_first + per));
 
   // ---- this lane's rows ----
-  int qt[MT], qh[MT];
-  bool live[MT];
+  // A row's token and query head; taken again for the stores rather than held through the loop.
+  struct Row {
+    int i, t, qh;
+    bool live;
+  };
+  auto row_of = [&](int m, int ln) __attribute__((always_inline)) {
+    const int row = row0 + (wave * MT + m) * 32 + (ln & 31);
+    Row r;
+    r.i = row / p.G;
+    r.t = rq.t0 + r.i;
+    r.qh = head * p.G + row % p.G;
+    r.live = r.i < rq.fresh && r.t >= 0 && r.t < p.T;
+    return r;
+  };
   VisRange vis[MT];
   int all_lo = 0, all_hi = held;  // keys that every row of the wave sees
   i16x8 qf[MT][KT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    const int row = row0 + (wave * MT + m) * 32 + l32;
-    const int i = row / p.G;
-    qt[m] = rq.t0 + i;
-    qh[m] = head * p.G + row % p.G;
-    live[m] = i < rq.fresh && qt[m] >= 0 && qt[m] < p.T;
-    const int pos = pos0 + i;
-    const int last = live[m] ? min(p.causal ? pos : rq.len - 1, held - 1) : -1;
+    const Row r = row_of(m, lane);
+    const int pos = pos0 + r.i;
+    const int last = r.live ? min(p.causal ? pos : rq.len - 1, held - 1) : -1;
     vis[m] = make_range(p.causal && p.window > 0 ? max(pos - p.window + 1, 0) : 0, last);
-    const int tc = live[m] ? qt[m] : 0;  // rows past the last read another's query; nothing of theirs goes out
-    const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)qh[m] * p.qsh + (tc % p.N) * p.qsn;
+    const int tc = r.live ? r.t : 0;  // rows past the last read another's query; nothing of theirs goes out
+    const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)r.qh * p.qsh + (tc % p.N) * p.qsn;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -173,30 +169,30 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
   const int* table = p.table + (int64_t)it.b * p.table_stride;
   auto block_of = [&](int tile) __attribute__((always_inline)) { return table_entry(table, min(tile, t_end - 1) >> tpb_log2); };
   int block_next = 0;
-  Kv4Copies<D> copies;
-  copies.init(wave, lane);
   const unsigned n_blocks = (unsigned)p.cache.num_blocks;
   bool held_next = false;
-  auto fetch = [&](int tile, char GFA_LDS* kt, char GFA_LDS* vt, char GFA_LDS* st) __attribute__((always_inline)) {
+  auto fetch = [&](int tile, int ln, char GFA_LDS* kt, char GFA_LDS* vt, char GFA_LDS* st) __attribute__((always_inline)) {
     const int block = block_next;
     block_next = block_of(tile + 1);
     const bool there = (unsigned)block < n_blocks;
     held_next = there && tile < t_end;
-    copies.load(p.cache, there ? block : 0, head, tile & ((1 << tpb_log2) - 1), kt, vt, st);
+    copy_tile<D>(p.cache, there ? block : 0, head, tile & ((1 << tpb_log2) - 1), wave, ln, kt, vt, st);
   };
 
   const unsigned nan2 = IS_BF16 ? 0x7fc07fc0u : 0x7e007e00u;
-  // LDS bytes of this lane: its K pieces (pair u of a chunk), K scales, V pieces, V scales
-  const int k_row = D == 64 ? l32 * 32 : l32 * 64;
-  const int k_swz = D == 64 ? (l32 >> 3) & 1 : (l32 >> 2) & 3;
-  const int v_piece = p16 * 16;
-  const int v_blk = p16 * L::PP / 32;
-
   auto step = [&](int tile, const char GFA_LDS* kt, const char GFA_LDS* vt, const char GFA_LDS* st, char GFA_LDS* kn,
                   char GFA_LDS* vn, char GFA_LDS* sn) __attribute__((always_inline)) {
     barrier_tile();
     const bool is_held = held_next;
-    fetch(tile + 1, kn, vn, sn);
+    const int ln = fresh_lane();
+    const int h = ln >> 5, l32 = ln & 31, p16 = ln & 15, hi = (ln >> 4) & 1;
+    fetch(tile + 1, ln, kn, vn, sn);
+
+    // LDS bytes of this lane: its K pieces (pair u of a chunk), its V pieces and the scale block of their channels
+    const int k_row = D == 64 ? l32 * 32 : l32 * 64;
+    const int k_swz = D == 64 ? (l32 >> 3) & 1 : (l32 >> 2) & 3;
+    const int v_piece = p16 * 16;
+    const int v_blk = p16 * L::PP / 32;
 
     // ---- S^T ----
     f32x16 s[MT];
@@ -393,7 +389,7 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
     }
     if (t_first < t_end) {
       block_next = block_of(t_first);
-      fetch(t_first, K0, V0, S0);
+      fetch(t_first, lane, K0, V0, S0);
     }
     for (int t = t_first; t < t_end; t += 2) {
       step(t, K0, V0, S0, K1, V1, S1);
@@ -410,21 +406,24 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
   }
 
   // ---- rows out ----
+  const int ln = opaque(lane);
+  const int ho = ln >> 5;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
+    const Row r0 = row_of(m, ln);
     float l = halves_sum(l_run[m]);
     if (m_ref[m] == -INFINITY && l == 0.f && seen[m]) l = 1.f;  // a mark, see row_inv
     if (it.nch > 1) {
-      const int64_t at = (int64_t)blockIdx.x * ROWS + (wave * MT + m) * 32 + l32;
-      if (h == 0) {
+      const int64_t at = (int64_t)blockIdx.x * ROWS + (wave * MT + m) * 32 + (ln & 31);
+      if (ho == 0) {
         p.part_ml[at * 2] = m_ref[m];
         p.part_ml[at * 2 + 1] = l;
       }
-      if (live[m] && t_first < t_end) {
+      if (r0.live && t_first < t_end) {
         float* part = p.part + at * D;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int idx = 8 * (r >> 2) + 4 * h + (r & 3);
+          const int idx = 8 * (r >> 2) + 4 * ho + (r & 3);
           float* d = part + (idx & 15) * L::PP + CPL * (idx >> 4);
           if constexpr (CPL >= 4) {
 #pragma unroll
@@ -438,13 +437,13 @@ __global__ __launch_bounds__(256, 1) void kv4_chunk_kernel(const Kv4AttnParams p
       }
       continue;
     }
-    if (!live[m]) continue;
+    if (!r0.live) continue;
     const bool none = m_ref[m] == -INFINITY && l == 0.f;
     const float inv = row_inv(m_ref[m], l);
-    uint16_t* op = p.o + (qt[m] / p.N) * p.osb + (int64_t)qh[m] * p.osh + (qt[m] % p.N) * p.osn;
+    uint16_t* op = p.o + (r0.t / p.N) * p.osb + (int64_t)r0.qh * p.osh + (r0.t % p.N) * p.osn;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int idx = 8 * (r >> 2) + 4 * h + (r & 3);
+      const int idx = 8 * (r >> 2) + 4 * ho + (r & 3);
       uint16_t* d = op + (idx & 15) * L::PP + CPL * (idx >> 4);
       constexpr int W = CPL < 4 ? CPL : 4;
 #pragma unroll

@@ -17,7 +17,7 @@ constexpr int kTile = 32;  // tokens
 struct Request {
   int t0, fresh, len;  // first new token, new tokens, tokens with the new ones
   int row_blocks;      // 0: not this kernel's
-  int first, tiles;    // key tiles that some row sees
+  int tiles;           // most key tiles that a row block sees
 };
 // Its three loads go out together (one wait: their latency is a good part of a short call).
 template <int ROWS, bool LARGE>
@@ -35,14 +35,23 @@ __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
   const int held = min(r.len, p.M << p.cache.bs_log2);
   const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : 0;
-  r.first = lo / kTile;
-  r.tiles = held > lo ? (held + kTile - 1) / kTile - r.first : 0;
+  r.tiles = held > lo ? (held + kTile - 1) / kTile - lo / kTile : 0;
+  if (p.window > 0) r.tiles = min(r.tiles, p.window_tiles);
   return r;
+}
+// Key tiles [x, y) that some row of the request's row block of `rows` rows from row0 on sees.
+__device__ __forceinline__ int2 tiles_of_rows(const Kv4AttnParams& p, const Request& r, int row0, int rows) {
+  const int i_lo = row0 / p.G, i_hi = min((row0 + rows - 1) / p.G, r.fresh - 1);
+  const int pos0 = r.len - r.fresh;  // position of new token 0
+  const int held = min(r.len, p.M << p.cache.bs_log2);
+  const int k_hi = p.causal ? min(held, pos0 + i_hi + 1) : held;
+  const int k_lo = p.window > 0 ? max(0, pos0 + i_lo - p.window + 1) : 0;
+  return k_hi > k_lo ? make_int2(k_lo / kTile, (k_hi + kTile - 1) / kTile) : make_int2(0, 0);
 }
 // Lane src's request in every lane.
 __device__ __forceinline__ Request request_from(const Request& r, int src) {
   auto at = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
-  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.first), at(r.tiles)};
+  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles)};
 }
 
 // Sum over the wave's lanes (the steps of wave_prefix_sum).
