@@ -10,10 +10,8 @@
 //    second product. A tile kept decoded in LDS would cost four times the LDS reads (64 D bytes per
 //    wave and product), which then take as long as the products; the codes cost a quarter, and the
 //    decoding (one instruction per two elements, two for V) issues in the products' shadow.
-//  * Softmax against a fixed reference per row, the maximum of the first tile it sees a key of, so that the
-//    loop never rescales O^T (which stays in AGPRs). A row whose scores pass the reference by more than
-//    2^kMargin (P ends at 2^16 in fp16) makes the workgroup redo its rows once against the exact maxima, seen
-//    along the way. Ordinary inputs never do. Row sums are held in 32 bits.
+//  * Softmax: a running reference per row, moved when a score passes it by more than 2^kMargin, so that O^T is
+//    rescaled once or twice per row and P stays within 2^kMargin. Row sums are held in 32 bits.
 #include "gfa_kv4_sched.h"
 #include "gfa_launch.h"
 
@@ -88,8 +86,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   constexpr int CPL = D / 32;                    // channels of an O^T operand row: 32-row blocks of O^T
   constexpr int NJ = D == 64 ? 1 : D / 128;
   constexpr bool PIN = D == 512;                 // O^T fills the AGPRs
-  constexpr float kMargin = IS_BF16 ? 64.0f : 15.0f;          // log2
-  __shared__ int redo_flag;
+  constexpr float kMargin = 8.0f;                // log2
   __shared__ __attribute__((aligned(1024))) char k_lds0[L::TILE_CODES], k_lds1[L::TILE_CODES];
   __shared__ __attribute__((aligned(1024))) char v_lds0[L::TILE_CODES], v_lds1[L::TILE_CODES];
   __shared__ __attribute__((aligned(1024))) char s_lds0[1024], s_lds1[1024];
@@ -156,14 +153,16 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   }
 
   f32x16 acc[MT][CPL];
-  float m_ref[MT], m_seen[MT], l_run[MT];
-  bool seen[MT], ovf = false;
+  float m_ref[MT], l_run[MT];
+  bool seen[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
-    m_ref[m] = m_seen[m] = -INFINITY;
+#pragma unroll
+    for (int x = 0; x < CPL; ++x) acc[m][x] = f32x16{};
+    m_ref[m] = -INFINITY;
+    l_run[m] = 0.f;
     seen[m] = false;
   }
-  if (threadIdx.x == 0) redo_flag = 0;  // read behind a later barrier
 
   const int tpb_log2 = p.cache.bs_log2 - 5;
   const int* table = p.table + (int64_t)it.b * p.table_stride;
@@ -242,6 +241,8 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
             mma32_decoded<IS_BF16, false>(s[m], __builtin_bit_cast(i16x8, a), q);
           }
         }
+        // few operands ahead: at two waves a SIMD and D = 256 the registers are full
+        if (D == 256 && (k & 1)) __builtin_amdgcn_sched_barrier(0);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -274,9 +275,25 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
         return halves_max(mt) * p.xs;
       };
       const float mt = row_max();
-      m_ref[m] = m_ref[m] == -INFINITY ? mt : m_ref[m];
-      ovf = ovf || mt > m_ref[m] + kMargin;
-      m_seen[m] = fmaxf(m_seen[m], mt);
+      if (__builtin_amdgcn_ballot_w64(mt > m_ref[m] + (m_ref[m] == -INFINITY ? 0.f : kMargin)) != 0) {
+        const float m_new = fmaxf(m_ref[m], mt);
+        const float a = m_new == -INFINITY ? 0.f : fast_exp2(m_ref[m] - m_new);
+        l_run[m] *= a;
+        m_ref[m] = m_new;
+#pragma unroll
+        for (int x = 0; x < CPL; ++x) {
+          // by way of a whole VGPR block: scaled element by element the block would live in two AGPR blocks at once
+          f32x16 c = acc[m][x];
+          if constexpr (PIN) pin_vgpr(c);
+          c *= a;
+          if constexpr (PIN) pin_vgpr(c);
+          acc[m][x] = c;
+          if constexpr (PIN) {
+            pin_agpr(acc[m][x]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      }
       const float m_use = m_ref[m] == -INFINITY ? 0.f : m_ref[m];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
@@ -379,34 +396,19 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   char GFA_LDS* const S0 = (char GFA_LDS*)s_lds0;
   char GFA_LDS* const S1 = (char GFA_LDS*)s_lds1;
   // Two tiles a turn, straight-line: an odd number of tiles gets one that nothing sees, and the last step a copy that
-  // nothing reads. 
-  auto run_pass = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int x = 0; x < CPL; ++x) acc[m][x] = f32x16{};
-      l_run[m] = 0.f;
-    }
-    if (t_first < t_end) {
-      block_next = block_of(t_first);
-      fetch(t_first, lane, K0, V0, S0);
-    }
-    for (int t = t_first; t < t_end; t += 2) {
-      step(t, K0, V0, S0, K1, V1, S1);
-      step(t + 1, K1, V1, S1, K0, V0, S0);
-    }
-  };
-  for (int pass = 0;; ++pass) {
-    run_pass();
-    if (__builtin_amdgcn_ballot_w64(ovf) != 0 && lane == 0) redo_flag = 1;
-    barrier_tile();  // the last copy has landed too
-    if (pass == 1 || redo_flag == 0) break;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) m_ref[m] = m_seen[m];
+  // nothing reads.
+  if (t_first < t_end) {
+    block_next = block_of(t_first);
+    fetch(t_first, lane, K0, V0, S0);
   }
+  for (int t = t_first; t < t_end; t += 2) {
+    step(t, K0, V0, S0, K1, V1, S1);
+    step(t + 1, K1, V1, S1, K0, V0, S0);
+  }
+  drain_tile_copies();
 
   // ---- rows out ----
-  const int ln = opaque(lane);
+  const int ln = fresh_lane();
   const int ho = ln >> 5;
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
