@@ -132,7 +132,8 @@ struct Kv4AttnParams {
   float share;
   int nblocks;    // workgroups of the split or chunk grid
   int row_limit;  // requests with more query rows than this belong to the chunk kernel
-  int row_blocks, join_rows, join_slice;  // the join grid: most row blocks, workgroups for the rows of one, channels of each
+  // the join grid: most row blocks, workgroups for the rows of one, channels of each, groups of lanes that share a row
+  int row_blocks, join_rows, join_slice, join_parts;
   float* part;    // (nblocks, rows, D) sums and (nblocks, rows, 2) row maxima and sums
   float* part_ml;
 };

@@ -88,7 +88,7 @@ struct Part {
   int min_tiles;
   float share;
   int64_t nblocks, row_blocks;
-  int join_rows, join_slice, window_tiles;
+  int join_rows, join_slice, join_parts, window_tiles;
   bool join;  // some row block may take more than one chunk
   size_t part_bytes, ml_bytes;
   size_t bytes() const { return part_bytes + ml_bytes; }
@@ -99,7 +99,10 @@ struct Split {
 };
 
 constexpr int kRows = gfa::kSplitRows;
-constexpr int kRowLimit = 32;
+// A request's rows from which the chunk kernel is faster: 16 requests at 8k, D = 512, 32 rows 101 us (chunk kernel 170),
+// 64 rows 158 (185), 128 rows 270 (203); D = 128, 64 rows 102 (124), 128 rows 178 (139). One request alone leaves the
+// GPU to the split kernel's smaller workgroups longer: 128 rows at 8k, D = 512, 25 us (47).
+int row_limit(const gfa_kv4_attn_args* a) { return (int64_t)a->requests * a->cache.heads_kv <= 4 ? 128 : 64; }
 
 void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
@@ -114,14 +117,15 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   s.join = chunks > 1;
   s.min_tiles = s.join ? min_tiles : 0x3fffffff;
   s.row_blocks = row_blocks;
-  // The join: a large row block's rows sixteen to a workgroup (few chunks); a small one's each in a workgroup, and where
-  // there are few of them in one per 128 channels, so that many lanes share the chunks (8 rows of 64 chunks
-  // at D = 512: 6.7 us, one workgroup a row: 8 us; 256 rows of 8 chunks: the other way round).
-  s.join_rows = rows == kRows ? (int)std::min<int64_t>(rows, most_rows) : rows / 16;
+  // The join. Where rows are few, a workgroup takes one row of 128 channels and its lanes share the chunks; else whole
+  // rows, where they are many one per group of lanes.
+  const int64_t hkv = a->cache.heads_kv, row_bound = std::min<int64_t>(rows, most_rows), n = row_blocks * hkv * row_bound;
   const int D = a->cache.head_dim;
-  s.join_slice = rows == kRows && D > 128 && row_blocks * s.join_rows * a->cache.heads_kv * (D / 128) <= 1024 ? 128 : D;
-  // items: one per row block, and as many more as there are full chunks
-  const int64_t hkv = a->cache.heads_kv;
+  s.join_slice = D > 128 && n * (D / 128) <= 1024 ? 128 : D;
+  const int groups = 1024 / s.join_slice;
+  s.join_parts = n <= 2048 ? groups : 1;
+  const int64_t wgs = (row_bound * s.join_parts + groups - 1) / groups, most_wgs = 4096 / std::max<int64_t>(1, row_blocks * hkv);
+  s.join_rows = (int)std::max<int64_t>(1, std::min(wgs, most_wgs));
   s.share = (float)((double)hkv / target * (1.0 + 1.0 / 4096));  // see chunk_tiles
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
   s.nblocks = items * hkv + spare;
@@ -137,7 +141,8 @@ Split split_of(const gfa_kv4_attn_args* a) {
   const int64_t T = (int64_t)a->batch * a->seq_len;
   const int64_t most = a->cu == nullptr ? T / R : a->max_new > 0 ? std::min<int64_t>(a->max_new, T) : T;
   // No request can have more rows than the limit: then all are the split kernel's, whatever max_new promised.
-  s.row_limit = most * G <= kRowLimit ? 0x7fffffff : kRowLimit;
+  const int limit = row_limit(a);
+  s.row_limit = most * G <= limit ? 0x7fffffff : limit;
   const int D = a->cache.head_dim, big = gfa::kv4_chunk_rows(D);
   int64_t few, many = 0;
   if (a->cu == nullptr) {
@@ -146,18 +151,20 @@ Split split_of(const gfa_kv4_attn_args* a) {
     many = large ? R * ((most * G + big - 1) / big) : 0;
   } else {
     few = (T * G + (kRows - 1) * R) / kRows;
-    if (s.row_limit == kRowLimit) {
-      few = std::min<int64_t>(few, R * ((kRowLimit + kRows - 1) / kRows));
-      many = T * G / big + std::min<int64_t>(R, T * G / (kRowLimit + 1));
+    if (s.row_limit == limit) {
+      few = std::min<int64_t>(few, R * ((limit + kRows - 1) / kRows));
+      many = T * G / big + std::min<int64_t>(R, T * G / (limit + 1));
     }
   }
   // with cu, workgroups to spare: rows behind the last request's
   // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 20.1 us; of 4: 21.8, of 2: 27.4). Twice the CUs' number
   // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us); of the
   // chunk kernel as many as the CUs hold at once (256 tokens at 16k, D = 512: 298 us, twice as many 327; 1024 tokens,
-  // D = 128: 256 482 us, 512 375, 768 354, 1024 360).
+  // D = 128: 256 482 us, 512 375, 768 354, 1024 360). A chunk of it costs as much again as eight tiles: where the row
+  // blocks alone take half the CUs, only rows of more than 64 tiles are split (512 tokens of four requests, window
+  // 1024: 70 us, split 79-94; 256 of one: 38 us, unsplit 57).
   size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
-  size_part(s.many, a, many, big, most * G, 8, 256 * gfa::kv4_chunk_wgs(D), 0);
+  size_part(s.many, a, many, big, most * G, many * a->cache.heads_kv >= 128 ? 64 : 8, 256 * gfa::kv4_chunk_wgs(D), 0);
   return s;
 }
 
@@ -286,6 +293,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     p.row_blocks = (int)part.row_blocks;
     p.join_rows = part.join_rows;
     p.join_slice = part.join_slice;
+    p.join_parts = part.join_parts;
     p.nblocks = (int)part.nblocks;
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);

@@ -16,8 +16,8 @@ template <int D, bool IS_BF16, int ROWS, bool LARGE>
 __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   const int LPR = p.join_slice / 4;  // a power of two
   const int GR = kTpb / LPR;
-  __shared__ f32x4 o_lds[LARGE ? 1 : kTpb];
-  __shared__ float ml_lds[LARGE ? 1 : kTpb / 16][2];
+  __shared__ f32x4 o_lds[kTpb];
+  __shared__ float ml_lds[kTpb / 16][2];
   const int lane = threadIdx.x & 63;
   int id = (int)blockIdx.x;
   const int head = id % p.cache.Hkv;
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   if ((int64_t)(blk.item + blk.nch) * p.cache.Hkv > p.nblocks) return;  // cu that is no prefix sum: no such chunks
   const int rb = LARGE ? blk.rq.row_blocks - 1 - blk.rb : blk.rb;       // the chunk kernel takes the last rows first
   const int rows = min(ROWS, blk.rq.fresh * p.G - rb * ROWS);
-  const int parts = LARGE ? 1 : min(GR, 1 << (32 - __builtin_clz(blk.nch - 1)));
+  const int parts = min(p.join_parts, 1 << (32 - __builtin_clz(blk.nch - 1)));
   const int at_once = GR / parts;
   const int group = threadIdx.x / LPR, part = group % parts, d = slice * p.join_slice + threadIdx.x % LPR * 4;
   for (int r0 = id % p.join_rows * at_once; r0 < rows; r0 += p.join_rows * at_once) {
@@ -48,7 +48,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
         join_rows(m, l, o, ml.x, ml.y, v);
       }
     }
-    if constexpr (!LARGE) {
+    if (parts > 1) {
       o_lds[threadIdx.x] = o;
       if (threadIdx.x % LPR == 0) {
         ml_lds[group][0] = m;
