@@ -117,14 +117,16 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   s.join = chunks > 1;
   s.min_tiles = s.join ? min_tiles : 0x3fffffff;
   s.row_blocks = row_blocks;
-  // The join. Where rows are few, a workgroup takes one row of 128 channels and its lanes share the chunks; else whole
-  // rows, where they are many one per group of lanes.
+  // The join. Of the chunk kernel: its runs of 1 KB, four waves a workgroup. Of the split kernel: where rows are few, a
+  // workgroup takes one row of 128 channels and its lanes share the chunks; else whole rows, where they are many
+  // one per group of lanes.
   const int64_t hkv = a->cache.heads_kv, row_bound = std::min<int64_t>(rows, most_rows), n = row_blocks * hkv * row_bound;
   const int D = a->cache.head_dim;
-  s.join_slice = D > 128 && n * (D / 128) <= 1024 ? 128 : D;
+  s.join_slice = rows == kRows && D > 128 && n * (D / 128) <= 1024 ? 128 : D;
   const int groups = 1024 / s.join_slice;
   s.join_parts = n <= 2048 ? groups : 1;
-  const int64_t wgs = (row_bound * s.join_parts + groups - 1) / groups, most_wgs = 4096 / std::max<int64_t>(1, row_blocks * hkv);
+  const int64_t wgs = rows == kRows ? (row_bound * s.join_parts + groups - 1) / groups : rows / 32 * (D <= 128 ? 16 : D / 8) / 4;
+  const int64_t most_wgs = 4096 / std::max<int64_t>(1, row_blocks * hkv);
   s.join_rows = (int)std::max<int64_t>(1, std::min(wgs, most_wgs));
   s.share = (float)((double)hkv / target * (1.0 + 1.0 / 4096));  // see chunk_tiles
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
@@ -158,13 +160,15 @@ Split split_of(const gfa_kv4_attn_args* a) {
   }
   // with cu, workgroups to spare: rows behind the last request's
   // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 20.1 us; of 4: 21.8, of 2: 27.4). Twice the CUs' number
-  // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us); of the
-  // chunk kernel as many as the CUs hold at once (256 tokens at 16k, D = 512: 298 us, twice as many 327; 1024 tokens,
-  // D = 128: 256 482 us, 512 375, 768 354, 1024 360). A chunk of it costs as much again as eight tiles: where the row
-  // blocks alone take half the CUs, only rows of more than 64 tiles are split (512 tokens of four requests, window
-  // 1024: 70 us, split 79-94; 256 of one: 38 us, unsplit 57).
+  // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us).
   size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
-  size_part(s.many, a, many, big, most * G, many * a->cache.heads_kv >= 128 ? 64 : 8, 256 * gfa::kv4_chunk_wgs(D), 0);
+  // Of the chunk kernel as many workgroups as the CUs hold at once (256 tokens at 16k, D = 512: 290 us, twice as many 314;
+  // 1024 tokens, D = 128: 256 482 us, 512 375, 768 354, 1024 360). Its chunks cost as much again as some tiles, so the
+  // more of the GPU the row blocks take by themselves the longer a chunk has to be: 256 tokens of one request, window
+  // 1024, 33 us with chunks of 8 tiles, 57 unsplit; 1000 tokens beside seven requests 66 us with 18 tiles, 74 unsplit;
+  // 512 tokens of four requests 76-84 us split, 71 unsplit.
+  const int64_t alone = many * a->cache.heads_kv;
+  size_part(s.many, a, many, big, most * G, alone >= 256 ? 64 : alone >= 128 ? 32 : 8, 256 * gfa::kv4_chunk_wgs(D), 0);
   return s;
 }
 

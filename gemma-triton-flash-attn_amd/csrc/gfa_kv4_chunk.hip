@@ -410,6 +410,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   // ---- rows out ----
   const int ln = fresh_lane();
   const int ho = ln >> 5;
+  constexpr int W = CPL < 4 ? CPL : 4;  // neighbouring channels stored at once
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
     const Row r0 = row_of(m, ln);
@@ -421,19 +422,18 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
         p.part_ml[at * 2] = m_ref[m];
         p.part_ml[at * 2 + 1] = l;
       }
-      if (r0.live && t_first < t_end) {
-        float* part = p.part + at * D;
+      if (t_first < t_end) {
+        // in the order the lanes hold them, whole 1 KB runs (kv4_join_large_kernel): by rows a store would touch 64 of them
+        float* part = p.part + ((int64_t)blockIdx.x * ROWS + (wave * MT + m) * 32) * D + ln * W;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const int idx = 8 * (r >> 2) + 4 * ho + (r & 3);
-          float* d = part + (idx & 15) * L::PP + CPL * (idx >> 4);
-          if constexpr (CPL >= 4) {
 #pragma unroll
-            for (int x = 0; x < CPL; x += 4)
-              *reinterpret_cast<f32x4*>(d + x) = f32x4{acc[m][x][r], acc[m][x + 1][r], acc[m][x + 2][r], acc[m][x + 3][r]};
-          } else {
-            d[0] = acc[m][0][r];
-            d[1] = acc[m][1][r];
+          for (int x = 0; x < CPL; x += W) {
+            typedef float vec __attribute__((ext_vector_type(W)));
+            vec v;
+#pragma unroll
+            for (int e = 0; e < W; ++e) v[e] = acc[m][x + e][r];
+            *reinterpret_cast<vec*>(part + (r * (CPL / W) + x / W) * (64 * W)) = v;
           }
         }
       }
@@ -447,7 +447,6 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
     for (int r = 0; r < 16; ++r) {
       const int idx = 8 * (r >> 2) + 4 * ho + (r & 3);
       uint16_t* d = op + (idx & 15) * L::PP + CPL * (idx >> 4);
-      constexpr int W = CPL < 4 ? CPL : 4;
 #pragma unroll
       for (int x = 0; x < CPL; x += W) {
         typedef short vec __attribute__((ext_vector_type(W)));
