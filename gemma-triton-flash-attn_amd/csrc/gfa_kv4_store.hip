@@ -7,36 +7,80 @@ namespace gfa {
 namespace {
 
 constexpr int kTpb = 256;
-// One lane owns one scale block: 32 channels of a token, K and V.
+
+// Rows and the cache. A lane takes 8 channels of four tokens in a row: its 16-byte pieces of K and V are loaded and
+// stored in whole 1 KB runs, the four lanes of a scale block sit side by side, and where the four tokens are a quarter of
+// an operand row of V (consecutive slots from a multiple of four, as a prompt's are) their codes go in one
+// piece. Bound: memory. 16384 tokens of 8 heads at D = 256, 170 MB each way: stored in 36 us (4.7 TB/s), read in
+// 27 us (6.4 TB/s); with a scale block a lane, 64-byte strides between lanes, 41 and 47 us.
+template <int D>
+struct Rows {
+  static constexpr int LPT = D / 8;     // lanes per token
+  static constexpr int GPW = 64 / LPT;  // groups of four tokens per wave
+};
 
 __device__ __forceinline__ bool slot_ok(int64_t slot, const Kv4Cache& c) {
   return slot >= 0 && slot < (int64_t)c.num_blocks << c.bs_log2;
 }
 
-// The block's scale byte and 16 bytes of codes. amax = the largest magnitude's float bits; its exponent
-// field less 2 puts amax in [4, 8) of the scale; one more where it is above 7, the midpoint of 6 and the
-// next scale's 8 (rms error of normal values 11.19% of theirs, 11.50% without). The conversion
-// rounds to the nearest code, ties to the even one, and saturates at 6.
+// Where a lane is: head, first of its four tokens, its 8 channels; the tokens' slots (-1: none).
+template <int D>
+struct Place {
+  int head, lane_t;  // lane within the token's lanes
+  int64_t t0;
+  int64_t slot[4];
+  bool quad;  // the four slots are one piece of V's order
+  __device__ __forceinline__ Place(const Kv4RowsParams& p) {
+    const int lane = threadIdx.x & 63;
+    const int64_t w = (int64_t)blockIdx.x * (kTpb / 64) + (threadIdx.x >> 6);
+    head = (int)(w % p.cache.Hkv);
+    t0 = (w / p.cache.Hkv * Rows<D>::GPW + lane / Rows<D>::LPT) * 4;
+    lane_t = lane % Rows<D>::LPT;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t s = t0 + i < p.T ? p.slots[t0 + i] : -1;
+      slot[i] = slot_ok(s, p.cache) ? s : -1;
+    }
+    quad = slot[0] >= 0 && (slot[0] & 3) == 0 && slot[1] == slot[0] + 1 && slot[2] == slot[0] + 2 && slot[3] == slot[0] + 3;
+  }
+};
+
+// A slot's bytes of one head: codes and scales of K and V, from the start of its tile.
+template <int D>
+struct SlotBytes {
+  uint8_t *k, *v, *ks, *vs;
+  int t;
+  __device__ __forceinline__ SlotBytes(const Kv4Cache& c, int64_t slot, int head) {
+    using L = Kv4Layout<D>;
+    const int block = (int)(slot >> c.bs_log2), off = (int)(slot & ((1 << c.bs_log2) - 1)), tile = off >> 5;
+    t = off & 31;
+    k = c.codes + kv4_codes_at<D>(c, block, head, 0) + tile * L::TILE_CODES;
+    v = c.codes + kv4_codes_at<D>(c, block, head, 1) + tile * L::TILE_CODES;
+    ks = c.scales + kv4_scales_at<D>(c, block, head, 0) + tile * L::TILE_SCALES;
+    vs = c.scales + kv4_scales_at<D>(c, block, head, 1) + tile * L::TILE_SCALES;
+  }
+};
+
+// The scale byte of the block whose four lanes each hold 8 values, and this lane's codes. amax = the largest
+// magnitude's float bits; its exponent field less 2 puts amax in [4, 8) of the scale; one more where it is
+// above 7, the midpoint of 6 and the next scale's 8 (rms error of normal values 11.19% of theirs, 11.50%
+// without). The conversion rounds to the nearest code, ties to the even one, and saturates at 6.
 template <bool IS_BF16>
-__device__ __forceinline__ int kv4_encode(const i16x8 (&x)[4], unsigned (&codes)[4]) {
+__device__ __forceinline__ int kv4_encode(const i16x8& x, unsigned& codes) {
   unsigned top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(from16<IS_BF16>(x[i][e])) & 0x7fffffffu);
-  }
+  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(from16<IS_BF16>(x[e])) & 0x7fffffffu);
+  top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, true));  // quad_perm [1, 0, 3, 2]
+  top = max(top, (unsigned)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, true));  // quad_perm [2, 3, 0, 1]
   const bool bad = top >= 0x7f800000u;
   const int byte = min(max((int)((top + 0x1fffffu) >> 23) - 2, Kv4Range<IS_BF16>::lo), Kv4Range<IS_BF16>::hi);
   const float scale = __uint_as_float((unsigned)byte << 23);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    unsigned c = 0;
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[i][0]), from16<IS_BF16>(x[i][1]), scale, 0);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[i][2]), from16<IS_BF16>(x[i][3]), scale, 1);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[i][4]), from16<IS_BF16>(x[i][5]), scale, 2);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[i][6]), from16<IS_BF16>(x[i][7]), scale, 3);
-    codes[i] = bad ? 0u : c;
-  }
+  unsigned c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[0]), from16<IS_BF16>(x[1]), scale, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[2]), from16<IS_BF16>(x[3]), scale, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[4]), from16<IS_BF16>(x[5]), scale, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, from16<IS_BF16>(x[6]), from16<IS_BF16>(x[7]), scale, 3);
+  codes = bad ? 0u : c;
   return bad ? kKv4Nan : byte;
 }
 
@@ -53,113 +97,121 @@ __device__ __forceinline__ i16x8 kv4_decode8(unsigned codes, int byte) {
 
 }  // namespace
 
-// Rows to the cache. A wave takes 2048 / D tokens of one head, a lane one scale block of K and of V. A
-// token's slot is read by its lanes; a slot outside the cache (padding: -1) stores nothing.
+// Rows to the cache; a slot outside it (padding: -1) stores nothing.
 template <int D, bool IS_BF16>
 __global__ __launch_bounds__(kTpb) void kv4_write_kernel(const Kv4RowsParams p) {
   using L = Kv4Layout<D>;
-  constexpr int SC = L::SC, TPW = 64 / SC;
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * (kTpb / 64) + (threadIdx.x >> 6);
-  const int head = (int)(w % p.cache.Hkv);
-  const int64_t t64 = w / p.cache.Hkv * TPW + lane / SC;
-  const int c = lane % SC;
-  const int64_t slot = t64 < p.T ? p.slots[t64] : -1;
-  const bool live = slot_ok(slot, p.cache);
-  i16x8 kx[4] = {}, vx[4] = {};
-  if (live) {
-    const int row = (int)t64 / p.N, n = (int)t64 % p.N;
-    const uint16_t* kp = p.k + row * p.ksb + head * p.ksh + n * p.ksn + 32 * c;
-    const uint16_t* vp = p.v + row * p.vsb + head * p.vsh + n * p.vsn + 32 * c;
+  constexpr int LPT = Rows<D>::LPT;
+  const Place<D> at(p);
+  const int lane = threadIdx.x & 63, d = 8 * at.lane_t, c = d / 32;
+  i16x8 kx[4], vx[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      kx[i] = *reinterpret_cast<const i16x8*>(kp + 8 * i);
-      vx[i] = *reinterpret_cast<const i16x8*>(vp + 8 * i);
+  for (int i = 0; i < 4; ++i) {
+    kx[i] = vx[i] = i16x8{};
+    if (at.slot[i] >= 0) {
+      const int row = (int)(at.t0 + i) / p.N, n = (int)(at.t0 + i) % p.N;
+      kx[i] = *reinterpret_cast<const i16x8*>(p.k + row * p.ksb + at.head * p.ksh + n * p.ksn + d);
+      vx[i] = *reinterpret_cast<const i16x8*>(p.v + row * p.vsb + at.head * p.vsh + n * p.vsn + d);
     }
   }
   unsigned kc[4], vc[4];
-  int ks = kv4_encode<IS_BF16>(kx, kc);
-  const int vs = kv4_encode<IS_BF16>(vx, vc);
-  // A value that is no number marks the token's first key block too: the attention kernel answers NaN to
-  // whoever attends to the token, through its score, and keeps the value out of every other row.
-  const uint64_t bad = __builtin_amdgcn_ballot_w64(vs == kKv4Nan);
-  const uint64_t mine = (SC == 64 ? ~0ull : (1ull << SC) - 1) << (lane / SC * SC);
-  if (c == 0 && (bad & mine) != 0) ks = kKv4Nan;
-  if (!live) return;
-  const int block = (int)(slot >> p.cache.bs_log2);
-  const int off = (int)(slot & ((1 << p.cache.bs_log2) - 1));
-  const int t = off & 31;
-  uint8_t* kb = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 0) + (off >> 5) * L::TILE_CODES;
-  uint8_t* vb = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 1) + (off >> 5) * L::TILE_CODES;
-  *reinterpret_cast<uint4*>(kb + L::k_code(t, c)) = make_uint4(kc[0], kc[1], kc[2], kc[3]);
+  int ks[4], vs[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // channels 32 c + 8 i ..
-    const int d = 32 * c + 8 * i;
-    if constexpr (D == 64) {
-      *reinterpret_cast<uint16_t*>(vb + L::v_code(t, d / 4, 0)) = (uint16_t)vc[i];
-      *reinterpret_cast<uint16_t*>(vb + L::v_code(t, d / 4 + 1, 0)) = (uint16_t)(vc[i] >> 16);
-    } else {
-      *reinterpret_cast<unsigned*>(vb + L::v_code(t, d / L::PP, d % L::PP / 8)) = vc[i];
-    }
+    ks[i] = kv4_encode<IS_BF16>(kx[i], kc[i]);
+    vs[i] = kv4_encode<IS_BF16>(vx[i], vc[i]);
+    // A value that is no number marks the token's first key block too: the attention kernels answer NaN to whoever
+    // attends to the token, through its score, and keep the value out of every other row.
+    const uint64_t bad = __builtin_amdgcn_ballot_w64(vs[i] == kKv4Nan);
+    const uint64_t mine = (LPT == 64 ? ~0ull : (1ull << LPT) - 1) << (lane / LPT * LPT);
+    if (c == 0 && (bad & mine) != 0) ks[i] = kKv4Nan;
   }
-  uint8_t* kse = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 0) + (off >> 5) * L::TILE_SCALES;
-  uint8_t* vse = p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 1) + (off >> 5) * L::TILE_SCALES;
-  kse[L::k_scale(t, c)] = (uint8_t)ks;
-  vse[L::v_scale(t, c)] = (uint8_t)vs;
+  const bool first = (at.lane_t & 3) == 0;  // of its block's four lanes
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (at.slot[i] < 0) continue;
+    const SlotBytes<D> b(p.cache, at.slot[i], at.head);
+    *reinterpret_cast<unsigned*>(b.k + L::k_code(b.t, c) + (d & 31) / 2) = kc[i];
+    if (first) b.ks[L::k_scale(b.t, c)] = (uint8_t)ks[i];
+    if (at.quad) continue;
+    if constexpr (D == 64) {
+      *reinterpret_cast<uint16_t*>(b.v + L::v_code(b.t, d / 4, 0)) = (uint16_t)vc[i];
+      *reinterpret_cast<uint16_t*>(b.v + L::v_code(b.t, d / 4 + 1, 0)) = (uint16_t)(vc[i] >> 16);
+    } else {
+      *reinterpret_cast<unsigned*>(b.v + L::v_code(b.t, d / L::PP, d % L::PP / 8)) = vc[i];
+    }
+    if (first) b.vs[L::v_scale(b.t, c)] = (uint8_t)vs[i];
+  }
+  if (at.quad) {
+    const SlotBytes<D> b(p.cache, at.slot[0], at.head);
+    if constexpr (D == 64) {
+      // two operand rows of 4 channels: tokens' 2 bytes side by side
+      *reinterpret_cast<uint2*>(b.v + L::v_code(b.t, d / 4, 0)) =
+          make_uint2(__builtin_amdgcn_perm(vc[1], vc[0], 0x05040100u), __builtin_amdgcn_perm(vc[3], vc[2], 0x05040100u));
+      *reinterpret_cast<uint2*>(b.v + L::v_code(b.t, d / 4 + 1, 0)) =
+          make_uint2(__builtin_amdgcn_perm(vc[1], vc[0], 0x07060302u), __builtin_amdgcn_perm(vc[3], vc[2], 0x07060302u));
+    } else {
+      *reinterpret_cast<uint4*>(b.v + L::v_code(b.t, d / L::PP, d % L::PP / 8)) = make_uint4(vc[0], vc[1], vc[2], vc[3]);
+    }
+    if (first)
+      *reinterpret_cast<unsigned*>(b.vs + L::v_scale(b.t, c)) = (unsigned)vs[0] | (unsigned)vs[1] << 8 | (unsigned)vs[2] << 16 | (unsigned)vs[3] << 24;
+  }
 }
 
-// Rows from the cache, the same split; a slot outside the cache reads as zeros.
+// Rows from the cache; a slot outside it reads as zeros.
 template <int D, bool IS_BF16>
 __global__ __launch_bounds__(kTpb) void kv4_read_kernel(const Kv4RowsParams p) {
   using L = Kv4Layout<D>;
-  constexpr int SC = L::SC, TPW = 64 / SC;
-  const int lane = threadIdx.x & 63;
-  const int64_t w = (int64_t)blockIdx.x * (kTpb / 64) + (threadIdx.x >> 6);
-  const int head = (int)(w % p.cache.Hkv);
-  const int64_t t64 = w / p.cache.Hkv * TPW + lane / SC;
-  const int c = lane % SC;
-  if (t64 >= p.T) return;
-  const int64_t slot = p.slots[t64];
-  unsigned kc[4] = {}, vc[4] = {};
-  int ks = 0, vs = 0;
-  if (slot_ok(slot, p.cache)) {
-    const int block = (int)(slot >> p.cache.bs_log2);
-    const int off = (int)(slot & ((1 << p.cache.bs_log2) - 1));
-    const int t = off & 31;
-    const uint8_t* kb = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 0) + (off >> 5) * L::TILE_CODES;
-    const uint8_t* vb = p.cache.codes + kv4_codes_at<D>(p.cache, block, head, 1) + (off >> 5) * L::TILE_CODES;
-    const uint4 k4 = *reinterpret_cast<const uint4*>(kb + L::k_code(t, c));
-    kc[0] = k4.x;
-    kc[1] = k4.y;
-    kc[2] = k4.z;
-    kc[3] = k4.w;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 32 * c + 8 * i;
-      if constexpr (D == 64) {
-        vc[i] = *reinterpret_cast<const uint16_t*>(vb + L::v_code(t, d / 4, 0)) |
-                (unsigned)*reinterpret_cast<const uint16_t*>(vb + L::v_code(t, d / 4 + 1, 0)) << 16;
-      } else {
-        vc[i] = *reinterpret_cast<const unsigned*>(vb + L::v_code(t, d / L::PP, d % L::PP / 8));
-      }
+  const Place<D> at(p);
+  const int d = 8 * at.lane_t, c = d / 32;
+  unsigned kc[4] = {}, vc[4] = {}, vs4 = 0;
+  int ks[4] = {};
+  if (at.quad) {
+    const SlotBytes<D> b(p.cache, at.slot[0], at.head);
+    if constexpr (D == 64) {
+      const uint2 x = *reinterpret_cast<const uint2*>(b.v + L::v_code(b.t, d / 4, 0));
+      const uint2 y = *reinterpret_cast<const uint2*>(b.v + L::v_code(b.t, d / 4 + 1, 0));
+      vc[0] = __builtin_amdgcn_perm(y.x, x.x, 0x05040100u);
+      vc[1] = __builtin_amdgcn_perm(y.x, x.x, 0x07060302u);
+      vc[2] = __builtin_amdgcn_perm(y.y, x.y, 0x05040100u);
+      vc[3] = __builtin_amdgcn_perm(y.y, x.y, 0x07060302u);
+    } else {
+      const uint4 x = *reinterpret_cast<const uint4*>(b.v + L::v_code(b.t, d / L::PP, d % L::PP / 8));
+      vc[0] = x.x;
+      vc[1] = x.y;
+      vc[2] = x.z;
+      vc[3] = x.w;
     }
-    ks = (p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 0) + (off >> 5) * L::TILE_SCALES)[L::k_scale(t, c)];
-    vs = (p.cache.scales + kv4_scales_at<D>(p.cache, block, head, 1) + (off >> 5) * L::TILE_SCALES)[L::v_scale(t, c)];
+    vs4 = *reinterpret_cast<const unsigned*>(b.vs + L::v_scale(b.t, c));
   }
-  const int row = (int)t64 / p.N, n = (int)t64 % p.N;
-  uint16_t* kp = p.ko + row * p.ksb + head * p.ksh + n * p.ksn + 32 * c;
-  uint16_t* vp = p.vo + row * p.vsb + head * p.vsh + n * p.vsn + 32 * c;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    *reinterpret_cast<i16x8*>(kp + 8 * i) = kv4_decode8<IS_BF16>(kc[i], ks);
-    *reinterpret_cast<i16x8*>(vp + 8 * i) = kv4_decode8<IS_BF16>(vc[i], vs);
+    if (at.slot[i] < 0) continue;
+    const SlotBytes<D> b(p.cache, at.slot[i], at.head);
+    kc[i] = *reinterpret_cast<const unsigned*>(b.k + L::k_code(b.t, c) + (d & 31) / 2);
+    ks[i] = b.ks[L::k_scale(b.t, c)];
+    if (at.quad) continue;
+    if constexpr (D == 64) {
+      vc[i] = *reinterpret_cast<const uint16_t*>(b.v + L::v_code(b.t, d / 4, 0)) |
+              (unsigned)*reinterpret_cast<const uint16_t*>(b.v + L::v_code(b.t, d / 4 + 1, 0)) << 16;
+    } else {
+      vc[i] = *reinterpret_cast<const unsigned*>(b.v + L::v_code(b.t, d / L::PP, d % L::PP / 8));
+    }
+    vs4 |= (unsigned)b.vs[L::v_scale(b.t, c)] << (8 * i);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (at.t0 + i >= p.T) continue;
+    const int row = (int)(at.t0 + i) / p.N, n = (int)(at.t0 + i) % p.N;
+    // read once by whoever asked: past the caches
+    __builtin_nontemporal_store(kv4_decode8<IS_BF16>(kc[i], ks[i]), reinterpret_cast<i16x8*>(p.ko + row * p.ksb + at.head * p.ksh + n * p.ksn + d));
+    __builtin_nontemporal_store(kv4_decode8<IS_BF16>(vc[i], (int)(vs4 >> (8 * i) & 255)), reinterpret_cast<i16x8*>(p.vo + row * p.vsb + at.head * p.vsh + n * p.vsn + d));
   }
 }
 
 template <bool WRITE>
 hipError_t launch_rows(const Kv4RowsParams& p, int D, bool bf16, hipStream_t stream) {
-  const int64_t tpw = 2048 / D;
+  const int64_t tpw = 2048 / D;  // four tokens a group
   const int64_t waves = (p.T + tpw - 1) / tpw * p.cache.Hkv;
   const dim3 grid((unsigned)((waves + kTpb / 64 - 1) / (kTpb / 64)));
   auto go = [&](auto d, auto b) {

@@ -340,6 +340,14 @@ int64_t check_table(const Tensor& table, int64_t requests, const c10::Device& de
   return requests == 1 ? table.size(1) : table.stride(0);
 }
 
+// A tensor over part of a buffer's memory: outputs of one call from one allocation (an allocation through the
+// dispatcher takes about 0.8 us of host time, as a view through it would).
+Tensor part_of(const Tensor& buffer, int64_t offset, at::IntArrayRef sizes, at::IntArrayRef strides) {
+  auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, buffer.storage_offset() + offset);
+  return t;
+}
+
 gfa_kv4_rows_args rows_args(const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& k, const Tensor& v,
                             const Tensor& slots) {
   gfa_kv4_rows_args a{};
@@ -370,7 +378,8 @@ void kv4_write(const Tensor& codes, const Tensor& scales, bool bf16, const Tenso
   check(api.kv4_write(&a));
 }
 
-std::tuple<Tensor, Tensor> kv4_read(const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& slots) {
+// `apart`: outputs with memory of their own, as a registered op's have to be.
+std::tuple<Tensor, Tensor> kv4_read(const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& slots, bool apart) {
   check_cache(codes, scales);
   check_array("slots", slots, at::kLong, 1, codes.device());
   TORCH_CHECK_VALUE(slots.size(0) <= INT32_MAX, "slots holds more than 2^31 - 1 entries");
@@ -378,8 +387,9 @@ std::tuple<Tensor, Tensor> kv4_read(const Tensor& codes, const Tensor& scales, b
   const auto options = codes.options().dtype(bf16 ? at::kBFloat16 : at::kHalf);
   const int64_t T = slots.size(0), H = codes.size(1), D = 2 * codes.size(4);
   // (1, H, T, D) views of token-major rows
-  const Tensor k = at::empty_strided({1, H, T, D}, {T * H * D, D, H * D, 1}, options);
-  const Tensor v = at::empty_strided({1, H, T, D}, {T * H * D, D, H * D, 1}, options);
+  const Tensor kv = at::empty({(apart ? 1 : 2) * T * H * D}, options), kv2 = apart ? at::empty({T * H * D}, options) : kv;
+  const Tensor k = part_of(kv, 0, {1, H, T, D}, {T * H * D, D, H * D, 1});
+  const Tensor v = part_of(kv2, apart ? 0 : T * H * D, {1, H, T, D}, {T * H * D, D, H * D, 1});
   if (T > 0) {
     const Tensor sp = dense(slots);
     const auto a = rows_args(codes, scales, bf16, k, v, sp);
@@ -390,7 +400,7 @@ std::tuple<Tensor, Tensor> kv4_read(const Tensor& codes, const Tensor& scales, b
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv4_plan(const Tensor& lens, const Tensor& fresh, const Tensor& table,
                                                             const Tensor& free_ids, const Tensor& used, int64_t block_size,
-                                                            int64_t tokens) {
+                                                            int64_t tokens, bool apart) {
   const auto device = lens.device();
   check_array("lens", lens, at::kInt, 1, device);
   const int64_t B = lens.size(0);
@@ -404,9 +414,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv4_plan(const Tensor& lens, 
   TORCH_CHECK_VALUE(tokens >= 0 && tokens <= INT32_MAX, "tokens=", tokens, " must be in [0, 2^31)");
   const c10::DeviceGuard guard(device);
   const Tensor l = dense(lens), n = dense(fresh), f = dense(free_ids), u = dense(used);
-  const Tensor slots = at::empty({tokens}, lens.options().dtype(at::kLong)), positions = at::empty({tokens}, lens.options());
-  const Tensor cu = at::empty({B + 1}, lens.options()), lens_out = at::empty({B}, lens.options());
-  const Tensor used_out = at::empty({1}, lens.options());
+  const Tensor slots = at::empty({tokens}, lens.options().dtype(at::kLong));
+  const Tensor rest = apart ? Tensor() : at::empty({tokens + 2 * B + 2}, lens.options());
+  const auto out = [&](int64_t offset, int64_t n) { return apart ? at::empty({n}, lens.options()) : part_of(rest, offset, {n}, {1}); };
+  const Tensor positions = out(0, tokens), cu = out(tokens, B + 1), lens_out = out(tokens + B + 1, B);
+  const Tensor used_out = out(tokens + 2 * B + 1, 1);
   const auto ints = [](const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); };
   gfa_kv4_plan_args a{};
   a.lens = ints(l);

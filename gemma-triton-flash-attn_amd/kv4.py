@@ -100,8 +100,9 @@ def plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch
     order. ``tokens``: the step's static token count, at least the sum of ``new``; what lies behind is padding
     (slot -1). A table entry past the free list is -1, and so are the slots there; ``Plan.used`` above F tells
     of it. The next step takes ``Plan.lens`` and ``Plan.used``."""
-    fn = _lib.native().kv4_plan if _plain(lens) else torch.ops.gfa.kv4_plan
-    return Plan(*fn(lens, new, table, free, used, block_size, tokens))
+    if _plain(lens):
+        return Plan(*_lib.native().kv4_plan(lens, new, table, free, used, block_size, tokens, False))
+    return Plan(*torch.ops.gfa.kv4_plan(lens, new, table, free, used, block_size, tokens))
 
 
 def write(cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -114,8 +115,9 @@ def write(cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -
 def read(cache: Cache, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values at ``slots`` (int64, (T,)), as (1, Hkv, T, D) of the cache's dtype; zeros for a slot
     outside the cache."""
-    fn = _lib.native().kv4_read if _plain(slots) else torch.ops.gfa.kv4_read
-    return fn(cache.codes, cache.scales, cache.dtype is torch.bfloat16, slots)
+    if _plain(slots):
+        return _lib.native().kv4_read(cache.codes, cache.scales, cache.dtype is torch.bfloat16, slots, False)
+    return torch.ops.gfa.kv4_read(cache.codes, cache.scales, cache.dtype is torch.bfloat16, slots)
 
 
 def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None, *,
@@ -146,7 +148,7 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
 @torch.library.custom_op("gfa::kv4_plan", mutates_args=("table",))
 def _plan_op(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, used: torch.Tensor,
              block_size: int, tokens: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _lib.native().kv4_plan(lens, new, table, free, used, block_size, tokens)
+    return _lib.native().kv4_plan(lens, new, table, free, used, block_size, tokens, True)
 
 
 @_plan_op.register_fake
@@ -168,7 +170,7 @@ def _write_fake(codes, scales, bf16, k, v, slots):
 
 @torch.library.custom_op("gfa::kv4_read", mutates_args=())
 def _read_op(codes: torch.Tensor, scales: torch.Tensor, bf16: bool, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    return _lib.native().kv4_read(codes, scales, bf16, slots)
+    return _lib.native().kv4_read(codes, scales, bf16, slots, True)
 
 
 @_read_op.register_fake

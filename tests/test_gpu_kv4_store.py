@@ -143,3 +143,29 @@ def test_a_cache_past_4_gib(device):
     ko, vo = kv4.read(cache, slots.to(device))
     _same(ko, orc.rounded(k))
     _same(vo, orc.rounded(v))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+def test_runs_of_slots(D, dtype, device):
+    """Slots in a row from every alignment, ends inside a group of four, a gap and a repeat-free reversal."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    g = torch.Generator().manual_seed(D)
+    runs = [list(range(a, a + n)) for a, n in [(0, 1), (4, 9), (17, 4), (23, 6), (31, 3), (64, 33), (101, 2)]]
+    runs += [[104, 105, -1, 107, 108, 109, 110, 111], [115, 114, 113, 112], [120, 121, 122, -1]]
+    cache = kv4.allocate(2, 3, D, 64, dtype, device)
+    cache.codes.fill_(255)
+    cache.scales.fill_(255)
+    for run in runs:
+        k, v = (torch.randn(1, 3, len(run), D, generator=g).to(dtype) for _ in range(2))
+        slots = torch.tensor(run, device=device)
+        kv4.write(cache, k.to(device), v.to(device), slots)
+        dead = torch.tensor(run) < 0
+        for got, x in zip(kv4.read(cache, slots), (k, v)):
+            want = orc.rounded(x)
+            want[:, :, dead] = 0
+            _same(got, want)
+    untouched = torch.tensor([3, 13, 16, 21, 22, 29, 34, 63, 97, 103, 106, 123], device=device)
+    for got in kv4.read(cache, untouched):
+        assert torch.isnan(got).all()
