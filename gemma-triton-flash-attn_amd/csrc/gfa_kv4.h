@@ -31,6 +31,32 @@ struct Kv4Range {
 };
 constexpr int kKv4Nan = 255;  // scale byte of a block that holds an infinity or a NaN
 
+// Division by a number that the host knows: x / d = x m >> s for x below 2^31 (m = ceil(2^s / d), s = 31 + ceil(log2 d),
+// after Granlund and Montgomery). A division by a kernel argument takes some twenty instructions, and the short calls
+// are made of little else.
+struct Div {
+  unsigned m, s, d;
+  __host__ void set(unsigned divisor) {
+    unsigned log2 = 0;
+    while ((1ull << log2) < divisor) ++log2;
+    d = divisor;
+    s = 31 + log2;
+    m = (unsigned)(((1ull << s) + divisor - 1) / divisor);
+  }
+  __device__ __forceinline__ int quot(int x) const { return (int)(((uint64_t)(unsigned)x * m) >> s); }
+  __device__ __forceinline__ int rem(int x) const { return x - quot(x) * (int)d; }
+};
+
+// x / d for 0 <= x < 2^31 and d > 0 known on the device alone: a float's quotient, off by at most one where the result is below
+// 2^22, put right.
+__device__ __forceinline__ int quotient(int x, int d) {
+  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
+  const int r = x - q * d;
+  q += r >= d;
+  q -= r < 0;
+  return q;
+}
+
 struct Kv4Cache {
   uint8_t* codes;   // (num_blocks, Hkv, 2, block_size, D / 2)
   uint8_t* scales;  // (num_blocks, Hkv, 2, block_size, D / 32)
@@ -96,7 +122,8 @@ struct Kv4RowsParams {
   uint16_t *ko, *vo;      // read
   int64_t ksb, ksh, ksn, vsb, vsh, vsn;
   const int64_t* slots;   // (T,), T = rows * N
-  int N, T;
+  int T;
+  Div n, hkv;  // N, Hkv
 };
 
 struct Kv4PlanParams {
@@ -120,7 +147,9 @@ struct Kv4AttnParams {
   const uint16_t* q;
   uint16_t* o;
   int64_t qsb, qsh, qsn, osb, osh, osn;
-  int N, T;  // tokens per batch row of q and o, and altogether
+  int T;       // tokens of q
+  Div n, g, hkv;  // tokens per batch row of q and o, query heads per KV head, KV heads
+  int each;    // without cu: new tokens of a request
   const int *table, *lens, *cu;
   int64_t table_stride;
   int B, M, Hq, G;

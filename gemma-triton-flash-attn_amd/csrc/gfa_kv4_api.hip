@@ -72,7 +72,8 @@ int rows_call(const gfa_kv4_rows_args* a, bool write) {
   p.vsh = a->v_strides.head;
   p.vsn = a->v_strides.row;
   p.slots = a->slots;
-  p.N = a->seq_len;
+  p.n.set(a->seq_len);
+  p.hkv.set(a->cache.heads_kv);
   p.T = (int)tokens;
   const auto stream = static_cast<hipStream_t>(a->stream);
   const bool bf16 = a->cache.dtype == GFA_DTYPE_BF16;
@@ -268,8 +269,11 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   p.osb = a->o_strides.batch;
   p.osh = a->o_strides.head;
   p.osn = a->o_strides.row;
-  p.N = a->seq_len;
   p.T = a->batch * a->seq_len;
+  p.n.set(a->seq_len);
+  p.hkv.set(a->cache.heads_kv);
+  p.g.set(a->heads_q / a->cache.heads_kv);
+  p.each = p.T / a->requests;
   p.table = a->table;
   p.lens = a->lens;
   p.cu = a->cu;

@@ -64,9 +64,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c16 = lane & 15;
-  const int head = (int)blockIdx.x % p.cache.Hkv;
+  const int head = p.hkv.rem((int)blockIdx.x);
 
-  const Item it = find_item<kRows, false>(p, (int)blockIdx.x / p.cache.Hkv, lane);
+  const Item it = find_item<kRows, false>(p, p.hkv.quot((int)blockIdx.x), lane);
   const Request& rq = it.rq;
   if (it.b < 0) {
     // No item: tokens behind the last request's are zeros, the workgroups without an item take them in turn.
@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
     for (int64_t i = extra * blockDim.x + threadIdx.x; i < pieces; i += n_extra * blockDim.x) {
       const int64_t hd = i / (D / 8);
       const int t = (int)(n0 + hd / p.Hq);
-      uint16_t* at = p.o + (t / p.N) * p.osb + hd % p.Hq * p.osh + (t % p.N) * p.osn + i % (D / 8) * 8;
+      uint16_t* at = p.o + p.n.quot(t) * p.osb + hd % p.Hq * p.osh + p.n.rem(t) * p.osn + i % (D / 8) * 8;
       *reinterpret_cast<i16x8*>(at) = i16x8{};
     }
     return;
@@ -87,8 +87,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   // ---- the chunk's tiles ----
   const int per = chunk_len(rq, it.nch);
   const int2 tiles = tiles_of_rows(p, rq, it.rb * kRows, kRows);
-  const int t_first = tiles.x + it.ch * per;
-  const int t_end = min(tiles.y, t_first + per);
+  const int t_first = __builtin_amdgcn_readfirstlane(tiles.x + it.ch * per);
+  const int t_end = __builtin_amdgcn_readfirstlane(min(tiles.y, t_first + per));
   const int tpb_log2 = p.cache.bs_log2 - 5;
   const int* table = p.table + (int64_t)it.b * p.table_stride;
   auto block_of = [&](int tile) __attribute__((always_inline)) { return table_entry(table, min(tile, t_end - 1) >> tpb_log2); };
@@ -99,8 +99,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
 
   // ---- this lane's row: token, head, visible keys ----
   const int row = it.rb * kRows + c16;
-  const int i = row / p.G;
-  const int qh = head * p.G + row % p.G;
+  const int i = p.g.quot(row);
+  const int qh = head * p.G + p.g.rem(row);
   const int t = rq.t0 + i;
   const bool live = i < rq.fresh && t >= 0 && t < p.T;
   const int pos = rq.len - rq.fresh + i;
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   i16x8 qf[KT];
   {
     const int tc = live ? t : 0;  // rows past the last read another's query; nothing of theirs goes out
-    const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)qh * p.qsh + (tc % p.N) * p.qsn;
+    const uint16_t* qp = p.q + p.n.quot(tc) * p.qsb + (int64_t)qh * p.qsh + p.n.rem(tc) * p.qsn;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   if (!live) return;
   const bool none = m_all == -INFINITY && l_all == 0.f;
   const float inv = row_inv(m_all, l_all);
-  uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn + d0;
+  uint16_t* op = p.o + p.n.quot(t) * p.osb + (int64_t)qh * p.osh + p.n.rem(t) * p.osn + d0;
   typedef short vec __attribute__((ext_vector_type(XW)));
 #pragma unroll
   for (int r = 0; r < 4; ++r) {

@@ -94,9 +94,9 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = lane >> 5;
-  const int head = (int)blockIdx.x % p.cache.Hkv;
+  const int head = p.hkv.rem((int)blockIdx.x);
 
-  const Item it = find_item<ROWS, true>(p, (int)blockIdx.x / p.cache.Hkv, lane);
+  const Item it = find_item<ROWS, true>(p, p.hkv.quot((int)blockIdx.x), lane);
   if (it.b < 0) return;
   const Request& rq = it.rq;
   const int rb = rq.row_blocks - 1 - it.rb;  // the rows that see most keys first
@@ -107,8 +107,8 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   const int pos0 = rq.len - rq.fresh;  // position of new token 0
   const int2 tiles = tiles_of_rows(p, rq, row0, ROWS);
   const int per = chunk_len(rq, it.nch);
-  const int t_first = tiles.x + it.ch * per;
-  const int t_end = max(t_first, min(tiles.y, t_first + per));
+  const int t_first = __builtin_amdgcn_readfirstlane(tiles.x + it.ch * per);
+  const int t_end = __builtin_amdgcn_readfirstlane(max(t_first, min(tiles.y, t_first + per)));
 
   // ---- this lane's rows ----
   // A row's token and query head; taken again for the stores rather than held through the loop.
@@ -119,9 +119,9 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   auto row_of = [&](int m, int ln) __attribute__((always_inline)) {
     const int row = row0 + (wave * MT + m) * 32 + (ln & 31);
     Row r;
-    r.i = row / p.G;
+    r.i = p.g.quot(row);
     r.t = rq.t0 + r.i;
-    r.qh = head * p.G + row % p.G;
+    r.qh = head * p.G + p.g.rem(row);
     r.live = r.i < rq.fresh && r.t >= 0 && r.t < p.T;
     return r;
   };
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
     const int last = r.live ? min(p.causal ? pos : rq.len - 1, held - 1) : -1;
     vis[m] = make_range(p.causal && p.window > 0 ? max(pos - p.window + 1, 0) : 0, last);
     const int tc = r.live ? r.t : 0;  // rows past the last read another's query; nothing of theirs goes out
-    const uint16_t* qp = p.q + (tc / p.N) * p.qsb + (int64_t)r.qh * p.qsh + (tc % p.N) * p.qsn;
+    const uint16_t* qp = p.q + p.n.quot(tc) * p.qsb + (int64_t)r.qh * p.qsh + p.n.rem(tc) * p.qsn;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
 #pragma unroll
@@ -148,10 +148,13 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   }
   if (p.causal) {
     const int first = row0 + wave * MT * 32;
-    all_hi = min(all_hi, pos0 + first / p.G + 1);
-    if (p.window > 0) all_lo = pos0 + (first + MT * 32 - 1) / p.G - p.window + 1;
+    all_hi = min(all_hi, pos0 + p.g.quot(first) + 1);
+    if (p.window > 0) all_lo = pos0 + p.g.quot(first + MT * 32 - 1) - p.window + 1;
   }
 
+  // the wave's, in scalar registers: what the compiler divides it keeps in vector ones
+  all_lo = __builtin_amdgcn_readfirstlane(all_lo);
+  all_hi = __builtin_amdgcn_readfirstlane(all_hi);
   f32x16 acc[MT][CPL];
   float m_ref[MT], l_run[MT];
   bool seen[MT];
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
     if (!r0.live) continue;
     const bool none = m_ref[m] == -INFINITY && l == 0.f;
     const float inv = row_inv(m_ref[m], l);
-    uint16_t* op = p.o + (r0.t / p.N) * p.osb + (int64_t)r0.qh * p.osh + (r0.t % p.N) * p.osn;
+    uint16_t* op = p.o + p.n.quot(r0.t) * p.osb + (int64_t)r0.qh * p.osh + p.n.rem(r0.t) * p.osn;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int idx = 8 * (r >> 2) + 4 * ho + (r & 3);

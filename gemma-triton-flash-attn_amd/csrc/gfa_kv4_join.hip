@@ -21,8 +21,8 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   __shared__ float ml_lds[kTpb / 16][2];
   const int lane = threadIdx.x & 63;
   int id = (int)blockIdx.x;
-  const int head = id % p.cache.Hkv;
-  id /= p.cache.Hkv;
+  const int head = p.hkv.rem(id);
+  id = p.hkv.quot(id);
   const int slice = id % (D / p.join_slice);
   id /= D / p.join_slice;
   const RowBlock blk = find_row_block<ROWS, false>(p, id / p.join_rows, lane);
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   for (int r0 = id % p.join_rows * at_once; r0 < rows; r0 += p.join_rows * at_once) {
     const int rr = r0 + group / parts;
     const int row = rb * ROWS + rr;
-    const int t = blk.rq.t0 + row / p.G, qh = head * p.G + row % p.G;
+    const int t = blk.rq.t0 + p.g.quot(row), qh = head * p.G + p.g.rem(row);
     const bool live = rr < rows && t >= 0 && t < p.T;
     float m = -INFINITY, l = 0.f;  // without a maximum l counts the rows' marks, see row_inv
     f32x4 o{};
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
     if (part == 0 && live) {
       const bool none = m == -INFINITY && l == 0.f;
       const float inv = row_inv(m, l);
-      uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn + d;
+      uint16_t* op = p.o + p.n.quot(t) * p.osb + (int64_t)qh * p.osh + p.n.rem(t) * p.osn + d;
       i16x4 v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = to16<IS_BF16>(none ? 0.f : o[e] * inv);
@@ -82,8 +82,8 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
   constexpr int RUNS = ROWS / 32 * 16 * (CPL / W);
   const int lane = threadIdx.x & 63;
   int id = (int)blockIdx.x;
-  const int head = id % p.cache.Hkv;
-  id /= p.cache.Hkv;
+  const int head = p.hkv.rem(id);
+  id = p.hkv.quot(id);
   const RowBlock blk = find_row_block<ROWS, true>(p, id / p.join_rows, lane);
   if (blk.b < 0 || blk.nch == 1) return;
   if ((int64_t)(blk.item + blk.nch) * p.cache.Hkv > p.nblocks) return;  // cu that is no prefix sum: no such chunks
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
   for (int run = id % p.join_rows * (kTpb / 64) + (threadIdx.x >> 6); run < RUNS; run += p.join_rows * (kTpb / 64)) {
     const int rr = run / (16 * (CPL / W)) * 32 + (lane & 31);
     const int row = rb * ROWS + rr;
-    const int t = blk.rq.t0 + row / p.G, qh = head * p.G + row % p.G;
+    const int t = blk.rq.t0 + p.g.quot(row), qh = head * p.G + p.g.rem(row);
     if (rr >= rows || t < 0 || t >= p.T) continue;
     float m = -INFINITY, l = 0.f;  // without a maximum l counts the rows' marks, see row_inv
     f32x4 o{};
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
     out v;
 #pragma unroll
     for (int e = 0; e < W; ++e) v[e] = to16<IS_BF16>(none ? 0.f : o[e] * inv);
-    uint16_t* op = p.o + (t / p.N) * p.osb + (int64_t)qh * p.osh + (t % p.N) * p.osn;
+    uint16_t* op = p.o + p.n.quot(t) * p.osb + (int64_t)qh * p.osh + p.n.rem(t) * p.osn;
     *reinterpret_cast<out*>(op + (idx & 15) * PP + CPL * (idx >> 4) + x) = v;
   }
 }

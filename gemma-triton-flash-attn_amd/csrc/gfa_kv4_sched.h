@@ -26,10 +26,9 @@ __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   const int bc = min(b, p.B - 1);
   const int* cu = p.cu != nullptr ? p.cu : p.lens;  // without cu read for nothing
   const int t0 = cu[bc], t1 = cu[p.cu != nullptr ? bc + 1 : bc], len = p.lens[bc];
-  const int each = p.T / p.B;
   if (b >= p.B) return r;
-  r.t0 = p.cu != nullptr ? t0 : b * each;
-  r.fresh = p.cu != nullptr ? min(max((int)((unsigned)t1 - (unsigned)t0), 0), p.T) : each;
+  r.t0 = p.cu != nullptr ? t0 : b * p.each;
+  r.fresh = p.cu != nullptr ? min(max((int)((unsigned)t1 - (unsigned)t0), 0), p.T) : p.each;
   r.len = max(len, 0);
   const int rows = r.fresh * p.G;
   r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
@@ -41,7 +40,7 @@ __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
 }
 // Key tiles [x, y) that some row of the request's row block of `rows` rows from row0 on sees.
 __device__ __forceinline__ int2 tiles_of_rows(const Kv4AttnParams& p, const Request& r, int row0, int rows) {
-  const int i_lo = row0 / p.G, i_hi = min((row0 + rows - 1) / p.G, r.fresh - 1);
+  const int i_lo = p.g.quot(row0), i_hi = min(p.g.quot(row0 + rows - 1), r.fresh - 1);
   const int pos0 = r.len - r.fresh;  // position of new token 0
   const int held = min(r.len, p.M << p.cache.bs_log2);
   const int k_hi = p.causal ? min(held, pos0 + i_hi + 1) : held;
@@ -85,11 +84,11 @@ __device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, const Request
     total += x;
   }
   const float each = ceilf(wave_sum(total) * p.share);
-  return max((int)fminf(each, 1.0e9f), p.min_tiles);
+  return __builtin_amdgcn_readfirstlane(max((int)fminf(each, 1.0e9f), p.min_tiles));
 }
-__device__ __forceinline__ int chunks_of(const Request& r, int per) { return max((r.tiles + per - 1) / per, 1); }
-// Chunks of one length each, not full ones and a rest: the grid's last workgroups end closer together.
-__device__ __forceinline__ int chunk_len(const Request& r, int nch) { return (r.tiles + nch - 1) / nch; }
+__device__ __forceinline__ int chunks_of(const Request& r, int per) { return max(quotient(r.tiles + per - 1, per), 1); }
+// (Of a request that is the wave's.) Chunks of one length each, not full ones and a rest: the grid's last workgroups end closer together.
+__device__ __forceinline__ int chunk_len(const Request& r, int nch) { return __builtin_amdgcn_readfirstlane(quotient(r.tiles + nch - 1, nch)); }
 
 struct Item {
   Request rq;
@@ -112,10 +111,10 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
       const int src = __builtin_ctzll(hit);
       it.b = b0 + src;
       it.rq = request_from(r, src);
-      it.nch = chunks_of(it.rq, per);
+      it.nch = __builtin_amdgcn_readfirstlane(chunks_of(it.rq, per));
       const int i = item - __builtin_amdgcn_readlane(before, src);
-      it.rb = i / it.nch;
-      it.ch = i % it.nch;
+      it.rb = __builtin_amdgcn_readfirstlane(quotient(i, it.nch));
+      it.ch = i - it.rb * it.nch;
       break;
     }
     it.items += __builtin_amdgcn_readlane(s, 63);
@@ -149,7 +148,7 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
       const int src = __builtin_ctzll(hit);
       out.b = b0 + src;
       out.rq = request_from(r, src);
-      out.nch = chunks_of(out.rq, per);
+      out.nch = __builtin_amdgcn_readfirstlane(chunks_of(out.rq, per));
       out.rb = block - __builtin_amdgcn_readlane(before, src);
       out.item = items + __builtin_amdgcn_readlane(t - mine, src) + out.rb * out.nch;
       break;

@@ -32,9 +32,9 @@ struct Place {
   bool quad;  // the four slots are one piece of V's order
   __device__ __forceinline__ Place(const Kv4RowsParams& p) {
     const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * (kTpb / 64) + (threadIdx.x >> 6);
-    head = (int)(w % p.cache.Hkv);
-    t0 = (w / p.cache.Hkv * Rows<D>::GPW + lane / Rows<D>::LPT) * 4;
+    const int w = (int)blockIdx.x * (kTpb / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    head = p.hkv.rem(w);
+    t0 = ((int64_t)p.hkv.quot(w) * Rows<D>::GPW + lane / Rows<D>::LPT) * 4;
     lane_t = lane % Rows<D>::LPT;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -109,7 +109,7 @@ __global__ __launch_bounds__(kTpb) void kv4_write_kernel(const Kv4RowsParams p) 
   for (int i = 0; i < 4; ++i) {
     kx[i] = vx[i] = i16x8{};
     if (at.slot[i] >= 0) {
-      const int row = (int)(at.t0 + i) / p.N, n = (int)(at.t0 + i) % p.N;
+      const int t = (int)at.t0 + i, row = p.n.quot(t), n = t - row * (int)p.n.d;
       kx[i] = *reinterpret_cast<const i16x8*>(p.k + row * p.ksb + at.head * p.ksh + n * p.ksn + d);
       vx[i] = *reinterpret_cast<const i16x8*>(p.v + row * p.vsb + at.head * p.vsh + n * p.vsn + d);
     }
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kTpb) void kv4_read_kernel(const Kv4RowsParams p) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (at.t0 + i >= p.T) continue;
-    const int row = (int)(at.t0 + i) / p.N, n = (int)(at.t0 + i) % p.N;
+    const int t = (int)at.t0 + i, row = p.n.quot(t), n = t - row * (int)p.n.d;
     // read once by whoever asked: past the caches
     __builtin_nontemporal_store(kv4_decode8<IS_BF16>(kc[i], ks[i]), reinterpret_cast<i16x8*>(p.ko + row * p.ksb + at.head * p.ksh + n * p.ksn + d));
     __builtin_nontemporal_store(kv4_decode8<IS_BF16>(vc[i], (int)(vs4 >> (8 * i) & 255)), reinterpret_cast<i16x8*>(p.vo + row * p.vsb + at.head * p.vsh + n * p.vsn + d));
