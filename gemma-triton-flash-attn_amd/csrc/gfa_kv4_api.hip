@@ -96,6 +96,7 @@ struct Part {
 };
 struct Split {
   int row_limit;  // requests of more query rows (new tokens times heads of a KV head) take the chunk kernel
+  bool one_block;  // as far as max_new says, no request has more than one row block
   Part few, many;
 };
 
@@ -144,6 +145,7 @@ Split split_of(const gfa_kv4_attn_args* a) {
   const int64_t T = (int64_t)a->batch * a->seq_len;
   const int64_t most = a->cu == nullptr ? T / R : a->max_new > 0 ? std::min<int64_t>(a->max_new, T) : T;
   // No request can have more rows than the limit: then all are the split kernel's, whatever max_new promised.
+  s.one_block = most * G <= kRows;
   const int limit = row_limit(a);
   s.row_limit = most * G <= limit ? 0x7fffffff : limit;
   const int D = a->cache.head_dim, big = gfa::kv4_chunk_rows(D);
@@ -306,7 +308,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);
     ws += part.bytes();
-    hipError_t err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, stream) : gfa::launch_kv4_split(p, D, bf16, cap, stream);
+    hipError_t err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, stream) : gfa::launch_kv4_split(p, D, bf16, cap, s.one_block, stream);
     if (err == hipSuccess && part.join) err = gfa::launch_kv4_join(p, D, bf16, large, stream);
     if (err != hipSuccess) return launched(err, "cache attention");
   }

@@ -40,6 +40,14 @@ constexpr int kRows = kSplitRows;
 constexpr int kWaves = 4;
 constexpr float kMargin = 8.0f;  // log2
 
+// 16 bytes of codes; ONCE: non-temporal, for tiles that no other workgroup reads.
+template <bool ONCE>
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  typedef unsigned vec __attribute__((ext_vector_type(4)));
+  if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const vec*>(p)));
+  return *reinterpret_cast<const uint4*>(p);
+}
+
 // What a lane holds of a 32-token tile.
 template <int D>
 struct TileRegs {
@@ -52,7 +60,7 @@ struct TileRegs {
 
 }  // namespace
 
-template <int D, bool IS_BF16, bool CAP>
+template <int D, bool IS_BF16, bool CAP, bool ONCE>
 __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kernel(const Kv4AttnParams p) {
   using L = Kv4Layout<D>;
   constexpr int KT = D / 32;   // products of a score block
@@ -153,7 +161,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
         r.ks[hh] = ks[tok * 2 + (g >> 1)];
       } else {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) r.k[hh * NJ + j] = *reinterpret_cast<const uint4*>(kc + j * 2048 + tok * 64 + g * 16);
+        for (int j = 0; j < NJ; ++j) r.k[hh * NJ + j] = load16<ONCE>(kc + j * 2048 + tok * 64 + g * 16);
         const uint8_t* sp = ks + tok * L::SC + g * NJ;
         if constexpr (NJ == 4) {
           r.ks[hh] = *reinterpret_cast<const unsigned*>(sp);
@@ -165,7 +173,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
       }
     }
 #pragma unroll
-    for (int j = 0; j < (D == 64 ? 1 : 2 * NJ); ++j) r.v[j] = *reinterpret_cast<const uint4*>(vc + j * 1024 + lane * 16);
+    for (int j = 0; j < (D == 64 ? 1 : 2 * NJ); ++j) r.v[j] = load16<ONCE>(vc + j * 1024 + lane * 16);
     r.vs = *reinterpret_cast<const uint2*>(vs + (g * L::SC + c16 * L::PP / 32) * 8);
   };
 
@@ -365,11 +373,18 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   }
 }
 
-hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, hipStream_t stream) {
+// Codes are loaded non-temporally: 64 requests at 16k, 32:8 D = 128, 170 -> 153 us, 16:8 D = 256 112 -> 98. At D = 512 only
+// where a request's rows are one row block (99 -> 95 us; two, which share tiles in L2, 96 -> 107).
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, bool once, hipStream_t stream) {
   auto go = [&](auto d, auto b, auto c) {
     constexpr int DD = decltype(d)::value;
     constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;
-    hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC>), dim3((unsigned)p.nblocks), dim3(kWaves * 64), 0, stream, p);
+    const dim3 grid((unsigned)p.nblocks), wg(kWaves * 64);
+    if (DD < 512 || once) {
+      hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC, true>), grid, wg, 0, stream, p);
+    } else {
+      hipLaunchKernelGGL((kv4_split_kernel<512, BB, CC, false>), grid, wg, 0, stream, p);
+    }
   };
   auto by_type = [&](auto d) {
     if (bf16 && cap) go(d, std::true_type{}, std::true_type{});

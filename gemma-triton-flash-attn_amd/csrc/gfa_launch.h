@@ -27,7 +27,7 @@ hipError_t launch_bwd_dq_ds(const BwdDqDsParams& p, int head_dim, bool bf16, hip
 hipError_t launch_kv4_write(const Kv4RowsParams& p, int head_dim, bool bf16, hipStream_t stream);
 hipError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, bool bf16, hipStream_t stream);
 hipError_t launch_kv4_plan(const Kv4PlanParams& p, hipStream_t stream);
-hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, hipStream_t stream);
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, bool once, hipStream_t stream);
 hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, hipStream_t stream);
 hipError_t launch_kv4_join(const Kv4AttnParams& p, int head_dim, bool bf16, bool large, hipStream_t stream);
 
