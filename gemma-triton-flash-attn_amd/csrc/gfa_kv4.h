@@ -160,10 +160,11 @@ struct Kv4AttnParams {
   int min_tiles;  // work split, see chunk_tiles in gfa_kv4_sched.h
   float share;
   int nblocks;    // workgroups of the split or chunk grid
+  int slots;      // of a split row block's chunk, per KV head (more only for a cu that is no prefix sum: left out)
   int row_limit;  // requests with more query rows than this belong to the chunk kernel
   // the join grid: most row blocks, workgroups for the rows of one, channels of each, groups of lanes that share a row
   int row_blocks, join_rows, join_slice, join_parts;
-  float* part;    // (nblocks, rows, D) sums and (nblocks, rows, 2) row maxima and sums
+  float* part;    // (slots, Hkv, rows, D) sums and (slots, Hkv, rows, 2) row maxima and sums
   float* part_ml;
 };
 

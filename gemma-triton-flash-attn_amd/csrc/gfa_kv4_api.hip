@@ -88,7 +88,7 @@ struct Part {
   bool runs;
   int min_tiles;
   float share;
-  int64_t nblocks, row_blocks;
+  int64_t nblocks, row_blocks, slots;
   int join_rows, join_slice, join_parts, window_tiles;
   bool join;  // some row block may take more than one chunk
   size_t part_bytes, ml_bytes;
@@ -134,8 +134,9 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
   s.nblocks = items * hkv + spare;
   if (s.join) {
-    s.part_bytes = (size_t)s.nblocks * rows * a->cache.head_dim * sizeof(float);
-    s.ml_bytes = (size_t)s.nblocks * rows * 2 * sizeof(float);
+    s.slots = std::min(row_blocks * chunks, 2 * target / hkv + 1);
+    s.part_bytes = (size_t)(s.slots * hkv) * rows * a->cache.head_dim * sizeof(float);
+    s.ml_bytes = (size_t)(s.slots * hkv) * rows * 2 * sizeof(float);
   }
 }
 
@@ -305,6 +306,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     p.join_slice = part.join_slice;
     p.join_parts = part.join_parts;
     p.nblocks = (int)part.nblocks;
+    p.slots = (int)part.slots;
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);
     ws += part.bytes();

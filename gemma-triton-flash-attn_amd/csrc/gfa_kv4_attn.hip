@@ -342,7 +342,8 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
 
   const int d0 = 4 * g * L::PP + wave * XW;
   if (it.nch > 1) {
-    const int64_t at = (int64_t)blockIdx.x * kRows + c16;
+    if ((unsigned)it.slot >= (unsigned)p.slots) return;
+    const int64_t at = ((int64_t)it.slot * p.cache.Hkv + head) * kRows + c16;
     if (live) {
       typedef float vec __attribute__((ext_vector_type(XW)));
 #pragma unroll

@@ -413,6 +413,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   // ---- rows out ----
   const int ln = fresh_lane();
   const int ho = ln >> 5;
+  const int64_t part_at = (int64_t)it.slot * p.cache.Hkv + head;
   constexpr int W = CPL < 4 ? CPL : 4;  // neighbouring channels stored at once
 #pragma unroll
   for (int m = 0; m < MT; ++m) {
@@ -420,14 +421,15 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
     float l = halves_sum(l_run[m]);
     if (m_ref[m] == -INFINITY && l == 0.f && seen[m]) l = 1.f;  // a mark, see row_inv
     if (it.nch > 1) {
-      const int64_t at = (int64_t)blockIdx.x * ROWS + (wave * MT + m) * 32 + (ln & 31);
+      if ((unsigned)it.slot >= (unsigned)p.slots) return;
+      const int64_t at = part_at * ROWS + (wave * MT + m) * 32 + (ln & 31);
       if (ho == 0) {
         p.part_ml[at * 2] = m_ref[m];
         p.part_ml[at * 2 + 1] = l;
       }
       if (t_first < t_end) {
         // in the order the lanes hold them, whole 1 KB runs (kv4_join_large_kernel): by rows a store would touch 64 of them
-        float* part = p.part + ((int64_t)blockIdx.x * ROWS + (wave * MT + m) * 32) * D + ln * W;
+        float* part = p.part + (part_at * ROWS + (wave * MT + m) * 32) * D + ln * W;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
 #pragma unroll

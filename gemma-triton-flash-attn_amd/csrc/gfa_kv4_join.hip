@@ -27,7 +27,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   id /= D / p.join_slice;
   const RowBlock blk = find_row_block<ROWS, false>(p, id / p.join_rows, lane);
   if (blk.b < 0 || blk.nch == 1) return;
-  if ((int64_t)(blk.item + blk.nch) * p.cache.Hkv > p.nblocks) return;  // cu that is no prefix sum: no such chunks
+  if (blk.slot < 0 || (int64_t)blk.slot + blk.nch > p.slots) return;  // cu that is no prefix sum: no such chunks
   const int rb = blk.rb;
   const int rows = min(ROWS, blk.rq.fresh * p.G - rb * ROWS);
   const int parts = min(p.join_parts, 1 << (32 - __builtin_clz(blk.nch - 1)));
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
     if (live) {
 #pragma unroll 8
       for (int c = part; c < blk.nch; c += parts) {
-        const int64_t at = ((int64_t)(blk.item + c) * p.cache.Hkv + head) * ROWS + rr;
+        const int64_t at = (((int64_t)blk.slot + c) * p.cache.Hkv + head) * ROWS + rr;
         const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
         const f32x4 v = *reinterpret_cast<const f32x4*>(p.part + at * D + d);
         join_rows(m, l, o, ml.x, ml.y, v);
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
   id = p.hkv.quot(id);
   const RowBlock blk = find_row_block<ROWS, true>(p, id / p.join_rows, lane);
   if (blk.b < 0 || blk.nch == 1) return;
-  if ((int64_t)(blk.item + blk.nch) * p.cache.Hkv > p.nblocks) return;  // cu that is no prefix sum: no such chunks
+  if (blk.slot < 0 || (int64_t)blk.slot + blk.nch > p.slots) return;  // cu that is no prefix sum: no such chunks
   const int rb = blk.rq.row_blocks - 1 - blk.rb;                        // the chunk kernel takes the last rows first
   const int rows = min(ROWS, blk.rq.fresh * p.G - rb * ROWS);
   typedef float vec __attribute__((ext_vector_type(W)));
@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
     f32x4 o{};
 #pragma unroll 8
     for (int c = 0; c < blk.nch; ++c) {
-      const int64_t item = (int64_t)(blk.item + c) * p.cache.Hkv + head;
+      const int64_t item = ((int64_t)blk.slot + c) * p.cache.Hkv + head;
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + (item * ROWS + rr) * 2);
       const vec v = *reinterpret_cast<const vec*>(p.part + item * (ROWS * D) + run * (64 * W) + lane * W);
       f32x4 v4{};

@@ -2,7 +2,9 @@
 // on the device from the requests' lengths, the same in every wave of every kernel of the call.
 //
 // The rows of a request and KV head are the G query heads of each of its new tokens, row r = token r / G, head r % G.
-// An item is a row block of ROWS of them and a chunk of the key tiles they see. Requests of up to
+// An item is a row block of ROWS of them and a chunk of the key tiles they see. A row block of several chunks leaves
+// their sums in slots of the workspace: a request is split where it has more than `per` tiles, so into fewer than
+// 2 tiles / per chunks, and with per at least the call's tiles / target there are fewer than 2 target slots. Requests of up to
 // row_limit rows are the split kernel's, the others the chunk kernel's (LARGE).
 #pragma once
 #include <type_traits>
@@ -95,6 +97,7 @@ struct Item {
   int b;            // -1: there is no such item
   int rb, ch, nch;  // row block, chunk of nch
   int items;        // of the whole call, where b < 0
+  int slot;         // of nch > 1: its place among the items of split row blocks
 };
 template <int ROWS, bool LARGE>
 __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int lane) {
@@ -103,8 +106,9 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
   Request r = request_of<ROWS, LARGE>(p, lane);
   const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
   for (int b0 = 0;;) {
-    const int mine = r.row_blocks * chunks_of(r, per);
-    const int s = wave_prefix_sum(mine);
+    const int nch = chunks_of(r, per);
+    const int mine = r.row_blocks * nch, split = nch > 1 ? mine : 0;
+    const int s = wave_prefix_sum(mine), z = wave_prefix_sum(split);
     const int before = it.items + s - mine;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
     if (hit != 0) {
@@ -115,21 +119,23 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
       const int i = item - __builtin_amdgcn_readlane(before, src);
       it.rb = __builtin_amdgcn_readfirstlane(quotient(i, it.nch));
       it.ch = i - it.rb * it.nch;
+      it.slot += __builtin_amdgcn_readlane(z - split, src) + i;
       break;
     }
     it.items += __builtin_amdgcn_readlane(s, 63);
+    it.slot += __builtin_amdgcn_readlane(z, 63);
     if ((b0 += 64) >= p.B) break;
     r = request_of<ROWS, LARGE>(p, b0 + lane);
   }
   return it;
 }
 
-// Row block `block` of the call, counted through the requests: rq, b, rb, nch, and the first chunk's item.
+// Row block `block` of the call, counted through the requests: rq, b, rb, nch, and the first chunk's slot.
 struct RowBlock {
   Request rq;
   int b;           // -1: there is no such row block
   int rb, nch;
-  int item;
+  int slot;
 };
 template <int ROWS, bool LARGE>
 __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int block, int lane) {
@@ -137,11 +143,11 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
   out.b = -1;
   Request r = request_of<ROWS, LARGE>(p, lane);
   const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
-  int blocks = 0, items = 0;
+  int blocks = 0;
   for (int b0 = 0;;) {
     const int s = wave_prefix_sum(r.row_blocks);
-    const int mine = r.row_blocks * chunks_of(r, per);
-    const int t = wave_prefix_sum(mine);
+    const int nch = chunks_of(r, per), split = nch > 1 ? r.row_blocks * nch : 0;
+    const int z = wave_prefix_sum(split);
     const int before = blocks + s - r.row_blocks;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(block >= before && block < before + r.row_blocks);
     if (hit != 0) {
@@ -150,11 +156,11 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
       out.rq = request_from(r, src);
       out.nch = __builtin_amdgcn_readfirstlane(chunks_of(out.rq, per));
       out.rb = block - __builtin_amdgcn_readlane(before, src);
-      out.item = items + __builtin_amdgcn_readlane(t - mine, src) + out.rb * out.nch;
+      out.slot += __builtin_amdgcn_readlane(z - split, src) + out.rb * out.nch;
       break;
     }
     blocks += __builtin_amdgcn_readlane(s, 63);
-    items += __builtin_amdgcn_readlane(t, 63);
+    out.slot += __builtin_amdgcn_readlane(z, 63);
     if ((b0 += 64) >= p.B) break;
     r = request_of<ROWS, LARGE>(p, b0 + lane);
   }

@@ -168,3 +168,44 @@ def test_a_cache_past_4_gib(device):
     big.scales[shift:shift + r.cache.num_blocks] = r.cache.scales
     o = kv4.attention(r.q.to(device), big, torch.where(r.table >= 0, r.table + shift, -1), r.lens_dev, r.cu)
     assert torch.equal(o, r.attend())
+
+
+def test_max_new_only_chooses_kernels(device):
+    """Too small, too large or none: the same rows within the roundings, nothing left out."""
+    r = Requests(device, [400, 260, 700, 33], [150, 3, 40, 1], 8, 2, 128, pad=2).store()
+    want, bound = r.expected()
+    for most in (1, 2, 150, 1 << 20, None):
+        check(r.attend(max_new=most), want, bound)
+
+
+def test_offsets_that_are_no_prefix_sums(device):
+    """cu, lens and tables of any content keep the call inside its arrays: other requests' rows stay right."""
+    r = Requests(device, [3000, 90, 260], [2, 1, 5], 8, 2, 128, pad=2).store()
+    want = r.attend()
+    good = r.cu.clone()
+    big = 2 ** 31 - 1
+    for cu in ([0, big, 3, 8], [0, 2, -5, 8], [-big, big, 3, 8], [5, 0, 3, 8], [big] * 4, [0, 2, 3, -1]):
+        r.cu.copy_(torch.tensor(cu, dtype=torch.int32))
+        r.attend()
+        r.attend(slide_size=50, max_new=1)
+    r.cu.copy_(good)
+    lens = r.lens_dev.clone()
+    r.lens_dev.copy_(torch.tensor([big, -big, 4], dtype=torch.int32))
+    r.attend()
+    r.attend(causal=False)
+    r.lens_dev.copy_(lens)
+    table = r.table.clone()
+    r.table.fill_(big)
+    assert not r.attend().any()
+    r.table.copy_(table)
+    assert torch.equal(r.attend(), want)
+
+
+def test_ragged_splits_of_chunks(device):
+    """Prompt chunks of unequal lengths that are split over their keys, beside single tokens over a long axis."""
+    for D, Hq, Hkv in ((512, 8, 1), (256, 4, 2), (64, 2, 2)):
+        r = Requests(device, [2100, 900, 1500, 40, 3000], [70, 300, 1, 2, 1], Hq, Hkv, D, 64, pad=3, seed=D).store()
+        a, b = r.attend(), r.attend()
+        assert torch.equal(a, b)
+        check(a, *r.expected())
+        check(r.attend(slide_size=600), *r.expected(window=600))

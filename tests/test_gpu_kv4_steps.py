@@ -244,3 +244,15 @@ def test_the_prompt_through_the_forward_kernel(device):
     want, bound = r.expected(window=100)
     check(r.attend(slide_size=100), want, bound)
     check(o, want, bound)
+
+
+def test_inference_mode(device):
+    r = Requests(device, [50, 90], [2, 1], 4, 2, 64, pad=1).store()
+    want = r.attend()
+    with torch.inference_mode():
+        assert torch.equal(r.attend(), want)
+        s = Server(device, 2, LAYERS)
+        rows = s.rows(45)
+        outs = s.step([40, 3], rows, 45)
+        assert s.lens.is_inference() and outs[0].is_inference()
+    s.check([40, 3], rows, outs)

@@ -1,5 +1,5 @@
 """The key/value cache in 4 bits without a GPU: the oracle's own rules, refusals before any launch, the C layout, and that the
-grid the host sizes holds every work item of any lengths."""
+workspace the host sizes holds the partial sums of any lengths."""
 from __future__ import annotations
 
 import ctypes
@@ -230,7 +230,8 @@ def test_other_refusals():
 # ---- the work split ----
 
 def _items(lens, new, G, Hkv, rows, target, window, min_tiles):
-    """Work items of one kernel for these requests, as the device counts them (gfa_kv4_sched.h)."""
+    """(work items, those of split row blocks) of one kernel for these requests, as the device counts them
+    (gfa_kv4_sched.h)."""
     f32 = np.float32
     blocks, tiles = [], []
     for n, k in zip(lens, new):
@@ -245,12 +246,13 @@ def _items(lens, new, G, Hkv, rows, target, window, min_tiles):
         total = f32(total + f32(f32(b) * f32(t)))
     share = f32(Hkv / target * (1.0 + 1.0 / 4096))
     per = max(int(min(math.ceil(f32(total * share)), 1e9)), min_tiles)
-    return sum(b * max(1, -(-t // per)) for b, t in zip(blocks, tiles)), max(tiles)
+    counts = [(b, max(1, -(-t // per))) for b, t in zip(blocks, tiles)]
+    return sum(b * n for b, n in counts), sum(b * n for b, n in counts if n > 1)
 
 
 @pytest.mark.parametrize("seed", range(40))
-def test_the_grid_holds_every_item(seed):
-    """Requests of one token count: all are one kernel's, whose workgroups the workspace counts."""
+def test_the_workspace_holds_every_part(seed):
+    """Requests of one token count: all are one kernel's, whose slots the workspace counts; and the grid's bound."""
     rng = random.Random(seed)
     lib = _lib.load()
     D, G, Hkv = rng.choice([64, 128, 256, 512]), rng.choice([1, 2, 3, 8, 16]), rng.choice([1, 2, 4, 8])
@@ -268,12 +270,13 @@ def test_the_grid_holds_every_item(seed):
     target = 256 * {512: 1, 256: 2, 128: 3, 64: 2}[D] if large else 512
     alone = R * -(-n * G // rows) * Hkv
     min_tiles = (64 if alone >= 256 else 32 if alone >= 128 else 8) if large else 8
-    items, most = _items(lens, [n] * R, G, Hkv, rows, target, window, min_tiles)
+    items, parts = _items(lens, [n] * R, G, Hkv, rows, target, window, min_tiles)
     if need == 0:  # one chunk each
         assert width * 2 <= max(16, min_tiles) or window
         return
     groups, rest = divmod(need, rows * (D + 2) * 4)
-    assert rest == 0 and items * Hkv <= groups
+    assert rest == 0 and groups % Hkv == 0 and parts <= groups // Hkv <= 2 * target // Hkv + 1
+    assert items <= R * -(-n * G // rows) + -(-target // Hkv)
 
 
 def test_workspace_follows_the_call():
