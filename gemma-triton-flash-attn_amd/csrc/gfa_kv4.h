@@ -109,6 +109,27 @@ __device__ __forceinline__ unsigned kv4_pair(unsigned codes, float scale) {
   }
 }
 
+// c + the sum of a row's rounded weights in p (32 bits). The weights that multiply V then add up to the sum that divides them:
+// what rounding does to a row's largest weight drops out (rms error of one token over 333 keys 0.0024 of the
+// result with the unrounded sum, 0.0017 with this one, which rounding the result alone gives).
+template <bool IS_BF16>
+__device__ __forceinline__ float kv4_add_weights(const i16x8& p, float c) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 w = __builtin_bit_cast(u32x4, p);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned two = w[i];  // a copy: the compiler's bit cast of a vector's element takes element 0
+    if constexpr (IS_BF16) {
+      typedef __bf16 pair __attribute__((ext_vector_type(2)));
+      c = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, two), pair{(__bf16)1.0f, (__bf16)1.0f}, c, false);
+    } else {
+      typedef _Float16 pair __attribute__((ext_vector_type(2)));
+      c = __builtin_amdgcn_fdot2(__builtin_bit_cast(pair, two), pair{(_Float16)1.0f, (_Float16)1.0f}, c, false);
+    }
+  }
+  return c;
+}
+
 // Power of two of byte I of a dword of scale bytes, as a float's bits.
 template <int I>
 __device__ __forceinline__ unsigned kv4_scale_bits(unsigned bytes) {

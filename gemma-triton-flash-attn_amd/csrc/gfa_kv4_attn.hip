@@ -247,10 +247,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
     i16x8 pb;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float pv = fast_exp2(x[e] - m_use);
-      l_run += pv;
-      pb[e] = to16<IS_BF16>(pv);
+      pb[e] = to16<IS_BF16>(fast_exp2(x[e] - m_use));
     }
+    l_run = kv4_add_weights<IS_BF16>(pb, l_run);
 
     // ---- O^T += V^T P^T ----
     float sc[8];

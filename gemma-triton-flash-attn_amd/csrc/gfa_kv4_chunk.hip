@@ -300,10 +300,9 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
       const float m_use = m_ref[m] == -INFINITY ? 0.f : m_ref[m];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float pv = fast_exp2(s[m][r] * p.xs - m_use);
-        l_run[m] += pv;
-        pb[m][r >> 3][r & 7] = to16<IS_BF16>(pv);
+        pb[m][r >> 3][r & 7] = to16<IS_BF16>(fast_exp2(s[m][r] * p.xs - m_use));
       }
+      l_run[m] = kv4_add_weights<IS_BF16>(pb[m][1], kv4_add_weights<IS_BF16>(pb[m][0], l_run[m]));
     }
 
     __builtin_amdgcn_sched_barrier(0);

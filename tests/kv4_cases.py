@@ -72,7 +72,9 @@ class Requests:
                 q = self.q[0, :, t:t + m]
                 ob, w = orc.attend(q, k, v, n, causal, window, sc, softcap, None if held is None else held[b])
                 o[:, t:t + m] = ob
-                # p and o are each rounded to the type once: half a step of p's weight, half a step of o. A p below the
+                # p and o are each rounded to the type once, and the row sum is that of the rounded p: with p_j (1 + e_j),
+                # |e_j| <= u, the numerator moves by at most u sum p |v| (the weight), the sum by at most u of itself, the
+                # quotient so by at most u (weight + |o|) to first order, and its rounding adds u |o|. A p below the
                 # type's normal range is off by half its smallest step instead. Scores are 32-bit sums of D products,
                 # each rounding at most 2^-24 of the sum of magnitudes so far; a shift of a score by x moves p and
                 # the row sum by x each; exp2 and tanh are good to 2^-22 (tanh times the cap).
@@ -81,7 +83,7 @@ class Requests:
                 mag = float((top(q).amax((0, 1)) * top(k).amax((0, 1))).sum() * sc) if n else 0.0
                 shift = self.D * 2.0 ** -24 * mag + 2.0 ** -21 + softcap * 2.0 ** -22
                 tiny = n * torch.finfo(self.dtype).smallest_normal * u * (float(top(v).max()) if n else 0.0)
-                bound[:, t:t + m] = (u + 2 * shift) * w + u * ob.abs() + tiny + 1e-30
+                bound[:, t:t + m] = (u + 2 * shift) * w + 2 * u * ob.abs() + 4 * u * u * w + tiny + 1e-30
             t += m
         return o, bound
 

@@ -57,10 +57,10 @@ class Server:
                 if n:
                     kk, vv = orc.rounded(self.k[i][b]), orc.rounded(self.v[i][b])
                     want, w = orc.attend(q[0, :, t:t + n], kk, vv, kk.shape[1], True, window)
-                    # one rounding of p, one of o, 32-bit score sums (kv4_cases.Requests.expected)
+                    # one rounding of p, in the sum too, one of o, 32-bit score sums (kv4_cases.Requests.expected)
                     u = half_step(self.dtype)
                     mag = float((q.double().abs().amax((0, 1, 2)) * kk.abs().amax((0, 1))).sum() * D ** -0.5)
-                    bound = (u + 2 * (D * 2.0 ** -24 * mag + 2.0 ** -21)) * w + u * want.abs() + 1e-30
+                    bound = (u + 2 * (D * 2.0 ** -24 * mag + 2.0 ** -21)) * w + 2 * u * want.abs() + 4 * u * u * w + 1e-30
                     check(o[:, :, t:t + n], want, bound)
                 t += n
             assert not o[:, :, t:].any()
