@@ -451,12 +451,13 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
     for (int r = 0; r < 16; ++r) {
       const int idx = 8 * (r >> 2) + 4 * ho + (r & 3);
       uint16_t* d = op + (idx & 15) * L::PP + CPL * (idx >> 4);
+      constexpr int WO = CPL < 8 ? CPL : 8;
 #pragma unroll
-      for (int x = 0; x < CPL; x += W) {
-        typedef short vec __attribute__((ext_vector_type(W)));
+      for (int x = 0; x < CPL; x += WO) {
+        typedef short vec __attribute__((ext_vector_type(WO)));
         vec v;
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] = to16<IS_BF16>(none ? 0.f : acc[m][x + e][r] * inv);
+        for (int e = 0; e < WO; ++e) v[e] = to16<IS_BF16>(none ? 0.f : acc[m][x + e][r] * inv);
         *reinterpret_cast<vec*>(d + x) = v;
       }
     }
