@@ -11,8 +11,8 @@ constexpr int kTpb = 256;
 // Rows and the cache. A lane takes 8 channels of four tokens in a row: its 16-byte pieces of K and V are loaded and
 // stored in whole 1 KB runs, the four lanes of a scale block sit side by side, and where the four tokens are a quarter of
 // an operand row of V (consecutive slots from a multiple of four, as a prompt's are) their codes go in one
-// piece. Bound: memory. 16384 tokens of 8 heads at D = 256, 170 MB each way: stored in 36 us (4.7 TB/s), read in
-// 27 us (6.4 TB/s); with a scale block a lane, 64-byte strides between lanes, 41 and 47 us.
+// piece. Bound: memory. 16384 tokens of 8 heads at D = 256, 172 MB each way: stored in 31 us (5.5 TB/s), read in
+// 26 us (6.6 TB/s); with a scale block a lane, 64-byte strides between lanes, 41 and 47 us.
 template <int D>
 struct Rows {
   static constexpr int LPT = D / 8;     // lanes per token
