@@ -47,15 +47,20 @@ struct Div {
   __device__ __forceinline__ int rem(int x) const { return x - quot(x) * (int)d; }
 };
 
-// x / d for 0 <= x < 2^31 and d > 0 known on the device alone: a float's quotient, off by at most one where the result is below
-// 2^22, put right.
-__device__ __forceinline__ int quotient(int x, int d) {
-  int q = (int)((float)x * __builtin_amdgcn_rcpf((float)d));
-  const int r = x - q * d;
+// x / d for 0 <= x < 2^31 and d > 0 known on the device alone, rcp = 1 / d within a unit in the last place: a float's
+// quotient, off by 2^-22 of itself (512) and one more at most, and by the remainder's, which is off by less than one.
+__host__ __device__ __forceinline__ int quotient_by(int x, int d, float rcp) {
+  // unsigned: q d may pass 2^31, the remainder does not
+  unsigned q = (unsigned)((float)x * rcp);
+  int r = (int)((unsigned)x - q * (unsigned)d);
+  const int more = (int)((float)r * rcp);
+  q += (unsigned)more;
+  r -= more * d;
   q += r >= d;
   q -= r < 0;
-  return q;
+  return (int)q;
 }
+__device__ __forceinline__ int quotient(int x, int d) { return quotient_by(x, d, __builtin_amdgcn_rcpf((float)d)); }
 
 struct Kv4Cache {
   uint8_t* codes;   // (num_blocks, Hkv, 2, block_size, D / 2)

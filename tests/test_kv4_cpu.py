@@ -19,6 +19,7 @@ from oracle import kv4_oracle as orc
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 HEADER = os.path.join(ROOT, "include", "gfa.h")
+CSRC = os.path.join(ROOT, "gemma-triton-flash-attn_amd", "csrc")
 no_gpu = pytest.mark.skipif(torch.cuda.is_available(), reason="passes fake device pointers; runs only without a visible GPU")
 
 
@@ -289,3 +290,42 @@ def test_workspace_follows_the_call():
 
 def test_exports():
     assert "kv4" in gfa.__all__ and gfa.kv4 is kv4
+
+
+# ---- the kernels' divisions ----
+
+@pytest.mark.skipif(shutil.which("hipcc") is None, reason="hipcc not available")
+def test_divisions_are_exact(tmp_path):
+    """Quotients of the work split over their whole range, with reciprocals a unit in the last place off to either side: a
+    wrong one loses key tiles of a long table, or counts a row block's chunks from below zero."""
+    src = tmp_path / "div.hip"
+    src.write_text(r'''
+#include "gfa_kv4.h"
+#include <cstdio>
+#include <random>
+static long check(int x, int d) {
+  long wrong = 0;
+  const float r = 1.0f / (float)d;
+  for (const float rcp : {std::nextafter(r, 0.f), r, std::nextafter(r, 2.f)}) wrong += gfa::quotient_by(x, d, rcp) != x / d;
+  return wrong;
+}
+int main() {
+  std::mt19937 gen(5);
+  long wrong = 0;
+  for (int d = 1; d < 2100; ++d) {
+    for (const long q : {0l, 1l, 2l, 1l << 22, (1l << 22) + 1, 0x7fffffffl / d}) {
+      for (long x = q * d - 2; x <= q * d + 2; ++x)
+        if (x >= 0 && x <= 0x7fffffffl) wrong += check((int)x, d);
+    }
+    for (int i = 0; i < 2000; ++i) wrong += check((int)(gen() >> 1), d) + check((int)(gen() >> (1 + gen() % 31)), d);
+  }
+  for (int i = 0; i < 1000000; ++i) wrong += check((int)(gen() >> 1), (int)(gen() >> (1 + gen() % 31)) | 1);
+  for (const int d : {1 << 30, 0x3fffffff, 0x7fffffff, 0x7ffffffe})
+    for (const int x : {0, 1, d - 1, d, 0x7fffffff}) wrong += check(x, d);
+  std::printf("%ld\n", wrong);
+}
+''')
+    exe = tmp_path / "div"
+    subprocess.run(["hipcc", "--offload-host-only", "-O2", "-std=c++17", "-I", CSRC, "-I", os.path.dirname(HEADER), str(src), "-o", str(exe)],
+                   check=True, capture_output=True)
+    assert subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.strip() == "0"
