@@ -101,9 +101,9 @@ struct Split {
 };
 
 constexpr int kRows = gfa::kSplitRows;
-// A request's rows from which the chunk kernel is faster: 16 requests at 8k, D = 512, 32 rows 101 us (chunk kernel 170),
-// 64 rows 158 (185), 128 rows 270 (203); D = 128, 64 rows 102 (124), 128 rows 178 (139). One request alone leaves the
-// GPU to the split kernel's smaller workgroups longer: 128 rows at 8k, D = 512, 25 us (47).
+// A request's rows from which the chunk kernel is faster: 16 requests at 8k, D = 512, 32 rows 101 us (chunk kernel 172),
+// 64 rows 159 (176), 128 rows 261 (190); D = 128, 64 rows 97 (122), 128 rows 161 (127). One request alone leaves the
+// GPU to the split kernel's smaller workgroups longer: 128 rows at 8k, D = 512, 25 us (46).
 int row_limit(const gfa_kv4_attn_args* a) { return (int64_t)a->requests * a->cache.heads_kv <= 4 ? 128 : 64; }
 
 void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
@@ -163,8 +163,9 @@ Split split_of(const gfa_kv4_attn_args* a) {
     }
   }
   // with cu, workgroups to spare: rows behind the last request's
-  // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 20.1 us; of 4: 21.8, of 2: 27.4). Twice the CUs' number
-  // of workgroups where there is work for them (32 ragged requests: 512 108 us, 1024 119 us, 2048 123-141 us).
+  // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 19.7 us; of 4: 21.0, of 2: 26.2). Twice the CUs' number
+  // of workgroups where there is work for them (32 ragged requests: 512 96 us, 1024 107 us, 2048 129 us; 64 full
+  // ones 152-154 us with each).
   size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
   // Of the chunk kernel as many workgroups as the CUs hold at once (256 tokens at 16k, D = 512: 290 us, twice as many 314;
   // 1024 tokens, D = 128: 256 482 us, 512 375, 768 354, 1024 360). Its chunks cost as much again as some tiles, so the
