@@ -209,3 +209,34 @@ def test_ragged_splits_of_chunks(device):
         assert torch.equal(a, b)
         check(a, *r.expected())
         check(r.attend(slide_size=600), *r.expected(window=600))
+
+
+def test_the_longest_table(device):
+    """One request of 2^30 tokens, its table naming one block 2^20 - 1 times and another one at the end. Head 0 looks for the
+    last block alone, head 1 sees the others."""
+    from gemma_triton_flash_attn_amd import kv4
+    from oracle import kv4_oracle as orc
+
+    D, bs, M = 64, 1024, 1 << 20
+    g = torch.Generator().manual_seed(7)
+    k = torch.zeros(1, 1, 2 * bs, D)
+    k[:, :, bs:, 0] = 16.0  # a value of the format
+    v = torch.randn(1, 1, 2 * bs, D, generator=g)
+    v[:, :, bs:] += 3.0
+    k, v = k.bfloat16(), v.bfloat16()
+    cache = kv4.allocate(2, 1, D, bs, torch.bfloat16, device)
+    kv4.write(cache, k.to(device), v.to(device), torch.arange(2 * bs, device=device))
+    table = torch.zeros(1, M, dtype=torch.int32, device=device)
+    table[0, -1] = 1
+    q = torch.zeros(1, 2, 1, D, dtype=torch.bfloat16)
+    q[0, 0, 0, 0], q[0, 1, 0, 0] = 32.0, -32.0  # scores 64 and -64 at the end, 0 elsewhere
+    lens = torch.tensor([M * bs], dtype=torch.int32, device=device)
+    got = kv4.attention(q.to(device), cache, table, lens)[0, :, 0].double().cpu()
+    vr = orc.rounded(v[0]).double()[0]
+    # e^64 against 2^30 e^0: the other side weighs less than 2^-50
+    want = torch.stack([vr[bs:].mean(0), vr[:bs].mean(0)])
+    weight = torch.stack([vr[bs:].abs().mean(0), vr[:bs].abs().mean(0)])
+    # P is 1 where it counts, so sums round alone: a lane adds 2^30 / (512 workgroups, 4 waves) keys of a tile 4 or 32 at a time,
+    # at most 2^17 sums of at most 2^-24 of the total, in O^T and in the row sum; joining adds less than 2^10.
+    bound = 2 * (2 ** 17 + 2 ** 10) * 2.0 ** -24 * weight + 2.0 ** -8 * want.abs()
+    assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() - bound).max())
