@@ -10,8 +10,8 @@
 //    4 g + r, 16 + 4 g + r, in which V is stored. No LDS and no barrier until the end.
 //  * Every wave keeps its own running maximum m, row sum l and O^T; they are joined once through LDS,
 //    and the chunks' results by the join kernels from fp32 partial sums, in a fixed order.
-// Bound: memory for batches (64 requests of 16k, 32:8 D = 128: 822 MB in 140 us, 5.9 TB/s), at D = 512 the decoding of
-// one wave per SIMD (32 ragged requests, 32:4: 371 MB in 87 us, 4.3 TB/s), latency for one request (16k, D = 512: 13 us).
+// Bound: memory for batches (64 requests of 16k, 32:8 D = 128: 822 MB in 142 us, 5.8 TB/s), at D = 512 the decoding of
+// one wave per SIMD (32 ragged requests, 32:4: 371 MB in 88 us, 4.2 TB/s), latency for one request (16k, D = 512: 13 us).
 #include "gfa_kv4_sched.h"
 #include "gfa_launch.h"
 

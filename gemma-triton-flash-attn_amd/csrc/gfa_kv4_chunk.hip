@@ -13,7 +13,7 @@
 //  * Softmax: a running reference per row, moved when a score passes it by more than 2^kMargin, so that O^T is
 //    rescaled once or twice per row and P stays within 2^kMargin. Row sums are held in 32 bits.
 // Bound: issue of one wave per SIMD at D = 512, products and decoding together. 4096 tokens over 16384: 32:4 D = 512 3.5 ms,
-// 1.09 PFLOP/s (matrix cores 43% busy by their counter), 16:8 D = 256 980, 32:8 D = 128 831, 16:16 D = 64 556 TFLOP/s.
+// 1.09 PFLOP/s (matrix cores 42% busy by their counter), 16:8 D = 256 980, 32:8 D = 128 831, 16:16 D = 64 556 TFLOP/s.
 #include "gfa_kv4_sched.h"
 #include "gfa_launch.h"
 
