@@ -78,15 +78,16 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   const Item it = find_item<kRows, false>(p, p.hkv.quot((int)blockIdx.x), lane);
   const Request& rq = it.rq;
   if (it.b < 0) {
-    // No item: tokens behind the last request's are zeros, the workgroups without an item take them in turn.
+    // No item: tokens ahead of the first request's and behind the last one's are zeros, the workgroups without an item take
+    // them in turn.
     if (p.cu == nullptr) return;
-    const int n0 = max(p.cu[p.B], 0);
+    const int lead = min(max(p.cu[0], 0), p.T), n0 = min(max(p.cu[p.B], 0), p.T);
     const int64_t taken = (int64_t)it.items * p.cache.Hkv;
     const int64_t extra = (int)blockIdx.x - taken, n_extra = p.nblocks - taken;
-    const int64_t pieces = (int64_t)(p.T - n0) * p.Hq * (D / 8);
+    const int64_t pieces = ((int64_t)lead + p.T - n0) * p.Hq * (D / 8);
     for (int64_t i = extra * blockDim.x + threadIdx.x; i < pieces; i += n_extra * blockDim.x) {
-      const int64_t hd = i / (D / 8);
-      const int t = (int)(n0 + hd / p.Hq);
+      const int64_t hd = i / (D / 8), n = hd / p.Hq;
+      const int t = (int)(n < lead ? n : n0 + (n - lead));
       uint16_t* at = p.o + p.n.quot(t) * p.osb + hd % p.Hq * p.osh + p.n.rem(t) * p.osn + i % (D / 8) * 8;
       *reinterpret_cast<i16x8*>(at) = i16x8{};
     }

@@ -130,7 +130,7 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
     without it every request has B N / R tokens. A request's new tokens are its last ones: the one at
     position p attends to positions <= p, with ``slide_size`` W > 0 only to those > p - W, without ``causal``
     (cross attention) to all of them. Positions whose table entry is no block are not attended to. A row that
-    attends to nothing is 0, and so are rows behind the last request's tokens.
+    attends to nothing is 0, and so are rows of no request (ahead of ``cu[0]``, from ``cu[R]`` on).
 
     ``max_new``: the most new tokens of any request, if known (1 for a decoding step): it only chooses
     kernels. ``scale`` defaults to 1/sqrt(D); ``softcap`` as in ``flash_attn_gqa_train``. There is no gradient."""

@@ -319,8 +319,8 @@ int gfa_kv4_plan(const gfa_kv4_plan_args* args);
  * token cu[b] on (cu NULL: every request has batch * seq_len / requests). New token i, at position
  * p = lens - fresh + i, attends to positions <= p, with a window W > 0 only to those > p - W; without
  * causal to all lens positions. Positions without a block are not attended to; a row that attends to
- * nothing is zero, and so are rows behind the last request's. max_new, when not 0, is the most new tokens
- * of any request and only chooses the kernel. Values in the tables, lens and cu cannot make the call
+ * nothing is zero, and so are rows of no request (ahead of cu[0], from cu[requests] on). max_new, when not
+ * 0, is the most new tokens of any request and only chooses the kernel. Values in the tables, lens and cu cannot make the call
  * address memory outside its arrays. */
 typedef struct {
   gfa_kv4_cache cache;
