@@ -90,6 +90,11 @@ def _plain(t: torch.Tensor) -> bool:
     return type(t) in _ORDINARY and _lib.plain_setting()
 
 
+def _refuse_gradients(what: str, *rows: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in rows):
+        raise NotImplementedError(f"{what} has no gradient (call it under torch.no_grad())")
+
+
 def plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, used: torch.Tensor, *,
          block_size: int, tokens: int) -> Plan:
     """Places for a step's new tokens, in one launch.
@@ -107,7 +112,8 @@ def plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch
 
 def write(cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Store k, v (B, Hkv, N, D) in the cache, token t at ``slots[t]`` (int64, B N of them). A slot outside the
-    cache (-1) stores nothing; the slots of one call must differ."""
+    cache (-1) stores nothing; the slots of one call must differ. There is no gradient."""
+    _refuse_gradients("a write to the cache", k, v)
     fn = _lib.native().kv4_write if _plain(k) else torch.ops.gfa.kv4_write
     fn(cache.codes, cache.scales, cache.dtype is torch.bfloat16, k, v, slots)
 
@@ -134,8 +140,7 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
 
     ``max_new``: the most new tokens of any request, if known (1 for a decoding step): it only chooses
     kernels. ``scale`` defaults to 1/sqrt(D); ``softcap`` as in ``flash_attn_gqa_train``. There is no gradient."""
-    if q.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("attention over the cache has no gradient (call it under torch.no_grad())")
+    _refuse_gradients("attention over the cache", q)
     if max_new is not None and max_new < 1:
         raise ValueError("max_new must be at least 1")
     fn = _lib.native().kv4_attention if _plain(q) else torch.ops.gfa.kv4_attention

@@ -1,0 +1,31 @@
+"""What the cache operators refuse, each by its message, on CPU tensors: none of it comes as far as the device's refusal."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from gemma_triton_flash_attn_amd import kv4
+from test_kv4_cpu import _codes, _Held
+
+
+def _ints(*s):
+    return torch.zeros(*s, dtype=torch.int32)
+
+
+def _rows(h, **kw):
+    return torch.zeros(1, h, 3, 128, dtype=torch.bfloat16, **kw)
+
+
+SLOTS = torch.zeros(3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_rows_that_want_a_gradient(which):
+    """Stored rows keep no graph: a write of rows that want one would cut their gradients off unseen."""
+    c = _Held(*_codes(), torch.bfloat16)
+    rows = {"k": _rows(2), "v": _rows(2)}
+    rows[which] = rows[which].requires_grad_(True)
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        kv4.write(c, rows["k"], rows["v"], SLOTS)
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):  # past it, to the device's refusal
+        kv4.write(c, rows["k"], rows["v"], SLOTS)
