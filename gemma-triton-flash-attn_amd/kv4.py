@@ -30,6 +30,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .attention import _DTYPES, _ORDINARY, _check_softcap, _default_scale
@@ -90,9 +91,11 @@ def _plain(t: torch.Tensor) -> bool:
     return type(t) in _ORDINARY and _lib.plain_setting()
 
 
-def _refuse_gradients(what: str, *rows: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in rows):
+def _refuse_gradients(what: str, a: torch.Tensor, b: torch.Tensor) -> None:
+    if (a.requires_grad or b.requires_grad) and torch.is_grad_enabled():
         raise NotImplementedError(f"{what} has no gradient (call it under torch.no_grad())")
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in (a, b)):
+        raise NotImplementedError(f"{what} has no gradient, in forward mode neither")
 
 
 def plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch.Tensor, used: torch.Tensor, *,
@@ -140,7 +143,7 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
 
     ``max_new``: the most new tokens of any request, if known (1 for a decoding step): it only chooses
     kernels. ``scale`` defaults to 1/sqrt(D); ``softcap`` as in ``flash_attn_gqa_train``. There is no gradient."""
-    _refuse_gradients("attention over the cache", q)
+    _refuse_gradients("attention over the cache", q, q)
     if max_new is not None and max_new < 1:
         raise ValueError("max_new must be at least 1")
     fn = _lib.native().kv4_attention if _plain(q) else torch.ops.gfa.kv4_attention

@@ -29,3 +29,21 @@ def test_rows_that_want_a_gradient(which):
         kv4.write(c, rows["k"], rows["v"], SLOTS)
     with torch.no_grad(), pytest.raises(ValueError, match="GPU"):  # past it, to the device's refusal
         kv4.write(c, rows["k"], rows["v"], SLOTS)
+
+
+def test_forward_mode_tangents():
+    """A dual tensor's tangent would be dropped, under no_grad too (which does not end forward mode): refused."""
+    c = _Held(*_codes(), torch.bfloat16)
+    calls = [lambda x: kv4.attention(x, c, _ints(3, 2), _ints(3)),
+             lambda x: kv4.write(c, x[:, :2], _rows(2), SLOTS), lambda x: kv4.write(c, _rows(2), x[:, :2], SLOTS)]
+    for call in calls:
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(_rows(4), torch.ones_like(_rows(4)))
+            with pytest.raises(NotImplementedError, match="no gradient"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="no gradient"):
+                call(dual)
+            with pytest.raises(ValueError, match="GPU"):  # rows without a tangent pass
+                call(_rows(4))
+        with pytest.raises(NotImplementedError, match="no gradient"):
+            torch.func.jvp(call, (_rows(4),), (torch.ones_like(_rows(4)),))
