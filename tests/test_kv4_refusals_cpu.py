@@ -47,3 +47,24 @@ def test_forward_mode_tangents():
                 call(_rows(4))
         with pytest.raises(NotImplementedError, match="no gradient"):
             torch.func.jvp(call, (_rows(4),), (torch.ones_like(_rows(4)),))
+
+
+@pytest.mark.parametrize("over,exc,message", [
+    (dict(max_new=0), ValueError, "max_new"), (dict(max_new=-3), ValueError, "max_new"), (dict(softcap=-1.0), ValueError, "softcap"),
+    (dict(softcap=float("nan")), ValueError, "softcap")])
+def test_options_of_attention(over, exc, message):
+    c = _Held(*_codes(), torch.bfloat16)
+    with pytest.raises(exc, match=message):
+        kv4.attention(_rows(4), c, _ints(3, 2), _ints(3), **over)
+
+
+@pytest.mark.parametrize("arrays,exc,message", [
+    (lambda c, s: (c.float(), s), TypeError, "uint8"), (lambda c, s: (c, s.float()), TypeError, "uint8"),
+    (lambda c, s: (c[0], s), ValueError, "5-D"), (lambda c, s: (c, s[:1]), ValueError, "belong together"),
+    (lambda c, s: (c[..., ::2], s), ValueError, "belong together"), (lambda c, s: _codes(bs=16), ValueError, "block_size"),
+    (lambda c, s: _codes(bs=96), ValueError, "block_size"), (lambda c, s: _codes(d=96), ValueError, "HEAD_DIM"),
+    (lambda c, s: _codes(n=0), ValueError, "0 blocks"), (lambda c, s: (c, s), ValueError, "GPU"),
+    (lambda c, s: (c.transpose(0, 1).contiguous().transpose(0, 1), s), ValueError, "contiguous")])
+def test_caches(arrays, exc, message):
+    with pytest.raises(exc, match=message):
+        kv4.Cache(*arrays(*_codes()), torch.bfloat16)
