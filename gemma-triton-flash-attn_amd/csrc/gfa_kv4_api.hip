@@ -102,8 +102,9 @@ struct Split {
 
 constexpr int kRows = gfa::kSplitRows;
 // A request's rows from which the chunk kernel is faster: 16 requests at 8k, D = 512, 32 rows 101 us (chunk kernel 172),
-// 64 rows 159 (176), 128 rows 261 (190); D = 128, 64 rows 97 (122), 128 rows 161 (127). One request alone leaves the
-// GPU to the split kernel's smaller workgroups longer: 128 rows at 8k, D = 512, 25 us (46).
+// 64 rows 159 (176), 128 rows 261 (190); D = 128, 64 rows 97 (122), 128 rows 161 (127). Up to four requests and KV heads
+// leave the GPU to the split kernel's smaller workgroups longer, 128 rows at every head dim from 1k to 16k: one request at
+// 8k, D = 512, 25 us (45), D = 64 12 (29); the nearest, four requests at 8k and 16k, D = 512, 47 (52) and 60 (66).
 int row_limit(const gfa_kv4_attn_args* a) { return (int64_t)a->requests * a->cache.heads_kv <= 4 ? 128 : 64; }
 
 void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
@@ -113,7 +114,12 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
     s.window_tiles = (int)std::min<int64_t>((a->window + tokens + 29) / 32 + 1, 0x40000000);
     tiles = std::min<int64_t>(tiles, s.window_tiles);
   }
-  // Requests of 512 tokens or less are one chunk: one token of 333 at D = 256 takes 8.5 us, 10.9-11.6 us with a join.
+  // One chunk and no join where no row block can see more than 16 tiles: tables of up to 512 tokens, windows of up to 466 (few
+  // rows, one query head per KV head) to 480 (many heads). Lengths are not the host's to see, so a short request in a wide table is split and
+  // joined like any other, and so is a window of 512, which can touch 18 tiles. One token of a request, one chunk against split
+  // and join, us (16:16 D = 64, 32:8 D = 128, 8:1 D = 256, 8:1 D = 512; the same from 512-token and 16k-token tables):
+  //   512 tokens  5.7 7.7, 7.0 8.8, 9.5 10.6, 14.9 15.6    768  6.9 8.1, 8.5 8.9, 11.6 10.9, 18.4 15.2
+  //   1024        8.0 8.2, 9.9 9.0, 13.8 10.9, 21.9 15.2   window 512 of 16k  5.7 7.8, 7.0 8.8, 9.4 10.7, 15.0 15.2
   const int64_t chunks = tiles <= 16 ? 1 : (tiles + min_tiles - 1) / min_tiles;
   s.runs = row_blocks > 0;
   s.join = chunks > 1;

@@ -7,13 +7,16 @@
 //  * A tile's codes and scales (34 D bytes for 32 tokens; K swizzled) are copied global -> LDS once per
 //    workgroup, one tile ahead, and every wave decodes what it multiplies in registers: S^T = K Q^T
 //    and O^T += V^T P^T with v_mfma_f32_32x32x16, rows on lanes, P in registers in the B layout of the
-//    second product. A tile kept decoded in LDS would cost four times the LDS reads (64 D bytes per
+//    second product. At D = 512 a tile kept decoded in LDS would cost four times the LDS reads (64 D bytes per
 //    wave and product), which then take as long as the products; the codes cost a quarter, and the
-//    decoding (one instruction per two elements, two for V) issues in the products' shadow.
+//    decoding (one instruction per two elements, two for V) issues in the products' shadow. At D = 64 and 128
+//    no 16-bit tiles were tried.
 //  * Softmax: a running reference per row, moved when a score passes it by more than 2^kMargin, so that O^T is
 //    rescaled once or twice per row and P stays within 2^kMargin. Row sums are held in 32 bits.
-// Bound: issue of one wave per SIMD at D = 512, products and decoding together. 4096 tokens over 16384: 32:4 D = 512 3.5 ms,
-// 1.09 PFLOP/s (matrix cores 42% busy by their counter), 16:8 D = 256 980, 32:8 D = 128 831, 16:16 D = 64 556 TFLOP/s.
+// Bound: issue of one wave per SIMD at D = 512, products and decoding together. 4096 tokens over 16384: 32:4 D = 512 3.6 ms,
+// 1.06 PFLOP/s (matrix cores 41-42% busy by their counter), 16:8 D = 256 960, 32:8 D = 128 811, 16:16 D = 64 558 TFLOP/s: there
+// the vector unit, 81 and 70% busy. It issues 10, 12, 17.5 and 18 instructions a product (D = 512 to 64, the product among
+// them), 7 of them for decoding (D = 64: 3.5), most of the others per score whatever D.
 #include "gfa_kv4_sched.h"
 #include "gfa_launch.h"
 

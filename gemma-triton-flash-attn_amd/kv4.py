@@ -107,7 +107,9 @@ def plan(lens: torch.Tensor, new: torch.Tensor, table: torch.Tensor, free: torch
     free blocks, of which the first ``used`` ((1,) int32) are handed out; requests take the next ones in their
     order. ``tokens``: the step's static token count, at least the sum of ``new``; what lies behind is padding
     (slot -1). A table entry past the free list is -1, and so are the slots there; ``Plan.used`` above F tells
-    of it. The next step takes ``Plan.lens`` and ``Plan.used``."""
+    of it. A request that outgrows the table's M blocks takes them from the free list all the same: they stand in no
+    table, and the slots there are -1. The next step takes ``Plan.lens`` and ``Plan.used`` (outside of torch.compile views
+    of one allocation with ``positions`` and ``cu``)."""
     if _plain(lens):
         return Plan(*_lib.native().kv4_plan(lens, new, table, free, used, block_size, tokens, False))
     return Plan(*torch.ops.gfa.kv4_plan(lens, new, table, free, used, block_size, tokens))
@@ -123,7 +125,7 @@ def write(cache: Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -
 
 def read(cache: Cache, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values at ``slots`` (int64, (T,)), as (1, Hkv, T, D) of the cache's dtype; zeros for a slot
-    outside the cache."""
+    outside the cache. Outside of torch.compile both are views of one allocation: whoever keeps one keeps both."""
     if _plain(slots):
         return _lib.native().kv4_read(cache.codes, cache.scales, cache.dtype is torch.bfloat16, slots, False)
     return torch.ops.gfa.kv4_read(cache.codes, cache.scales, cache.dtype is torch.bfloat16, slots)

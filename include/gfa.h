@@ -292,8 +292,8 @@ int gfa_kv4_read(const gfa_kv4_rows_args* args);
  * in the order of the requests. It holds ceil(lens / block_size) blocks; further ones it needs are the
  * next entries of free_ids behind the *used that are taken, handed out in the order of the requests
  * and entered in its row of the table. Where the free list ends, -1 is entered: *used_out above
- * free_count tells of it. One launch; the inputs other than the table are only read, the outputs must not
- * overlap them. */
+ * free_count tells of it. Blocks past the table's width are handed out too, and entered nowhere. One launch; the inputs other
+ * than the table are only read, the outputs must not overlap them. */
 typedef struct {
   const int32_t* lens;  /* (requests) */
   const int32_t* fresh; /* (requests) */
