@@ -16,6 +16,8 @@ namespace {
 
 using gfa::api_fail;
 
+constexpr int64_t kMostWorkgroups = (1 << 24) - 1;  // of 256 threads: a launch holds fewer than 2^32
+
 bool aligned(const void* p, unsigned n) { return p != nullptr && reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int check_cache(const gfa_kv4_cache& c) {
@@ -59,7 +61,8 @@ int rows_call(const gfa_kv4_rows_args* a, bool write) {
   if (!aligned(a->slots, 8)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "slots must be an 8-byte aligned pointer");
   const int64_t tokens = (int64_t)a->batch * a->seq_len;
   // a wave per 2048 / head_dim tokens and head, four waves a workgroup
-  if (tokens > 0x7fffffff || (tokens + 3) * a->cache.heads_kv / 4 >= 0x7fffffff)
+  const int64_t per_wave = 2048 / a->cache.head_dim, waves = (tokens + per_wave - 1) / per_wave * a->cache.heads_kv;
+  if (tokens > 0x7fffffff || (waves + 3) / 4 > kMostWorkgroups)
     return api_fail(GFA_ERR_UNSUPPORTED, "%lld tokens of %d heads exceed one launch", (long long)tokens, a->cache.heads_kv);
   gfa::Kv4RowsParams p{};
   p.cache = cache_of(a->cache);
@@ -263,9 +266,11 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   if (!aligned(a->table, 4) || !aligned(a->lens, 4) || (a->cu != nullptr && !aligned(a->cu, 4)))
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "table, lens and cu must be 4-byte aligned pointers");
   const Split s = split_of(a);
-  for (const Part* part : {&s.few, &s.many})
-    if (part->nblocks > 0x7fffffff || part->row_blocks * part->join_rows * a->cache.heads_kv > 0x1fffffff)
-      return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)part->nblocks);
+  for (const Part* part : {&s.few, &s.many}) {
+    const int64_t join = part->join ? part->row_blocks * part->join_rows * (a->cache.head_dim / part->join_slice) * a->cache.heads_kv : 0;
+    if (std::max(part->nblocks, join) > kMostWorkgroups)
+      return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)std::max(part->nblocks, join));
+  }
   const size_t need = s.few.bytes() + s.many.bytes();
   if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
     return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, a->workspace_bytes);

@@ -1,11 +1,13 @@
 """What the cache operators refuse, each by its message, on CPU tensors: none of it comes as far as the device's refusal."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from gemma_triton_flash_attn_amd import kv4
-from test_kv4_cpu import _codes, _Held
+from gemma_triton_flash_attn_amd import _lib, kv4
+from test_kv4_cpu import UNSUPPORTED, _attn, _cache, _codes, _Held, no_gpu
 
 
 def _ints(*s):
@@ -68,3 +70,24 @@ def test_options_of_attention(over, exc, message):
 def test_caches(arrays, exc, message):
     with pytest.raises(exc, match=message):
         kv4.Cache(*arrays(*_codes()), torch.bfloat16)
+
+
+@no_gpu
+def test_grids_past_one_launch():
+    """A launch holds fewer than 2^32 threads, 2^24 workgroups of 256: calls that would need more are refused for what they are,
+    not by whatever the runtime says. Calls just below come as far as the launch, which fails for want of a GPU."""
+    lib = _lib.load()
+    wide = lambda heads, requests: _attn(cache=_cache(heads_kv=heads), heads_q=heads, cu=0, requests=requests, seq_len=requests)  # noqa: E731
+    for heads, requests, status in ((256, 65536, UNSUPPORTED), (65535, 256, UNSUPPORTED), (255, 65535, 4)):
+        got = lib.gfa_kv4_attn(ctypes.byref(wide(heads, requests)))
+        assert got == status, (heads, requests, got, lib.gfa_last_error())
+
+    a = _lib.Kv4RowsArgs()
+    a.k = a.v = 256
+    a.k_strides = a.v_strides = _lib.Strides(0, 128, 256)
+    a.batch, a.slots = 1, 64
+    # a wave holds 2048 / head_dim tokens of a head
+    for heads, tokens, D, status in ((1 << 10, 1 << 18, 512, UNSUPPORTED), (1 << 10, (1 << 18) - 4, 512, 4), (1 << 13, 1 << 18, 64, UNSUPPORTED)):
+        a.cache, a.seq_len = _cache(heads_kv=heads, head_dim=D), tokens
+        for fn in (lib.gfa_kv4_write, lib.gfa_kv4_read):
+            assert fn(ctypes.byref(a)) == status, (heads, tokens, D, lib.gfa_last_error())
