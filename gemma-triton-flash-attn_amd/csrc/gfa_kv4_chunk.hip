@@ -13,9 +13,9 @@
 //    no 16-bit tiles were tried.
 //  * Softmax: a running reference per row, moved when a score passes it by more than 2^kMargin, so that O^T is
 //    rescaled once or twice per row and P stays within 2^kMargin. Row sums are held in 32 bits.
-// Bound: issue of one wave per SIMD at D = 512, products and decoding together. 4096 tokens over 16384: 32:4 D = 512 3.6 ms,
-// 1.06 PFLOP/s (matrix cores 41-42% busy by their counter), 16:8 D = 256 960, 32:8 D = 128 811, 16:16 D = 64 558 TFLOP/s: there
-// the vector unit, 81 and 70% busy. It issues 10, 12, 17.5 and 18 instructions a product (D = 512 to 64, the product among
+// Bound: issue of one wave per SIMD at D = 512, products and decoding together. 4096 tokens over 16384: 32:4 D = 512 3.6 ms
+// (3.58 to 3.70 from card to card), 1.06 PFLOP/s (matrix cores 41-42% busy by their counter), 16:8 D = 256 960, 32:8 D = 128 811,
+// 16:16 D = 64 558 TFLOP/s. Bound at D = 128 and 64: the vector unit, 81 and 70% busy. It issues 10, 12, 17.5 and 18 instructions a product (D = 512 to 64, the product among
 // them), 7 of them for decoding (D = 64: 3.5), most of the others per score whatever D.
 #include "gfa_kv4_sched.h"
 #include "gfa_launch.h"
