@@ -38,12 +38,14 @@ STATUS_NAMES = {
 # GFA_VERSION of include/gfa.h whose struct layouts FwdArgs / BwdArgs below mirror. A library
 # built from other sources reads another prefix of the argument structs (an older one ignores the
 # segment, soft-cap and dropout fields), so load() refuses it instead of computing wrong results.
-ABI_VERSION = 108
+ABI_VERSION = 109
 
 EXPORTED = ("gfa_fwd", "gfa_bwd", "gfa_bwd_noalloc", "gfa_bwd_workspace_size", "gfa_bwd_workspace_bytes",
             "gfa_bwd_ds_limit", "gfa_config", "gfa_last_error", "gfa_version", "gfa_set_runtime_scheduling",
             "gfa_segments_from_positions", "gfa_segments_from_mask", "gfa_kv4_write", "gfa_kv4_read", "gfa_kv4_plan",
-            "gfa_kv4_attn", "gfa_kv4_attn_workspace_bytes")
+            "gfa_kv4_attn", "gfa_kv4_attn_workspace_bytes", "gfa_kv4_fork", "gfa_kv4_compact",
+            "gfa_kv4_pages_workspace_bytes", "gfa_kv4_copy", "gfa_kv4_share", "gfa_kv4_verify",
+            "gfa_kv4_verify_workspace_bytes")
 NOALLOC_SCRATCH_BYTES = 64 << 20  # GFA_NOALLOC_SCRATCH_BYTES
 
 
@@ -129,7 +131,34 @@ class Kv4AttnArgs(ctypes.Structure):
                 ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p),
                 ("table_width", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
                 ("max_new", ctypes.c_int32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
-                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p)]
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
+                ("shared_skip", ctypes.c_void_p), ("shared_cu", ctypes.c_void_p), ("shared_lens", ctypes.c_void_p)]
+
+
+class Kv4PagesArgs(ctypes.Structure):
+    _fields_ = [("caches", ctypes.POINTER(Kv4Cache)), ("layers", ctypes.c_int32), ("table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p), ("requests", ctypes.c_int32),
+                ("table_width", ctypes.c_int32), ("parents", ctypes.c_void_p), ("keep", ctypes.c_void_p),
+                ("rows", ctypes.c_int32), ("free_count", ctypes.c_int32), ("free_ids", ctypes.c_void_p),
+                ("used", ctypes.c_void_p), ("table_out", ctypes.c_void_p), ("lens_out", ctypes.c_void_p),
+                ("used_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                ("stream", ctypes.c_void_p)]
+
+
+class Kv4ShareArgs(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p),
+                ("requests", ctypes.c_int32), ("table_width", ctypes.c_int32), ("block_size", ctypes.c_int32),
+                ("least", ctypes.c_int32), ("skip", ctypes.c_void_p), ("cu_out", ctypes.c_void_p), ("lens_out", ctypes.c_void_p),
+                ("stream", ctypes.c_void_p)]
+
+
+class Kv4VerifyArgs(ctypes.Structure):
+    _fields_ = [("target", ctypes.c_void_p), ("draft", ctypes.c_void_p), ("target_stride", ctypes.c_int64),
+                ("draft_stride", ctypes.c_int64), ("type", ctypes.c_int32), ("token_count", ctypes.c_int32),
+                ("vocab", ctypes.c_int32), ("requests", ctypes.c_int32), ("tokens", ctypes.c_void_p), ("accept", ctypes.c_void_p),
+                ("sample", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("follows", ctypes.c_void_p),
+                ("accepted", ctypes.c_void_p), ("lens_out", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+                ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p)]
 
 
 _lib = None
@@ -175,11 +204,18 @@ def load() -> ctypes.CDLL:
         lib.gfa_segments_from_mask.argtypes = [ptr, i64, i32, i32, ptr, ptr, ptr, ptr]
         lib.gfa_segments_from_mask.restype = ctypes.c_int
         for name, args in (("gfa_kv4_write", Kv4RowsArgs), ("gfa_kv4_read", Kv4RowsArgs), ("gfa_kv4_plan", Kv4PlanArgs),
-                           ("gfa_kv4_attn", Kv4AttnArgs)):
+                           ("gfa_kv4_attn", Kv4AttnArgs), ("gfa_kv4_fork", Kv4PagesArgs), ("gfa_kv4_compact", Kv4PagesArgs),
+                           ("gfa_kv4_share", Kv4ShareArgs), ("gfa_kv4_verify", Kv4VerifyArgs)):
             getattr(lib, name).argtypes = [ctypes.POINTER(args)]
             getattr(lib, name).restype = ctypes.c_int
         lib.gfa_kv4_attn_workspace_bytes.argtypes = [ctypes.POINTER(Kv4AttnArgs)]
         lib.gfa_kv4_attn_workspace_bytes.restype = ctypes.c_size_t
+        lib.gfa_kv4_copy.argtypes = [ctypes.POINTER(Kv4Cache), i32, ptr, ptr, i32, ptr]
+        lib.gfa_kv4_copy.restype = ctypes.c_int
+        lib.gfa_kv4_pages_workspace_bytes.argtypes = [i32]
+        lib.gfa_kv4_pages_workspace_bytes.restype = ctypes.c_size_t
+        lib.gfa_kv4_verify_workspace_bytes.argtypes = [i32, i32]
+        lib.gfa_kv4_verify_workspace_bytes.restype = ctypes.c_size_t
         built = int(lib.gfa_version())
         if built != ABI_VERSION:
             raise RuntimeError(
@@ -232,6 +268,9 @@ def native():
                  address("gfa_segments_from_positions"), address("gfa_last_error"), GfaError)
         mod.bind_kv4(address("gfa_kv4_write"), address("gfa_kv4_read"), address("gfa_kv4_plan"), address("gfa_kv4_attn"),
                      address("gfa_kv4_attn_workspace_bytes"))
+        mod.bind_kv4_pages(address("gfa_kv4_fork"), address("gfa_kv4_compact"), address("gfa_kv4_pages_workspace_bytes"),
+                           address("gfa_kv4_copy"), address("gfa_kv4_share"), address("gfa_kv4_verify"),
+                           address("gfa_kv4_verify_workspace_bytes"))
         _native = mod
         return mod
 

@@ -161,12 +161,53 @@ struct Kv4PlanParams {
   int *positions, *cu, *lens_out, *used_out;
 };
 
+// Pages (gfa_kv4_pages.hip): bit maps of blocks in LDS, counted in groups of 8 words, one per thread of a workgroup.
+constexpr int kKv4PagesBlocks = 1 << 18, kKv4PagesRows = 4096;  // most blocks of a pool, rows of a table
+constexpr int kKv4CopyPiece = 16384;                             // bytes
+constexpr int kKv4CopyArrays = 64;                               // of one launch: codes and scales of 32 layers
+constexpr int kKv4ShareMost = 4096;                              // requests
+inline int kv4_pages_words(int num_blocks) { return (num_blocks + 255) / 256 * 8; }
+inline size_t kv4_fork_lds_words(int words, int requests, int rows) {
+  return (size_t)3 * words + 2 * (words / 8) + requests + 2 * (size_t)rows;
+}
+
+struct Kv4PagesParams {
+  const int *table, *lens, *parents, *keep, *used;
+  int64_t table_stride;
+  int B, M, rows, F, num_blocks, words, bs_log2;
+  Div m;  // M
+  int* free_ids;
+  int *table_out, *lens_out, *used_out;
+  int *src, *dst, *count;  // blocks to copy
+};
+
+struct Kv4CopyParams {
+  uint8_t* base[kKv4CopyArrays];
+  int64_t bytes[kKv4CopyArrays];    // of a block
+  int first[kKv4CopyArrays];        // an array's first piece of a pair's
+  int arrays, num_blocks, pairs;
+  Div pieces;                       // of a pair
+  const int *src, *dst, *count;     // count NULL: all pairs
+};
+
+struct Kv4ShareParams {
+  const int *table, *lens, *cu;
+  int64_t table_stride;
+  int R, M, bs_log2, least;
+  int *skip, *cu_out, *lens_out;
+};
+
 // Query rows of a workgroup of the split and of the chunk kernel.
 constexpr int kSplitRows = 16;
 constexpr int kv4_chunk_rows(int D) { return D >= 128 ? 128 : 256; }
 
 // Workgroups of the chunk kernel that a CU holds (by their registers).
 constexpr int kv4_chunk_wgs(int D) { return D == 512 ? 1 : D == 128 ? 3 : 2; }
+
+// What a launch of the attention kernels does: a whole call; or, where requests share prefixes (gfa_kv4_share), the groups'
+// prefixes as requests of their own, and the requests' keys behind them. The last two leave sums alone (kPrefix a row's in row_o
+// and row_ml), which kRest's join brings together.
+enum Kv4Part : int { kWhole, kPrefix, kRest };
 
 struct Kv4AttnParams {
   Kv4Cache cache;
@@ -192,6 +233,8 @@ struct Kv4AttnParams {
   int row_blocks, join_rows, join_slice, join_parts;
   float* part;    // (slots, Hkv, rows, D) sums and (slots, Hkv, rows, 2) row maxima and sums
   float* part_ml;
+  const int* skip;       // kRest: (B) tokens of the request's prefix
+  float *row_o, *row_ml;  // (T, Hq, D) sums and (T, Hq, 2) maxima and sums of the prefixes
 };
 
 }  // namespace gfa

@@ -6,6 +6,7 @@
 #include "gfa.h"
 #include "gfa_kv4.h"
 #include "gfa_launch.h"
+#include "gfa_verify.h"
 
 namespace gfa {
 int api_fail(int code, const char* fmt, ...);  // gfa_api.hip
@@ -108,11 +109,11 @@ constexpr int kRows = gfa::kSplitRows;
 // 64 rows 159 (176), 128 rows 261 (190); D = 128, 64 rows 97 (122), 128 rows 161 (127). Up to four requests and KV heads
 // leave the GPU to the split kernel's smaller workgroups longer, 128 rows at every head dim from 1k to 16k: one request at
 // 8k, D = 512, 25 us (45), D = 64 12 (29); the nearest, four requests at 8k and 16k, D = 512, 47 (52) and 60 (66).
-int row_limit(const gfa_kv4_attn_args* a) { return (int64_t)a->requests * a->cache.heads_kv <= 4 ? 128 : 64; }
+int row_limit(const gfa_kv4_attn_args* a, int64_t requests) { return requests * a->cache.heads_kv <= 4 ? 128 : 64; }
 
-void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
+void size_part(Part& s, const gfa_kv4_attn_args* a, gfa::Kv4Part kind, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
-  if (a->causal && a->window > 0) {
+  if (kind == gfa::kWhole && a->causal && a->window > 0) {
     const int64_t g = a->heads_q / a->cache.heads_kv, tokens = (rows + g - 2) / g + 1;  // a row block's, at most
     s.window_tiles = (int)std::min<int64_t>((a->window + tokens + 29) / 32 + 1, 0x40000000);
     tiles = std::min<int64_t>(tiles, s.window_tiles);
@@ -125,8 +126,8 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   //   1024        8.0 8.2, 9.9 9.0, 13.8 10.9, 21.9 15.2   window 512 of 16k  5.7 7.8, 7.0 8.8, 9.4 10.7, 15.0 15.2
   const int64_t chunks = tiles <= 16 ? 1 : (tiles + min_tiles - 1) / min_tiles;
   s.runs = row_blocks > 0;
-  s.join = chunks > 1;
-  s.min_tiles = s.join ? min_tiles : 0x3fffffff;
+  s.join = chunks > 1 || kind != gfa::kWhole;
+  s.min_tiles = chunks > 1 ? min_tiles : 0x3fffffff;
   s.row_blocks = row_blocks;
   // The join. Of the chunk kernel: its runs of 1 KB, four waves a workgroup. Of the split kernel: where rows are few, a
   // workgroup takes one row of 128 channels and its lanes share the chunks; else whole rows, where they are many
@@ -143,21 +144,28 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, int64_t row_blocks, int rows
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
   s.nblocks = items * hkv + spare;
   if (s.join) {
-    s.slots = std::min(row_blocks * chunks, 2 * target / hkv + 1);
+    s.slots = kind != gfa::kWhole ? items : std::min(row_blocks * chunks, 2 * target / hkv + 1);
     s.part_bytes = (size_t)(s.slots * hkv) * rows * a->cache.head_dim * sizeof(float);
     s.ml_bytes = (size_t)(s.slots * hkv) * rows * 2 * sizeof(float);
   }
 }
 
-Split split_of(const gfa_kv4_attn_args* a) {
-  Split s{};
-  const int64_t G = a->heads_q / a->cache.heads_kv, R = a->requests;
+// Most new tokens of a request, as far as the host knows.
+int64_t most_new(const gfa_kv4_attn_args* a) {
   const int64_t T = (int64_t)a->batch * a->seq_len;
-  const int64_t most = a->cu == nullptr ? T / R : a->max_new > 0 ? std::min<int64_t>(a->max_new, T) : T;
+  return a->cu == nullptr ? T / a->requests : a->max_new > 0 ? std::min<int64_t>(a->max_new, T) : T;
+}
+
+Split split_of(const gfa_kv4_attn_args* a, gfa::Kv4Part kind) {
+  Split s{};
+  const int64_t G = a->heads_q / a->cache.heads_kv, T = (int64_t)a->batch * a->seq_len;
+  // a prefix is that of two requests at least, and of any number of them
+  const int64_t R = kind == gfa::kPrefix ? std::max<int64_t>(1, a->requests / 2) : a->requests;
+  const int64_t most = kind == gfa::kPrefix ? T : most_new(a);
   // No request can have more rows than the limit: then all are the split kernel's, whatever max_new promised.
   s.one_block = most * G <= kRows;
-  const int limit = row_limit(a);
-  s.row_limit = most * G <= limit ? 0x7fffffff : limit;
+  const int limit = row_limit(a, R);
+  s.row_limit = kind == gfa::kRest || most * G <= limit ? 0x7fffffff : limit;
   const int D = a->cache.head_dim, big = gfa::kv4_chunk_rows(D);
   int64_t few, many = 0;
   if (a->cu == nullptr) {
@@ -175,14 +183,47 @@ Split split_of(const gfa_kv4_attn_args* a) {
   // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 19.7 us; of 4: 21.0, of 2: 26.2). Twice the CUs' number
   // of workgroups where there is work for them (32 ragged requests: 512 96 us, 1024 107 us, 2048 129 us; 64 full
   // ones 152-154 us with each).
-  size_part(s.few, a, few, kRows, most * G, 8, 512, a->cu ? 64 : 0);
+  size_part(s.few, a, kind, few, kRows, most * G, 8, 512, a->cu && kind != gfa::kPrefix ? 64 : 0);
   // Of the chunk kernel as many workgroups as the CUs hold at once (256 tokens at 16k, D = 512: 290 us, twice as many 314;
   // 1024 tokens, D = 128: 256 482 us, 512 375, 768 354, 1024 360). Its chunks cost as much again as some tiles, so the
   // more of the GPU the row blocks take by themselves the longer a chunk has to be: 256 tokens of one request, window
   // 1024, 33 us with chunks of 8 tiles, 57 unsplit; 1000 tokens beside seven requests 66 us with 18 tiles, 74 unsplit;
   // 512 tokens of four requests 76-84 us split, 71 unsplit.
   const int64_t alone = many * a->cache.heads_kv;
-  size_part(s.many, a, many, big, most * G, alone >= 256 ? 64 : alone >= 128 ? 32 : 8, 256 * gfa::kv4_chunk_wgs(D), 0);
+  size_part(s.many, a, kind, many, big, most * G, alone >= 256 ? 64 : alone >= 128 ? 32 : 8, 256 * gfa::kv4_chunk_wgs(D), 0);
+  return s;
+}
+
+// Whether prefixes are taken apart: without a window, which bounds what a request reads, and for requests of few rows; where
+// max_new is not known, of few rows on average.
+bool takes_prefixes(const gfa_kv4_attn_args* a) {
+  if (a->shared_skip == nullptr || (a->causal && a->window > 0) || a->requests < 2) return false;
+  const int64_t T = (int64_t)a->batch * a->seq_len;
+  const int64_t rows = a->max_new > 0 ? a->max_new : (T + a->requests - 1) / a->requests;
+  return rows * (a->heads_q / a->cache.heads_kv) <= row_limit(a, a->requests);
+}
+
+// The launches of a call: each a kernel over a part of the work and, where it leaves sums, their join.
+struct Steps {
+  Split whole, prefix, rest;  // whole, or the two others
+  bool shared;
+  size_t rows_o, rows_ml;  // bytes of the prefixes' rows
+  size_t bytes() const {
+    return shared ? rows_o + rows_ml + prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() : whole.few.bytes() + whole.many.bytes();
+  }
+};
+Steps steps_of(const gfa_kv4_attn_args* a) {
+  Steps s{};
+  s.shared = takes_prefixes(a);
+  if (!s.shared) {
+    s.whole = split_of(a, gfa::kWhole);
+    return s;
+  }
+  s.prefix = split_of(a, gfa::kPrefix);
+  s.rest = split_of(a, gfa::kRest);
+  const size_t rows = (size_t)a->batch * a->seq_len * a->heads_q;
+  s.rows_o = rows * a->cache.head_dim * sizeof(float);
+  s.rows_ml = (rows * 2 * sizeof(float) + 15) / 16 * 16;
   return s;
 }
 
@@ -208,6 +249,135 @@ int check_attn(const gfa_kv4_attn_args* a) {
   if (a->table_stride < a->table_width && a->requests > 1)
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "table_stride=%lld below table_width=%d", (long long)a->table_stride, a->table_width);
   return GFA_OK;
+}
+
+int log2_of(int block_size) {
+  int log2 = 5;
+  while ((1 << log2) < block_size) ++log2;
+  return log2;
+}
+
+// ---- pages ----
+
+int check_layers(const gfa_kv4_cache* caches, int layers) {
+  if (caches == nullptr || layers < 1) return api_fail(GFA_ERR_INVALID_ARGUMENT, "at least one cache is needed");
+  for (int i = 0; i < layers; ++i) {
+    if (int rc = check_cache(caches[i])) return rc;
+    if (caches[i].num_blocks != caches[0].num_blocks || caches[i].block_size != caches[0].block_size)
+      return api_fail(GFA_ERR_INVALID_ARGUMENT, "caches of %d blocks of %d and %d blocks of %d tokens do not belong to one table",
+                      caches[0].num_blocks, caches[0].block_size, caches[i].num_blocks, caches[i].block_size);
+  }
+  return GFA_OK;
+}
+
+constexpr int kLayersAtOnce = gfa::kKv4CopyArrays / 2;
+
+int64_t block_bytes(const gfa_kv4_cache& c, bool scales) {
+  return (int64_t)c.heads_kv * 2 * c.block_size * (scales ? c.head_dim / 32 : c.head_dim / 2);
+}
+int64_t pieces_of(int64_t bytes) { return (bytes + gfa::kKv4CopyPiece - 1) / gfa::kKv4CopyPiece; }
+
+int check_copy(const gfa_kv4_cache* caches, int layers, int64_t pairs) {
+  for (int l0 = 0; l0 < layers; l0 += kLayersAtOnce) {
+    int64_t pieces = 0;
+    for (int i = l0; i < std::min(layers, l0 + kLayersAtOnce); ++i) pieces += pieces_of(block_bytes(caches[i], false)) + pieces_of(block_bytes(caches[i], true));
+    if (pieces * pairs > 0x7fffffff)
+      return api_fail(GFA_ERR_UNSUPPORTED, "%lld pieces of %lld blocks exceed one launch", (long long)pieces, (long long)pairs);
+  }
+  return GFA_OK;
+}
+
+// (Of a call that check_copy has passed.)
+int copy_blocks(const gfa_kv4_cache* caches, int layers, const int32_t* src, const int32_t* dst, const int32_t* count, int pairs, hipStream_t stream) {
+  for (int l0 = 0; l0 < layers; l0 += kLayersAtOnce) {
+    gfa::Kv4CopyParams p{};
+    int pieces = 0;
+    for (int i = l0; i < std::min(layers, l0 + kLayersAtOnce); ++i) {
+      for (const bool scales : {false, true}) {
+        p.base[p.arrays] = static_cast<uint8_t*>(scales ? caches[i].scales : caches[i].codes);
+        p.bytes[p.arrays] = block_bytes(caches[i], scales);
+        p.first[p.arrays] = pieces;
+        pieces += (int)pieces_of(p.bytes[p.arrays]);
+        ++p.arrays;
+      }
+    }
+    p.num_blocks = caches[0].num_blocks;
+    p.pairs = pairs;
+    p.pieces.set(pieces);
+    p.src = src;
+    p.dst = dst;
+    p.count = count;
+    if (const hipError_t err = gfa::launch_kv4_copy(p, stream); err != hipSuccess) return launched(err, "block copy");
+  }
+  return gfa::api_ok();
+}
+
+int pages_call(const gfa_kv4_pages_args* a, bool fork) {
+  if (a == nullptr) return api_fail(GFA_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (int rc = check_layers(a->caches, a->layers)) return rc;
+  const int blocks = a->caches[0].num_blocks, bs = a->caches[0].block_size, rows = fork ? a->rows : a->requests;
+  if (blocks > gfa::kKv4PagesBlocks) return api_fail(GFA_ERR_UNSUPPORTED, "a pool of %d blocks (most %d)", blocks, gfa::kKv4PagesBlocks);
+  if (a->requests < 1 || a->table_width < 1 || rows < 1 || a->free_count < 0)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "requests=%d, table_width=%d and rows=%d must be positive, free_count=%d not negative",
+                    a->requests, a->table_width, rows, a->free_count);
+  if (a->requests > gfa::kKv4PagesRows || rows > gfa::kKv4PagesRows)
+    return api_fail(GFA_ERR_UNSUPPORTED, "%d requests and %d rows (most %d)", a->requests, rows, gfa::kKv4PagesRows);
+  if ((int64_t)a->table_width * bs > 0x40000000)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block tables of %lld tokens (most 2^30)", (long long)a->table_width * bs);
+  if ((int64_t)std::max(a->requests, rows) * a->table_width > 0x40000000)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block tables of %d x %d entries (most 2^30)", std::max(a->requests, rows), a->table_width);
+  if (a->table_stride < a->table_width && a->requests > 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "table_stride=%lld below table_width=%d", (long long)a->table_stride, a->table_width);
+  if (!fork && a->free_count != blocks)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "free_count=%d: a compacted pool's free list holds all of its %d blocks", a->free_count, blocks);
+  for (const void* p : {(const void*)a->table, (const void*)a->lens, (const void*)a->table_out, (const void*)a->used_out})
+    if (!aligned(p, 4)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "page arrays must be 4-byte aligned pointers");
+  if ((a->free_count > 0 && !aligned(a->free_ids, 4)) || (fork && (!aligned(a->used, 4) || !aligned(a->lens_out, 4))) ||
+      (fork && a->parents != nullptr && !aligned(a->parents, 4)) || (fork && a->keep != nullptr && !aligned(a->keep, 4)))
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "page arrays must be 4-byte aligned pointers");
+  const int most = fork ? rows : blocks / 2;  // pairs
+  if (int rc = check_copy(a->caches, a->layers, most)) return rc;
+  const size_t need = gfa_kv4_pages_workspace_bytes(fork ? rows : blocks);
+  if (!aligned(a->workspace, 4) || a->workspace_bytes < need)
+    return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (4-byte aligned) needed, got %zu", need, a->workspace_bytes);
+  gfa::Kv4PagesParams p{};
+  p.table = a->table;
+  p.lens = a->lens;
+  p.parents = fork ? a->parents : nullptr;
+  p.keep = fork ? a->keep : nullptr;
+  p.used = a->used;
+  p.table_stride = a->table_stride;
+  p.B = a->requests;
+  p.M = a->table_width;
+  p.rows = rows;
+  p.F = a->free_count;
+  p.num_blocks = blocks;
+  p.words = gfa::kv4_pages_words(blocks);
+  p.bs_log2 = log2_of(bs);
+  p.m.set(a->table_width);
+  p.free_ids = a->free_ids;
+  p.table_out = a->table_out;
+  p.lens_out = a->lens_out;
+  p.used_out = a->used_out;
+  p.count = static_cast<int*>(a->workspace);
+  p.src = p.count + 1;
+  p.dst = p.src + most;
+  const auto stream = static_cast<hipStream_t>(a->stream);
+  const hipError_t err = fork ? gfa::launch_kv4_fork(p, stream) : gfa::launch_kv4_compact(p, stream);
+  if (err != hipSuccess) return launched(err, fork ? "fork" : "compaction");
+  return copy_blocks(a->caches, a->layers, p.src, p.dst, p.count, most, stream);
+}
+
+// ---- verification ----
+
+// Waves of a request: about 4096 of a call, of at least one step.
+struct Segments {
+  int length;
+  int64_t count;
+};
+Segments verify_segments(int64_t requests, int64_t vocab) {
+  const int64_t step = gfa::kVerifyStep, length = std::max<int64_t>(1, (vocab * requests + 4096 * step - 1) / (4096 * step)) * step;
+  return Segments{(int)std::min<int64_t>(length, (vocab + step - 1) / step * step), (vocab + length - 1) / length};
 }
 
 }  // namespace
@@ -253,10 +423,102 @@ int gfa_kv4_plan(const gfa_kv4_plan_args* a) {
   return launched(gfa::launch_kv4_plan(p, static_cast<hipStream_t>(a->stream)), "plan");
 }
 
+size_t gfa_kv4_pages_workspace_bytes(int32_t n) { return n < 0 ? 0 : (2 * (size_t)n + 1) * sizeof(int32_t); }
+
+int gfa_kv4_copy(const gfa_kv4_cache* caches, int32_t layers, const int32_t* src, const int32_t* dst, int32_t pairs, void* stream) {
+  if (int rc = check_layers(caches, layers)) return rc;
+  if (pairs < 0) return api_fail(GFA_ERR_INVALID_ARGUMENT, "pairs=%d must not be negative", pairs);
+  if (pairs == 0) return gfa::api_ok();
+  if (!aligned(src, 4) || !aligned(dst, 4)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "src and dst must be 4-byte aligned pointers");
+  if (int rc = check_copy(caches, layers, pairs)) return rc;
+  return copy_blocks(caches, layers, src, dst, nullptr, pairs, static_cast<hipStream_t>(stream));
+}
+
+int gfa_kv4_fork(const gfa_kv4_pages_args* a) { return pages_call(a, true); }
+int gfa_kv4_compact(const gfa_kv4_pages_args* a) { return pages_call(a, false); }
+
+int gfa_kv4_share(const gfa_kv4_share_args* a) {
+  if (a == nullptr) return api_fail(GFA_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->block_size < 32 || a->block_size > 1024 || (a->block_size & (a->block_size - 1)) != 0)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block_size=%d must be a power of two, 32 to 1024", a->block_size);
+  if (a->requests < 1 || a->table_width < 1 || a->least < 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "requests=%d, table_width=%d and least=%d must be positive", a->requests, a->table_width, a->least);
+  if (a->requests > gfa::kKv4ShareMost) return api_fail(GFA_ERR_UNSUPPORTED, "%d requests (most %d)", a->requests, gfa::kKv4ShareMost);
+  if ((int64_t)a->table_width * a->block_size > 0x40000000)
+    return api_fail(GFA_ERR_UNSUPPORTED, "block tables of %lld tokens (most 2^30)", (long long)a->table_width * a->block_size);
+  if (a->table_stride < a->table_width && a->requests > 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "table_stride=%lld below table_width=%d", (long long)a->table_stride, a->table_width);
+  for (const void* p : {(const void*)a->table, (const void*)a->lens, (const void*)a->cu, (const void*)a->skip, (const void*)a->cu_out,
+                        (const void*)a->lens_out})
+    if (!aligned(p, 4)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "share arrays must be 4-byte aligned pointers");
+  gfa::Kv4ShareParams p{};
+  p.table = a->table;
+  p.lens = a->lens;
+  p.cu = a->cu;
+  p.table_stride = a->table_stride;
+  p.R = a->requests;
+  p.M = a->table_width;
+  p.bs_log2 = log2_of(a->block_size);
+  p.least = a->least;
+  p.skip = a->skip;
+  p.cu_out = a->cu_out;
+  p.lens_out = a->lens_out;
+  return launched(gfa::launch_kv4_share(p, static_cast<hipStream_t>(a->stream)), "share");
+}
+
+size_t gfa_kv4_verify_workspace_bytes(int32_t requests, int32_t vocab) {
+  if (requests < 1 || vocab < 1) return 0;
+  return (size_t)requests * (verify_segments(requests, vocab).count * 2 * sizeof(double) + sizeof(double));
+}
+
+int gfa_kv4_verify(const gfa_kv4_verify_args* a) {
+  if (a == nullptr) return api_fail(GFA_ERR_INVALID_ARGUMENT, "args is NULL");
+  if (a->token_count < 1 || a->vocab < 1 || a->requests < 1)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "token_count=%d, vocab=%d and requests=%d must be positive", a->token_count, a->vocab, a->requests);
+  if (a->requests > 65535) return api_fail(GFA_ERR_UNSUPPORTED, "%d requests (most 65535)", a->requests);
+  if (a->vocab > 1 << 30) return api_fail(GFA_ERR_UNSUPPORTED, "a vocabulary of %d (most 2^30)", a->vocab);
+  if (a->type < 0 || a->type > 2) return api_fail(GFA_ERR_INVALID_ARGUMENT, "type=%d is none of 0, 1, 2", a->type);
+  if (a->cu == nullptr && a->token_count % a->requests != 0)
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "%d tokens do not divide among %d requests (pass cu)", a->token_count, a->requests);
+  if (a->target_stride < 0 || a->draft_stride < 0) return api_fail(GFA_ERR_INVALID_ARGUMENT, "row strides must not be negative");
+  const unsigned size = a->type == 2 ? 4 : 2;
+  if (!aligned(a->target, size) || (a->draft != nullptr && !aligned(a->draft, size)))
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "target and draft must be aligned to their type");
+  if (!aligned(a->tokens, 8) || !aligned(a->follows, 8)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "tokens and follows must be 8-byte aligned pointers");
+  for (const void* p : {(const void*)a->accept, (const void*)a->sample, (const void*)a->lens, (const void*)a->accepted, (const void*)a->lens_out})
+    if (!aligned(p, 4)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "verify arrays must be 4-byte aligned pointers");
+  if (a->cu != nullptr && !aligned(a->cu, 4)) return api_fail(GFA_ERR_INVALID_ARGUMENT, "cu must be a 4-byte aligned pointer");
+  const size_t need = gfa_kv4_verify_workspace_bytes(a->requests, a->vocab);
+  if (!aligned(a->workspace, 8) || a->workspace_bytes < need)
+    return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (8-byte aligned) needed, got %zu", need, a->workspace_bytes);
+  gfa::VerifyParams p{};
+  p.target = a->target;
+  p.draft = a->draft;
+  p.ts = a->target_stride;
+  p.ds = a->draft_stride;
+  p.tokens = a->tokens;
+  p.accept = a->accept;
+  p.sample = a->sample;
+  p.lens = a->lens;
+  p.cu = a->cu;
+  p.T = a->token_count;
+  p.V = a->vocab;
+  p.R = a->requests;
+  p.each = a->token_count / a->requests;
+  const Segments s = verify_segments(a->requests, a->vocab);
+  p.segment = s.length;
+  p.segments = s.count;
+  p.sums = static_cast<double*>(a->workspace);
+  p.taken = reinterpret_cast<int*>(p.sums + (size_t)a->requests * s.count * 2);
+  p.follows = a->follows;
+  p.accepted = a->accepted;
+  p.lens_out = a->lens_out;
+  return launched(gfa::launch_verify(p, a->type, static_cast<hipStream_t>(a->stream)), "verification");
+}
+
 size_t gfa_kv4_attn_workspace_bytes(const gfa_kv4_attn_args* a) {
   if (check_attn(a) != GFA_OK) return 0;
-  const Split s = split_of(a);
-  return s.few.bytes() + s.many.bytes();
+  return steps_of(a).bytes();
 }
 
 int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
@@ -265,13 +527,16 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   if (int rc = check_rows("o", a->o, a->o_strides)) return rc;
   if (!aligned(a->table, 4) || !aligned(a->lens, 4) || (a->cu != nullptr && !aligned(a->cu, 4)))
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "table, lens and cu must be 4-byte aligned pointers");
-  const Split s = split_of(a);
-  for (const Part* part : {&s.few, &s.many}) {
+  if (a->shared_skip != nullptr &&
+      (a->cu == nullptr || !aligned(a->shared_skip, 4) || !aligned(a->shared_cu, 4) || !aligned(a->shared_lens, 4)))
+    return api_fail(GFA_ERR_INVALID_ARGUMENT, "shared prefixes need cu, and 4-byte aligned pointers");
+  const Steps s = steps_of(a);
+  for (const Part* part : {&s.whole.few, &s.whole.many, &s.prefix.few, &s.prefix.many, &s.rest.few}) {
     const int64_t join = part->join ? part->row_blocks * part->join_rows * (a->cache.head_dim / part->join_slice) * a->cache.heads_kv : 0;
     if (std::max(part->nblocks, join) > kMostWorkgroups)
       return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)std::max(part->nblocks, join));
   }
-  const size_t need = s.few.bytes() + s.many.bytes();
+  const size_t need = s.bytes();
   if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
     return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, a->workspace_bytes);
   gfa::Kv4AttnParams p{};
@@ -302,14 +567,15 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   const bool cap = a->softcap > 0.f;
   p.xs = (cap ? a->softcap : a->scale) * 1.4426950408889634f;
   p.cap_a = cap ? a->scale / a->softcap : 0.f;
-  p.row_limit = s.row_limit;
   const auto stream = static_cast<hipStream_t>(a->stream);
   const int D = a->cache.head_dim;
   const bool bf16 = a->cache.dtype == GFA_DTYPE_BF16;
   char* ws = static_cast<char*>(a->workspace);
-  for (const bool large : {true, false}) {
-    const Part& part = large ? s.many : s.few;
-    if (!part.runs) continue;
+  hipError_t err = hipSuccess;
+  auto run = [&](const Split& split, bool large, gfa::Kv4Part kind) {
+    const Part& part = large ? split.many : split.few;
+    if (!part.runs || err != hipSuccess) return;
+    p.row_limit = split.row_limit;
     p.min_tiles = part.min_tiles;
     p.share = part.share;
     p.window_tiles = part.window_tiles;
@@ -322,11 +588,27 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);
     ws += part.bytes();
-    hipError_t err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, stream) : gfa::launch_kv4_split(p, D, bf16, cap, s.one_block, stream);
-    if (err == hipSuccess && part.join) err = gfa::launch_kv4_join(p, D, bf16, large, stream);
-    if (err != hipSuccess) return launched(err, "cache attention");
+    err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, kind, stream) : gfa::launch_kv4_split(p, D, bf16, cap, split.one_block, kind, stream);
+    if (err == hipSuccess && part.join) err = gfa::launch_kv4_join(p, D, bf16, large, kind, stream);
+  };
+  if (s.shared) {
+    p.row_o = reinterpret_cast<float*>(ws);
+    p.row_ml = reinterpret_cast<float*>(ws + s.rows_o);
+    ws += s.rows_o + s.rows_ml;
+    const gfa::Kv4AttnParams whole = p;
+    p.cu = a->shared_cu;
+    p.lens = a->shared_lens;
+    p.causal = p.window = 0;
+    run(s.prefix, true, gfa::kPrefix);
+    run(s.prefix, false, gfa::kPrefix);
+    p = whole;
+    p.skip = a->shared_skip;
+    run(s.rest, false, gfa::kRest);
+  } else {
+    run(s.whole, true, gfa::kWhole);
+    run(s.whole, false, gfa::kWhole);
   }
-  return gfa::api_ok();
+  return err != hipSuccess ? launched(err, "cache attention") : gfa::api_ok();
 }
 
 }  // extern "C"

@@ -61,7 +61,7 @@ struct TileRegs {
 
 }  // namespace
 
-template <int D, bool IS_BF16, bool CAP, bool ONCE>
+template <int D, bool IS_BF16, bool CAP, bool ONCE, Kv4Part PART = kWhole>
 __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kernel(const Kv4AttnParams p) {
   using L = Kv4Layout<D>;
   constexpr int KT = D / 32;   // products of a score block
@@ -75,12 +75,12 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   const int g = lane >> 4, c16 = lane & 15;
   const int head = p.hkv.rem((int)blockIdx.x);
 
-  const Item it = find_item<kRows, false>(p, p.hkv.quot((int)blockIdx.x), lane);
+  const Item it = find_item<kRows, false, PART>(p, p.hkv.quot((int)blockIdx.x), lane);
   const Request& rq = it.rq;
   if (it.b < 0) {
     // No item: tokens ahead of the first request's and behind the last one's are zeros, the workgroups without an item take
     // them in turn.
-    if (p.cu == nullptr) return;
+    if (p.cu == nullptr || PART == kPrefix) return;
     const int lead = min(max(p.cu[0], 0), p.T), n0 = min(max(p.cu[p.B], 0), p.T);
     const int64_t taken = (int64_t)it.items * p.cache.Hkv;
     const int64_t extra = (int)blockIdx.x - taken, n_extra = p.nblocks - taken;
@@ -345,7 +345,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   }
 
   const int d0 = 4 * g * L::PP + wave * XW;
-  if (it.nch > 1) {
+  if (PART != kWhole || it.nch > 1) {
     if ((unsigned)it.slot >= (unsigned)p.slots) return;
     const int64_t at = ((int64_t)it.slot * p.cache.Hkv + head) * kRows + c16;
     if (live) {
@@ -380,12 +380,18 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
 
 // Codes are loaded non-temporally: 64 requests at 16k, 32:8 D = 128, 170 -> 153 us, 16:8 D = 256 112 -> 98. At D = 512 only
 // where a request's rows are one row block (99 -> 95 us; two, which share tiles in L2, 96 -> 107).
-hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, bool once, hipStream_t stream) {
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int D, bool bf16, bool cap, bool once, Kv4Part part, hipStream_t stream) {
   auto go = [&](auto d, auto b, auto c) {
     constexpr int DD = decltype(d)::value;
     constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;
     const dim3 grid((unsigned)p.nblocks), wg(kWaves * 64);
-    if (DD < 512 || once) {
+    if (part == kPrefix) {
+      hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC, false, kPrefix>), grid, wg, 0, stream, p);
+    } else if (part == kRest && (DD < 512 || once)) {
+      hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC, true, kRest>), grid, wg, 0, stream, p);
+    } else if (part == kRest) {
+      hipLaunchKernelGGL((kv4_split_kernel<512, BB, CC, false, kRest>), grid, wg, 0, stream, p);
+    } else if (DD < 512 || once) {
       hipLaunchKernelGGL((kv4_split_kernel<DD, BB, CC, true>), grid, wg, 0, stream, p);
     } else {
       hipLaunchKernelGGL((kv4_split_kernel<512, BB, CC, false>), grid, wg, 0, stream, p);

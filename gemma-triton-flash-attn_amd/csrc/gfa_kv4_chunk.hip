@@ -82,7 +82,7 @@ __device__ __forceinline__ void mma32_decoded(f32x16& c, const i16x8& a, const i
 
 }  // namespace
 
-template <int D, bool IS_BF16, bool CAP>
+template <int D, bool IS_BF16, bool CAP, Kv4Part PART>
 __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const Kv4AttnParams p) {
   using L = Kv4Layout<D>;
   constexpr int ROWS = kv4_chunk_rows(D);
@@ -101,7 +101,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
   const int h = lane >> 5;
   const int head = p.hkv.rem((int)blockIdx.x);
 
-  const Item it = find_item<ROWS, true>(p, p.hkv.quot((int)blockIdx.x), lane);
+  const Item it = find_item<ROWS, true, PART>(p, p.hkv.quot((int)blockIdx.x), lane);
   if (it.b < 0) return;
   const Request& rq = it.rq;
   const int rb = rq.row_blocks - 1 - it.rb;  // the rows that see most keys first
@@ -424,7 +424,7 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
     const Row r0 = row_of(m, ln);
     float l = halves_sum(l_run[m]);
     if (m_ref[m] == -INFINITY && l == 0.f && seen[m]) l = 1.f;  // a mark, see row_inv
-    if (it.nch > 1) {
+    if (PART != kWhole || it.nch > 1) {
       if ((unsigned)it.slot >= (unsigned)p.slots) return;
       const int64_t at = part_at * ROWS + (wave * MT + m) * 32 + (ln & 31);
       if (ho == 0) {
@@ -470,22 +470,30 @@ __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const 
 }
 
 // Explicit instantiations: the host launch stubs must exist for each variant.
-#define GFA_KV4_CHUNK_INST(DD)                                                      \
-  template __global__ void kv4_chunk_kernel<DD, true, true>(const Kv4AttnParams);   \
-  template __global__ void kv4_chunk_kernel<DD, true, false>(const Kv4AttnParams);  \
-  template __global__ void kv4_chunk_kernel<DD, false, true>(const Kv4AttnParams);  \
-  template __global__ void kv4_chunk_kernel<DD, false, false>(const Kv4AttnParams);
+#define GFA_KV4_CHUNK_INST1(DD, PART)                                                     \
+  template __global__ void kv4_chunk_kernel<DD, true, true, PART>(const Kv4AttnParams);   \
+  template __global__ void kv4_chunk_kernel<DD, true, false, PART>(const Kv4AttnParams);  \
+  template __global__ void kv4_chunk_kernel<DD, false, true, PART>(const Kv4AttnParams);  \
+  template __global__ void kv4_chunk_kernel<DD, false, false, PART>(const Kv4AttnParams);
+#define GFA_KV4_CHUNK_INST(DD)      \
+  GFA_KV4_CHUNK_INST1(DD, kWhole)   \
+  GFA_KV4_CHUNK_INST1(DD, kPrefix)
 GFA_KV4_CHUNK_INST(64)
 GFA_KV4_CHUNK_INST(128)
 GFA_KV4_CHUNK_INST(256)
 GFA_KV4_CHUNK_INST(512)
 #undef GFA_KV4_CHUNK_INST
+#undef GFA_KV4_CHUNK_INST1
 
-hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int D, bool bf16, bool cap, hipStream_t stream) {
+hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int D, bool bf16, bool cap, Kv4Part part, hipStream_t stream) {
   auto go = [&](auto d, auto b, auto c) {
     constexpr int DD = decltype(d)::value;
     constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;
-    hipLaunchKernelGGL((kv4_chunk_kernel<DD, BB, CC>), dim3((unsigned)p.nblocks), dim3(256), 0, stream, p);
+    if (part == kPrefix) {
+      hipLaunchKernelGGL((kv4_chunk_kernel<DD, BB, CC, kPrefix>), dim3((unsigned)p.nblocks), dim3(256), 0, stream, p);
+    } else {
+      hipLaunchKernelGGL((kv4_chunk_kernel<DD, BB, CC, kWhole>), dim3((unsigned)p.nblocks), dim3(256), 0, stream, p);
+    }
   };
   auto by_type = [&](auto d) {
     if (bf16 && cap) go(d, std::true_type{}, std::true_type{});

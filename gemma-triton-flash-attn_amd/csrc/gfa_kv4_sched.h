@@ -20,22 +20,27 @@ struct Request {
   int t0, fresh, len;  // first new token, new tokens, tokens with the new ones
   int row_blocks;      // 0: not this kernel's
   int tiles;           // most key tiles that a row block sees
+  int skip;            // kRest: tokens of its prefix
 };
 // Its three loads go out together (one wait: their latency is a good part of a short call).
-template <int ROWS, bool LARGE>
+template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
 __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   Request r{};
   const int bc = min(b, p.B - 1);
   const int* cu = p.cu != nullptr ? p.cu : p.lens;  // without cu read for nothing
   const int t0 = cu[bc], t1 = cu[p.cu != nullptr ? bc + 1 : bc], len = p.lens[bc];
+  int skip = 0;
+  if constexpr (PART == kRest) skip = p.skip[bc];
   if (b >= p.B) return r;
   r.t0 = p.cu != nullptr ? t0 : b * p.each;
   r.fresh = p.cu != nullptr ? min(max((int)((unsigned)t1 - (unsigned)t0), 0), p.T) : p.each;
   r.len = max(len, 0);
+  if constexpr (PART == kPrefix) r.fresh = r.len > 0 ? r.fresh : 0;  // no prefix: nothing to do
+  if constexpr (PART == kRest) r.skip = max(skip, 0);
   const int rows = r.fresh * p.G;
   r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
   const int held = min(r.len, p.M << p.cache.bs_log2);
-  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : 0;
+  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : PART == kRest ? r.skip : 0;
   r.tiles = held > lo ? (held + kTile - 1) / kTile - lo / kTile : 0;
   if (p.window > 0) r.tiles = min(r.tiles, p.window_tiles);
   return r;
@@ -46,13 +51,14 @@ __device__ __forceinline__ int2 tiles_of_rows(const Kv4AttnParams& p, const Requ
   const int pos0 = r.len - r.fresh;  // position of new token 0
   const int held = min(r.len, p.M << p.cache.bs_log2);
   const int k_hi = p.causal ? min(held, pos0 + i_hi + 1) : held;
-  const int k_lo = p.window > 0 ? max(0, pos0 + i_lo - p.window + 1) : 0;
+  const int k_lo = p.window > 0 ? max(0, pos0 + i_lo - p.window + 1) : r.skip;
   return k_hi > k_lo ? make_int2(k_lo / kTile, (k_hi + kTile - 1) / kTile) : make_int2(0, 0);
 }
 // Lane src's request in every lane.
+template <Kv4Part PART = kWhole>
 __device__ __forceinline__ Request request_from(const Request& r, int src) {
   auto at = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
-  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles)};
+  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles), PART == kRest ? at(r.skip) : 0};
 }
 
 // Sum over the wave's lanes (the steps of wave_prefix_sum).
@@ -76,12 +82,12 @@ __device__ __forceinline__ float wave_sum(float x) {
 // sum is a float's (a product of two counts can pass 32 bits); `share` = Hkv / target is rounded up by more than the
 // sum can be off, so that the grid the host sized holds every item. The same operations in the same order wherever
 // it is taken: contraction is off.
-template <int ROWS, bool LARGE>
+template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
 __device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, const Request& r0, int lane) {
 #pragma clang fp contract(off)
   float total = (float)r0.row_blocks * (float)r0.tiles;
   for (int b0 = 64; b0 < p.B; b0 += 64) {
-    const Request r = request_of<ROWS, LARGE>(p, b0 + lane);
+    const Request r = request_of<ROWS, LARGE, PART>(p, b0 + lane);
     const float x = (float)r.row_blocks * (float)r.tiles;
     total += x;
   }
@@ -99,22 +105,22 @@ struct Item {
   int items;        // of the whole call, where b < 0
   int slot;         // of nch > 1: its place among the items of split row blocks
 };
-template <int ROWS, bool LARGE>
+template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
 __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int lane) {
   Item it{};
   it.b = -1;
-  Request r = request_of<ROWS, LARGE>(p, lane);
-  const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
+  Request r = request_of<ROWS, LARGE, PART>(p, lane);
+  const int per = chunk_tiles<ROWS, LARGE, PART>(p, r, lane);
   for (int b0 = 0;;) {
     const int nch = chunks_of(r, per);
-    const int mine = r.row_blocks * nch, split = nch > 1 ? mine : 0;
+    const int mine = r.row_blocks * nch, split = PART != kWhole || nch > 1 ? mine : 0;
     const int s = wave_prefix_sum(mine), z = wave_prefix_sum(split);
     const int before = it.items + s - mine;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
       it.b = b0 + src;
-      it.rq = request_from(r, src);
+      it.rq = request_from<PART>(r, src);
       it.nch = __builtin_amdgcn_readfirstlane(chunks_of(it.rq, per));
       const int i = item - __builtin_amdgcn_readlane(before, src);
       it.rb = __builtin_amdgcn_readfirstlane(quotient(i, it.nch));
@@ -125,7 +131,7 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
     it.items += __builtin_amdgcn_readlane(s, 63);
     it.slot += __builtin_amdgcn_readlane(z, 63);
     if ((b0 += 64) >= p.B) break;
-    r = request_of<ROWS, LARGE>(p, b0 + lane);
+    r = request_of<ROWS, LARGE, PART>(p, b0 + lane);
   }
   return it;
 }
@@ -137,23 +143,23 @@ struct RowBlock {
   int rb, nch;
   int slot;
 };
-template <int ROWS, bool LARGE>
+template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
 __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int block, int lane) {
   RowBlock out{};
   out.b = -1;
-  Request r = request_of<ROWS, LARGE>(p, lane);
-  const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
+  Request r = request_of<ROWS, LARGE, PART>(p, lane);
+  const int per = chunk_tiles<ROWS, LARGE, PART>(p, r, lane);
   int blocks = 0;
   for (int b0 = 0;;) {
     const int s = wave_prefix_sum(r.row_blocks);
-    const int nch = chunks_of(r, per), split = nch > 1 ? r.row_blocks * nch : 0;
+    const int nch = chunks_of(r, per), split = PART != kWhole || nch > 1 ? r.row_blocks * nch : 0;
     const int z = wave_prefix_sum(split);
     const int before = blocks + s - r.row_blocks;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(block >= before && block < before + r.row_blocks);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
       out.b = b0 + src;
-      out.rq = request_from(r, src);
+      out.rq = request_from<PART>(r, src);
       out.nch = __builtin_amdgcn_readfirstlane(chunks_of(out.rq, per));
       out.rb = block - __builtin_amdgcn_readlane(before, src);
       out.slot += __builtin_amdgcn_readlane(z - split, src) + out.rb * out.nch;
@@ -162,7 +168,7 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
     blocks += __builtin_amdgcn_readlane(s, 63);
     out.slot += __builtin_amdgcn_readlane(z, 63);
     if ((b0 += 64) >= p.B) break;
-    r = request_of<ROWS, LARGE>(p, b0 + lane);
+    r = request_of<ROWS, LARGE, PART>(p, b0 + lane);
   }
   return out;
 }

@@ -8,6 +8,11 @@ namespace gfa {
 struct Kv4RowsParams;
 struct Kv4PlanParams;
 struct Kv4AttnParams;
+enum Kv4Part : int;
+struct Kv4PagesParams;
+struct Kv4CopyParams;
+struct Kv4ShareParams;
+struct VerifyParams;
 
 hipError_t launch_fwd(const FwdParams& p, int head_dim, int block_kv, int nwaves, bool bf16, bool cap, bool drop,
                       hipStream_t stream);
@@ -27,8 +32,14 @@ hipError_t launch_bwd_dq_ds(const BwdDqDsParams& p, int head_dim, bool bf16, hip
 hipError_t launch_kv4_write(const Kv4RowsParams& p, int head_dim, bool bf16, hipStream_t stream);
 hipError_t launch_kv4_read(const Kv4RowsParams& p, int head_dim, bool bf16, hipStream_t stream);
 hipError_t launch_kv4_plan(const Kv4PlanParams& p, hipStream_t stream);
-hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, bool once, hipStream_t stream);
-hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, hipStream_t stream);
-hipError_t launch_kv4_join(const Kv4AttnParams& p, int head_dim, bool bf16, bool large, hipStream_t stream);
+hipError_t launch_kv4_fork(const Kv4PagesParams& p, hipStream_t stream);
+hipError_t launch_kv4_compact(const Kv4PagesParams& p, hipStream_t stream);
+hipError_t launch_kv4_copy(const Kv4CopyParams& p, hipStream_t stream);
+hipError_t launch_kv4_share(const Kv4ShareParams& p, hipStream_t stream);
+hipError_t launch_verify(const VerifyParams& p, int kind, hipStream_t stream);
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, bool once, Kv4Part part,
+                            hipStream_t stream);
+hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, Kv4Part part, hipStream_t stream);
+hipError_t launch_kv4_join(const Kv4AttnParams& p, int head_dim, bool bf16, bool large, Kv4Part part, hipStream_t stream);
 
 }  // namespace gfa

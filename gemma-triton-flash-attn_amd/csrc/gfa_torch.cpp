@@ -42,6 +42,13 @@ struct Api {
   decltype(&gfa_kv4_plan) kv4_plan = nullptr;
   decltype(&gfa_kv4_attn) kv4_attn = nullptr;
   decltype(&gfa_kv4_attn_workspace_bytes) kv4_attn_workspace_bytes = nullptr;
+  decltype(&gfa_kv4_fork) kv4_fork = nullptr;
+  decltype(&gfa_kv4_compact) kv4_compact = nullptr;
+  decltype(&gfa_kv4_pages_workspace_bytes) kv4_pages_workspace_bytes = nullptr;
+  decltype(&gfa_kv4_copy) kv4_copy = nullptr;
+  decltype(&gfa_kv4_share) kv4_share = nullptr;
+  decltype(&gfa_kv4_verify) kv4_verify = nullptr;
+  decltype(&gfa_kv4_verify_workspace_bytes) kv4_verify_workspace_bytes = nullptr;
   decltype(&gfa_last_error) last_error = nullptr;
   PyObject* error_type = nullptr;  // GfaError(status, message); held for the process
 } api;
@@ -444,7 +451,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv4_plan(const Tensor& lens, 
 
 Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& table,
                      const Tensor& lens, const std::optional<Tensor>& cu, int64_t max_new, bool causal, int64_t window,
-                     double scale, double softcap) {
+                     double scale, double softcap, const std::optional<Tensor>& shared_skip, const std::optional<Tensor>& shared_cu,
+                     const std::optional<Tensor>& shared_lens) {
   check_cache(codes, scales);
   check_token_rows("q", q, codes, bf16, false);
   const int64_t B = q.size(0), Hq = q.size(1), N = q.size(2), Hkv = codes.size(1);
@@ -462,7 +470,17 @@ Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
   }
   TORCH_CHECK_VALUE(window >= 0, "slide_size must be >= 0");
   TORCH_CHECK_VALUE(max_new >= 0, "max_new must be at least 1");
+  const bool shared = shared_skip && shared_cu && shared_lens;
+  TORCH_CHECK_VALUE(shared || (!shared_skip && !shared_cu && !shared_lens), "shared must hold all of skip, cu and lens");
+  if (shared) {
+    check_array("shared.skip", *shared_skip, at::kInt, 1, device);
+    check_array("shared.cu", *shared_cu, at::kInt, 1, device);
+    check_array("shared.lens", *shared_lens, at::kInt, 1, device);
+    TORCH_CHECK_VALUE(cu && shared_skip->size(0) == R && shared_cu->size(0) == R + 1 && shared_lens->size(0) == R,
+                      "shared is for ", shared_skip->size(0), " requests with cu, the call has ", R, cu ? "" : " without");
+  }
   const c10::DeviceGuard guard(device);
+  const Tensor ss = shared ? dense(*shared_skip) : Tensor(), sc = shared ? dense(*shared_cu) : Tensor(), sl = shared ? dense(*shared_lens) : Tensor();
   const Tensor qp = prep(q), lp = dense(lens), cp = cu ? dense(*cu) : Tensor();
   const Tensor o = out_like(qp);
   gfa_kv4_attn_args a{};
@@ -486,6 +504,11 @@ Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
   a.scale = (float)scale;
   a.softcap = (float)softcap;
   a.stream = stream_of(q);
+  if (shared) {
+    a.shared_skip = static_cast<const int32_t*>(ss.data_ptr());
+    a.shared_cu = static_cast<const int32_t*>(sc.data_ptr());
+    a.shared_lens = static_cast<const int32_t*>(sl.data_ptr());
+  }
   Tensor ws;
   const size_t need = api.kv4_attn_workspace_bytes(&a);
   if (need > 0) {
@@ -495,6 +518,224 @@ Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
   }
   check(api.kv4_attn(&a));
   return o;
+}
+
+// ---- Requests with something in common (kv4.py) ----
+
+int32_t* ints_of(const Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+
+std::vector<gfa_kv4_cache> caches_of(const std::vector<Tensor>& codes, const std::vector<Tensor>& scales) {
+  TORCH_CHECK_VALUE(!codes.empty() && codes.size() == scales.size(), "at least one cache is needed");
+  std::vector<gfa_kv4_cache> out(codes.size());
+  for (size_t i = 0; i < codes.size(); ++i) {
+    check_cache(codes[i], scales[i]);
+    TORCH_CHECK_VALUE(codes[i].device() == codes[0].device() && codes[i].size(0) == codes[0].size(0) && codes[i].size(3) == codes[0].size(3),
+                      "caches of ", codes[0].sizes(), " on ", codes[0].device(), " and ", codes[i].sizes(), " on ", codes[i].device(),
+                      " do not belong to one table");
+    out[i] = cache_of(codes[i], scales[i], true);  // bytes, whatever the type
+  }
+  return out;
+}
+
+// The free list, which is changed in place.
+void check_free(const Tensor& free_ids, const c10::Device& device) {
+  check_array("free", free_ids, at::kInt, 1, device);
+  TORCH_CHECK_VALUE(free_ids.is_contiguous() && !free_ids.is_neg() && free_ids.size(0) <= INT32_MAX, "free must be contiguous");
+}
+
+void check_rows_of_pages(const Tensor& table, int64_t rows) {
+  TORCH_CHECK_VALUE(rows > 0 && rows <= 4096 && table.size(0) <= 4096, table.size(0), " requests and ", rows, " rows (1 to 4096)");
+}
+
+std::tuple<Tensor, Tensor, Tensor> kv4_fork(const std::vector<Tensor>& codes, const std::vector<Tensor>& scales, const Tensor& table,
+                                            const Tensor& lens, const Tensor& free_ids, const Tensor& used,
+                                            const std::optional<Tensor>& parents, const std::optional<Tensor>& keep, bool apart) {
+  const auto caches = caches_of(codes, scales);
+  const auto device = codes[0].device();
+  check_array("lens", lens, at::kInt, 1, device);
+  const int64_t B = lens.size(0), stride = check_table(table, B, device), M = table.size(1);
+  check_free(free_ids, device);
+  check_array("used", used, at::kInt, 1, device);
+  TORCH_CHECK_VALUE(used.size(0) == 1, "used must hold one entry");
+  if (parents) check_array("parents", *parents, at::kInt, 1, device);
+  const int64_t R = parents ? parents->size(0) : B;
+  if (keep) {
+    check_array("keep", *keep, at::kInt, 1, device);
+    TORCH_CHECK_VALUE(keep->size(0) == R, "keep holds ", keep->size(0), " entries for ", R, " rows");
+  }
+  check_rows_of_pages(table, R);
+  const c10::DeviceGuard guard(device);
+  const Tensor l = dense(lens), u = dense(used), pp = parents ? dense(*parents) : Tensor(), kp = keep ? dense(*keep) : Tensor();
+  const size_t need = api.kv4_pages_workspace_bytes((int32_t)R);
+  const int64_t ws_ints = (int64_t)(need / 4);
+  const Tensor rest = at::empty({apart ? ws_ints : R * M + R + 1 + ws_ints}, lens.options());
+  const Tensor table_out = apart ? at::empty({R, M}, lens.options()) : part_of(rest, 0, {R, M}, {M, 1});
+  const Tensor lens_out = apart ? at::empty({R}, lens.options()) : part_of(rest, R * M, {R}, {1});
+  const Tensor used_out = apart ? at::empty({1}, lens.options()) : part_of(rest, R * M + R, {1}, {1});
+  gfa_kv4_pages_args a{};
+  a.caches = caches.data();
+  a.layers = (int32_t)caches.size();
+  a.table = ints_of(table);
+  a.table_stride = stride;
+  a.lens = ints_of(l);
+  a.requests = (int32_t)B;
+  a.table_width = (int32_t)M;
+  a.parents = parents ? ints_of(pp) : nullptr;
+  a.keep = keep ? ints_of(kp) : nullptr;
+  a.rows = (int32_t)R;
+  a.free_count = (int32_t)free_ids.size(0);
+  a.free_ids = ints_of(free_ids);
+  a.used = ints_of(u);
+  a.table_out = ints_of(table_out);
+  a.lens_out = ints_of(lens_out);
+  a.used_out = ints_of(used_out);
+  a.workspace = ints_of(rest) + (apart ? 0 : R * M + R + 1);
+  a.workspace_bytes = need;
+  a.stream = stream_of(codes[0]);
+  check(api.kv4_fork(&a));
+  return {table_out, lens_out, used_out};
+}
+
+std::tuple<Tensor, Tensor> kv4_compact(const std::vector<Tensor>& codes, const std::vector<Tensor>& scales, const Tensor& table,
+                                       const Tensor& lens, const Tensor& free_ids, bool apart) {
+  const auto caches = caches_of(codes, scales);
+  const auto device = codes[0].device();
+  check_array("lens", lens, at::kInt, 1, device);
+  const int64_t B = lens.size(0), stride = check_table(table, B, device), M = table.size(1), blocks = codes[0].size(0);
+  check_free(free_ids, device);
+  TORCH_CHECK_VALUE(free_ids.size(0) == blocks, "free holds ", free_ids.size(0), " entries, a compacted pool's all of its ", blocks, " blocks");
+  check_rows_of_pages(table, B);
+  const c10::DeviceGuard guard(device);
+  const Tensor l = dense(lens);
+  const size_t need = api.kv4_pages_workspace_bytes((int32_t)blocks);
+  const int64_t ws_ints = (int64_t)(need / 4);
+  // the workspace is the larger part, and nobody keeps it
+  const Tensor ws = at::empty({ws_ints}, lens.options()), out = at::empty({apart ? B * M : B * M + 1}, lens.options());
+  const Tensor table_out = part_of(out, 0, {B, M}, {M, 1});
+  const Tensor used_out = apart ? at::empty({1}, lens.options()) : part_of(out, B * M, {1}, {1});
+  gfa_kv4_pages_args a{};
+  a.caches = caches.data();
+  a.layers = (int32_t)caches.size();
+  a.table = ints_of(table);
+  a.table_stride = stride;
+  a.lens = ints_of(l);
+  a.requests = (int32_t)B;
+  a.table_width = (int32_t)M;
+  a.free_count = (int32_t)blocks;
+  a.free_ids = ints_of(free_ids);
+  a.table_out = ints_of(table_out);
+  a.used_out = ints_of(used_out);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = need;
+  a.stream = stream_of(codes[0]);
+  check(api.kv4_compact(&a));
+  return {table_out, used_out};
+}
+
+void kv4_copy(const std::vector<Tensor>& codes, const std::vector<Tensor>& scales, const Tensor& src, const Tensor& dst) {
+  const auto caches = caches_of(codes, scales);
+  const auto device = codes[0].device();
+  check_array("src", src, at::kInt, 1, device);
+  check_array("dst", dst, at::kInt, 1, device);
+  TORCH_CHECK_VALUE(src.size(0) == dst.size(0) && src.size(0) <= INT32_MAX, "src holds ", src.size(0), " entries, dst ", dst.size(0));
+  const c10::DeviceGuard guard(device);
+  const Tensor s = dense(src), d = dense(dst);
+  check(api.kv4_copy(caches.data(), (int32_t)caches.size(), ints_of(s), ints_of(d), (int32_t)s.size(0), stream_of(codes[0])));
+}
+
+std::tuple<Tensor, Tensor, Tensor> kv4_share(const Tensor& table, const Tensor& lens, const Tensor& cu, int64_t block_size, int64_t least,
+                                             bool apart) {
+  const auto device = lens.device();
+  check_array("lens", lens, at::kInt, 1, device);
+  const int64_t R = lens.size(0), stride = check_table(table, R, device);
+  check_array("cu", cu, at::kInt, 1, device);
+  TORCH_CHECK_VALUE(cu.size(0) == R + 1, "cu holds ", cu.size(0), " entries for ", R, " requests");
+  TORCH_CHECK_VALUE(block_size_ok(block_size), "block_size=", block_size, " must be a power of two, 32 to 1024");
+  TORCH_CHECK_VALUE(least >= 1, "least=", least, " must be at least 1");
+  TORCH_CHECK_VALUE(R <= 4096, R, " requests (most 4096)");
+  const c10::DeviceGuard guard(device);
+  const Tensor l = dense(lens), c = dense(cu);
+  const Tensor all = apart ? Tensor() : at::empty({3 * R + 1}, lens.options());
+  const auto out = [&](int64_t offset, int64_t n) { return apart ? at::empty({n}, lens.options()) : part_of(all, offset, {n}, {1}); };
+  const Tensor skip = out(0, R), cu_out = out(R, R + 1), lens_out = out(2 * R + 1, R);
+  gfa_kv4_share_args a{};
+  a.table = ints_of(table);
+  a.table_stride = stride;
+  a.lens = ints_of(l);
+  a.cu = ints_of(c);
+  a.requests = (int32_t)R;
+  a.table_width = (int32_t)table.size(1);
+  a.block_size = (int32_t)block_size;
+  a.least = (int32_t)std::min<int64_t>(least, INT32_MAX);
+  a.skip = ints_of(skip);
+  a.cu_out = ints_of(cu_out);
+  a.lens_out = ints_of(lens_out);
+  a.stream = stream_of(lens);
+  check(api.kv4_share(&a));
+  return {skip, cu_out, lens_out};
+}
+
+// Rows of probabilities, read in place where their entries are side by side.
+Tensor probability_rows(const Tensor& t) {
+  if (t.is_neg()) return t.resolve_neg().contiguous();
+  return (t.size(1) == 1 || t.stride(1) == 1) && t.stride(0) >= 0 ? t : t.contiguous();
+}
+
+std::tuple<Tensor, Tensor, Tensor> kv4_verify(const Tensor& target, const std::optional<Tensor>& draft, const Tensor& tokens,
+                                              const Tensor& accept, const Tensor& sample, const Tensor& lens, const std::optional<Tensor>& cu) {
+  const auto type = target.scalar_type();
+  TORCH_CHECK_TYPE(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, "target is ", type, " (fp32, fp16 or bf16)");
+  TORCH_CHECK_VALUE(target.dim() == 2, "target must be 2-D (tokens, vocabulary), got shape ", target.sizes());
+  TORCH_CHECK_VALUE(target.is_cuda(), "target must be on a GPU (the engine has no CPU path), is on ", target.device());
+  const auto device = target.device();
+  const int64_t T = target.size(0), V = target.size(1);
+  TORCH_CHECK_VALUE(T > 0 && V > 0 && T <= INT32_MAX && V <= 1 << 30, "target of shape ", target.sizes());
+  if (draft) {
+    TORCH_CHECK_TYPE(draft->scalar_type() == type, "draft is ", draft->scalar_type(), ", target ", type);
+    TORCH_CHECK_VALUE(draft->sizes() == target.sizes(), "shape mismatch: target ", target.sizes(), ", draft ", draft->sizes());
+    TORCH_CHECK_VALUE(on_gpu(*draft, device), "draft must be on the call's GPU (", device, "), is on ", draft->device());
+  }
+  check_array("tokens", tokens, at::kLong, 1, device);
+  check_array("accept", accept, at::kFloat, 1, device);
+  TORCH_CHECK_VALUE(tokens.size(0) == T && accept.size(0) == T, "tokens holds ", tokens.size(0), " entries and accept ", accept.size(0),
+                    " for ", T, " rows of target");
+  check_array("lens", lens, at::kInt, 1, device);
+  check_array("sample", sample, at::kFloat, 1, device);
+  const int64_t R = lens.size(0);
+  TORCH_CHECK_VALUE(R > 0 && R <= 65535 && sample.size(0) == R, "sample holds ", sample.size(0), " entries for ", R, " requests (1 to 65535)");
+  if (cu) {
+    check_array("cu", *cu, at::kInt, 1, device);
+    TORCH_CHECK_VALUE(cu->size(0) == R + 1, "cu holds ", cu->size(0), " entries for ", R, " requests");
+  } else {
+    TORCH_CHECK_VALUE(T % R == 0, T, " tokens do not divide among ", R, " requests (pass cu)");
+  }
+  const c10::DeviceGuard guard(device);
+  const Tensor p = probability_rows(target), q = draft ? probability_rows(*draft) : Tensor();
+  const Tensor x = dense(tokens), u = dense(accept), r = dense(sample), l = dense(lens), c = cu ? dense(*cu) : Tensor();
+  const Tensor follows = at::empty({T}, tokens.options()), accepted = at::empty({R}, lens.options()), lens_out = at::empty({R}, lens.options());
+  gfa_kv4_verify_args a{};
+  a.target = p.data_ptr();
+  a.draft = draft ? q.data_ptr() : nullptr;
+  a.target_stride = p.stride(0);
+  a.draft_stride = draft ? q.stride(0) : 0;
+  a.type = type == at::kFloat ? 2 : type == at::kBFloat16 ? 1 : 0;
+  a.token_count = (int32_t)T;
+  a.vocab = (int32_t)V;
+  a.requests = (int32_t)R;
+  a.tokens = static_cast<const int64_t*>(x.data_ptr());
+  a.accept = static_cast<const float*>(u.data_ptr());
+  a.sample = static_cast<const float*>(r.data_ptr());
+  a.lens = ints_of(l);
+  a.cu = cu ? ints_of(c) : nullptr;
+  a.follows = static_cast<int64_t*>(follows.data_ptr());
+  a.accepted = ints_of(accepted);
+  a.lens_out = ints_of(lens_out);
+  a.workspace_bytes = api.kv4_verify_workspace_bytes(a.requests, a.vocab);
+  const Tensor ws = at::empty({(int64_t)a.workspace_bytes}, lens.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.stream = stream_of(target);
+  check(api.kv4_verify(&a));
+  return {follows, accepted, lens_out};
 }
 
 template <typename F>
@@ -522,6 +763,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     api.kv4_attn = pointer<decltype(api.kv4_attn)>(attn);
     api.kv4_attn_workspace_bytes = pointer<decltype(api.kv4_attn_workspace_bytes)>(workspace_bytes);
   });
+  m.def("bind_kv4_pages", [](uintptr_t fork, uintptr_t compact, uintptr_t workspace_bytes, uintptr_t copy, uintptr_t share, uintptr_t verify,
+                             uintptr_t verify_workspace_bytes) {
+    api.kv4_fork = pointer<decltype(api.kv4_fork)>(fork);
+    api.kv4_compact = pointer<decltype(api.kv4_compact)>(compact);
+    api.kv4_pages_workspace_bytes = pointer<decltype(api.kv4_pages_workspace_bytes)>(workspace_bytes);
+    api.kv4_copy = pointer<decltype(api.kv4_copy)>(copy);
+    api.kv4_share = pointer<decltype(api.kv4_share)>(share);
+    api.kv4_verify = pointer<decltype(api.kv4_verify)>(verify);
+    api.kv4_verify_workspace_bytes = pointer<decltype(api.kv4_verify_workspace_bytes)>(verify_workspace_bytes);
+  });
+  m.def("kv4_fork", torch::wrap_pybind_function_no_gil(kv4_fork));
+  m.def("kv4_compact", torch::wrap_pybind_function_no_gil(kv4_compact));
+  m.def("kv4_copy", torch::wrap_pybind_function_no_gil(kv4_copy));
+  m.def("kv4_share", torch::wrap_pybind_function_no_gil(kv4_share));
+  m.def("kv4_verify", torch::wrap_pybind_function_no_gil(kv4_verify));
   m.def("kv4_cache", torch::wrap_pybind_function_no_gil(check_cache));
   m.def("kv4_write", torch::wrap_pybind_function_no_gil(kv4_write));
   m.def("kv4_read", torch::wrap_pybind_function_no_gil(kv4_read));

@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define GFA_VERSION 108 /* 1.0.8: key/value cache in 4 bits (1.0.7: segment tables from position ids and masks, 1.0.6: materialised backward, 1.0.5: run-time work distribution, 1.0.4: attention dropout, 1.0.3: soft-capping) */
+#define GFA_VERSION 109 /* 1.0.8: key/value cache in 4 bits (1.0.7: segment tables from position ids and masks, 1.0.6: materialised backward, 1.0.5: run-time work distribution, 1.0.4: attention dropout, 1.0.3: soft-capping) */
 
 typedef enum {
   GFA_DTYPE_FP16 = 0,
@@ -337,11 +337,115 @@ typedef struct {
   void* workspace;      /* >= gfa_kv4_attn_workspace_bytes(args), 16-byte aligned */
   size_t workspace_bytes;
   void* stream;
+  /* gfa_kv4_share's results for this table, lens and cu, or NULL: the groups' prefixes are attended to once for all of a
+   * group's queries. The same result, but for the order of sums. Without effect with a window or for requests of many rows. */
+  const int32_t* shared_skip; /* (requests) */
+  const int32_t* shared_cu;   /* (requests + 1) */
+  const int32_t* shared_lens; /* (requests) */
 } gfa_kv4_attn_args;
 
 int gfa_kv4_attn(const gfa_kv4_attn_args* args);
 /* Workspace of gfa_kv4_attn(args) in bytes; pointers are not read, but for whether cu is NULL. */
 size_t gfa_kv4_attn_workspace_bytes(const gfa_kv4_attn_args* args);
+
+/* ---- Requests with something in common ----
+ *
+ * Pages. Rows of a block table may hold the same blocks. caches is a host array of the layers' caches, all of one num_blocks (at
+ * most 2^18) and block_size, whose blocks the table's rows hold; at most 4096 requests and rows. Entries of the table outside
+ * [0, num_blocks) are no block, request b holds the first ceil(lens[b] / block_size). Values in the arrays cannot
+ * make a call address memory outside them.
+ *
+ * gfa_kv4_fork: the block tables of the next step's requests. Row r takes request parents[r] (outside [0, requests): an empty
+ * row; NULL: request r) and keeps its first min(lens, keep[r]) tokens (keep NULL: all). A block of which a row keeps only a part is
+ * the row's to write to: it stays with the first such row if no row keeps it whole, and every other such row gets a copy
+ * of it, in every cache. Blocks of the requests that no row holds any more are given back: in ascending order they become the
+ * last ones ahead of *used in free_ids (at most *used of them). Copies take, in the order of the rows, the blocks just given
+ * back and then the entries from *used on; where the list ends the row's entry is -1, and *used_out above free_count tells of it.
+ * gfa_kv4_compact: of the n blocks that requests hold, the k-th (in ascending order) at or past n is moved, in every cache, to
+ * the k-th block below n that no request holds; free_ids (num_blocks entries: all of the pool) becomes 0, 1, ... and *used_out n.
+ * parents, keep, rows, used and lens_out are not read.
+ * table_out (rows, compact: requests; table_width) and lens_out must not overlap the inputs. Two launches and more: the tables
+ * first, then the blocks' bytes. */
+typedef struct {
+  const gfa_kv4_cache* caches;
+  int32_t layers;
+  const int32_t* table; /* (requests, table_width), rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* lens; /* (requests) */
+  int32_t requests, table_width;
+  const int32_t* parents; /* (rows) or NULL */
+  const int32_t* keep;    /* (rows) or NULL */
+  int32_t rows;
+  int32_t free_count;
+  int32_t* free_ids;   /* (free_count), changed in place */
+  const int32_t* used; /* (1) */
+  int32_t* table_out;  /* (rows, table_width) */
+  int32_t* lens_out;   /* (rows) */
+  int32_t* used_out;   /* (1) */
+  void* workspace;     /* >= gfa_kv4_pages_workspace_bytes, 4-byte aligned */
+  size_t workspace_bytes;
+  void* stream;
+} gfa_kv4_pages_args;
+
+int gfa_kv4_fork(const gfa_kv4_pages_args* args);
+int gfa_kv4_compact(const gfa_kv4_pages_args* args);
+/* Workspace of gfa_kv4_fork with so many rows, or of gfa_kv4_compact of so many blocks. */
+size_t gfa_kv4_pages_workspace_bytes(int32_t rows_or_blocks);
+
+/* Copies block src[i] to block dst[i] in every cache; pairs with an id outside [0, num_blocks) are left out. No block may be a
+ * destination twice, or a destination and a source. */
+int gfa_kv4_copy(const gfa_kv4_cache* caches, int32_t layers, const int32_t* src, const int32_t* dst, int32_t pairs, void* stream);
+
+/* What neighbouring requests of a step have in common, as gfa_kv4_attn takes it: the whole blocks that a request's row and the row
+ * before it begin with, ahead of both requests' new tokens (cu). Neighbours with at least `least` tokens in common are a group, the
+ * fewest tokens that two neighbours in it have in common are its prefix. skip (requests): tokens of the request's prefix, 0
+ * without a group; cu_out (requests + 1) and lens_out (requests): the groups' new tokens as one request's, cu_out[b + 1] -
+ * cu_out[b] of them over lens_out[b] tokens (0 for all requests but a group's first). At most 4096 requests. */
+typedef struct {
+  const int32_t* table; /* (requests, table_width), rows table_stride apart */
+  int64_t table_stride;
+  const int32_t* lens; /* (requests): tokens with the new ones */
+  const int32_t* cu;   /* (requests + 1) */
+  int32_t requests, table_width, block_size, least;
+  int32_t* skip;
+  int32_t* cu_out;
+  int32_t* lens_out;
+  void* stream;
+} gfa_kv4_share_args;
+
+int gfa_kv4_share(const gfa_kv4_share_args* args);
+
+/* Verification of drafted tokens. Request b's tokens of the step are cu[b] .. cu[b + 1] - 1 (cu NULL: token_count / requests
+ * each): its last known token and the drafted ones. target (token_count, vocab): row t the target's probabilities of what follows
+ * token t; draft: row t the probabilities that token t was drawn from (not read for a request's first; NULL: the tokens were
+ * proposed for certain). Token t is accepted, in the order of a request's, while accept[t] * draft[t, x] < target[t - 1, x], x = tokens[t]
+ * (a token outside the vocabulary is not). Behind the accepted ones a token is drawn: where one was not accepted from max(target -
+ * draft, 0), else from the target: the first entry at which the running sum of weights exceeds sample[b] times their sum, in 64 bits.
+ * Where no weight is left the target's probabilities are taken instead, and without any of those the token is -1. What is
+ * not a finite positive number counts as probability 0, sample as the nearest in [0, 1].
+ * follows[t]: the token that follows token t in the request: a drafted one that was accepted, the drawn one, then -1 (also for
+ * tokens of no request). accepted (requests): drafted tokens accepted. lens_out = lens less the drafted tokens that were not. */
+typedef struct {
+  const void* target;
+  const void* draft;
+  int64_t target_stride, draft_stride; /* elements from row to row */
+  int32_t type;                        /* 0 fp16, 1 bf16, 2 fp32 */
+  int32_t token_count, vocab, requests;
+  const int64_t* tokens; /* (token_count) */
+  const float* accept;   /* (token_count), uniform in [0, 1) */
+  const float* sample;   /* (requests), uniform in [0, 1) */
+  const int32_t* lens;   /* (requests) */
+  const int32_t* cu;     /* (requests + 1) or NULL */
+  int64_t* follows;      /* (token_count) */
+  int32_t* accepted;     /* (requests) */
+  int32_t* lens_out;     /* (requests) */
+  void* workspace;       /* >= gfa_kv4_verify_workspace_bytes(requests, vocab), 8-byte aligned */
+  size_t workspace_bytes;
+  void* stream;
+} gfa_kv4_verify_args;
+
+int gfa_kv4_verify(const gfa_kv4_verify_args* args);
+size_t gfa_kv4_verify_workspace_bytes(int32_t requests, int32_t vocab);
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* gfa_last_error(void);

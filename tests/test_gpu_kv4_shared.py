@@ -1,0 +1,256 @@
+"""What requests have in common, and attention that computes it once: against the definition, and against the plain call."""
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from kv4_cases import check
+from kv4_sharing_cases import Answers, ints
+from oracle import kv4_sharing_oracle as orc
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- share ----
+
+def same_as_defined(table, lens, cu, bs, least, device):
+    from gemma_triton_flash_attn_amd import kv4
+
+    t = table if isinstance(table, torch.Tensor) else ints(table, device)
+    got = kv4.share(t, ints(lens, device), ints(cu, device), block_size=bs, least=least)
+    want = orc.share(t.tolist(), lens, cu, bs, least)
+    assert [x.tolist() for x in got] == [list(x) for x in want]
+    return want
+
+
+def test_share_by_hand(device):
+    table = [[5, 6, 7, 1], [5, 6, 7, 2], [5, 6, 8, 3], [9, 6, 7, 1], [9, 4, 0, 0]]
+    want = same_as_defined(table, [256, 250, 200, 130, 70], [0, 1, 3, 4, 5, 6], 64, 64, device)
+    assert want == ([128, 128, 128, 64, 64], [0, 4, 4, 4, 6, 6], [128, 0, 0, 64, 0])
+    # a longer least keeps the third apart; the first two share what is full ahead of their new tokens
+    want = same_as_defined(table, [256, 250, 200, 130, 70], [0, 1, 3, 4, 5, 6], 64, 129, device)
+    assert want == ([192, 192, 0, 0, 0], [0, 3, 3, 4, 5, 6], [192, 0, 0, 0, 0])
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_share_any(seed, device):
+    r = random.Random(seed)
+    R, M, bs = r.choice([1, 2, 33, 300]), r.choice([1, 7, 130, 400]), r.choice([32, 64, 1024])
+    rows = [[r.randint(-1, 9) for _ in range(M)]]
+    for _ in range(R - 1):
+        n = r.choice([0, 1, M // 2, M, M])
+        rows.append(rows[-1][:n] + [r.randint(-1, 9) for _ in range(M - n)])
+    lens = [r.choice([0, 5, M * bs, r.randint(0, M * bs), M * bs + 70]) for _ in range(R)]
+    cu = [r.choice([0, 4])]
+    for n in lens:
+        cu.append(cu[-1] + r.choice([0, 1, 1, 8, min(n, 100)]))
+    wide = torch.cat([ints(rows, device), torch.full((R, 3), 7, dtype=torch.int32, device=device)], 1)[:, :M]
+    same_as_defined(wide, lens, cu, bs, r.choice([1, bs, 4 * bs, 1 << 40]) if seed else 1, device)
+
+
+def test_share_many(device):
+    """As many requests as a call takes, in groups of 1 to 1500."""
+    r = random.Random(3)
+    rows, n = [], 0
+    while len(rows) < 4096:
+        for _ in range(r.choice([1, 2, 30, 1500])):
+            rows.append([n, n + 1, r.randint(0, 3)])
+        n += 2
+    rows = rows[:4096]
+    same_as_defined(rows, [r.randint(90, 96) for _ in rows], list(range(4097)), 32, 64, device)
+
+
+# ---- attention ----
+
+CASES = {
+    # groups (requests, common tokens), own tokens of a request (least, most), new tokens, Hq, Hkv, D, bs, dtype
+    "d512_few": ([(4, 700)], (1, 90), 1, 8, 1, 512, 64, torch.bfloat16),
+    "d512_many": ([(20, 900)], (1, 90), 1, 16, 2, 512, 64, torch.bfloat16),
+    "d256_few": ([(2, 1300), (1, 0)], (1, 40), 1, 8, 4, 256, 128, torch.float16),
+    "d256_many": ([(30, 640), (3, 2000), (2, 64)], (1, 200), 1, 16, 4, 256, 64, torch.bfloat16),
+    "d128_many": ([(40, 2100), (1, 77), (17, 333)], (1, 70), 1, 32, 8, 128, 32, torch.bfloat16),
+    "d128_drafts": ([(9, 1500), (1, 10), (2, 700)], (8, 300), 5, 16, 8, 128, 64, torch.float16),
+    "d64_many": ([(70, 1111)], (1, 33), 1, 8, 2, 64, 32, torch.bfloat16),
+    "d64_drafts": ([(5, 4000), (70, 512)], (3, 50), 3, 15, 5, 64, 64, torch.float16),
+    "d512_drafts": ([(7, 1000), (2, 320)], (4, 100), 4, 8, 1, 512, 64, torch.float16),
+    "long": ([(3, 20000)], (1, 3000), 1, 8, 2, 128, 256, torch.bfloat16),
+}
+
+
+def answers(name, device, seed=0, pad=0, **kw):
+    groups, (lo, hi), new, Hq, Hkv, D, bs, dtype = CASES[name]
+    r = random.Random(name)
+    lens = [c // bs * bs + r.randint(max(lo, new), hi) for n, c in groups for _ in range(n)]
+    return Answers(device, lens, [new] * len(lens), Hq, Hkv, D, groups, bs=bs, dtype=dtype, seed=seed, pad=pad, **kw).store()
+
+
+def run(a, shared, **kw):
+    return a.attend(max_new=max(a.new), shared=shared, **kw)
+
+
+@pytest.mark.parametrize("name", list(CASES))
+def test_against_the_definition(name, device):
+    a = answers(name, device, pad=3)
+    s = a.share()
+    assert int(s.lens.max()) >= 64 and int(s.skip.max()) == int(s.lens.max())
+    o = run(a, s)
+    want, bound = a.expected()
+    check(o, want, bound)
+    assert not o[:, :, -3:].any()
+    assert torch.equal(o, run(a, s))  # the order of sums is fixed
+
+
+@pytest.mark.parametrize("name", ["d512_many", "d128_drafts", "d64_drafts", "d256_few"])
+def test_masks_and_caps(name, device):
+    """Cross attention, soft-capping, a scale; with a window the plain path, bit for bit."""
+    a = answers(name, device, seed=1)
+    s = a.share()
+    for kw in (dict(causal=False), dict(softcap=20.0), dict(scale=0.3, softcap=5.0, causal=False)):
+        o = run(a, s, **kw)
+        want, bound = a.expected(causal=kw.get("causal", True), softcap=kw.get("softcap", 0.0), scale=kw.get("scale"))
+        check(o, want, bound)
+    assert torch.equal(run(a, s, slide_size=100), run(a, None, slide_size=100))
+
+
+def test_mixed_counts(device):
+    """Requests with no new tokens, one, several: in a group, and between groups; max_new unknown or wrong; an empty request."""
+    lens, new = [400, 410, 390, 0, 5, 850, 860, 849], [1, 0, 6, 0, 2, 3, 1, 2]
+    a = Answers(device, lens, new, 8, 2, 128, [(3, 384), (2, 0), (3, 832)], bs=32, pad=2).store()
+    want, bound = a.expected()
+    s = a.share()
+    assert s.skip.tolist() == [384, 384, 384, 0, 0, 832, 832, 832]
+    for kw in (dict(max_new=6), dict(), dict(max_new=1)):
+        check(a.attend(shared=s, **kw), want, bound)
+    q = a.q.to(device)
+    assert torch.equal(q.cpu(), a.q)
+
+
+def test_many_rows_take_the_plain_path(device):
+    """A prompt's chunk of each of two answers: bit for bit the call without shared."""
+    a = Answers(device, [700, 710], [100, 60], 8, 2, 128, [(2, 512)], bs=64).store()
+    assert a.share().lens.tolist() == [512, 0]
+    assert torch.equal(run(a, a.share()), run(a, None))
+
+
+def test_nothing_in_common(device):
+    """No group: sums are joined all the same, within the same bound."""
+    a = Answers(device, [300, 1000, 64, 1], [1, 1, 1, 1], 8, 2, 128, [(4, 0)], bs=64).store()
+    s = a.share()
+    assert not s.skip.any() and not s.lens.any()
+    check(run(a, s), *a.expected())
+
+
+def test_missing_blocks(device):
+    """Blocks missing in a prefix, all of a prefix, all of a request's own."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    for holes, whole in (([2], False), ([0, 1, 2, 3, 4, 5, 6, 7], False), ([1], True)):
+        a = Answers(device, [530, 545, 513], [1, 1, 1], 8, 2, 128, [(3, 512)], bs=64).store()
+        held = [torch.ones(n, dtype=torch.bool) for n in a.lens]
+        for c in holes:
+            a.table[:, c] = -1
+            for h in held:
+                h[c * 64:(c + 1) * 64] = False
+        if whole:
+            a.table[1, 8:] = 1 << 20
+            held[1][512:] = False
+        s = kv4.share(a.table, a.lens_dev, a.cu, block_size=64, least=64)
+        assert s.skip.tolist() == [512] * 3
+        check(run(a, s), *a.expected(held=held))
+    a.table.fill_(-1)  # nothing at all: zeros
+    assert not run(a, kv4.share(a.table, a.lens_dev, a.cu, block_size=64, least=64)).any()
+
+
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_values_that_are_no_numbers(where, device):
+    """A token of no number in the prefix reaches its whole group, one in a request's own keys that request alone."""
+    a = Answers(device, [530, 545, 513, 300, 300], [1] * 5, 8, 2, 128, [(3, 512), (2, 256)], bs=64)
+    for b in range(3) if where == "prefix" else [1]:
+        a.k[b][0, 100 if where == "prefix" else 530, 3] = float("inf")
+    a.store()
+    o = run(a, a.share())
+    want, bound = a.expected()
+    assert torch.isnan(want[:, 1]).any() and not torch.isnan(want[:, 3:]).any()
+    check(o, want, bound)
+
+
+def test_infinite_queries(device):
+    """A query of infinities answers NaN in both parts and leaves its neighbours alone."""
+    a = Answers(device, [530, 545, 513], [1, 1, 1], 8, 2, 128, [(3, 512)], bs=64).store()
+    plain = run(a, a.share())
+    a.q[0, 2, 1] = float("inf")
+    o = run(a, a.share())
+    assert torch.isnan(o[0, 2, 1]).all()
+    keep = torch.ones_like(o, dtype=torch.bool)
+    keep[0, 2, 1] = False
+    assert torch.equal(o[keep], plain[keep])
+
+
+def test_one_token_per_batch_entry(device):
+    """(R, Hq, 1, D) queries, strided, with cu."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    a = answers("d128_many", device)
+    s = a.share()
+    want = run(a, s)
+    q = a.q[0].transpose(0, 1)[:, :, None].contiguous().to(device)  # (R, Hq, 1, D)
+    wide = torch.cat([q, q], 3)[..., :128]
+    for x in (q, wide, wide.transpose(1, 2).contiguous().transpose(1, 2)):
+        o = kv4.attention(x, a.cache, a.table, a.lens_dev, a.cu, max_new=1, shared=s)
+        assert o.shape == x.shape and torch.equal(o[:, :, 0].transpose(0, 1), want[0])
+
+
+def test_captured(device):
+    """A graph of share and attention replayed while lengths and tables change in device memory; another call's workspace in
+    between."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    a, other = answers("d256_many", device, junk=0), answers("d128_many", device)  # rows that look past what was stored: numbers
+    table, lens, q = a.table.clone(), a.lens_dev.clone(), a.q.to(device)
+
+    def step():
+        s = kv4.share(table, lens, a.cu, block_size=a.bs, least=64)
+        return kv4.attention(q, a.cache, table, lens, a.cu, max_new=1, shared=s)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    s = other.share()
+    oq = other.q.to(device)
+    with torch.cuda.graph(second):
+        got2 = kv4.attention(oq, other.cache, other.table, other.lens_dev, other.cu, max_new=1, shared=s)
+    r = random.Random(0)
+    for i in range(4):
+        lens.copy_(ints([n - r.choice([0, 0, 64, 200]) if n > 300 else n for n in a.lens], device))
+        table.copy_(a.table.roll(i, 0) if i == 2 else a.table)
+        q.copy_(a.q.roll(i, 3))
+        graph.replay()
+        second.replay()
+        seen, seen2 = got.clone(), got2.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(seen, step()) and torch.equal(seen2, run(other, s))
+
+
+def test_registered(device):
+    from gemma_triton_flash_attn_amd import kv4
+
+    a = answers("d64_many", device)
+    s = a.share()
+    q = a.q.to(device)
+    torch.library.opcheck(torch.ops.gfa.kv4_share, (a.table, a.lens_dev, a.cu, a.bs, 64))
+    args = (q, a.cache.codes, a.cache.scales, True, a.table, a.lens_dev, a.cu, 1, True, 0, 0.125, 0.0, *s)
+    torch.library.opcheck(torch.ops.gfa.kv4_attention, args)
+
+    def step(q, codes, scales, table, lens, cu):
+        cache = kv4.Cache(codes, scales, torch.bfloat16)
+        return kv4.attention(q, cache, table, lens, cu, max_new=1, shared=kv4.share(table, lens, cu, block_size=a.bs, least=64))
+
+    args = (q, a.cache.codes, a.cache.scales, a.table, a.lens_dev, a.cu)
+    assert torch.equal(torch.compile(step, fullgraph=True, backend="aot_eager")(*args), step(*args))
