@@ -25,7 +25,7 @@ LIB = os.path.join(HERE, "libgfa.so")
 TORCH_LIB = os.path.join(HERE, "_gfa_torch.so")
 SOURCES = ["gfa_fwd.hip", "gfa_fwd_rows.hip", "gfa_bwd_dq.hip", "gfa_bwd_dkv.hip", "gfa_bwd_ds.hip", "gfa_segments.hip",
            "gfa_api.hip", "gfa_kv4_store.hip", "gfa_kv4_attn.hip", "gfa_kv4_chunk.hip",
-           "gfa_kv4_join.hip", "gfa_kv4_pages.hip", "gfa_verify.hip", "gfa_kv4_api.hip"]
+           "gfa_kv4_join.hip", "gfa_kv4_shared.hip", "gfa_kv4_pages.hip", "gfa_verify.hip", "gfa_kv4_api.hip"]
 ARCH = "gfx950"
 
 

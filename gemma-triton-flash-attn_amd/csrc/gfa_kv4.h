@@ -203,11 +203,12 @@ constexpr int kv4_chunk_rows(int D) { return D >= 128 ? 128 : 256; }
 
 // Workgroups of the chunk kernel that a CU holds (by their registers).
 constexpr int kv4_chunk_wgs(int D) { return D == 512 ? 1 : D == 128 ? 3 : 2; }
+// Workgroups of the shared prefixes' kernel that a CU holds (gfa_kv4_shared.hip).
+constexpr int kv4_shared_wgs(int D) { return D == 512 ? 1 : 2; }
 
-// What a launch of the attention kernels does: a whole call; or, where requests share prefixes (gfa_kv4_share), the groups'
-// prefixes as requests of their own, and the requests' keys behind them. The last two leave sums alone (kPrefix a row's in row_o
-// and row_ml), which kRest's join brings together.
-enum Kv4Part : int { kWhole, kPrefix, kRest };
+// What the attention kernels' device functions work on: a whole call; or, where requests share prefixes (gfa_kv4_share), the groups'
+// prefixes as requests of their own (skip NULL) or the requests' keys behind them, which leave sums alone.
+enum Kv4Part : int { kWhole, kPart };
 
 struct Kv4AttnParams {
   Kv4Cache cache;
@@ -233,8 +234,21 @@ struct Kv4AttnParams {
   int row_blocks, join_rows, join_slice, join_parts;
   float* part;    // (slots, Hkv, rows, D) sums and (slots, Hkv, rows, 2) row maxima and sums
   float* part_ml;
-  const int* skip;       // kRest: (B) tokens of the request's prefix
-  float *row_o, *row_ml;  // (T, Hq, D) sums and (T, Hq, 2) maxima and sums of the prefixes
+  const int* skip;  // kPart: (B) tokens of the request's prefix, or NULL
+};
+
+// A call over shared prefixes (gfa_kv4_shared.hip): the sums of one part of the work, see Kv4AttnParams.
+struct Kv4Sums {
+  int min_tiles;
+  float share;
+  int nblocks, slots;
+  float *part, *part_ml;
+};
+struct Kv4SharedParams {
+  Kv4AttnParams p;
+  const int *group_cu, *group_lens;
+  int row_limit;          // of the groups
+  Kv4Sums many, few, rest;  // prefixes of groups of many rows and of few, the requests behind their prefixes
 };
 
 }  // namespace gfa

@@ -111,9 +111,11 @@ constexpr int kRows = gfa::kSplitRows;
 // 8k, D = 512, 25 us (45), D = 64 12 (29); the nearest, four requests at 8k and 16k, D = 512, 47 (52) and 60 (66).
 int row_limit(const gfa_kv4_attn_args* a, int64_t requests) { return requests * a->cache.heads_kv <= 4 ? 128 : 64; }
 
-void size_part(Part& s, const gfa_kv4_attn_args* a, gfa::Kv4Part kind, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
+enum Kind { kWhole, kPrefix, kRest };  // a whole call, the groups' prefixes, the requests behind them
+
+void size_part(Part& s, const gfa_kv4_attn_args* a, Kind kind, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
-  if (kind == gfa::kWhole && a->causal && a->window > 0) {
+  if (kind == kWhole && a->causal && a->window > 0) {
     const int64_t g = a->heads_q / a->cache.heads_kv, tokens = (rows + g - 2) / g + 1;  // a row block's, at most
     s.window_tiles = (int)std::min<int64_t>((a->window + tokens + 29) / 32 + 1, 0x40000000);
     tiles = std::min<int64_t>(tiles, s.window_tiles);
@@ -126,7 +128,7 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, gfa::Kv4Part kind, int64_t r
   //   1024        8.0 8.2, 9.9 9.0, 13.8 10.9, 21.9 15.2   window 512 of 16k  5.7 7.8, 7.0 8.8, 9.4 10.7, 15.0 15.2
   const int64_t chunks = tiles <= 16 ? 1 : (tiles + min_tiles - 1) / min_tiles;
   s.runs = row_blocks > 0;
-  s.join = chunks > 1 || kind != gfa::kWhole;
+  s.join = chunks > 1 || kind != kWhole;
   s.min_tiles = chunks > 1 ? min_tiles : 0x3fffffff;
   s.row_blocks = row_blocks;
   // The join. Of the chunk kernel: its runs of 1 KB, four waves a workgroup. Of the split kernel: where rows are few, a
@@ -136,7 +138,8 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, gfa::Kv4Part kind, int64_t r
   const int D = a->cache.head_dim;
   s.join_slice = rows == kRows && D > 128 && n * (D / 128) <= 1024 ? 128 : D;
   const int groups = 1024 / s.join_slice;
-  s.join_parts = n <= 2048 ? groups : 1;
+  // (Over prefixes a row has many chunks: 64 answers to a 16k prompt, 32:8 D = 128, two groups of lanes a row 46.2 us, one 50.3.)
+  s.join_parts = n <= 2048 ? groups : kind == kRest ? 2 : 1;
   const int64_t wgs = rows == kRows ? (row_bound * s.join_parts + groups - 1) / groups : rows / 32 * (D <= 128 ? 16 : D / 8) / 4;
   const int64_t most_wgs = 4096 / std::max<int64_t>(1, row_blocks * hkv);
   s.join_rows = (int)std::max<int64_t>(1, std::min(wgs, most_wgs));
@@ -144,11 +147,16 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, gfa::Kv4Part kind, int64_t r
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
   s.nblocks = items * hkv + spare;
   if (s.join) {
-    s.slots = kind != gfa::kWhole ? items : std::min(row_blocks * chunks, 2 * target / hkv + 1);
+    s.slots = kind != kWhole ? items : std::min(row_blocks * chunks, 2 * target / hkv + 1);
     s.part_bytes = (size_t)(s.slots * hkv) * rows * a->cache.head_dim * sizeof(float);
     s.ml_bytes = (size_t)(s.slots * hkv) * rows * 2 * sizeof(float);
   }
 }
+
+// The same of a group's rows. Below a workgroup's 128 the chunk kernel's waves share the keys (gfa_kv4_chunk.inc), so the line is lower
+// where there are KV heads to fill the GPU with: four prompts of 8k with 12 answers each, 32:8 D = 128, 48 rows 37 us (split kernel 41),
+// 16:8 D = 256 60 (69), 32:4 D = 512 60 (66); one KV head at D = 256 24.5 (23.4), two at D = 64 24 (20), 32:8 at D = 64 35 (34).
+int group_limit(const gfa_kv4_attn_args* a) { return a->cache.heads_kv >= 4 && a->cache.head_dim >= 128 ? 32 : 64; }
 
 // Most new tokens of a request, as far as the host knows.
 int64_t most_new(const gfa_kv4_attn_args* a) {
@@ -156,16 +164,16 @@ int64_t most_new(const gfa_kv4_attn_args* a) {
   return a->cu == nullptr ? T / a->requests : a->max_new > 0 ? std::min<int64_t>(a->max_new, T) : T;
 }
 
-Split split_of(const gfa_kv4_attn_args* a, gfa::Kv4Part kind) {
+Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
   Split s{};
   const int64_t G = a->heads_q / a->cache.heads_kv, T = (int64_t)a->batch * a->seq_len;
   // a prefix is that of two requests at least, and of any number of them
-  const int64_t R = kind == gfa::kPrefix ? std::max<int64_t>(1, a->requests / 2) : a->requests;
-  const int64_t most = kind == gfa::kPrefix ? T : most_new(a);
+  const int64_t R = kind == kPrefix ? std::max<int64_t>(1, a->requests / 2) : a->requests;
+  const int64_t most = kind == kPrefix ? T : most_new(a);
   // No request can have more rows than the limit: then all are the split kernel's, whatever max_new promised.
   s.one_block = most * G <= kRows;
-  const int limit = row_limit(a, R);
-  s.row_limit = kind == gfa::kRest || most * G <= limit ? 0x7fffffff : limit;
+  const int limit = kind == kPrefix ? group_limit(a) : row_limit(a, R);
+  s.row_limit = kind == kRest || most * G <= limit ? 0x7fffffff : limit;
   const int D = a->cache.head_dim, big = gfa::kv4_chunk_rows(D);
   int64_t few, many = 0;
   if (a->cu == nullptr) {
@@ -180,17 +188,30 @@ Split split_of(const gfa_kv4_attn_args* a, gfa::Kv4Part kind) {
     }
   }
   // with cu, workgroups to spare: rows behind the last request's
-  // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 19.7 us; of 4: 21.0, of 2: 26.2). Twice the CUs' number
-  // of workgroups where there is work for them (32 ragged requests: 512 96 us, 1024 107 us, 2048 129 us; 64 full
-  // ones 152-154 us with each).
-  size_part(s.few, a, kind, few, kRows, most * G, 8, 512, a->cu && kind != gfa::kPrefix ? 64 : 0);
+  const int spare = a->cu && kind != kPrefix ? 64 : 0;
+  if (kind == kWhole) {
+    // Chunks of at least 8 tiles, two a wave (16k keys, D = 512: 19.7 us; of 4: 21.0, of 2: 26.2). Twice the CUs' number
+    // of workgroups where there is work for them (32 ragged requests: 512 96 us, 1024 107 us, 2048 129 us; 64 full
+    // ones 152-154 us with each).
+    size_part(s.few, a, kind, few, kRows, most * G, 8, 512, spare);
+  } else {
+    // At D = 512 a CU holds one workgroup, and the prefixes' and the requests' share the GPU (eight answers to each of four prompts,
+    // 32:4: 160 of the chunk kernel and 128 52.8 us, 160 and 256 57-61, 256 and 256 63-71). A few answers leave it to
+    // chunks of one tile a wave (four answers, 8:1 D = 512, 700 tokens: 15.8 us, of two 17.5).
+    const int min_tiles = (int64_t)a->requests * a->cache.heads_kv <= 16 ? 4 : 8;
+    size_part(s.few, a, kind, few, kRows, most * G, min_tiles, D < 512 ? 512 : kind == kPrefix ? 256 : 128, spare);
+  }
   // Of the chunk kernel as many workgroups as the CUs hold at once (256 tokens at 16k, D = 512: 290 us, twice as many 314;
   // 1024 tokens, D = 128: 256 482 us, 512 375, 768 354, 1024 360). Its chunks cost as much again as some tiles, so the
   // more of the GPU the row blocks take by themselves the longer a chunk has to be: 256 tokens of one request, window
   // 1024, 33 us with chunks of 8 tiles, 57 unsplit; 1000 tokens beside seven requests 66 us with 18 tiles, 74 unsplit;
   // 512 tokens of four requests 76-84 us split, 71 unsplit.
+  // Of prefixes one workgroup a CU: their sums are as much again as what they read (64 answers to a 16k prompt, D = 128: 46.2 us, two
+  // 57), chunks of 4 tiles where row blocks are few (16 answers of 4 drafted tokens, 3k, 8:4 D = 256: 24.3 us, of 8 27.8).
   const int64_t alone = many * a->cache.heads_kv;
-  size_part(s.many, a, kind, many, big, most * G, alone >= 256 ? 64 : alone >= 128 ? 32 : 8, 256 * gfa::kv4_chunk_wgs(D), 0);
+  const int target = kind != kPrefix ? 256 * gfa::kv4_chunk_wgs(D) : D < 512 ? 256 : 160;
+  const int min_tiles = alone >= 256 ? 64 : alone >= 128 ? 32 : kind == kPrefix && alone <= 16 ? 4 : 8;
+  size_part(s.many, a, kind, many, big, most * G, min_tiles, target, 0);
   return s;
 }
 
@@ -203,27 +224,23 @@ bool takes_prefixes(const gfa_kv4_attn_args* a) {
   return rows * (a->heads_q / a->cache.heads_kv) <= row_limit(a, a->requests);
 }
 
-// The launches of a call: each a kernel over a part of the work and, where it leaves sums, their join.
+// The parts of a call.
 struct Steps {
   Split whole, prefix, rest;  // whole, or the two others
   bool shared;
-  size_t rows_o, rows_ml;  // bytes of the prefixes' rows
   size_t bytes() const {
-    return shared ? rows_o + rows_ml + prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() : whole.few.bytes() + whole.many.bytes();
+    return shared ? prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() : whole.few.bytes() + whole.many.bytes();
   }
 };
 Steps steps_of(const gfa_kv4_attn_args* a) {
   Steps s{};
   s.shared = takes_prefixes(a);
   if (!s.shared) {
-    s.whole = split_of(a, gfa::kWhole);
+    s.whole = split_of(a, kWhole);
     return s;
   }
-  s.prefix = split_of(a, gfa::kPrefix);
-  s.rest = split_of(a, gfa::kRest);
-  const size_t rows = (size_t)a->batch * a->seq_len * a->heads_q;
-  s.rows_o = rows * a->cache.head_dim * sizeof(float);
-  s.rows_ml = (rows * 2 * sizeof(float) + 15) / 16 * 16;
+  s.prefix = split_of(a, kPrefix);
+  s.rest = split_of(a, kRest);
   return s;
 }
 
@@ -531,11 +548,12 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
       (a->cu == nullptr || !aligned(a->shared_skip, 4) || !aligned(a->shared_cu, 4) || !aligned(a->shared_lens, 4)))
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "shared prefixes need cu, and 4-byte aligned pointers");
   const Steps s = steps_of(a);
-  for (const Part* part : {&s.whole.few, &s.whole.many, &s.prefix.few, &s.prefix.many, &s.rest.few}) {
+  int64_t most = s.prefix.many.nblocks + s.prefix.few.nblocks + s.rest.few.nblocks;
+  for (const Part* part : {&s.whole.few, &s.whole.many, &s.rest.few}) {
     const int64_t join = part->join ? part->row_blocks * part->join_rows * (a->cache.head_dim / part->join_slice) * a->cache.heads_kv : 0;
-    if (std::max(part->nblocks, join) > kMostWorkgroups)
-      return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)std::max(part->nblocks, join));
+    most = std::max({most, part->nblocks, join});
   }
+  if (most > kMostWorkgroups) return api_fail(GFA_ERR_UNSUPPORTED, "%lld workgroups exceed one launch", (long long)most);
   const size_t need = s.bytes();
   if (need > 0 && (!aligned(a->workspace, 16) || a->workspace_bytes < need))
     return api_fail(GFA_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need, a->workspace_bytes);
@@ -572,41 +590,48 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   const bool bf16 = a->cache.dtype == GFA_DTYPE_BF16;
   char* ws = static_cast<char*>(a->workspace);
   hipError_t err = hipSuccess;
-  auto run = [&](const Split& split, bool large, gfa::Kv4Part kind) {
-    const Part& part = large ? split.many : split.few;
-    if (!part.runs || err != hipSuccess) return;
-    p.row_limit = split.row_limit;
-    p.min_tiles = part.min_tiles;
-    p.share = part.share;
+  auto sums_of = [&](const Part& part) {
+    gfa::Kv4Sums sums{part.min_tiles, part.share, (int)part.nblocks, (int)part.slots, reinterpret_cast<float*>(ws),
+                      reinterpret_cast<float*>(ws + part.part_bytes)};
+    ws += part.bytes();
+    return sums;
+  };
+  if (s.shared) {
+    gfa::Kv4SharedParams sp{};
+    p.row_limit = s.rest.row_limit;
+    p.row_blocks = (int)s.rest.few.row_blocks;
+    p.join_rows = s.rest.few.join_rows;
+    p.join_slice = s.rest.few.join_slice;
+    p.join_parts = s.rest.few.join_parts;
+    p.skip = a->shared_skip;
+    sp.p = p;
+    sp.group_cu = a->shared_cu;
+    sp.group_lens = a->shared_lens;
+    sp.row_limit = s.prefix.row_limit;
+    sp.many = sums_of(s.prefix.many);
+    sp.few = sums_of(s.prefix.few);
+    sp.rest = sums_of(s.rest.few);
+    return launched(gfa::launch_kv4_shared(sp, D, bf16, cap, stream), "attention over shared prefixes");
+  }
+  for (const bool large : {true, false}) {
+    const Part& part = large ? s.whole.many : s.whole.few;
+    if (!part.runs) continue;
+    p.row_limit = s.whole.row_limit;
     p.window_tiles = part.window_tiles;
     p.row_blocks = (int)part.row_blocks;
     p.join_rows = part.join_rows;
     p.join_slice = part.join_slice;
     p.join_parts = part.join_parts;
-    p.nblocks = (int)part.nblocks;
-    p.slots = (int)part.slots;
-    p.part = reinterpret_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float*>(ws + part.part_bytes);
-    ws += part.bytes();
-    err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, kind, stream) : gfa::launch_kv4_split(p, D, bf16, cap, split.one_block, kind, stream);
-    if (err == hipSuccess && part.join) err = gfa::launch_kv4_join(p, D, bf16, large, kind, stream);
-  };
-  if (s.shared) {
-    p.row_o = reinterpret_cast<float*>(ws);
-    p.row_ml = reinterpret_cast<float*>(ws + s.rows_o);
-    ws += s.rows_o + s.rows_ml;
-    const gfa::Kv4AttnParams whole = p;
-    p.cu = a->shared_cu;
-    p.lens = a->shared_lens;
-    p.causal = p.window = 0;
-    run(s.prefix, true, gfa::kPrefix);
-    run(s.prefix, false, gfa::kPrefix);
-    p = whole;
-    p.skip = a->shared_skip;
-    run(s.rest, false, gfa::kRest);
-  } else {
-    run(s.whole, true, gfa::kWhole);
-    run(s.whole, false, gfa::kWhole);
+    const gfa::Kv4Sums sums = sums_of(part);
+    p.min_tiles = sums.min_tiles;
+    p.share = sums.share;
+    p.nblocks = sums.nblocks;
+    p.slots = sums.slots;
+    p.part = sums.part;
+    p.part_ml = sums.part_ml;
+    err = large ? gfa::launch_kv4_chunk(p, D, bf16, cap, stream) : gfa::launch_kv4_split(p, D, bf16, cap, s.whole.one_block, stream);
+    if (err == hipSuccess && part.join) err = gfa::launch_kv4_join(p, D, bf16, large, stream);
+    if (err != hipSuccess) break;
   }
   return err != hipSuccess ? launched(err, "cache attention") : gfa::api_ok();
 }

@@ -13,7 +13,7 @@ constexpr int kTpb = 256;
 // running maxima and are joined through LDS: fp32 sums in a fixed order. Bound: latency, one pass of
 // loads behind the requests' lengths; every load of a lane's chunks is in flight at once. One
 // request of 16k at D = 512 6.7 us, 32 ragged ones 6.3.
-template <int D, bool IS_BF16, Kv4Part PART>
+template <int D, bool IS_BF16>
 __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   constexpr int ROWS = kSplitRows;
   const int LPR = p.join_slice / 4;  // a power of two
@@ -26,12 +26,12 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
   id = p.hkv.quot(id);
   const int slice = id % (D / p.join_slice);
   id /= D / p.join_slice;
-  const RowBlock blk = find_row_block<ROWS, false, PART>(p, id / p.join_rows, lane);
-  if (blk.b < 0 || (PART == kWhole && blk.nch == 1)) return;
+  const RowBlock blk = find_row_block<ROWS, false>(p, id / p.join_rows, lane);
+  if (blk.b < 0 || blk.nch == 1) return;
   if (blk.slot < 0 || (int64_t)blk.slot + blk.nch > p.slots) return;  // cu that is no prefix sum: no such chunks
   const int rb = blk.rb;
   const int rows = min(ROWS, blk.rq.fresh * p.G - rb * ROWS);
-  const int parts = min(p.join_parts, blk.nch > 1 ? 1 << (32 - __builtin_clz(blk.nch - 1)) : 1);
+  const int parts = min(p.join_parts, 1 << (32 - __builtin_clz(blk.nch - 1)));
   const int at_once = GR / parts;
   const int group = threadIdx.x / LPR, part = group % parts, d = slice * p.join_slice + threadIdx.x % LPR * 4;
   for (int r0 = id % p.join_rows * at_once; r0 < rows; r0 += p.join_rows * at_once) {
@@ -41,14 +41,6 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
     const bool live = rr < rows && t >= 0 && t < p.T;
     float m = -INFINITY, l = 0.f;  // without a maximum l counts the rows' marks, see row_inv
     f32x4 o{};
-    if constexpr (PART == kRest) {
-      if (live && part == 0 && blk.rq.skip > 0) {  // the prefix first
-        const int64_t at = (int64_t)t * p.Hq + qh;
-        m = p.row_ml[at * 2];
-        l = p.row_ml[at * 2 + 1];
-        o = *reinterpret_cast<const f32x4*>(p.row_o + at * D + d);
-      }
-    }
     if (live) {
 #pragma unroll 8
       for (int c = part; c < blk.nch; c += parts) {
@@ -70,15 +62,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
       }
       __syncthreads();
     }
-    if (PART == kPrefix && part == 0 && live) {
-      const int64_t at = (int64_t)t * p.Hq + qh;
-      if (d == 0) {
-        p.row_ml[at * 2] = m;
-        p.row_ml[at * 2 + 1] = l;
-      }
-      *reinterpret_cast<f32x4*>(p.row_o + at * D + d) = o;
-    }
-    if (PART != kPrefix && part == 0 && live) {
+    if (part == 0 && live) {
       const bool none = m == -INFINITY && l == 0.f;
       const float inv = row_inv(m, l);
       uint16_t* op = p.o + p.n.quot(t) * p.osb + (int64_t)qh * p.osh + p.n.rem(t) * p.osn + d;
@@ -93,7 +77,7 @@ __global__ __launch_bounds__(kTpb) void kv4_join_kernel(const Kv4AttnParams p) {
 // The chunk kernel's: its sums lie in the order its lanes held them (1 KB runs; per 32 rows, product row r and W
 // channels: lane (h, row) W channels), and are read the same way: a wave takes runs, a lane one row's W channels
 // of every chunk.
-template <int D, bool IS_BF16, Kv4Part PART>
+template <int D, bool IS_BF16>
 __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParams p) {
   constexpr int ROWS = kv4_chunk_rows(D), CPL = D / 32, PP = D / 16, W = CPL < 4 ? CPL : 4;
   constexpr int RUNS = ROWS / 32 * 16 * (CPL / W);
@@ -101,8 +85,8 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
   int id = (int)blockIdx.x;
   const int head = p.hkv.rem(id);
   id = p.hkv.quot(id);
-  const RowBlock blk = find_row_block<ROWS, true, PART>(p, id / p.join_rows, lane);
-  if (blk.b < 0 || (PART == kWhole && blk.nch == 1)) return;
+  const RowBlock blk = find_row_block<ROWS, true>(p, id / p.join_rows, lane);
+  if (blk.b < 0 || blk.nch == 1) return;
   if (blk.slot < 0 || (int64_t)blk.slot + blk.nch > p.slots) return;  // cu that is no prefix sum: no such chunks
   const int rb = blk.rq.row_blocks - 1 - blk.rb;                        // the chunk kernel takes the last rows first
   const int rows = min(ROWS, blk.rq.fresh * p.G - rb * ROWS);
@@ -126,19 +110,6 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
     }
     const int r = run / (CPL / W) % 16, x = run % (CPL / W) * W;
     const int idx = 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-    if constexpr (PART == kPrefix) {
-      const int64_t at = (int64_t)t * p.Hq + qh;
-      const int d = (idx & 15) * PP + CPL * (idx >> 4) + x;
-      if (d == 0) {
-        p.row_ml[at * 2] = m;
-        p.row_ml[at * 2 + 1] = l;
-      }
-      vec v;
-#pragma unroll
-      for (int e = 0; e < W; ++e) v[e] = o[e];
-      *reinterpret_cast<vec*>(p.row_o + at * D + d) = v;
-      continue;
-    }
     const bool none = m == -INFINITY && l == 0.f;
     const float inv = row_inv(m, l);
     typedef short out __attribute__((ext_vector_type(W)));
@@ -150,22 +121,16 @@ __global__ __launch_bounds__(kTpb) void kv4_join_large_kernel(const Kv4AttnParam
   }
 }
 
-hipError_t launch_kv4_join(const Kv4AttnParams& p, int D, bool bf16, bool large, Kv4Part part, hipStream_t stream) {
+hipError_t launch_kv4_join(const Kv4AttnParams& p, int D, bool bf16, bool large, hipStream_t stream) {
   auto go = [&](auto d, auto b) {
     constexpr int DD = decltype(d)::value;
     constexpr bool BB = decltype(b)::value;
     const int slices = large ? 1 : DD / p.join_slice;
     const dim3 grid((unsigned)((int64_t)p.row_blocks * p.join_rows * slices * p.cache.Hkv));
-    if (large && part == kPrefix) {
-      hipLaunchKernelGGL((kv4_join_large_kernel<DD, BB, kPrefix>), grid, dim3(kTpb), 0, stream, p);
-    } else if (large) {
-      hipLaunchKernelGGL((kv4_join_large_kernel<DD, BB, kWhole>), grid, dim3(kTpb), 0, stream, p);
-    } else if (part == kPrefix) {
-      hipLaunchKernelGGL((kv4_join_kernel<DD, BB, kPrefix>), grid, dim3(kTpb), 0, stream, p);
-    } else if (part == kRest) {
-      hipLaunchKernelGGL((kv4_join_kernel<DD, BB, kRest>), grid, dim3(kTpb), 0, stream, p);
+    if (large) {
+      hipLaunchKernelGGL((kv4_join_large_kernel<DD, BB>), grid, dim3(kTpb), 0, stream, p);
     } else {
-      hipLaunchKernelGGL((kv4_join_kernel<DD, BB, kWhole>), grid, dim3(kTpb), 0, stream, p);
+      hipLaunchKernelGGL((kv4_join_kernel<DD, BB>), grid, dim3(kTpb), 0, stream, p);
     }
   };
   auto by_type = [&](auto d) {

@@ -6,6 +6,9 @@
 // their sums in slots of the workspace: a request is split where it has more than `per` tiles, so into fewer than
 // 2 tiles / per chunks, and with per at least the call's tiles / target there are fewer than 2 target slots. Requests of up to
 // row_limit rows are the split kernel's, the others the chunk kernel's (LARGE).
+//
+// Where requests share prefixes (kPart) the same split is taken twice: of the groups' prefixes, each group a request whose
+// keys all its rows see (p.skip NULL), and of the requests behind their prefixes. Every row block leaves sums then.
 #pragma once
 #include <type_traits>
 
@@ -20,7 +23,7 @@ struct Request {
   int t0, fresh, len;  // first new token, new tokens, tokens with the new ones
   int row_blocks;      // 0: not this kernel's
   int tiles;           // most key tiles that a row block sees
-  int skip;            // kRest: tokens of its prefix
+  int skip;            // kPart: tokens of its prefix
 };
 // Its three loads go out together (one wait: their latency is a good part of a short call).
 template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
@@ -30,35 +33,41 @@ __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   const int* cu = p.cu != nullptr ? p.cu : p.lens;  // without cu read for nothing
   const int t0 = cu[bc], t1 = cu[p.cu != nullptr ? bc + 1 : bc], len = p.lens[bc];
   int skip = 0;
-  if constexpr (PART == kRest) skip = p.skip[bc];
+  if constexpr (PART == kPart) skip = (p.skip != nullptr ? p.skip : p.lens)[bc];
   if (b >= p.B) return r;
   r.t0 = p.cu != nullptr ? t0 : b * p.each;
   r.fresh = p.cu != nullptr ? min(max((int)((unsigned)t1 - (unsigned)t0), 0), p.T) : p.each;
   r.len = max(len, 0);
-  if constexpr (PART == kPrefix) r.fresh = r.len > 0 ? r.fresh : 0;  // no prefix: nothing to do
-  if constexpr (PART == kRest) r.skip = max(skip, 0);
+  if constexpr (PART == kPart) {
+    if (p.skip == nullptr) {
+      r.fresh = r.len > 0 ? r.fresh : 0;  // a group without a prefix
+    } else {
+      r.skip = max(skip, 0);
+    }
+  }
   const int rows = r.fresh * p.G;
   r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
   const int held = min(r.len, p.M << p.cache.bs_log2);
-  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : PART == kRest ? r.skip : 0;
+  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : PART == kPart ? r.skip : 0;
   r.tiles = held > lo ? (held + kTile - 1) / kTile - lo / kTile : 0;
   if (p.window > 0) r.tiles = min(r.tiles, p.window_tiles);
   return r;
 }
 // Key tiles [x, y) that some row of the request's row block of `rows` rows from row0 on sees.
+template <Kv4Part PART = kWhole>
 __device__ __forceinline__ int2 tiles_of_rows(const Kv4AttnParams& p, const Request& r, int row0, int rows) {
   const int i_lo = p.g.quot(row0), i_hi = min(p.g.quot(row0 + rows - 1), r.fresh - 1);
   const int pos0 = r.len - r.fresh;  // position of new token 0
   const int held = min(r.len, p.M << p.cache.bs_log2);
   const int k_hi = p.causal ? min(held, pos0 + i_hi + 1) : held;
-  const int k_lo = p.window > 0 ? max(0, pos0 + i_lo - p.window + 1) : r.skip;
+  const int k_lo = p.window > 0 ? max(0, pos0 + i_lo - p.window + 1) : PART == kPart ? r.skip : 0;
   return k_hi > k_lo ? make_int2(k_lo / kTile, (k_hi + kTile - 1) / kTile) : make_int2(0, 0);
 }
 // Lane src's request in every lane.
 template <Kv4Part PART = kWhole>
 __device__ __forceinline__ Request request_from(const Request& r, int src) {
   auto at = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
-  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles), PART == kRest ? at(r.skip) : 0};
+  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles), PART == kPart ? at(r.skip) : 0};
 }
 
 // Sum over the wave's lanes (the steps of wave_prefix_sum).
@@ -113,7 +122,7 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
   const int per = chunk_tiles<ROWS, LARGE, PART>(p, r, lane);
   for (int b0 = 0;;) {
     const int nch = chunks_of(r, per);
-    const int mine = r.row_blocks * nch, split = PART != kWhole || nch > 1 ? mine : 0;
+    const int mine = r.row_blocks * nch, split = PART == kPart || nch > 1 ? mine : 0;
     const int s = wave_prefix_sum(mine), z = wave_prefix_sum(split);
     const int before = it.items + s - mine;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
@@ -152,7 +161,7 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
   int blocks = 0;
   for (int b0 = 0;;) {
     const int s = wave_prefix_sum(r.row_blocks);
-    const int nch = chunks_of(r, per), split = PART != kWhole || nch > 1 ? r.row_blocks * nch : 0;
+    const int nch = chunks_of(r, per), split = PART == kPart || nch > 1 ? r.row_blocks * nch : 0;
     const int z = wave_prefix_sum(split);
     const int before = blocks + s - r.row_blocks;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(block >= before && block < before + r.row_blocks);

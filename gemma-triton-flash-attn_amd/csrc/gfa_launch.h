@@ -8,7 +8,7 @@ namespace gfa {
 struct Kv4RowsParams;
 struct Kv4PlanParams;
 struct Kv4AttnParams;
-enum Kv4Part : int;
+struct Kv4SharedParams;
 struct Kv4PagesParams;
 struct Kv4CopyParams;
 struct Kv4ShareParams;
@@ -37,9 +37,9 @@ hipError_t launch_kv4_compact(const Kv4PagesParams& p, hipStream_t stream);
 hipError_t launch_kv4_copy(const Kv4CopyParams& p, hipStream_t stream);
 hipError_t launch_kv4_share(const Kv4ShareParams& p, hipStream_t stream);
 hipError_t launch_verify(const VerifyParams& p, int kind, hipStream_t stream);
-hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, bool once, Kv4Part part,
-                            hipStream_t stream);
-hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, Kv4Part part, hipStream_t stream);
-hipError_t launch_kv4_join(const Kv4AttnParams& p, int head_dim, bool bf16, bool large, Kv4Part part, hipStream_t stream);
+hipError_t launch_kv4_split(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, bool once, hipStream_t stream);
+hipError_t launch_kv4_chunk(const Kv4AttnParams& p, int head_dim, bool bf16, bool cap, hipStream_t stream);
+hipError_t launch_kv4_join(const Kv4AttnParams& p, int head_dim, bool bf16, bool large, hipStream_t stream);
+hipError_t launch_kv4_shared(const Kv4SharedParams& s, int head_dim, bool bf16, bool cap, hipStream_t stream);
 
 }  // namespace gfa
