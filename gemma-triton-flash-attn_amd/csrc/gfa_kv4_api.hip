@@ -387,13 +387,13 @@ int pages_call(const gfa_kv4_pages_args* a, bool fork) {
 
 // ---- verification ----
 
-// Waves of a request: about 4096 of a call, of at least one step.
+// A wave's entries: about 4096 waves a call, one to four steps each (the entry drawn is then found in one pass of a workgroup).
 struct Segments {
   int length;
   int64_t count;
 };
 Segments verify_segments(int64_t requests, int64_t vocab) {
-  const int64_t step = gfa::kVerifyStep, length = std::max<int64_t>(1, (vocab * requests + 4096 * step - 1) / (4096 * step)) * step;
+  const int64_t step = gfa::kVerifyStep, length = std::max<int64_t>(1, std::min<int64_t>(4, (vocab * requests + 4096 * step - 1) / (4096 * step))) * step;
   return Segments{(int)std::min<int64_t>(length, (vocab + step - 1) / step * step), (vocab + length - 1) / length};
 }
 

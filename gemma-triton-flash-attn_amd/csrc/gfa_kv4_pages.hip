@@ -4,6 +4,8 @@
 // Sets of blocks are bit maps in LDS, built by every workgroup for itself from the block tables; ranks and k-th members come
 // from prefix counts over 256-block groups, so every list is in ascending order whatever the order of the atomics (all of
 // them OR, MIN and MAX of integers). One launch decides, a second one moves the bytes.
+#include <algorithm>
+
 #include "gfa_kv4.h"
 #include "gfa_launch.h"
 
@@ -308,7 +310,9 @@ __global__ __launch_bounds__(kTpb) void kv4_compact_kernel(const Kv4PagesParams 
 }
 
 // Whole blocks of every layer, bytes as they are: a piece of 16 KB of one layer's codes or scales a turn, the workgroups
-// counting through (pair, piece). Bound: memory.
+// counting through (pair, piece). Stores go past the caches, where blocks are read again from other addresses; loads do not: a
+// fork's copies are often of one block (24 prompts' last blocks seven times each, 8 layers: 20 us, with loads past the
+// caches too 25-30). Bound: memory. 1140 blocks of 4 layers, 317 MB each way, 105 us, 6.0 TB/s (stores through the caches 128).
 constexpr int kCopyTpb = 256, kCopyUnroll = 4;
 static_assert(kCopyTpb * kCopyUnroll * 16 == kKv4CopyPiece, "a workgroup's turn is one piece");
 __global__ __launch_bounds__(kCopyTpb) void kv4_copy_kernel(const Kv4CopyParams p) {
@@ -331,7 +335,7 @@ __global__ __launch_bounds__(kCopyTpb) void kv4_copy_kernel(const Kv4CopyParams 
       x[i] = *reinterpret_cast<const vec*>(s + min(off + i * (kCopyTpb * 16), size - 16));
 #pragma unroll
     for (int i = 0; i < kCopyUnroll; ++i)
-      if (off + i * (kCopyTpb * 16) < size) *reinterpret_cast<vec*>(d + off + i * (kCopyTpb * 16)) = x[i];
+      if (off + i * (kCopyTpb * 16) < size) __builtin_nontemporal_store(x[i], reinterpret_cast<vec*>(d + off + i * (kCopyTpb * 16)));
   }
 }
 
@@ -410,8 +414,8 @@ __global__ __launch_bounds__(kTpb) void kv4_share_kernel(const Kv4ShareParams p)
 namespace {
 template <typename Kernel>
 hipError_t launch_pages(Kernel kernel, const Kv4PagesParams& p, int64_t work, size_t lds, hipStream_t stream) {
-  // A workgroup for every 8192 results, each marking the tables for itself: past 32 that costs more than it saves.
-  const unsigned wgs = (unsigned)(work <= 8192 ? 1 : work >= 32 * 8192 ? 32 : (work + 8191) / 8192);
+  // A workgroup for every 2048 results, each marking the tables for itself.
+  const unsigned wgs = (unsigned)std::min<int64_t>(32, (work + 2047) / 2048);
   if (lds > 65536) {
     const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (err != hipSuccess) return err;
@@ -429,7 +433,7 @@ hipError_t launch_kv4_compact(const Kv4PagesParams& p, hipStream_t stream) {
 }
 hipError_t launch_kv4_copy(const Kv4CopyParams& p, hipStream_t stream) {
   const int64_t units = (int64_t)p.pairs * p.pieces.d;
-  const unsigned wgs = (unsigned)(units < 2048 ? units : 2048);  // eight of 256 threads a CU
+  const unsigned wgs = (unsigned)std::min<int64_t>(units, 4096);  // twice what the CUs hold
   if (wgs == 0) return hipSuccess;
   hipLaunchKernelGGL(kv4_copy_kernel, dim3(wgs), dim3(kCopyTpb), 0, stream, p);
   return hipGetLastError();

@@ -682,7 +682,8 @@ Tensor probability_rows(const Tensor& t) {
 }
 
 std::tuple<Tensor, Tensor, Tensor> kv4_verify(const Tensor& target, const std::optional<Tensor>& draft, const Tensor& tokens,
-                                              const Tensor& accept, const Tensor& sample, const Tensor& lens, const std::optional<Tensor>& cu) {
+                                              const Tensor& accept, const Tensor& sample, const Tensor& lens, const std::optional<Tensor>& cu,
+                                              bool apart) {
   const auto type = target.scalar_type();
   TORCH_CHECK_TYPE(type == at::kFloat || type == at::kHalf || type == at::kBFloat16, "target is ", type, " (fp32, fp16 or bf16)");
   TORCH_CHECK_VALUE(target.dim() == 2, "target must be 2-D (tokens, vocabulary), got shape ", target.sizes());
@@ -712,7 +713,12 @@ std::tuple<Tensor, Tensor, Tensor> kv4_verify(const Tensor& target, const std::o
   const c10::DeviceGuard guard(device);
   const Tensor p = probability_rows(target), q = draft ? probability_rows(*draft) : Tensor();
   const Tensor x = dense(tokens), u = dense(accept), r = dense(sample), l = dense(lens), c = cu ? dense(*cu) : Tensor();
-  const Tensor follows = at::empty({T}, tokens.options()), accepted = at::empty({R}, lens.options()), lens_out = at::empty({R}, lens.options());
+  // the workspace in front: its numbers are of 64 bits
+  const size_t need = api.kv4_verify_workspace_bytes((int32_t)R, (int32_t)V);
+  const int64_t ws_ints = (int64_t)(need / 4);
+  const Tensor rest = at::empty({ws_ints + (apart ? 0 : 2 * R)}, lens.options());
+  const auto out = [&](int64_t offset) { return apart ? at::empty({R}, lens.options()) : part_of(rest, offset, {R}, {1}); };
+  const Tensor follows = at::empty({T}, tokens.options()), accepted = out(ws_ints), lens_out = out(ws_ints + R);
   gfa_kv4_verify_args a{};
   a.target = p.data_ptr();
   a.draft = draft ? q.data_ptr() : nullptr;
@@ -730,9 +736,8 @@ std::tuple<Tensor, Tensor, Tensor> kv4_verify(const Tensor& target, const std::o
   a.follows = static_cast<int64_t*>(follows.data_ptr());
   a.accepted = ints_of(accepted);
   a.lens_out = ints_of(lens_out);
-  a.workspace_bytes = api.kv4_verify_workspace_bytes(a.requests, a.vocab);
-  const Tensor ws = at::empty({(int64_t)a.workspace_bytes}, lens.options().dtype(at::kByte));
-  a.workspace = ws.data_ptr();
+  a.workspace = rest.data_ptr();
+  a.workspace_bytes = need;
   a.stream = stream_of(target);
   check(api.kv4_verify(&a));
   return {follows, accepted, lens_out};

@@ -118,14 +118,21 @@ __device__ __forceinline__ double wave_total(double x) {
   return x;
 }
 
-// Inclusive prefix over the workgroup in the threads' order, and the total; two barriers.
-__device__ __forceinline__ double block_prefix(double x, double* sums, double& total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// Inclusive prefix over the wave's lanes.
+__device__ __forceinline__ double wave_prefix(double x) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) {
     const double y = __shfl_up(x, m);
     if (lane >= m) x += y;
   }
+  return x;
+}
+
+// Inclusive prefix over the workgroup in the threads' order, and the total; two barriers.
+__device__ __forceinline__ double block_prefix(double x, double* sums, double& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  x = wave_prefix(x);
   if (lane == 63) sums[wave] = x;
   __syncthreads();
   double before = 0.0;
@@ -139,16 +146,22 @@ __device__ __forceinline__ double block_prefix(double x, double* sums, double& t
   return before + x;
 }
 
-// The least of the threads' values; two barriers.
-__device__ __forceinline__ int block_min(int x, int* least) {
+// The least of the threads' x and the largest of their y; two barriers.
+__device__ __forceinline__ int2 block_ends(int x, int y, int2* ends) {
 #pragma unroll
-  for (int m = 32; m > 0; m >>= 1) x = min(x, __shfl_xor(x, m));
-  if ((threadIdx.x & 63) == 0) least[threadIdx.x >> 6] = x;
+  for (int m = 32; m > 0; m >>= 1) {
+    x = min(x, __shfl_xor(x, m));
+    y = max(y, __shfl_xor(y, m));
+  }
+  if ((threadIdx.x & 63) == 0) ends[threadIdx.x >> 6] = make_int2(x, y);
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kWaves; ++w) x = min(x, least[w]);
+  for (int w = 0; w < kWaves; ++w) {
+    x = min(x, ends[w].x);
+    y = max(y, ends[w].y);
+  }
   __syncthreads();
-  return x;
+  return make_int2(x, y);
 }
 
 }  // namespace
@@ -187,8 +200,8 @@ __global__ __launch_bounds__(kTpb) void verify_sums_kernel(const VerifyParams p)
 template <Kind K>
 __global__ __launch_bounds__(kTpb) void verify_pick_kernel(const VerifyParams p) {
   __shared__ double sums[kWaves];
-  __shared__ int least[kWaves];
-  const int tid = threadIdx.x, b = (int)blockIdx.x;
+  __shared__ int2 ends[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63, b = (int)blockIdx.x;
   const Tokens r = tokens_of(p, b);
   // tokens of no request
   if (b == 0) {
@@ -206,69 +219,69 @@ __global__ __launch_bounds__(kTpb) void verify_pick_kernel(const VerifyParams p)
   }
   const int taken = p.taken[b];
   const Row<K> row(p, r, taken);
+  // ---- the segment: the first at which the running sum passes the goal, else the last with weight ----
+  // Every wave for itself, a lane neighbouring segments: no barrier.
   const double* seg = p.sums + (int64_t)b * p.segments * 2;
-  // ---- the sum; a residual without weight (the draft's probabilities are the target's) leaves the target's ----
-  double all[2] = {0.0, 0.0};
-  for (int s0 = 0; s0 < p.segments; s0 += kTpb) {
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      double total;
-      block_prefix(s0 + tid < p.segments ? seg[(s0 + tid) * 2 + e] : 0.0, sums, total);
-      all[e] += total;
-    }
+  const int per = (p.segments + 63) / 64, s0 = lane * per, s1 = min(s0 + per, p.segments);
+  double mine[2] = {0.0, 0.0};
+  for (int s = s0; s < s1; ++s) {
+    mine[0] += seg[s * 2];
+    mine[1] += seg[s * 2 + 1];
   }
-  const int use = all[0] > 0.0 ? 0 : 1;
+  // a residual without weight (the draft's probabilities are the target's) leaves the target's
+  const int use = wave_total(mine[0]) > 0.0 ? 0 : 1;
+  const double x = use == 0 ? mine[0] : mine[1];
+  const double upto = wave_prefix(x), total = __shfl(upto, 63);
   const float u = p.sample[b];
-  const double goal = (u > 0.f ? fmin((double)u, 1.0) : 0.0) * all[use];
-  // ---- its segment: the first whose running sum passes the goal, else the last with weight ----
-  double before = 0.0;
-  int pick = -1, heavy = -1;  // heavy: negative index of the last segment with weight, less 2
-  double base = 0.0;
-  for (int s0 = 0; s0 < p.segments && pick < 0; s0 += kTpb) {
-    const double x = s0 + tid < p.segments ? seg[(s0 + tid) * 2 + use] : 0.0;
-    double total;
-    const double upto = before + block_prefix(x, sums, total);
-    const int hit = block_min(x > 0.0 && upto > goal ? s0 + tid : 0x7fffffff, least);
-    if (hit != 0x7fffffff) pick = hit;
-    heavy = min(heavy, block_min(x > 0.0 ? -2 - (s0 + tid) : -1, least));
-    before += total;
-  }
-  const bool passed = pick >= 0;
-  if (!passed && heavy < -1) pick = -2 - heavy;
-  int next = -1;
-  if (pick >= 0) {
-    // weight ahead of the segment, in the order of the sums above
-    for (int s0 = 0; s0 < pick; s0 += kTpb) {
-      double total;
-      block_prefix(s0 + tid < pick ? seg[(s0 + tid) * 2 + use] : 0.0, sums, total);
-      base += total;
+  const double goal = (u > 0.f ? fmin((double)u, 1.0) : 0.0) * total;
+  double run = upto - x, before = 0.0;  // weight ahead of the lane's segments, of its pick
+  int pick = -1, last = -1;
+  for (int s = s0; s < s1; ++s) {
+    const double w = seg[s * 2 + use];
+    if (w > 0.0) {
+      last = s;
+      if (pick < 0 && run + w > goal) {
+        pick = s;
+        before = run;
+      }
     }
-    // ---- its entry ----
+    run += w;
+  }
+  const uint64_t hits = __builtin_amdgcn_ballot_w64(pick >= 0), heavy = __builtin_amdgcn_ballot_w64(last >= 0);
+  int next = -1;
+  if (heavy != 0) {
+    const bool passed = hits != 0;
+    const int src = passed ? __builtin_ctzll(hits) : 63 - __builtin_clzll(heavy);
+    pick = __shfl(passed ? pick : last, src);
+    double base = __shfl(before, src);
+    // ---- its entry, by the whole workgroup ----
     const int first = pick * p.segment, end = min(p.V, first + p.segment);
-    int hit = 0x7fffffff, last = -1;
+    int hit = 0x7fffffff, most = -1;
     for (int i0 = first; i0 < end && hit == 0x7fffffff; i0 += kTpb * kLane) {
-      const int i = i0 + tid * kLane;
-      double w[kLane], whole[kLane], mine = 0.0;
-      row.weights(min(i, end), end, w, whole);
+      const int i = min(i0 + tid * kLane, end);
+      double w[kLane], whole[kLane], sum = 0.0;
+      row.weights(i, end, w, whole);
 #pragma unroll
       for (int e = 0; e < kLane; ++e) {
         if (use == 1) w[e] = whole[e];
-        mine += w[e];
+        sum += w[e];
       }
-      double total;
-      double run = base + (block_prefix(mine, sums, total) - mine);
+      double all;
+      double at = base + (block_prefix(sum, sums, all) - sum);
       int found = 0x7fffffff, heaviest = -1;
 #pragma unroll
       for (int e = 0; e < kLane; ++e) {
-        run += w[e];
-        if (w[e] > 0.0 && run > goal && found == 0x7fffffff) found = i + e;
+        at += w[e];
+        if (w[e] > 0.0 && at > goal && found == 0x7fffffff) found = i + e;
         if (w[e] > 0.0) heaviest = i + e;
       }
-      hit = block_min(passed ? found : 0x7fffffff, least);
-      last = max(last, -block_min(-heaviest, least));
-      base += total;
+      // one pass for both: the least entry that passes the goal, the last with weight
+      const int2 both = block_ends(passed ? found : 0x7fffffff, heaviest, ends);
+      hit = both.x;
+      most = max(most, both.y);
+      base += all;
     }
-    next = hit != 0x7fffffff ? hit : last;
+    next = hit != 0x7fffffff ? hit : most;
   }
   for (int i = tid; i < r.n; i += kTpb) {
     const int64_t t = r.t0 + i;

@@ -273,11 +273,11 @@ def verify(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Te
     target and draft leave no weight, the target's probabilities are taken; without any of those the token is -1. Values that are no
     finite positive number count as 0.
 
-    lens: (R,) int32 (``Plan.lens``); ``Verified.lens`` is less the tokens not accepted, which ``fork``'s ``keep`` takes back. There is no
-    gradient."""
+    lens: (R,) int32 (``Plan.lens``); ``Verified.lens`` is less the tokens not accepted, which ``fork``'s ``keep`` takes back; outside of
+    torch.compile it shares an allocation with ``accepted``. There is no gradient."""
     _refuse_gradients("verification", target, target if draft is None else draft)
     if _plain(target):
-        return Verified(*_lib.native().kv4_verify(target, draft, tokens, accept, sample, lens, cu))
+        return Verified(*_lib.native().kv4_verify(target, draft, tokens, accept, sample, lens, cu, False))
     return Verified(*torch.ops.gfa.kv4_verify(target, draft, tokens, accept, sample, lens, cu))
 
 
@@ -381,7 +381,7 @@ def _share_fake(table, lens, cu, block_size, least):
 @torch.library.custom_op("gfa::kv4_verify", mutates_args=())
 def _verify_op(target: torch.Tensor, draft: Optional[torch.Tensor], tokens: torch.Tensor, accept: torch.Tensor, sample: torch.Tensor,
                lens: torch.Tensor, cu: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _lib.native().kv4_verify(target, draft, tokens, accept, sample, lens, cu)
+    return _lib.native().kv4_verify(target, draft, tokens, accept, sample, lens, cu, True)
 
 
 @_verify_op.register_fake
