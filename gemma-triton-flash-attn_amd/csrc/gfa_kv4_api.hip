@@ -497,6 +497,9 @@ int gfa_kv4_verify(const gfa_kv4_verify_args* a) {
   if (a->type < 0 || a->type > 2) return api_fail(GFA_ERR_INVALID_ARGUMENT, "type=%d is none of 0, 1, 2", a->type);
   if (a->cu == nullptr && a->token_count % a->requests != 0)
     return api_fail(GFA_ERR_INVALID_ARGUMENT, "%d tokens do not divide among %d requests (pass cu)", a->token_count, a->requests);
+  const Segments s = verify_segments(a->requests, a->vocab);
+  if ((s.count + 3) / 4 * a->requests > kMostWorkgroups)
+    return api_fail(GFA_ERR_UNSUPPORTED, "%d requests over a vocabulary of %d exceed one launch", a->requests, a->vocab);
   if (a->target_stride < 0 || a->draft_stride < 0) return api_fail(GFA_ERR_INVALID_ARGUMENT, "row strides must not be negative");
   const unsigned size = a->type == 2 ? 4 : 2;
   if (!aligned(a->target, size) || (a->draft != nullptr && !aligned(a->draft, size)))
@@ -522,7 +525,6 @@ int gfa_kv4_verify(const gfa_kv4_verify_args* a) {
   p.V = a->vocab;
   p.R = a->requests;
   p.each = a->token_count / a->requests;
-  const Segments s = verify_segments(a->requests, a->vocab);
   p.segment = s.length;
   p.segments = s.count;
   p.sums = static_cast<double*>(a->workspace);
