@@ -114,6 +114,29 @@ def test_masks_and_caps(name, device):
     assert torch.equal(run(a, s, slide_size=100), run(a, None, slide_size=100))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256, 512])
+@pytest.mark.parametrize("rows", [16, 17, 32, 33, 64, 65, 128, 129, 260])
+def test_rows_of_a_group(D, rows, device):
+    """Every form a prefix's rows can take: a row block of 16 and several, half a workgroup whose waves share the keys, whole ones.
+    Prefixes of one tile, of an odd number, of one that is split; two groups of different rows side by side, and a request alone."""
+    G, Hkv, bs = {17: 1, 33: 3, 65: 5, 129: 3}.get(rows, 4), 4, 32 if rows % 2 else 64
+    n = rows // G
+    for tiles in (2, 5, 37) if n <= 17 else (2, 11):
+        common = -(-tiles * 32 // bs) * bs
+        lens = [common + 1 + i % 9 for i in range(n)] + [common + 3, common + 40, 7]
+        a = Answers(device, lens, [1] * len(lens), G * Hkv, Hkv, D, [(n, common), (2, common), (1, 0)], bs=bs, seed=rows,
+                    dtype=torch.float16 if rows in (33, 129) else torch.bfloat16).store()
+        s = a.share(least=32)
+        assert s.skip.tolist() == [common] * (n + 2) + [0]
+        check(run(a, s), *a.expected())
+        if rows in (33, 65):
+            check(run(a, s, softcap=10.0), *a.expected(softcap=10.0))
+
+
+# Requests of a group, by the kernel that takes its prefix: 12 rows the split kernel's, 48 the chunk kernel's with shared keys, 160 its own.
+SIZES = [3, 12, 40]
+
+
 def test_mixed_counts(device):
     """Requests with no new tokens, one, several: in a group, and between groups; max_new unknown or wrong; an empty request."""
     lens, new = [400, 410, 390, 0, 5, 850, 860, 849], [1, 0, 6, 0, 2, 3, 1, 2]
@@ -142,13 +165,15 @@ def test_nothing_in_common(device):
     check(run(a, s), *a.expected())
 
 
-def test_missing_blocks(device):
+@pytest.mark.parametrize("n", SIZES)
+def test_missing_blocks(n, device):
     """Blocks missing in a prefix, all of a prefix, all of a request's own."""
     from gemma_triton_flash_attn_amd import kv4
 
-    for holes, whole in (([2], False), ([0, 1, 2, 3, 4, 5, 6, 7], False), ([1], True)):
-        a = Answers(device, [530, 545, 513], [1, 1, 1], 8, 2, 128, [(3, 512)], bs=64).store()
-        held = [torch.ones(n, dtype=torch.bool) for n in a.lens]
+    lens = [513 + 16 * i % 50 for i in range(n)]
+    for holes, whole in (([2], False), ([0, 1, 2, 3, 4, 5, 6, 7], False), ([1], True), ([0, 7], False)):
+        a = Answers(device, lens, [1] * n, 16, 4, 128, [(n, 512)], bs=64).store()
+        held = [torch.ones(m, dtype=torch.bool) for m in a.lens]
         for c in holes:
             a.table[:, c] = -1
             for h in held:
@@ -157,28 +182,31 @@ def test_missing_blocks(device):
             a.table[1, 8:] = 1 << 20
             held[1][512:] = False
         s = kv4.share(a.table, a.lens_dev, a.cu, block_size=64, least=64)
-        assert s.skip.tolist() == [512] * 3
+        assert s.skip.tolist() == [512] * n
         check(run(a, s), *a.expected(held=held))
     a.table.fill_(-1)  # nothing at all: zeros
     assert not run(a, kv4.share(a.table, a.lens_dev, a.cu, block_size=64, least=64)).any()
 
 
+@pytest.mark.parametrize("n", SIZES)
 @pytest.mark.parametrize("where", ["prefix", "own"])
-def test_values_that_are_no_numbers(where, device):
+def test_values_that_are_no_numbers(where, n, device):
     """A token of no number in the prefix reaches its whole group, one in a request's own keys that request alone."""
-    a = Answers(device, [530, 545, 513, 300, 300], [1] * 5, 8, 2, 128, [(3, 512), (2, 256)], bs=64)
-    for b in range(3) if where == "prefix" else [1]:
+    lens = [530 + i for i in range(n)] + [300, 300]
+    a = Answers(device, lens, [1] * len(lens), 16, 4, 128, [(n, 512), (2, 256)], bs=64)
+    for b in range(n) if where == "prefix" else [1]:
         a.k[b][0, 100 if where == "prefix" else 530, 3] = float("inf")
     a.store()
     o = run(a, a.share())
     want, bound = a.expected()
-    assert torch.isnan(want[:, 1]).any() and not torch.isnan(want[:, 3:]).any()
+    assert torch.isnan(want[:, 1]).any() and not torch.isnan(want[:, n:]).any()
     check(o, want, bound)
 
 
-def test_infinite_queries(device):
+@pytest.mark.parametrize("n", SIZES)
+def test_infinite_queries(n, device):
     """A query of infinities answers NaN in both parts and leaves its neighbours alone."""
-    a = Answers(device, [530, 545, 513], [1, 1, 1], 8, 2, 128, [(3, 512)], bs=64).store()
+    a = Answers(device, [530 + i for i in range(n)], [1] * n, 16, 4, 128, [(n, 512)], bs=64).store()
     plain = run(a, a.share())
     a.q[0, 2, 1] = float("inf")
     o = run(a, a.share())
@@ -186,6 +214,28 @@ def test_infinite_queries(device):
     keep = torch.ones_like(o, dtype=torch.bool)
     keep[0, 2, 1] = False
     assert torch.equal(o[keep], plain[keep])
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_any_groups(seed, device):
+    """Random groups, lengths, counts and layers."""
+    r = random.Random(100 + seed)
+    D, (Hq, Hkv) = r.choice([64, 128, 256, 512]), r.choice([(4, 4), (8, 1), (16, 4), (6, 2), (32, 4)])
+    bs = r.choice([32, 64, 256, 1024])
+    groups, lens, new = [], [], []
+    for _ in range(r.choice([1, 3, 6])):
+        n, common = r.choice([1, 2, 5, 20, 66]), r.choice([0, 1, 3]) * bs
+        groups.append((n, common))
+        for _ in range(n):
+            k = r.choice([0, 1, 1, 1, r.randint(1, 4)])
+            new.append(k)
+            lens.append(common + r.choice([k, k + r.randint(0, 70), k + r.randint(0, 700)]))
+    a = Answers(device, lens, new, Hq, Hkv, D, groups, bs=bs, seed=seed, dtype=r.choice([torch.bfloat16, torch.float16]), pad=r.choice([0, 3])).store()
+    if a.T == 0:
+        return
+    kw = dict(softcap=r.choice([None, 15.0]), causal=r.random() < 0.8)
+    want, bound = a.expected(causal=kw["causal"], softcap=kw["softcap"] or 0.0)
+    check(a.attend(max_new=max(max(new), 1), shared=a.share(least=r.choice([1, bs])), **kw), want, bound)
 
 
 def test_one_token_per_batch_entry(device):
