@@ -132,7 +132,8 @@ class Kv4AttnArgs(ctypes.Structure):
                 ("table_width", ctypes.c_int32), ("causal", ctypes.c_int32), ("window", ctypes.c_int32),
                 ("max_new", ctypes.c_int32), ("scale", ctypes.c_float), ("softcap", ctypes.c_float),
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p),
-                ("shared_skip", ctypes.c_void_p), ("shared_cu", ctypes.c_void_p), ("shared_lens", ctypes.c_void_p)]
+                ("shared_skip", ctypes.c_void_p), ("shared_cu", ctypes.c_void_p), ("shared_lens", ctypes.c_void_p),
+                ("shared_apart", ctypes.c_int32)]
 
 
 class Kv4PagesArgs(ctypes.Structure):

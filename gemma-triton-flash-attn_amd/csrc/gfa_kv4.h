@@ -201,13 +201,11 @@ struct Kv4ShareParams {
 constexpr int kSplitRows = 16;
 constexpr int kv4_chunk_rows(int D) { return D >= 128 ? 128 : 256; }
 
-// Workgroups of the chunk kernel that a CU holds (by their registers).
+// Workgroups of the chunk kernel that a CU holds (by their registers), and of the shared prefixes' kernel (gfa_kv4_shared.hip).
 constexpr int kv4_chunk_wgs(int D) { return D == 512 ? 1 : D == 128 ? 3 : 2; }
-// Workgroups of the shared prefixes' kernel that a CU holds (gfa_kv4_shared.hip).
-constexpr int kv4_shared_wgs(int D) { return D == 512 ? 1 : 2; }
 
 // What the attention kernels' device functions work on: a whole call; or, where requests share prefixes (gfa_kv4_share), the groups'
-// prefixes as requests of their own (skip NULL) or the requests' keys behind them, which leave sums alone.
+// prefixes as requests of their own or the requests' keys behind them.
 enum Kv4Part : int { kWhole, kPart };
 
 struct Kv4AttnParams {
@@ -234,7 +232,7 @@ struct Kv4AttnParams {
   int row_blocks, join_rows, join_slice, join_parts;
   float* part;    // (slots, Hkv, rows, D) sums and (slots, Hkv, rows, 2) row maxima and sums
   float* part_ml;
-  const int* skip;  // kPart: (B) tokens of the request's prefix, or NULL
+  const int* skip;  // kPart: (B) tokens of the request's prefix
 };
 
 // A call over shared prefixes (gfa_kv4_shared.hip): the sums of one part of the work, see Kv4AttnParams.
@@ -244,11 +242,19 @@ struct Kv4Sums {
   int nblocks, slots;
   float *part, *part_ml;
 };
+// A row block of a request: its chunks' sums (slot -1: it is out already), its first token and new ones, and its group's sums.
+struct Kv4Join {
+  int slot, nch, rb, t0, fresh;
+  int group_nch, group_slot, group_blocks, group_t0, group_rows, large, unused;
+};
 struct Kv4SharedParams {
   Kv4AttnParams p;
   const int *group_cu, *group_lens;
   int row_limit;          // of the groups
   Kv4Sums many, few, rest;  // prefixes of groups of many rows and of few, the requests behind their prefixes
+  float many_cost, apart_cost, worth;  // see plan_of in gfa_kv4_shared.hip
+  int* joined;              // row blocks of the requests, and where their sums are
+  Kv4Join* joins;
 };
 
 }  // namespace gfa

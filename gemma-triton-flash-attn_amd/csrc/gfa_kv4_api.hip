@@ -113,6 +113,8 @@ int row_limit(const gfa_kv4_attn_args* a, int64_t requests) { return requests * 
 
 enum Kind { kWhole, kPrefix, kRest };  // a whole call, the groups' prefixes, the requests behind them
 
+float share_of(int64_t hkv, int target) { return (float)((double)hkv / target * (1.0 + 1.0 / 4096)); }  // see chunk_tiles
+
 void size_part(Part& s, const gfa_kv4_attn_args* a, Kind kind, int64_t row_blocks, int rows, int64_t most_rows, int min_tiles, int target, int spare) {
   int64_t tiles = (int64_t)a->table_width * a->cache.block_size / 32;  // most tiles of a row block
   if (kind == kWhole && a->causal && a->window > 0) {
@@ -143,7 +145,7 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, Kind kind, int64_t row_block
   const int64_t wgs = rows == kRows ? (row_bound * s.join_parts + groups - 1) / groups : rows / 32 * (D <= 128 ? 16 : D / 8) / 4;
   const int64_t most_wgs = 4096 / std::max<int64_t>(1, row_blocks * hkv);
   s.join_rows = (int)std::max<int64_t>(1, std::min(wgs, most_wgs));
-  s.share = (float)((double)hkv / target * (1.0 + 1.0 / 4096));  // see chunk_tiles
+  s.share = share_of(hkv, target);
   const int64_t items = std::min(row_blocks * chunks, row_blocks + (target + hkv - 1) / hkv);
   s.nblocks = items * hkv + spare;
   if (s.join) {
@@ -207,21 +209,38 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
   // 1024, 33 us with chunks of 8 tiles, 57 unsplit; 1000 tokens beside seven requests 66 us with 18 tiles, 74 unsplit;
   // 512 tokens of four requests 76-84 us split, 71 unsplit.
   // Of prefixes one workgroup a CU: their sums are as much again as what they read (64 answers to a 16k prompt, D = 128: 46.2 us, two
-  // 57), chunks of 4 tiles where row blocks are few (16 answers of 4 drafted tokens, 3k, 8:4 D = 256: 24.3 us, of 8 27.8).
+  // 57), chunks of 8 tiles however many the row blocks could be (31 answers to each of three prompts of 500, 32:8 D = 128: 30 us, of 32
+  // 36), of 4 where they are few (16 answers of 4 drafted tokens, 3k, 8:4 D = 256: 24.3 us, of 8 27.8).
   const int64_t alone = many * a->cache.heads_kv;
   const int target = kind != kPrefix ? 256 * gfa::kv4_chunk_wgs(D) : D < 512 ? 256 : 160;
-  const int min_tiles = alone >= 256 ? 64 : alone >= 128 ? 32 : kind == kPrefix && alone <= 16 ? 4 : 8;
+  const int min_tiles = kind == kPrefix ? (alone <= 16 ? 4 : 8) : alone >= 256 ? 64 : alone >= 128 ? 32 : 8;
   size_part(s.many, a, kind, many, big, most * G, min_tiles, target, 0);
   return s;
 }
 
-// Whether prefixes are taken apart: without a window, which bounds what a request reads, and for requests of few rows; where
-// max_new is not known, of few rows on average.
+// What taking prefixes apart saves is counted in passes of the split kernel over a tile (one row block, one KV head): `tiles` of them take
+// a us of the whole GPU, one of the chunk kernel takes as long as many_cost of them. From calls of 40 to 300 requests, by head dim: 151k
+// passes 72 us and 60k 52 us, 24k 43 us, 43k 133 us; the chunk kernel's 2.1 us a tile and CU at D = 512, 1.3, 1.1, 0.8.
+struct Rate {
+  float tiles, many_cost;
+};
+Rate rate_of(int D) { return D == 64 ? Rate{2100.f, 6.5f} : D == 128 ? Rate{1200.f, 5.f} : D == 256 ? Rate{570.f, 2.9f} : Rate{320.f, 2.6f}; }
+// A row block whose request is taken apart leaves sums in two parts and is joined, about as much again as 10 tiles of it; a call has one
+// kernel's latency more: it pays from 4 us on. Apart against whole, us: two answers of 5 tokens to a 2k prompt, 32:4 D = 512, 35.7 24.0;
+// 16 answers of 8 to each of eight prompts of 740 tokens, 8:4 D = 256, 66 51; two answers to each of six prompts of 8k, 8:1 D = 512,
+// 27.8 31.7; 16 of 4 drafted tokens, 3k, 8:4 D = 256, 24.2 25.7; 44 to each of four of 1352, 32:8 D = 128, 41 52; 64 to one of 16k, 47 215.
+constexpr float kApartCost = 10.f, kApartLeast = 4.f;
+float worth_of(const gfa_kv4_attn_args* a) { return kApartLeast * rate_of(a->cache.head_dim).tiles / (float)a->cache.heads_kv; }
+
+// Whether prefixes may be taken apart: without a window, which bounds what a request reads, and for requests of few rows; where
+// max_new is not known, of few rows on average. Not where the tables are too narrow for it to pay.
 bool takes_prefixes(const gfa_kv4_attn_args* a) {
   if (a->shared_skip == nullptr || (a->causal && a->window > 0) || a->requests < 2) return false;
-  const int64_t T = (int64_t)a->batch * a->seq_len;
+  const int64_t T = (int64_t)a->batch * a->seq_len, G = a->heads_q / a->cache.heads_kv;
   const int64_t rows = a->max_new > 0 ? a->max_new : (T + a->requests - 1) / a->requests;
-  return rows * (a->heads_q / a->cache.heads_kv) <= row_limit(a, a->requests);
+  if (rows * G > row_limit(a, a->requests)) return false;
+  const double tiles = (double)a->table_width * a->cache.block_size / 32, row_blocks = (double)(T * G + (kRows - 1) * (int64_t)a->requests) / kRows;
+  return a->shared_apart != 0 || (tiles - kApartCost) * row_blocks > worth_of(a);
 }
 
 // The parts of a call.
@@ -229,7 +248,8 @@ struct Steps {
   Split whole, prefix, rest;  // whole, or the two others
   bool shared;
   size_t bytes() const {
-    return shared ? prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() : whole.few.bytes() + whole.many.bytes();
+    if (!shared) return whole.few.bytes() + whole.many.bytes();
+    return prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() + 64 + (size_t)rest.few.row_blocks * sizeof(gfa::Kv4Join);
   }
 };
 Steps steps_of(const gfa_kv4_attn_args* a) {
@@ -613,6 +633,11 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     sp.many = sums_of(s.prefix.many);
     sp.few = sums_of(s.prefix.few);
     sp.rest = sums_of(s.rest.few);
+    sp.joined = reinterpret_cast<int*>(ws);
+    sp.joins = reinterpret_cast<gfa::Kv4Join*>(ws + 64);
+    sp.many_cost = rate_of(D).many_cost;
+    sp.apart_cost = kApartCost;
+    sp.worth = a->shared_apart != 0 ? -INFINITY : worth_of(a);
     return launched(gfa::launch_kv4_shared(sp, D, bf16, cap, stream), "attention over shared prefixes");
   }
   for (const bool large : {true, false}) {

@@ -7,7 +7,19 @@ namespace gfa {
 template <int D, bool IS_BF16, bool CAP, bool ONCE>
 __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kernel(const Kv4AttnParams p) {
   constexpr Kv4Part PART = kWhole;
+  __shared__ __attribute__((aligned(16))) f32x4 sums_lds[kWaves][D / 16 * 64];
+  auto o_lds = [&](int w) __attribute__((always_inline)) { return sums_lds[w]; };
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int block = (int)blockIdx.x;
+  const int head = p.hkv.rem(block);
+  const Item it = find_item<kRows, false>(p, p.hkv.quot(block), lane);
+  if (it.b < 0) {
+    if (p.cu == nullptr) return;
+    const int64_t taken = (int64_t)it.items * p.cache.Hkv;
+    zero_rows<D>(p, block - taken, p.nblocks - taken);
+    return;
+  }
 #include "gfa_kv4_split.inc"
 }
 

@@ -7,7 +7,21 @@ namespace gfa {
 template <int D, bool IS_BF16, bool CAP>
 __global__ __launch_bounds__(256, kv4_chunk_wgs(D)) void kv4_chunk_kernel(const Kv4AttnParams p) {
   constexpr Kv4Part PART = kWhole;
+  constexpr int TILE = Kv4Layout<D>::TILE_CODES;
+  __shared__ __attribute__((aligned(1024))) char k_lds0[TILE], k_lds1[TILE], v_lds0[TILE], v_lds1[TILE], s_lds0[1024], s_lds1[1024];
+  char GFA_LDS* const K0 = (char GFA_LDS*)k_lds0;
+  char GFA_LDS* const K1 = (char GFA_LDS*)k_lds1;
+  char GFA_LDS* const V0 = (char GFA_LDS*)v_lds0;
+  char GFA_LDS* const V1 = (char GFA_LDS*)v_lds1;
+  char GFA_LDS* const S0 = (char GFA_LDS*)s_lds0;
+  char GFA_LDS* const S1 = (char GFA_LDS*)s_lds1;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int block = (int)blockIdx.x;
+  const int head = p.hkv.rem(block);
+  constexpr int ROWS = kv4_chunk_rows(D);
+  const Item it = find_item<ROWS, true>(p, p.hkv.quot(block), lane);
+  if (it.b < 0) return;
 #include "gfa_kv4_chunk.inc"
 }
 

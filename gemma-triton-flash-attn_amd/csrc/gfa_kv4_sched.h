@@ -7,8 +7,8 @@
 // 2 tiles / per chunks, and with per at least the call's tiles / target there are fewer than 2 target slots. Requests of up to
 // row_limit rows are the split kernel's, the others the chunk kernel's (LARGE).
 //
-// Where requests share prefixes (kPart) the same split is taken twice: of the groups' prefixes, each group a request whose
-// keys all its rows see (p.skip NULL), and of the requests behind their prefixes. Every row block leaves sums then.
+// Where requests share prefixes (kPart) there are two kinds of request, groups with their prefix and requests behind theirs
+// (gfa_kv4_shared.hip, which finds the items of a call as the functions here do).
 #pragma once
 #include <type_traits>
 
@@ -23,38 +23,29 @@ struct Request {
   int t0, fresh, len;  // first new token, new tokens, tokens with the new ones
   int row_blocks;      // 0: not this kernel's
   int tiles;           // most key tiles that a row block sees
-  int skip;            // kPart: tokens of its prefix
+  int skip;            // kPart: tokens of its prefix that others see to
 };
 // Its three loads go out together (one wait: their latency is a good part of a short call).
-template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
+template <int ROWS, bool LARGE>
 __device__ __forceinline__ Request request_of(const Kv4AttnParams& p, int b) {
   Request r{};
   const int bc = min(b, p.B - 1);
   const int* cu = p.cu != nullptr ? p.cu : p.lens;  // without cu read for nothing
   const int t0 = cu[bc], t1 = cu[p.cu != nullptr ? bc + 1 : bc], len = p.lens[bc];
-  int skip = 0;
-  if constexpr (PART == kPart) skip = (p.skip != nullptr ? p.skip : p.lens)[bc];
   if (b >= p.B) return r;
   r.t0 = p.cu != nullptr ? t0 : b * p.each;
   r.fresh = p.cu != nullptr ? min(max((int)((unsigned)t1 - (unsigned)t0), 0), p.T) : p.each;
   r.len = max(len, 0);
-  if constexpr (PART == kPart) {
-    if (p.skip == nullptr) {
-      r.fresh = r.len > 0 ? r.fresh : 0;  // a group without a prefix
-    } else {
-      r.skip = max(skip, 0);
-    }
-  }
   const int rows = r.fresh * p.G;
   r.row_blocks = (rows > p.row_limit) != LARGE ? 0 : (int)(((unsigned)rows + ROWS - 1) / ROWS);
   const int held = min(r.len, p.M << p.cache.bs_log2);
-  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : PART == kPart ? r.skip : 0;
+  const int lo = p.window > 0 ? (int)max((int64_t)r.len - r.fresh - p.window + 1, (int64_t)0) : 0;
   r.tiles = held > lo ? (held + kTile - 1) / kTile - lo / kTile : 0;
   if (p.window > 0) r.tiles = min(r.tiles, p.window_tiles);
   return r;
 }
 // Key tiles [x, y) that some row of the request's row block of `rows` rows from row0 on sees.
-template <Kv4Part PART = kWhole>
+template <Kv4Part PART>
 __device__ __forceinline__ int2 tiles_of_rows(const Kv4AttnParams& p, const Request& r, int row0, int rows) {
   const int i_lo = p.g.quot(row0), i_hi = min(p.g.quot(row0 + rows - 1), r.fresh - 1);
   const int pos0 = r.len - r.fresh;  // position of new token 0
@@ -64,10 +55,9 @@ __device__ __forceinline__ int2 tiles_of_rows(const Kv4AttnParams& p, const Requ
   return k_hi > k_lo ? make_int2(k_lo / kTile, (k_hi + kTile - 1) / kTile) : make_int2(0, 0);
 }
 // Lane src's request in every lane.
-template <Kv4Part PART = kWhole>
 __device__ __forceinline__ Request request_from(const Request& r, int src) {
   auto at = [&](int x) { return __builtin_amdgcn_readlane(x, src); };
-  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles), PART == kPart ? at(r.skip) : 0};
+  return Request{at(r.t0), at(r.fresh), at(r.len), at(r.row_blocks), at(r.tiles), at(r.skip)};
 }
 
 // Sum over the wave's lanes (the steps of wave_prefix_sum).
@@ -91,12 +81,12 @@ __device__ __forceinline__ float wave_sum(float x) {
 // sum is a float's (a product of two counts can pass 32 bits); `share` = Hkv / target is rounded up by more than the
 // sum can be off, so that the grid the host sized holds every item. The same operations in the same order wherever
 // it is taken: contraction is off.
-template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
+template <int ROWS, bool LARGE>
 __device__ __forceinline__ int chunk_tiles(const Kv4AttnParams& p, const Request& r0, int lane) {
 #pragma clang fp contract(off)
   float total = (float)r0.row_blocks * (float)r0.tiles;
   for (int b0 = 64; b0 < p.B; b0 += 64) {
-    const Request r = request_of<ROWS, LARGE, PART>(p, b0 + lane);
+    const Request r = request_of<ROWS, LARGE>(p, b0 + lane);
     const float x = (float)r.row_blocks * (float)r.tiles;
     total += x;
   }
@@ -112,24 +102,24 @@ struct Item {
   int b;            // -1: there is no such item
   int rb, ch, nch;  // row block, chunk of nch
   int items;        // of the whole call, where b < 0
-  int slot;         // of nch > 1: its place among the items of split row blocks
+  int slot;         // of nch > 1: its place among the items of split row blocks (kPart: of all that leave sums, else -1)
 };
-template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
+template <int ROWS, bool LARGE>
 __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int lane) {
   Item it{};
   it.b = -1;
-  Request r = request_of<ROWS, LARGE, PART>(p, lane);
-  const int per = chunk_tiles<ROWS, LARGE, PART>(p, r, lane);
+  Request r = request_of<ROWS, LARGE>(p, lane);
+  const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
   for (int b0 = 0;;) {
     const int nch = chunks_of(r, per);
-    const int mine = r.row_blocks * nch, split = PART == kPart || nch > 1 ? mine : 0;
+    const int mine = r.row_blocks * nch, split = nch > 1 ? mine : 0;
     const int s = wave_prefix_sum(mine), z = wave_prefix_sum(split);
     const int before = it.items + s - mine;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= before && item < before + mine);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
       it.b = b0 + src;
-      it.rq = request_from<PART>(r, src);
+      it.rq = request_from(r, src);
       it.nch = __builtin_amdgcn_readfirstlane(chunks_of(it.rq, per));
       const int i = item - __builtin_amdgcn_readlane(before, src);
       it.rb = __builtin_amdgcn_readfirstlane(quotient(i, it.nch));
@@ -140,7 +130,7 @@ __device__ __forceinline__ Item find_item(const Kv4AttnParams& p, int item, int 
     it.items += __builtin_amdgcn_readlane(s, 63);
     it.slot += __builtin_amdgcn_readlane(z, 63);
     if ((b0 += 64) >= p.B) break;
-    r = request_of<ROWS, LARGE, PART>(p, b0 + lane);
+    r = request_of<ROWS, LARGE>(p, b0 + lane);
   }
   return it;
 }
@@ -152,23 +142,23 @@ struct RowBlock {
   int rb, nch;
   int slot;
 };
-template <int ROWS, bool LARGE, Kv4Part PART = kWhole>
+template <int ROWS, bool LARGE>
 __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int block, int lane) {
   RowBlock out{};
   out.b = -1;
-  Request r = request_of<ROWS, LARGE, PART>(p, lane);
-  const int per = chunk_tiles<ROWS, LARGE, PART>(p, r, lane);
+  Request r = request_of<ROWS, LARGE>(p, lane);
+  const int per = chunk_tiles<ROWS, LARGE>(p, r, lane);
   int blocks = 0;
   for (int b0 = 0;;) {
     const int s = wave_prefix_sum(r.row_blocks);
-    const int nch = chunks_of(r, per), split = PART == kPart || nch > 1 ? r.row_blocks * nch : 0;
+    const int nch = chunks_of(r, per), split = nch > 1 ? r.row_blocks * nch : 0;
     const int z = wave_prefix_sum(split);
     const int before = blocks + s - r.row_blocks;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(block >= before && block < before + r.row_blocks);
     if (hit != 0) {
       const int src = __builtin_ctzll(hit);
       out.b = b0 + src;
-      out.rq = request_from<PART>(r, src);
+      out.rq = request_from(r, src);
       out.nch = __builtin_amdgcn_readfirstlane(chunks_of(out.rq, per));
       out.rb = block - __builtin_amdgcn_readlane(before, src);
       out.slot += __builtin_amdgcn_readlane(z - split, src) + out.rb * out.nch;
@@ -177,7 +167,7 @@ __device__ __forceinline__ RowBlock find_row_block(const Kv4AttnParams& p, int b
     blocks += __builtin_amdgcn_readlane(s, 63);
     out.slot += __builtin_amdgcn_readlane(z, 63);
     if ((b0 += 64) >= p.B) break;
-    r = request_of<ROWS, LARGE, PART>(p, b0 + lane);
+    r = request_of<ROWS, LARGE>(p, b0 + lane);
   }
   return out;
 }

@@ -452,7 +452,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> kv4_plan(const Tensor& lens, 
 Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales, bool bf16, const Tensor& table,
                      const Tensor& lens, const std::optional<Tensor>& cu, int64_t max_new, bool causal, int64_t window,
                      double scale, double softcap, const std::optional<Tensor>& shared_skip, const std::optional<Tensor>& shared_cu,
-                     const std::optional<Tensor>& shared_lens) {
+                     const std::optional<Tensor>& shared_lens, bool apart) {
   check_cache(codes, scales);
   check_token_rows("q", q, codes, bf16, false);
   const int64_t B = q.size(0), Hq = q.size(1), N = q.size(2), Hkv = codes.size(1);
@@ -508,6 +508,7 @@ Tensor kv4_attention(const Tensor& q, const Tensor& codes, const Tensor& scales,
     a.shared_skip = static_cast<const int32_t*>(ss.data_ptr());
     a.shared_cu = static_cast<const int32_t*>(sc.data_ptr());
     a.shared_lens = static_cast<const int32_t*>(sl.data_ptr());
+    a.shared_apart = apart;
   }
   Tensor ws;
   const size_t need = api.kv4_attn_workspace_bytes(&a);

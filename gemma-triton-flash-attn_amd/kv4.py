@@ -147,7 +147,7 @@ def read(cache: Cache, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]
 
 def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Tensor, cu: Optional[torch.Tensor] = None, *,
               max_new: Optional[int] = None, causal: bool = True, slide_size: int = 0, scale: Optional[float] = None,
-              softcap: Optional[float] = None, shared: Optional[Shared] = None) -> torch.Tensor:
+              softcap: Optional[float] = None, shared: Optional[Shared] = None, apart: bool = False) -> torch.Tensor:
     """Attention of a step's new tokens over the cache, which holds their own keys and values already.
 
     q: (B, Hq, N, D), Hq a multiple of the cache's heads. table: (R, M) int32, lens: (R,) int32 tokens of each
@@ -161,16 +161,17 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
     kernels. ``scale`` defaults to 1/sqrt(D); ``softcap`` as in ``flash_attn_gqa_train``. There is no gradient.
 
     ``shared``: ``share``'s result for this table, lens and cu. The prefix of a group of requests is then read once for all
-    of them, and the parts are joined: the same result, but for the order in which 32-bit sums are taken. It has no
-    effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average, times Hq / Hkv above 64; 128
-    where requests times KV heads are at most four), which are bound by products."""
+    of them, and the parts are joined: the same result, but for the order in which 32-bit sums are taken. That is done
+    where it is faster, which is found on the device from the lengths of all requests, or with ``apart`` wherever there is a
+    group. It has no effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average,
+    times Hq / Hkv above 64; 128 where requests times KV heads are at most four), which are bound by products."""
     _refuse_gradients("attention over the cache", q, q)
     if max_new is not None and max_new < 1:
         raise ValueError("max_new must be at least 1")
     fn = _lib.native().kv4_attention if _plain(q) else torch.ops.gfa.kv4_attention
     return fn(q, cache.codes, cache.scales, cache.dtype is torch.bfloat16, table, lens, cu, max_new or 0, bool(causal),
               int(slide_size or 0), _default_scale(q.shape[-1], scale), _check_softcap(softcap),
-              *(shared if shared is not None else (None, None, None)))
+              *(shared if shared is not None else (None, None, None)), bool(apart))
 
 
 class Fork(NamedTuple):
@@ -322,14 +323,14 @@ def _read_fake(codes, scales, bf16, slots):
 def _attention_op(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, bf16: bool, table: torch.Tensor,
                   lens: torch.Tensor, cu: Optional[torch.Tensor], max_new: int, causal: bool, window: int, scale: float,
                   softcap: float, shared_skip: Optional[torch.Tensor] = None, shared_cu: Optional[torch.Tensor] = None,
-                  shared_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+                  shared_lens: Optional[torch.Tensor] = None, apart: bool = False) -> torch.Tensor:
     return _lib.native().kv4_attention(q, codes, scales, bf16, table, lens, cu, max_new, causal, window, scale, softcap,
-                                       shared_skip, shared_cu, shared_lens)
+                                       shared_skip, shared_cu, shared_lens, apart)
 
 
 @_attention_op.register_fake
 def _attention_fake(q, codes, scales, bf16, table, lens, cu, max_new, causal, window, scale, softcap, shared_skip=None,
-                    shared_cu=None, shared_lens=None):
+                    shared_cu=None, shared_lens=None, apart=False):
     return _out_like(q)
 
 

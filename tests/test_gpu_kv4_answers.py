@@ -56,7 +56,7 @@ class Server:
         for i, (cache, (hq, hkv, D)) in enumerate(zip(self.caches, LAYERS)):
             q, k, v = (self.randn(1, h, T, D) for h in (hq, hkv, hkv))
             kv4.write(cache, k.to(self.device), v.to(self.device), p.slots)
-            o = kv4.attention(q.to(self.device), cache, self.table, p.lens, p.cu, max_new=max(max(new), 1), shared=s)
+            o = kv4.attention(q.to(self.device), cache, self.table, p.lens, p.cu, max_new=max(max(new), 1), shared=s, apart=True)
             t = 0
             for b, n in enumerate(new):
                 kb, vb = self.rows[b][i]
@@ -159,7 +159,7 @@ def test_a_captured_turn(device):
         outs = []
         for cache, q, k in zip(s.caches, x["q"], x["k"]):
             kv4.write(cache, k, k, p.slots)
-            outs.append(kv4.attention(q, cache, s.table, p.lens, p.cu, max_new=3, shared=shared))
+            outs.append(kv4.attention(q, cache, s.table, p.lens, p.cu, max_new=3, shared=shared, apart=True))
         v = kv4.verify(x["target"], x["draft"], x["tokens"], x["accept"], x["sample"], p.lens, p.cu)
         f = kv4.fork(s.caches, s.table, p.lens, s.free, p.used, keep=v.lens)
         s.table.copy_(f.table)

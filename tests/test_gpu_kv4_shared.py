@@ -87,7 +87,8 @@ def answers(name, device, seed=0, pad=0, **kw):
 
 
 def run(a, shared, **kw):
-    return a.attend(max_new=max(a.new), shared=shared, **kw)
+    """With every group's prefix taken apart, whatever that saves, unless kw has it otherwise."""
+    return a.attend(**{**dict(max_new=max(a.new), shared=shared, apart=True), **kw})
 
 
 @pytest.mark.parametrize("name", list(CASES))
@@ -145,7 +146,7 @@ def test_mixed_counts(device):
     s = a.share()
     assert s.skip.tolist() == [384, 384, 384, 0, 0, 832, 832, 832]
     for kw in (dict(max_new=6), dict(), dict(max_new=1)):
-        check(a.attend(shared=s, **kw), want, bound)
+        check(a.attend(shared=s, apart=True, **kw), want, bound)
     q = a.q.to(device)
     assert torch.equal(q.cpu(), a.q)
 
@@ -163,6 +164,42 @@ def test_nothing_in_common(device):
     s = a.share()
     assert not s.skip.any() and not s.lens.any()
     check(run(a, s), *a.expected())
+
+
+@pytest.mark.parametrize("D,Hkv", [(512, 1), (512, 4), (256, 4), (128, 8), (64, 16)])
+def test_where_it_pays(D, Hkv, device):
+    """The call's own choice, on either side of the line: many requests over a long prefix, few over a short one, none in common; the
+    same kernels with the lengths changed in place. Requests without a prefix in one chunk are the plain call's, bit for bit."""
+    a = Answers(device, [2100 + i for i in range(48)] + [90, 70], [1] * 50, 4 * Hkv, Hkv, D, [(48, 2048), (2, 64)], bs=64).store()
+    s = a.share()
+    assert s.lens.tolist()[0] == 2048 and s.lens.tolist()[48] == 64
+    want = a.expected()
+    for kw in (dict(), dict(apart=True), dict(apart=False)):
+        check(run(a, s, **kw), *want)
+    b = Answers(device, [150, 140, 400], [1, 2, 1], 4 * Hkv, Hkv, D, [(2, 128), (1, 0)], bs=64).store()
+    s = b.share()
+    assert s.lens.tolist() == [128, 0, 0]
+    check(run(b, s), *b.expected())
+    assert torch.equal(run(b, s, apart=False), run(b, None))
+
+
+@pytest.mark.parametrize("n", [64, 65, 128, 256, 257, 700])
+def test_many_requests(n, device):
+    """More requests than a wave looks through at once: dealt to four, several rounds each; groups that lie across the deal, requests
+    without tokens, tokens of no request ahead and behind."""
+    r = random.Random(n)
+    groups, left = [], n
+    while left:
+        k = min(left, r.choice([1, 2, 3, 40, 150]))
+        groups.append((k, r.choice([64, 128, 320]) if k > 1 else 0))
+        left -= k
+    lens = [c + r.randint(4, 70) for k, c in groups for _ in range(k)]
+    new = [r.choice([0, 1, 1, 2, 3]) for _ in lens]
+    a = Answers(device, lens, new, 4, 2, 64, groups, bs=64, pad=5, seed=n).store()
+    s = a.share(least=64)
+    want = a.expected()
+    for kw in (dict(), dict(apart=False), dict(max_new=1)):
+        check(run(a, s, **kw), *want)
 
 
 @pytest.mark.parametrize("n", SIZES)
@@ -235,7 +272,7 @@ def test_any_groups(seed, device):
         return
     kw = dict(softcap=r.choice([None, 15.0]), causal=r.random() < 0.8)
     want, bound = a.expected(causal=kw["causal"], softcap=kw["softcap"] or 0.0)
-    check(a.attend(max_new=max(max(new), 1), shared=a.share(least=r.choice([1, bs])), **kw), want, bound)
+    check(a.attend(max_new=max(max(new), 1), shared=a.share(least=r.choice([1, bs])), apart=seed % 5 > 0, **kw), want, bound)
 
 
 def test_one_token_per_batch_entry(device):
@@ -248,7 +285,7 @@ def test_one_token_per_batch_entry(device):
     q = a.q[0].transpose(0, 1)[:, :, None].contiguous().to(device)  # (R, Hq, 1, D)
     wide = torch.cat([q, q], 3)[..., :128]
     for x in (q, wide, wide.transpose(1, 2).contiguous().transpose(1, 2)):
-        o = kv4.attention(x, a.cache, a.table, a.lens_dev, a.cu, max_new=1, shared=s)
+        o = kv4.attention(x, a.cache, a.table, a.lens_dev, a.cu, max_new=1, shared=s, apart=True)
         assert o.shape == x.shape and torch.equal(o[:, :, 0].transpose(0, 1), want[0])
 
 
@@ -262,7 +299,7 @@ def test_captured(device):
 
     def step():
         s = kv4.share(table, lens, a.cu, block_size=a.bs, least=64)
-        return kv4.attention(q, a.cache, table, lens, a.cu, max_new=1, shared=s)
+        return kv4.attention(q, a.cache, table, lens, a.cu, max_new=1, shared=s, apart=True)
 
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -275,7 +312,7 @@ def test_captured(device):
     s = other.share()
     oq = other.q.to(device)
     with torch.cuda.graph(second):
-        got2 = kv4.attention(oq, other.cache, other.table, other.lens_dev, other.cu, max_new=1, shared=s)
+        got2 = kv4.attention(oq, other.cache, other.table, other.lens_dev, other.cu, max_new=1, shared=s, apart=True)
     r = random.Random(0)
     for i in range(4):
         lens.copy_(ints([n - r.choice([0, 0, 64, 200]) if n > 300 else n for n in a.lens], device))
@@ -297,6 +334,7 @@ def test_registered(device):
     torch.library.opcheck(torch.ops.gfa.kv4_share, (a.table, a.lens_dev, a.cu, a.bs, 64))
     args = (q, a.cache.codes, a.cache.scales, True, a.table, a.lens_dev, a.cu, 1, True, 0, 0.125, 0.0, *s)
     torch.library.opcheck(torch.ops.gfa.kv4_attention, args)
+    torch.library.opcheck(torch.ops.gfa.kv4_attention, (*args, True))
 
     def step(q, codes, scales, table, lens, cu):
         cache = kv4.Cache(codes, scales, torch.bfloat16)
