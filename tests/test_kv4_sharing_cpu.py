@@ -210,15 +210,15 @@ def test_verify_refusals():
     (dict(shared_skip=2), INVALID), (dict(shared_cu=0), INVALID), (dict(shared_lens=6), INVALID), (dict(cu=0), INVALID), (dict(workspace_bytes=64), WORKSPACE)])
 def test_shared_attention_refusals(over, status):
     lib = _lib.load()
-    a = dict(shared_skip=64, shared_cu=64, shared_lens=64, max_new=1)
+    a = dict(shared_skip=64, shared_cu=64, shared_lens=64, shared_apart=1, max_new=1)
     assert lib.gfa_kv4_attn(ctypes.byref(_attn(**{**a, **over}))) == status, lib.gfa_last_error()
 
 
 # ---- what the host sizes for shared prefixes ----
 
-def _parts(a, heads, D):
+def _parts(a, heads, D, besides):
     """(chunk kernel's slots, split kernel's) that the workspace can be made of: rows of sums and two statistics each."""
-    need = _lib.load().gfa_kv4_attn_workspace_bytes(ctypes.byref(a))
+    need = _lib.load().gfa_kv4_attn_workspace_bytes(ctypes.byref(a)) - besides
     assert need % (heads * (D + 2) * 4 * 16) == 0
     return need // (heads * (D + 2) * 4)  # rows
 
@@ -234,8 +234,8 @@ def test_the_workspace_holds_every_part(seed):
     if n * G > 64:
         n = 1
     a = _attn(cache=_cache(heads_kv=Hkv, head_dim=D), heads_q=G * Hkv, requests=R, seq_len=R * n, table_width=300, table_stride=300, max_new=n,
-              shared_skip=64, shared_cu=64, shared_lens=64)
-    rows = _parts(a, Hkv, D)
+              shared_skip=64, shared_cu=64, shared_lens=64, shared_apart=1)
+    rows = _parts(a, Hkv, D, 64 + (R * n * G + 15 * R) // 16 * 48)  # and where each row block's sums are
     big = 128 if D >= 128 else 256
     # any cut of the requests into groups of two and more
     left, groups = R, []
@@ -253,7 +253,11 @@ def test_workspace_without_effect():
     """With a window, or for requests of many rows, the call is the plain one."""
     ws = lambda **k: _lib.load().gfa_kv4_attn_workspace_bytes(ctypes.byref(_attn(**k)))  # noqa: E731
     shared = dict(shared_skip=64, shared_cu=64, shared_lens=64)
-    assert ws(max_new=1) != ws(max_new=1, **shared)
+    assert ws(max_new=1) != ws(max_new=1, shared_apart=1, **shared) and ws(max_new=1) == ws(max_new=1, shared_apart=1)
+    wide = dict(table_width=10000, table_stride=10000, requests=64, seq_len=64, max_new=1)
+    assert ws(**wide) != ws(**wide, **shared) == ws(**wide, **shared, shared_apart=1)
+    narrow = dict(wide, table_width=1, table_stride=1)  # nothing there that would pay
+    assert ws(**narrow) == ws(**narrow, **shared) != ws(**narrow, **shared, shared_apart=1)
     assert ws(window=3000, max_new=1) == ws(window=3000, max_new=1, **shared)
     assert ws(max_new=100, seq_len=400) == ws(max_new=100, seq_len=400, **shared)
     assert ws(requests=1, max_new=1) == ws(requests=1, max_new=1, **shared)
