@@ -18,6 +18,11 @@ computed by hand-written HIP kernels behind a C ABI (include/gfa.h, libgfa.so):
                                                                          (``segments=`` keyword)
     kv4.plan / write / read / attention                                  serving: a key/value cache
                                                                          in 4 bits (kv4.py)
+    kv4.fork / compact / copy / share                                    blocks that requests share:
+                                                                         several answers to a prompt,
+                                                                         beams, blocks given back
+    kv4.verify                                                           drafted tokens accepted or
+                                                                         replaced
 
 q: (B, N_Q_HEADS, N, D), k/v: (B, N_KV_HEADS, N, D), fp16/bf16, D in {64, 128, 256, 512}.
 """
