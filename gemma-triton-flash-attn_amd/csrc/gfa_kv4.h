@@ -252,7 +252,7 @@ struct Kv4SharedParams {
   const int *group_cu, *group_lens;
   int row_limit;          // of the groups
   Kv4Sums many, few, rest;  // prefixes of groups of many rows and of few, the requests behind their prefixes
-  float many_cost, apart_cost, worth;  // see plan_of in gfa_kv4_shared.hip
+  float many_cost, apart_cost, worth, group_blocks;  // see plan_of in gfa_kv4_shared.hip
   int* joined;              // row blocks of the requests, and where their sums are
   Kv4Join* joins;
 };

@@ -637,6 +637,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     sp.joins = reinterpret_cast<gfa::Kv4Join*>(ws + 64);
     sp.many_cost = rate_of(D).many_cost;
     sp.apart_cost = kApartCost;
+    sp.group_blocks = (float)(s.prefix.many.row_blocks + s.prefix.few.row_blocks);
     sp.worth = a->shared_apart != 0 ? -INFINITY : worth_of(a);
     return launched(gfa::launch_kv4_shared(sp, D, bf16, cap, stream), "attention over shared prefixes");
   }

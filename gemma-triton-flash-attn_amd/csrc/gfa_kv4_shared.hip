@@ -87,7 +87,7 @@ __device__ __forceinline__ Both both_of(const Kv4SharedParams& s, int b) {
   x.own.fresh = tokens(c0, c1);
   x.own.len = max(len, 0);
   x.own.skip = max(skip, 0);
-  x.own.row_blocks = blocks(x.own.fresh * p.G, 4);
+  x.own.row_blocks = blocks(min(x.own.fresh, max(p.T - max(c0, 0), 0)) * p.G, 4);  // tokens past q's have no rows
   const int held = min(x.own.len, most);
   x.own.tiles = (held + kTile - 1) / kTile;
   x.behind = held > x.own.skip ? x.own.tiles - x.own.skip / kTile : 0;
@@ -104,6 +104,7 @@ struct Plan {
   int first, end;  // this wave's requests
   bool alone;      // all of them
   bool apart;      // prefixes are taken apart
+  bool fits;       // the host's grid holds the requests (not only for a cu that is no prefix sum)
   int per_many, per_few, per_rest;  // key tiles per chunk
 };
 // A group's rows and sums.
@@ -112,7 +113,7 @@ struct Group {
   bool large;
 };
 struct PlanLds {
-  float total[4][5];
+  float total[4][6];
   int count[4][4], found[16], group[4][8];
 };
 
@@ -126,9 +127,9 @@ __device__ __forceinline__ Plan plan_of(const Kv4SharedParams& s, const Both& x0
   out.end = end;
   out.alone = alone;
   // the call's parameters all at once: a line of them on its own waits for memory
-  asm volatile("" ::"s"(s.many_cost), "s"(s.worth), "s"(s.apart_cost), "s"(s.many.share), "s"(s.few.share), "s"(s.rest.share),
+  asm volatile("" ::"s"(s.many_cost), "s"(s.worth), "s"(s.apart_cost), "s"(s.group_blocks), "s"(s.many.share), "s"(s.few.share), "s"(s.rest.share),
                "s"(s.many.min_tiles), "s"(s.few.min_tiles), "s"(s.rest.min_tiles));
-  float t[5] = {};  // kMany, kFew, kRests, whole requests; their row blocks
+  float t[6] = {};  // kMany, kFew, kRests, whole requests; their row blocks, the groups'
   Both x = x0;
   for (int b0 = first;;) {
     const float own = (float)x.own.row_blocks, group = (float)x.group.row_blocks * (float)x.group.tiles;
@@ -137,21 +138,23 @@ __device__ __forceinline__ Plan plan_of(const Kv4SharedParams& s, const Both& x0
     t[kRests] += own * (float)x.behind;
     t[3] += own * (float)x.own.tiles;
     t[4] += own;
+    t[5] += (float)x.group.row_blocks;
     if ((b0 += 64) >= end) break;
     x = both_of<BIG>(s, b0 + lane);
   }
 #pragma unroll
-  for (int k = 0; k < 5; ++k) t[k] = wave_sum(t[k]);
+  for (int k = 0; k < 6; ++k) t[k] = wave_sum(t[k]);
   if (!alone) {
     if (lane == 0) {
 #pragma unroll
-      for (int k = 0; k < 5; ++k) lds.total[wave][k] = t[k];
+      for (int k = 0; k < 6; ++k) lds.total[wave][k] = t[k];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < 5; ++k) t[k] = ((lds.total[0][k] + lds.total[1][k]) + lds.total[2][k]) + lds.total[3][k];
+    for (int k = 0; k < 6; ++k) t[k] = ((lds.total[0][k] + lds.total[1][k]) + lds.total[2][k]) + lds.total[3][k];
   }
-  out.apart = __builtin_amdgcn_readfirstlane(t[3] - t[kRests] - t[kFew] - t[kMany] * s.many_cost - t[4] * s.apart_cost > s.worth);
+  out.apart = __builtin_amdgcn_readfirstlane(t[3] - t[kRests] - t[kFew] - t[kMany] * s.many_cost - t[4] * s.apart_cost > s.worth) && t[5] <= s.group_blocks;
+  out.fits = t[4] <= (float)s.p.row_blocks;
   auto per = [&](float total, int min_tiles, float share) {
     return __builtin_amdgcn_readfirstlane(max((int)fminf(ceilf(total * share), 1.0e9f), min_tiles));
   };
@@ -256,15 +259,21 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
   wave_range(s.p.B, wave, first, end, alone);
   const Both x0 = both_of<BIG>(s, first + lane);
   const Plan plan = plan_of<BIG>(s, x0, first, end, alone, lds, lane, wave);
+  if (!plan.fits) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *s.joined = 0;
+    return;
+  }
   Round<BIG> r;
   r.take(x0, plan);
+  if (threadIdx.x == 0) lds.found[0] = -1;
   const Ahead a = ahead_of<BIG>(s, plan, r, lds, lane, wave);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *s.joined = a.all[kBlocks];
+  const int64_t taken = ((int64_t)a.all[kMany] + a.all[kFew] + a.all[kRests]) * s.p.cache.Hkv, grid = (int64_t)s.many.nblocks + s.few.nblocks + s.rest.nblocks;
+  // without room for all items some row blocks' places are not written down
+  if (blockIdx.x == 0 && threadIdx.x == 0) *s.joined = taken <= grid ? a.all[kBlocks] : 0;
   const int which = item < a.all[kMany] ? kMany : item < a.all[kMany] + a.all[kFew] ? kFew : kRests;
   item -= which == kMany ? 0 : which == kFew ? a.all[kMany] : a.all[kMany] + a.all[kFew];
   if (which == kRests && item >= a.all[kRests]) {
-    const int64_t taken = ((int64_t)a.all[kMany] + a.all[kFew] + a.all[kRests]) * s.p.cache.Hkv;
-    zero_rows<D>(s.p, (int64_t)blockIdx.x - taken, (int64_t)s.many.nblocks + s.few.nblocks + s.rest.nblocks - taken);
+    zero_rows<D>(s.p, (int64_t)blockIdx.x - taken, grid - taken);
     return;
   }
   Item it{};
@@ -325,14 +334,16 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
     __syncthreads();
     auto at = [&](int k) { return __builtin_amdgcn_readfirstlane(lds.found[k]); };
     it = Item{Request{at(5), at(6), at(7), at(8), at(9), at(10)}, at(0), at(1), at(2), at(3), 0, at(4)};
+    if (it.b < 0) return;
     block = at(11);
     int w = at(12);  // the group: of that wave's requests, or of one ahead of it
     while (w > 0 && __builtin_amdgcn_readfirstlane(lds.group[w][2]) == 0) --w;
     auto of = [&](int k) { return __builtin_amdgcn_readfirstlane(lds.group[w][k]); };
     grp = Group{of(0), of(1), of(2), of(3), of(4), of(5) != 0};
   }
+  if (it.b < 0) return;
   // for the join
-  if (which == kRests && head == 0 && it.ch == 0 && block < s.p.row_blocks && threadIdx.x == 0) {
+  if (which == kRests && head == 0 && it.ch == 0 && (unsigned)block < (unsigned)s.p.row_blocks && threadIdx.x == 0) {
     const Kv4Sums& sums = grp.large ? s.many : s.few;
     const bool there = it.rq.skip > 0 && (int64_t)grp.slot + (int64_t)grp.row_blocks * grp.nch <= sums.slots;
     s.joins[block] = Kv4Join{it.slot, it.nch, it.rb, it.rq.t0, it.rq.fresh, there ? grp.nch : 0, grp.slot, grp.row_blocks, grp.t0, grp.rows, grp.large, 0};

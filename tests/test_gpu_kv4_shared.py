@@ -202,6 +202,46 @@ def test_many_requests(n, device):
         check(run(a, s, **kw), *want)
 
 
+@pytest.mark.parametrize("n,D", [(5, 512), (64, 128), (90, 256), (300, 64)])
+def test_numbers_that_fit_nothing(n, D, device):
+    """Tables, lengths, offsets and results of share that are no such things: nothing outside the arrays is touched, the call ends,
+    and the next one is right. q and the cache keep their values."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    r = random.Random(n)
+    a = Answers(device, [300 + i % 40 for i in range(n)], [1] * n, 8, 2, D, [(n, 256)], bs=64).store()
+    s = a.share(least=64)
+    want = a.expected()
+    before = [t.clone() for t in (a.cache.codes, a.cache.scales)]
+    big = [-2 ** 31, -70000, -5, -1, 0, 1, 3, n, n + 1, 100, 5000, 2 ** 20, 2 ** 31 - 1]
+    wild = lambda t, p: torch.where(torch.rand(t.shape, generator=g) < p, torch.tensor([r.choice(big) for _ in range(t.numel())]).view(t.shape),  # noqa: E731
+                                    t.cpu().long()).to(torch.int32).to(device)
+    g = torch.Generator().manual_seed(n)
+    q = a.q.to(device)
+    for i in range(24):
+        p = [0.02, 0.3, 1.0][i % 3]
+        table, lens, cu = (wild(t, p if i >> k & 1 else 0) for k, t in enumerate((a.table, a.lens_dev, a.cu)))
+        bad = kv4.Shared(*(wild(t, p if (i + 1) >> k & 1 else 0) for k, t in enumerate(s)))
+        o = kv4.attention(q, a.cache, table, lens, cu, max_new=1, shared=bad, apart=i % 2 == 0)
+        assert o.shape == q.shape
+        torch.cuda.synchronize()
+    assert torch.equal(q.cpu(), a.q) and all(torch.equal(x, y) for x, y in zip(before, (a.cache.codes, a.cache.scales)))
+    check(run(a, s), *want)
+
+
+def test_more_tokens_than_q_has(device):
+    """cu of more tokens than q (not of one request): the rows that q has are right."""
+    a = Answers(device, [300 + i for i in range(70)], [2] * 70, 8, 2, 128, [(70, 256)], bs=64).store()
+    from gemma_triton_flash_attn_amd import kv4
+
+    s = a.share(least=64)
+    want, bound = a.expected()
+    for T in (2, 7, 101, 139):
+        for apart in (True, False):
+            o = kv4.attention(a.q[:, :, :T].contiguous().to(device), a.cache, a.table, a.lens_dev, a.cu, max_new=2, shared=s, apart=apart)
+            check(o, want[:, :T], bound[:, :T])
+
+
 @pytest.mark.parametrize("n", SIZES)
 def test_missing_blocks(n, device):
     """Blocks missing in a prefix, all of a prefix, all of a request's own."""
