@@ -253,6 +253,7 @@ struct Kv4SharedParams {
   int row_limit;          // of the groups
   Kv4Sums many, few, rest;  // prefixes of groups of many rows and of few, the requests behind their prefixes
   float many_cost, apart_cost, worth, group_blocks;  // see plan_of in gfa_kv4_shared.hip
+  int grid;                 // workgroups, that take items in turn
   int* joined;              // row blocks of the requests, and where their sums are
   Kv4Join* joins;
 };

@@ -637,6 +637,8 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     sp.joins = reinterpret_cast<gfa::Kv4Join*>(ws + 64);
     sp.many_cost = rate_of(D).many_cost;
     sp.apart_cost = kApartCost;
+    const int64_t bound = s.prefix.many.nblocks + s.prefix.few.nblocks + s.rest.few.nblocks;
+    sp.grid = (int)std::min<int64_t>(bound, 256 * gfa::kv4_chunk_wgs(D) * 3);
     sp.group_blocks = (float)(s.prefix.many.row_blocks + s.prefix.few.row_blocks);
     sp.worth = a->shared_apart != 0 ? -INFINITY : worth_of(a);
     return launched(gfa::launch_kv4_shared(sp, D, bf16, cap, stream), "attention over shared prefixes");

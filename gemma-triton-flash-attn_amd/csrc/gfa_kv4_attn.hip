@@ -17,7 +17,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 512 ? 1 : 2) void kv4_split_kerne
   if (it.b < 0) {
     if (p.cu == nullptr) return;
     const int64_t taken = (int64_t)it.items * p.cache.Hkv;
-    zero_rows<D>(p, block - taken, p.nblocks - taken);
+    zero_rows<D>(p, threadIdx.x, block - taken, p.nblocks - taken);
     return;
   }
 #include "gfa_kv4_split.inc"

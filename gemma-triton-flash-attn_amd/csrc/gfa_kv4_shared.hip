@@ -25,6 +25,7 @@ namespace gfa {
 namespace {
 
 constexpr int kTpb = 256;
+constexpr int kSpare = 64;  // workgroups for rows of no request
 
 template <int D, bool IS_BF16, bool CAP>
 __device__ __forceinline__ void many_rows(const Kv4AttnParams& p, const int lane, const int wave, const int head, const Item& it, char GFA_LDS* const K0,
@@ -62,8 +63,10 @@ __device__ __forceinline__ Kv4AttnParams part_of(const Kv4SharedParams& s, const
 
 // ---- the split of the call ----
 // As in gfa_kv4_sched.h, of three kinds of items in this order: row blocks of groups of many rows, of groups of few, of the
-// requests behind their prefixes. Items that exist come first: what the host's grid has to spare ends the launch (ahead of the
-// requests' it held them up: 312 requests in 12 groups, 8:1 D = 512, 132 us, 77 of them until the first).
+// requests behind their prefixes. A grid for any lengths would be several times the items there are, and one that finds nothing takes
+// 2 to 4 us to find that out: three times what the CUs hold are launched at most, and take the items in turn (308 requests without
+// prefixes, 16:8 D = 256, 87 -> 74 us, 93 in three groups, 32:8 D = 128, 28 -> 24; as many as the CUs hold 10 to 20% slower where there
+// is more to do, ten times as many as before).
 // Up to 64 requests every wave looks through all of them; more are dealt to the four waves, which trade what they found in LDS.
 enum Which : int { kMany, kFew, kRests, kBlocks };
 struct Both {
@@ -104,7 +107,7 @@ struct Plan {
   int first, end;  // this wave's requests
   bool alone;      // all of them
   bool apart;      // prefixes are taken apart
-  bool fits;       // the host's grid holds the requests (not only for a cu that is no prefix sum)
+  bool fits;       // the host's arrays hold the requests' row blocks (not only for a cu that is no prefix sum)
   int per_many, per_few, per_rest;  // key tiles per chunk
 };
 // A group's rows and sums.
@@ -238,7 +241,7 @@ __device__ __forceinline__ void wave_range(int B, int wave, int& first, int& end
 }  // namespace
 
 template <int D, bool IS_BF16, bool CAP>
-__global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(const Kv4SharedParams s) {
+__global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(const Kv4SharedParams) {
   constexpr int BIG = kv4_chunk_rows(D);
   __shared__ PlanLds lds;
   // The chunk kernel's tiles, or what the waves of the split kernel join: D * 32 bytes each (D = 64: 4 KB).
@@ -250,108 +253,116 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
   char GFA_LDS* const V1 = (char GFA_LDS*)v_lds1;
   char GFA_LDS* const S0 = (char GFA_LDS*)s_lds0;
   char GFA_LDS* const S1 = (char GFA_LDS*)s_lds1;
-  const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int head = s.p.hkv.rem((int)blockIdx.x);
-  int item = s.p.hkv.quot((int)blockIdx.x);
-  int first, end;
-  bool alone;
-  wave_range(s.p.B, wave, first, end, alone);
-  const Both x0 = both_of<BIG>(s, first + lane);
-  const Plan plan = plan_of<BIG>(s, x0, first, end, alone, lds, lane, wave);
-  if (!plan.fits) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) *s.joined = 0;
-    return;
-  }
-  Round<BIG> r;
-  r.take(x0, plan);
-  if (threadIdx.x == 0) lds.found[0] = -1;
-  const Ahead a = ahead_of<BIG>(s, plan, r, lds, lane, wave);
-  const int64_t taken = ((int64_t)a.all[kMany] + a.all[kFew] + a.all[kRests]) * s.p.cache.Hkv, grid = (int64_t)s.many.nblocks + s.few.nblocks + s.rest.nblocks;
-  // without room for all items some row blocks' places are not written down
-  if (blockIdx.x == 0 && threadIdx.x == 0) *s.joined = taken <= grid ? a.all[kBlocks] : 0;
-  const int which = item < a.all[kMany] ? kMany : item < a.all[kMany] + a.all[kFew] ? kFew : kRests;
-  item -= which == kMany ? 0 : which == kFew ? a.all[kMany] : a.all[kMany] + a.all[kFew];
-  if (which == kRests && item >= a.all[kRests]) {
-    zero_rows<D>(s.p, (int64_t)blockIdx.x - taken, grid - taken);
-    return;
-  }
-  Item it{};
-  it.b = -1;
-  Group grp{};
-  int block = 0, before[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) before[k] = a.before[k];
-  for (int b0 = plan.first;;) {
-    const int n = which == kMany ? r.c.n[kMany] : which == kFew ? r.c.n[kFew] : r.c.n[kRests];
-    const int upto = which == kMany ? r.upto[kMany] : which == kFew ? r.upto[kFew] : r.upto[kRests];
-    const int from = (which == kMany ? before[kMany] : which == kFew ? before[kFew] : before[kRests]) + upto - n;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= from && item < from + n);
-    const int src = hit != 0 ? __builtin_ctzll(hit) : 63;
-    if (which == kRests && plan.apart) {
-      // the last group that begins with the request or ahead of it
-      const uint64_t groups = __builtin_amdgcn_ballot_w64(r.x.group.row_blocks > 0 && lane <= src);
-      if (groups != 0) {
-        const int g = 63 - __builtin_clzll(groups);
-        auto at = [&](int x) { return __builtin_amdgcn_readlane(x, g); };
-        const bool large = at(r.x.large) != 0;
-        const int row_blocks = at(r.x.group.row_blocks), items = at(large ? r.c.n[kMany] : r.c.n[kFew]);
-        const int slot = (large ? before[kMany] : before[kFew]) + at(large ? r.upto[kMany] : r.upto[kFew]) - items;
-        grp = Group{at(r.x.group.t0), at(r.x.group.fresh) * s.p.G, row_blocks, __builtin_amdgcn_readfirstlane(quotient(items, row_blocks)), slot, large};
-      }
+  typedef const Kv4SharedParams __attribute__((address_space(4)))* Args;
+  for (int at = (int)blockIdx.x;;) {
+    // read anew each turn: held through the loop they spill
+    Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(args));
+    const Kv4SharedParams& s = *(const Kv4SharedParams*)args;
+    const int lane = fresh_lane();
+    const int head = s.p.hkv.rem(at);
+    int item = s.p.hkv.quot(at);
+    int first, end;
+    bool alone;
+    wave_range(s.p.B, wave, first, end, alone);
+    const Both x0 = both_of<BIG>(s, first + lane);
+    const Plan plan = plan_of<BIG>(s, x0, first, end, alone, lds, lane, wave);
+    if (!plan.fits) {
+      if (at == 0 && wave == 0 && lane == 0) *s.joined = 0;
+      return;
     }
-    if (hit != 0) {
-      it.b = b0 + src;
-      it.rq = request_from(which == kRests ? r.x.own : r.x.group, src);
-      if (which == kRests) {
-        it.rq.tiles = plan.apart ? __builtin_amdgcn_readlane(r.x.behind, src) : it.rq.tiles;
-        it.rq.skip = plan.apart ? it.rq.skip : 0;
-      }
-      it.nch = __builtin_amdgcn_readfirstlane(quotient(__builtin_amdgcn_readlane(n, src), it.rq.row_blocks));
-      const int i = item - __builtin_amdgcn_readlane(from, src);
-      it.rb = __builtin_amdgcn_readfirstlane(quotient(i, it.nch));
-      it.ch = i - it.rb * it.nch;
-      it.slot = which == kRests && it.nch == 1 && it.rq.skip == 0 ? -1 : item;
-      block = before[kBlocks] + __builtin_amdgcn_readlane(r.upto[kBlocks], src) - it.rq.row_blocks + it.rb;
-      break;
+    Round<BIG> r;
+    r.take(x0, plan);
+    if (wave == 0 && lane == 0) lds.found[0] = -1;
+    const Ahead a = ahead_of<BIG>(s, plan, r, lds, lane, wave);
+    const int taken = (a.all[kMany] + a.all[kFew] + a.all[kRests]) * s.p.cache.Hkv;
+    if (at == 0 && wave == 0 && lane == 0) *s.joined = a.all[kBlocks];
+    const int which = item < a.all[kMany] ? kMany : item < a.all[kMany] + a.all[kFew] ? kFew : kRests;
+    item -= which == kMany ? 0 : which == kFew ? a.all[kMany] : a.all[kMany] + a.all[kFew];
+    if (which == kRests && item >= a.all[kRests]) {
+      if (at < taken + kSpare) zero_rows<D>(s.p, wave * 64 + lane, at - taken, kSpare);
+      return;
     }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) before[k] += last_lane(r.upto[k]);
-    if ((b0 += 64) >= plan.end) break;
-    r.take(both_of<BIG>(s, b0 + lane), plan);
-  }
-  if (!alone) {
-    if (lane == 0) {
-      const int group[] = {grp.t0, grp.rows, grp.row_blocks, grp.nch, grp.slot, grp.large};
-#pragma unroll
-      for (int k = 0; k < 6; ++k) lds.group[wave][k] = group[k];
-      if (it.b >= 0) {
-        const int of[] = {it.b, it.rb, it.ch, it.nch, it.slot, it.rq.t0, it.rq.fresh, it.rq.len, it.rq.row_blocks, it.rq.tiles, it.rq.skip, block, wave};
-#pragma unroll
-        for (int k = 0; k < 13; ++k) lds.found[k] = of[k];
+    Item it{};
+    it.b = -1;
+    Group grp{};
+    int block = 0, before[4];
+  #pragma unroll
+    for (int k = 0; k < 4; ++k) before[k] = a.before[k];
+    for (int b0 = plan.first;;) {
+      const int n = which == kMany ? r.c.n[kMany] : which == kFew ? r.c.n[kFew] : r.c.n[kRests];
+      const int upto = which == kMany ? r.upto[kMany] : which == kFew ? r.upto[kFew] : r.upto[kRests];
+      const int from = (which == kMany ? before[kMany] : which == kFew ? before[kFew] : before[kRests]) + upto - n;
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(item >= from && item < from + n);
+      const int src = hit != 0 ? __builtin_ctzll(hit) : 63;
+      if (which == kRests && plan.apart) {
+        // the last group that begins with the request or ahead of it
+        const uint64_t groups = __builtin_amdgcn_ballot_w64(r.x.group.row_blocks > 0 && lane <= src);
+        if (groups != 0) {
+          const int g = 63 - __builtin_clzll(groups);
+          auto at = [&](int x) { return __builtin_amdgcn_readlane(x, g); };
+          const bool large = at(r.x.large) != 0;
+          const int row_blocks = at(r.x.group.row_blocks), items = at(large ? r.c.n[kMany] : r.c.n[kFew]);
+          const int slot = (large ? before[kMany] : before[kFew]) + at(large ? r.upto[kMany] : r.upto[kFew]) - items;
+          grp = Group{at(r.x.group.t0), at(r.x.group.fresh) * s.p.G, row_blocks, __builtin_amdgcn_readfirstlane(quotient(items, row_blocks)), slot, large};
+        }
       }
+      if (hit != 0) {
+        it.b = b0 + src;
+        it.rq = request_from(which == kRests ? r.x.own : r.x.group, src);
+        if (which == kRests) {
+          it.rq.tiles = plan.apart ? __builtin_amdgcn_readlane(r.x.behind, src) : it.rq.tiles;
+          it.rq.skip = plan.apart ? it.rq.skip : 0;
+        }
+        it.nch = __builtin_amdgcn_readfirstlane(quotient(__builtin_amdgcn_readlane(n, src), it.rq.row_blocks));
+        const int i = item - __builtin_amdgcn_readlane(from, src);
+        it.rb = __builtin_amdgcn_readfirstlane(quotient(i, it.nch));
+        it.ch = i - it.rb * it.nch;
+        it.slot = which == kRests && it.nch == 1 && it.rq.skip == 0 ? -1 : item;
+        block = before[kBlocks] + __builtin_amdgcn_readlane(r.upto[kBlocks], src) - it.rq.row_blocks + it.rb;
+        break;
+      }
+  #pragma unroll
+      for (int k = 0; k < 4; ++k) before[k] += last_lane(r.upto[k]);
+      if ((b0 += 64) >= plan.end) break;
+      r.take(both_of<BIG>(s, b0 + lane), plan);
     }
-    __syncthreads();
-    auto at = [&](int k) { return __builtin_amdgcn_readfirstlane(lds.found[k]); };
-    it = Item{Request{at(5), at(6), at(7), at(8), at(9), at(10)}, at(0), at(1), at(2), at(3), 0, at(4)};
+    if (!alone) {
+      if (lane == 0) {
+        const int group[] = {grp.t0, grp.rows, grp.row_blocks, grp.nch, grp.slot, grp.large};
+  #pragma unroll
+        for (int k = 0; k < 6; ++k) lds.group[wave][k] = group[k];
+        if (it.b >= 0) {
+          const int of[] = {it.b, it.rb, it.ch, it.nch, it.slot, it.rq.t0, it.rq.fresh, it.rq.len, it.rq.row_blocks, it.rq.tiles, it.rq.skip, block, wave};
+  #pragma unroll
+          for (int k = 0; k < 13; ++k) lds.found[k] = of[k];
+        }
+      }
+      __syncthreads();
+      auto at = [&](int k) { return __builtin_amdgcn_readfirstlane(lds.found[k]); };
+      it = Item{Request{at(5), at(6), at(7), at(8), at(9), at(10)}, at(0), at(1), at(2), at(3), 0, at(4)};
+      if (it.b < 0) return;
+      block = at(11);
+      int w = at(12);  // the group: of that wave's requests, or of one ahead of it
+      while (w > 0 && __builtin_amdgcn_readfirstlane(lds.group[w][2]) == 0) --w;
+      auto of = [&](int k) { return __builtin_amdgcn_readfirstlane(lds.group[w][k]); };
+      grp = Group{of(0), of(1), of(2), of(3), of(4), of(5) != 0};
+    }
     if (it.b < 0) return;
-    block = at(11);
-    int w = at(12);  // the group: of that wave's requests, or of one ahead of it
-    while (w > 0 && __builtin_amdgcn_readfirstlane(lds.group[w][2]) == 0) --w;
-    auto of = [&](int k) { return __builtin_amdgcn_readfirstlane(lds.group[w][k]); };
-    grp = Group{of(0), of(1), of(2), of(3), of(4), of(5) != 0};
-  }
-  if (it.b < 0) return;
-  // for the join
-  if (which == kRests && head == 0 && it.ch == 0 && (unsigned)block < (unsigned)s.p.row_blocks && threadIdx.x == 0) {
-    const Kv4Sums& sums = grp.large ? s.many : s.few;
-    const bool there = it.rq.skip > 0 && (int64_t)grp.slot + (int64_t)grp.row_blocks * grp.nch <= sums.slots;
-    s.joins[block] = Kv4Join{it.slot, it.nch, it.rb, it.rq.t0, it.rq.fresh, there ? grp.nch : 0, grp.slot, grp.row_blocks, grp.t0, grp.rows, grp.large, 0};
-  }
-  if (which == kMany) {
-    many_rows<D, IS_BF16, CAP>(part_of(s, s.many, true), lane, wave, head, it, K0, K1, V0, V1, S0, S1);
-  } else {
-    few_rows<D, IS_BF16, CAP>(part_of(s, which == kFew ? s.few : s.rest, which == kFew), lane, wave, head, it, K0, K1, V0, V1);
+    // for the join
+    if (which == kRests && head == 0 && it.ch == 0 && (unsigned)block < (unsigned)s.p.row_blocks && wave == 0 && lane == 0) {
+      const Kv4Sums& sums = grp.large ? s.many : s.few;
+      const bool there = it.rq.skip > 0 && (int64_t)grp.slot + (int64_t)grp.row_blocks * grp.nch <= sums.slots;
+      s.joins[block] = Kv4Join{it.slot, it.nch, it.rb, it.rq.t0, it.rq.fresh, there ? grp.nch : 0, grp.slot, grp.row_blocks, grp.t0, grp.rows, grp.large, 0};
+    }
+    if (which == kMany) {
+      many_rows<D, IS_BF16, CAP>(part_of(s, s.many, true), lane, wave, head, it, K0, K1, V0, V1, S0, S1);
+    } else {
+      few_rows<D, IS_BF16, CAP>(part_of(s, which == kFew ? s.few : s.rest, which == kFew), lane, wave, head, it, K0, K1, V0, V1);
+    }
+    if ((at += s.grid) >= taken + kSpare) return;
+    __syncthreads();
   }
 }
 
@@ -434,7 +445,7 @@ __global__ __launch_bounds__(kTpb) void kv4_shared_join_kernel(const Kv4SharedPa
 
 hipError_t launch_kv4_shared(const Kv4SharedParams& s, int D, bool bf16, bool cap, hipStream_t stream) {
   const dim3 wg(kTpb);
-  const dim3 grid((unsigned)((int64_t)s.many.nblocks + s.few.nblocks + s.rest.nblocks));
+  const dim3 grid((unsigned)s.grid);
   auto go = [&](auto d, auto b, auto c) {
     constexpr int DD = decltype(d)::value;
     constexpr bool BB = decltype(b)::value, CC = decltype(c)::value;

@@ -62,10 +62,10 @@ struct TileRegs {
 // Workgroup `extra` of n_extra without an item: tokens ahead of the first request's and behind the last one's are zeros, they
 // take them in turn.
 template <int D>
-__device__ __forceinline__ void zero_rows(const Kv4AttnParams& p, int64_t extra, int64_t n_extra) {
+__device__ __forceinline__ void zero_rows(const Kv4AttnParams& p, int tid, int64_t extra, int64_t n_extra) {
   const int lead = min(max(p.cu[0], 0), p.T), n0 = min(max(p.cu[p.B], 0), p.T);
   const int64_t pieces = ((int64_t)lead + p.T - n0) * p.Hq * (D / 8);
-  for (int64_t i = extra * blockDim.x + threadIdx.x; i < pieces; i += n_extra * blockDim.x) {
+  for (int64_t i = extra * (kWaves * 64) + tid; i < pieces; i += n_extra * (kWaves * 64)) {
     const int64_t hd = i / (D / 8), n = hd / p.Hq;
     const int t = (int)(n < lead ? n : n0 + (n - lead));
     uint16_t* at = p.o + p.n.quot(t) * p.osb + hd % p.Hq * p.osh + p.n.rem(t) * p.osn + i % (D / 8) * 8;

@@ -202,6 +202,20 @@ def test_many_requests(n, device):
         check(run(a, s, **kw), *want)
 
 
+@pytest.mark.parametrize("n,Hkv,D", [(500, 2, 512), (450, 4, 256), (400, 8, 128), (900, 2, 64)])
+def test_more_items_than_workgroups(n, Hkv, D, device):
+    """A workgroup takes several items in turn, prefixes of many rows and of few and requests behind them; rows of no request after all."""
+    groups = [(n // 2, 192), (3, 128), (n - n // 2 - 3, 64)]
+    lens = [c + 1 + i % 50 for k, c in groups for i in range(k)]
+    a = Answers(device, lens, [1] * n, 2 * Hkv, Hkv, D, groups, bs=64, pad=9, seed=n).store()
+    s = a.share(least=64)
+    want = a.expected()
+    for kw in (dict(), dict(apart=False)):
+        o = run(a, s, **kw)
+        check(o, want[0], want[1])
+        assert not o[:, :, -9:].any() and torch.equal(o, run(a, s, **kw))
+
+
 @pytest.mark.parametrize("n,D", [(5, 512), (64, 128), (90, 256), (300, 64)])
 def test_numbers_that_fit_nothing(n, D, device):
     """Tables, lengths, offsets and results of share that are no such things: nothing outside the arrays is touched, the call ends,
