@@ -10,10 +10,10 @@
 // requests' rests by the split kernel's, as three runs of workgroups. A second launch joins a row's chunks of both. Whether that
 // pays depends on the lengths: where it does not, the first launch takes the requests whole.
 //
-// Bound: issue of the chunk kernel's products and decoding (64 answers to a 16k prompt, 32:8 D = 128: 46.5 us against 215 without
+// Bound: issue of the chunk kernel's products and decoding (64 answers to a 16k prompt, 32:8 D = 128: 47.8 us against 215 without
 // sharing; the tiles' loop 31, 1.1 us a tile and CU), around it latency: 2.5 us until a workgroup has its work, 8 until its first
-// products, 2 (D = 128) to 7 us (D = 512) for sums out, 6 for the join. Eight answers to each of four prompts of 8k, 32:4 D = 512, 55 us
-// (90), 16 of 4 drafted tokens, 3k, 8:4 D = 256, 24 (21: by then it is even).
+// products, 2 (D = 128) to 7 us (D = 512) for sums out, 6 for the join. Eight answers to each of four prompts of 8k, 32:4 D = 512, 54 us
+// (90), 16 of 4 drafted tokens, 3k, 8:4 D = 256, 25 (21: there it does not pay yet).
 #include <algorithm>
 
 #include "gfa_kv4_chunk.h"
