@@ -66,7 +66,7 @@ __device__ __forceinline__ Kv4AttnParams part_of(const Kv4SharedParams& s, const
 // requests behind their prefixes. A grid for any lengths would be several times the items there are, and one that finds nothing takes
 // 2 to 4 us to find that out: three times what the CUs hold are launched at most, and take the items in turn (308 requests without
 // prefixes, 16:8 D = 256, 87 -> 74 us, 93 in three groups, 32:8 D = 128, 28 -> 24; as many as the CUs hold 10 to 20% slower where there
-// is more to do, ten times as many as before).
+// is more to do, ten times the same as a grid for any lengths).
 // Up to 64 requests every wave looks through all of them; more are dealt to the four waves, which trade what they found in LDS.
 enum Which : int { kMany, kFew, kRests, kBlocks };
 struct Both {
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
     it.b = -1;
     Group grp{};
     int block = 0, before[4];
-  #pragma unroll
+#pragma unroll
     for (int k = 0; k < 4; ++k) before[k] = a.before[k];
     for (int b0 = plan.first;;) {
       const int n = which == kMany ? r.c.n[kMany] : which == kFew ? r.c.n[kFew] : r.c.n[kRests];
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
         block = before[kBlocks] + __builtin_amdgcn_readlane(r.upto[kBlocks], src) - it.rq.row_blocks + it.rb;
         break;
       }
-  #pragma unroll
+#pragma unroll
       for (int k = 0; k < 4; ++k) before[k] += last_lane(r.upto[k]);
       if ((b0 += 64) >= plan.end) break;
       r.take(both_of<BIG>(s, b0 + lane), plan);
@@ -331,11 +331,11 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
     if (!alone) {
       if (lane == 0) {
         const int group[] = {grp.t0, grp.rows, grp.row_blocks, grp.nch, grp.slot, grp.large};
-  #pragma unroll
+#pragma unroll
         for (int k = 0; k < 6; ++k) lds.group[wave][k] = group[k];
         if (it.b >= 0) {
           const int of[] = {it.b, it.rb, it.ch, it.nch, it.slot, it.rq.t0, it.rq.fresh, it.rq.len, it.rq.row_blocks, it.rq.tiles, it.rq.skip, block, wave};
-  #pragma unroll
+#pragma unroll
           for (int k = 0; k < 13; ++k) lds.found[k] = of[k];
         }
       }

@@ -168,8 +168,8 @@ def test_nothing_in_common(device):
 
 @pytest.mark.parametrize("D,Hkv", [(512, 1), (512, 4), (256, 4), (128, 8), (64, 16)])
 def test_where_it_pays(D, Hkv, device):
-    """The call's own choice, on either side of the line: many requests over a long prefix, few over a short one, none in common; the
-    same kernels with the lengths changed in place. Requests without a prefix in one chunk are the plain call's, bit for bit."""
+    """The call's own choice, on either side of the line: many requests over a long prefix, few over a short one. In tables too narrow
+    to gain anything it is the plain call, bit for bit."""
     a = Answers(device, [2100 + i for i in range(48)] + [90, 70], [1] * 50, 4 * Hkv, Hkv, D, [(48, 2048), (2, 64)], bs=64).store()
     s = a.share()
     assert s.lens.tolist()[0] == 2048 and s.lens.tolist()[48] == 64
@@ -181,6 +181,37 @@ def test_where_it_pays(D, Hkv, device):
     assert s.lens.tolist() == [128, 0, 0]
     check(run(b, s), *b.expected())
     assert torch.equal(run(b, s, apart=False), run(b, None))
+
+
+@pytest.mark.parametrize("D,Hkv", [(512, 2), (128, 8)])
+def test_captured_where_it_pays(D, Hkv, device):
+    """The choice is the replay's, not the capture's: lengths on both sides of the line, two graphs at once on two streams."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    a = Answers(device, [2100 + i for i in range(48)], [1] * 48, 4 * Hkv, Hkv, D, [(48, 2048)], bs=64, junk=0).store()
+    q, lens = a.q.to(device), [a.lens_dev.clone(), a.lens_dev.clone()]
+
+    def step(n):
+        return kv4.attention(q, a.cache, a.table, n, a.cu, max_new=1, shared=kv4.share(a.table, n, a.cu, block_size=64))
+
+    step(lens[0])
+    torch.cuda.synchronize()
+    graphs, got = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph, n in zip(graphs, lens):
+        with torch.cuda.graph(graph):
+            got.append(step(n))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for cut in (0, 2040, 1500, 600, 0):
+        lens[0].copy_(a.lens_dev - cut)
+        lens[1].copy_(a.lens_dev - (2040 - cut))
+        torch.cuda.synchronize()
+        for stream, graph in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for n, o in zip(lens, got):
+            assert torch.equal(o, step(n))
+    check(got[0], *a.expected())
 
 
 @pytest.mark.parametrize("n", [64, 65, 128, 256, 257, 700])
