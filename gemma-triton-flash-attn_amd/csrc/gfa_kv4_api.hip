@@ -157,7 +157,8 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, Kind kind, int64_t row_block
 
 // The same of a group's rows. Below a workgroup's 128 the chunk kernel's waves share the keys (gfa_kv4_chunk.inc), so the line is lower
 // where there are KV heads to fill the GPU with: four prompts of 8k with 12 answers each, 32:8 D = 128, 48 rows 37 us (split kernel 41),
-// 16:8 D = 256 60 (69), 32:4 D = 512 60 (66); one KV head at D = 256 24.5 (23.4), two at D = 64 24 (20), 32:8 at D = 64 35 (34).
+// 16:8 D = 256 60 (69), 32:4 D = 512 60 (66); one KV head at D = 256 24.5 (23.4), 32:8 at D = 64 32.9 (30.3), 10 answers to four of 4k, 16:4
+// D = 64, 22.2 (19.0).
 int group_limit(const gfa_kv4_attn_args* a) { return a->cache.heads_kv >= 4 && a->cache.head_dim >= 128 ? 32 : 64; }
 
 // Most new tokens of a request, as far as the host knows.
@@ -176,7 +177,7 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
   s.one_block = most * G <= kRows;
   const int limit = kind == kPrefix ? group_limit(a) : row_limit(a, R);
   s.row_limit = kind == kRest || most * G <= limit ? 0x7fffffff : limit;
-  const int D = a->cache.head_dim, big = gfa::kv4_chunk_rows(D);
+  const int D = a->cache.head_dim, big = kind == kPrefix ? gfa::kSharedRows : gfa::kv4_chunk_rows(D);
   int64_t few, many = 0;
   if (a->cu == nullptr) {
     const bool large = most * G > s.row_limit;
@@ -220,11 +221,11 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
 
 // What taking prefixes apart saves is counted in passes of the split kernel over a tile (one row block, one KV head): `tiles` of them take
 // a us of the whole GPU, one of the chunk kernel takes as long as many_cost of them. From calls of 40 to 300 requests, by head dim: 151k
-// passes 72 us and 60k 52 us, 24k 43 us, 43k 133 us; the chunk kernel's 2.1 us a tile and CU at D = 512, 1.3, 1.1, 0.8.
+// passes 72 us and 60k 52 us, 24k 43 us, 43k 133 us; the chunk kernel's 2.1 us a tile and CU at D = 512, 1.3, 1.1, 0.5.
 struct Rate {
   float tiles, many_cost;
 };
-Rate rate_of(int D) { return D == 64 ? Rate{2100.f, 6.5f} : D == 128 ? Rate{1200.f, 5.f} : D == 256 ? Rate{570.f, 2.9f} : Rate{320.f, 2.6f}; }
+Rate rate_of(int D) { return D == 64 ? Rate{2100.f, 3.5f} : D == 128 ? Rate{1200.f, 5.f} : D == 256 ? Rate{570.f, 2.9f} : Rate{320.f, 2.6f}; }
 // A row block whose request is taken apart leaves sums in two parts and is joined, about as much again as 10 tiles of it; a call has one
 // kernel's latency more: it pays from 4 us on. Apart against whole, us: two answers of 5 tokens to a 2k prompt, 32:4 D = 512, 35.7 24.0;
 // 16 answers of 8 to each of eight prompts of 740 tokens, 8:4 D = 256, 66 51; two answers to each of six prompts of 8k, 8:1 D = 512,
@@ -638,7 +639,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     sp.many_cost = rate_of(D).many_cost;
     sp.apart_cost = kApartCost;
     const int64_t bound = s.prefix.many.nblocks + s.prefix.few.nblocks + s.rest.few.nblocks;
-    sp.grid = (int)std::min<int64_t>(bound, 256 * gfa::kv4_chunk_wgs(D) * 3);
+    sp.grid = (int)std::min<int64_t>(bound, 256 * gfa::kv4_shared_wgs(D) * 3);
     sp.group_blocks = (float)(s.prefix.many.row_blocks + s.prefix.few.row_blocks);
     sp.worth = a->shared_apart != 0 ? -INFINITY : worth_of(a);
     return launched(gfa::launch_kv4_shared(sp, D, bf16, cap, stream), "attention over shared prefixes");

@@ -33,7 +33,7 @@ __device__ __forceinline__ void many_rows(const Kv4AttnParams& p, const int lane
                                           char GFA_LDS* const S1) {
 #ifdef __HIP_DEVICE_COMPILE__
   constexpr Kv4Part PART = kPart;
-  constexpr int ROWS = kv4_chunk_rows(D);
+  constexpr int ROWS = kSharedRows;
 #include "gfa_kv4_chunk.inc"
 #endif
 }
@@ -85,7 +85,7 @@ __device__ __forceinline__ Both both_of(const Kv4SharedParams& s, int b) {
   const int most = p.M << p.cache.bs_log2;
   auto tokens = [&](int from, int to) { return min(max((int)((unsigned)to - (unsigned)from), 0), p.T); };
   auto blocks = [&](int rows, int log2) { return (int)(((unsigned)rows + (1u << log2) - 1) >> log2); };
-  static_assert(kSplitRows == 16 && (BIG == 128 || BIG == 256));
+  static_assert(kSplitRows == 16 && BIG == 128);
   x.own.t0 = c0;
   x.own.fresh = tokens(c0, c1);
   x.own.len = max(len, 0);
@@ -98,7 +98,7 @@ __device__ __forceinline__ Both both_of(const Kv4SharedParams& s, int b) {
   x.group.len = max(glen, 0);
   x.group.fresh = x.group.len > 0 ? tokens(g0, g1) : 0;
   x.large = x.group.fresh * p.G > s.row_limit;
-  x.group.row_blocks = blocks(x.group.fresh * p.G, x.large ? (BIG == 128 ? 7 : 8) : 4);
+  x.group.row_blocks = blocks(x.group.fresh * p.G, x.large ? 7 : 4);
   x.group.tiles = (min(x.group.len, most) + kTile - 1) / kTile;
   return x;
 }
@@ -241,8 +241,8 @@ __device__ __forceinline__ void wave_range(int B, int wave, int& first, int& end
 }  // namespace
 
 template <int D, bool IS_BF16, bool CAP>
-__global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(const Kv4SharedParams) {
-  constexpr int BIG = kv4_chunk_rows(D);
+__global__ __launch_bounds__(kTpb, kv4_shared_wgs(D)) void kv4_shared_kernel(const Kv4SharedParams) {
+  constexpr int BIG = kSharedRows;
   __shared__ PlanLds lds;
   // The chunk kernel's tiles, or what the waves of the split kernel join: D * 32 bytes each (D = 64: 4 KB).
   constexpr int TILE = std::max(kv4_chunk_steps(kPart) * Kv4Layout<D>::TILE_CODES, D == 64 ? 4096 : D * 32), SCALES = kv4_chunk_steps(kPart) * 1024;
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kTpb, kv4_chunk_wgs(D)) void kv4_shared_kernel(cons
 // written down. Bound: latency, of a row block's place and of one pass of loads.
 template <int D, bool IS_BF16>
 __global__ __launch_bounds__(kTpb) void kv4_shared_join_kernel(const Kv4SharedParams s) {
-  constexpr int ROWS = kSplitRows, BIG = kv4_chunk_rows(D);
+  constexpr int ROWS = kSplitRows, BIG = kSharedRows;
   const Kv4AttnParams p = part_of(s, s.rest, false);
   const int LPR = p.join_slice / 4;  // a power of two
   const int GR = kTpb / LPR;
