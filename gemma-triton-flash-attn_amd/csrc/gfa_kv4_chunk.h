@@ -24,8 +24,8 @@ namespace gfa {
 
 namespace {
 
-// Tiles a step of the chunk kernel can take at once, see gfa_kv4_chunk.inc.
-__host__ __device__ constexpr int kv4_chunk_steps(Kv4Part part) { return part == kPart ? 2 : 1; }
+// Tiles a step of the chunk kernel can take at once, see gfa_kv4_chunk.inc (at D = 64 no group of so few rows comes to it).
+__host__ __device__ constexpr int kv4_chunk_steps(Kv4Part part, int D) { return part == kPart && D > 64 ? 2 : 1; }
 
 // Tile copies of one wave: 1 KB runs of codes (K, then V) and the scales, dealt to the four waves in turn. K pieces land
 // swizzled: a lane's 16-byte reads of a column of pieces then touch every bank once.

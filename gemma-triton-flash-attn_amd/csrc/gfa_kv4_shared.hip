@@ -245,7 +245,7 @@ __global__ __launch_bounds__(kTpb, kv4_shared_wgs(D)) void kv4_shared_kernel(con
   constexpr int BIG = kSharedRows;
   __shared__ PlanLds lds;
   // The chunk kernel's tiles, or what the waves of the split kernel join: D * 32 bytes each (D = 64: 4 KB).
-  constexpr int TILE = std::max(kv4_chunk_steps(kPart) * Kv4Layout<D>::TILE_CODES, D == 64 ? 4096 : D * 32), SCALES = kv4_chunk_steps(kPart) * 1024;
+  constexpr int TILE = std::max(kv4_chunk_steps(kPart, D) * Kv4Layout<D>::TILE_CODES, D == 64 ? 4096 : D * 32), SCALES = kv4_chunk_steps(kPart, D) * 1024;
   __shared__ __attribute__((aligned(1024))) char k_lds0[TILE], k_lds1[TILE], v_lds0[TILE], v_lds1[TILE], s_lds0[SCALES], s_lds1[SCALES];
   char GFA_LDS* const K0 = (char GFA_LDS*)k_lds0;
   char GFA_LDS* const K1 = (char GFA_LDS*)k_lds1;
