@@ -200,7 +200,7 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
   } else {
     // At D = 512 a CU holds one workgroup, and the prefixes' and the requests' share the GPU (eight answers to each of four prompts,
     // 32:4: 160 of the chunk kernel and 128 52.8 us, 160 and 256 57-61, 256 and 256 63-71). A few answers leave it to
-    // chunks of one tile a wave (four answers, 8:1 D = 512, 700 tokens: 15.8 us, of two 17.5).
+    // chunks of one tile a wave (four answers to 700 tokens, 8:1 D = 512, taken apart: 15.8 us, of two 17.5).
     const int min_tiles = (int64_t)a->requests * a->cache.heads_kv <= 16 ? 4 : 8;
     size_part(s.few, a, kind, few, kRows, most * G, min_tiles, D < 512 ? 512 : kind == kPrefix ? 256 : 128, spare);
   }
