@@ -234,7 +234,7 @@ constexpr float kApartCost = 10.f, kApartLeast = 4.f;
 float worth_of(const gfa_kv4_attn_args* a) { return kApartLeast * rate_of(a->cache.head_dim).tiles / (float)a->cache.heads_kv; }
 
 // Whether prefixes may be taken apart: without a window, which bounds what a request reads, and for requests of few rows; where
-// max_new is not known, of few rows on average. Not where the tables are too narrow for it to pay.
+// max_new is not known, of few rows on average (those of many are the chunk kernel's then, see steps_of). Not where the tables are too narrow for it to pay.
 bool takes_prefixes(const gfa_kv4_attn_args* a) {
   if (a->shared_skip == nullptr || (a->causal && a->window > 0) || a->requests < 2) return false;
   const int64_t T = (int64_t)a->batch * a->seq_len, G = a->heads_q / a->cache.heads_kv;
@@ -246,20 +246,21 @@ bool takes_prefixes(const gfa_kv4_attn_args* a) {
 
 // The parts of a call.
 struct Steps {
-  Split whole, prefix, rest;  // whole, or the two others
+  Split whole, prefix, rest;  // whole; or the two others, and of whole the chunk kernel's part
   bool shared;
   size_t bytes() const {
     if (!shared) return whole.few.bytes() + whole.many.bytes();
-    return prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() + 64 + (size_t)rest.few.row_blocks * sizeof(gfa::Kv4Join);
+    return prefix.few.bytes() + prefix.many.bytes() + rest.few.bytes() + 64 + (size_t)rest.few.row_blocks * sizeof(gfa::Kv4Join) + whole.many.bytes();
   }
 };
 Steps steps_of(const gfa_kv4_attn_args* a) {
   Steps s{};
   s.shared = takes_prefixes(a);
-  if (!s.shared) {
-    s.whole = split_of(a, kWhole);
-    return s;
-  }
+  s.whole = split_of(a, kWhole);
+  if (!s.shared) return s;
+  // Where max_new is not known a prompt's chunk may stand among requests of few rows, and belongs to the chunk kernel all the same: 8000
+  // tokens over 8000 beside 200 of one token, 16:16 D = 64, 769 us (by 16 rows at a time 1191), 1000 over 8000, 32:4 D = 512, 771 (1168).
+  s.whole.few = Part{};
   s.prefix = split_of(a, kPrefix);
   s.rest = split_of(a, kRest);
   return s;
@@ -621,7 +622,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
   };
   if (s.shared) {
     gfa::Kv4SharedParams sp{};
-    p.row_limit = s.rest.row_limit;
+    p.row_limit = s.whole.row_limit;
     p.row_blocks = (int)s.rest.few.row_blocks;
     p.join_rows = s.rest.few.join_rows;
     p.join_slice = s.rest.few.join_slice;
@@ -642,7 +643,8 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     sp.grid = (int)std::min<int64_t>(bound, 256 * gfa::kv4_shared_wgs(D) * 3);
     sp.group_blocks = (float)(s.prefix.many.row_blocks + s.prefix.few.row_blocks);
     sp.worth = a->shared_apart != 0 ? -INFINITY : worth_of(a);
-    return launched(gfa::launch_kv4_shared(sp, D, bf16, cap, stream), "attention over shared prefixes");
+    if (err = gfa::launch_kv4_shared(sp, D, bf16, cap, stream); err != hipSuccess) return launched(err, "attention over shared prefixes");
+    ws += 64 + s.rest.few.row_blocks * sizeof(gfa::Kv4Join);
   }
   for (const bool large : {true, false}) {
     const Part& part = large ? s.whole.many : s.whole.few;

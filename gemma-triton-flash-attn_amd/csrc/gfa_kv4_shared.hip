@@ -90,7 +90,8 @@ __device__ __forceinline__ Both both_of(const Kv4SharedParams& s, int b) {
   x.own.fresh = tokens(c0, c1);
   x.own.len = max(len, 0);
   x.own.skip = max(skip, 0);
-  x.own.row_blocks = blocks(min(x.own.fresh, max(p.T - max(c0, 0), 0)) * p.G, 4);  // tokens past q's have no rows
+  // tokens past q's have no rows; those of a request of many rows are the chunk kernel's
+  x.own.row_blocks = x.own.fresh * p.G > p.row_limit ? 0 : blocks(min(x.own.fresh, max(p.T - max(c0, 0), 0)) * p.G, 4);
   const int held = min(x.own.len, most);
   x.own.tiles = (held + kTile - 1) / kTile;
   x.behind = held > x.own.skip ? x.own.tiles - x.own.skip / kTile : 0;

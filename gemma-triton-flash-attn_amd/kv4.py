@@ -164,7 +164,8 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
     of them, and the parts are joined: the same result, but for the order in which 32-bit sums are taken. That is done
     where it is faster, which is found on the device from the lengths of all requests, or with ``apart`` wherever there is a
     group. It has no effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average,
-    times Hq / Hkv above 64; 128 where requests times KV heads are at most four), which are bound by products."""
+    times Hq / Hkv above 64; 128 where requests times KV heads are at most four), which are bound by products; without
+    ``max_new`` single requests of more rows than that are computed as without ``shared``."""
     _refuse_gradients("attention over the cache", q, q)
     if max_new is not None and max_new < 1:
         raise ValueError("max_new must be at least 1")
