@@ -220,18 +220,33 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
 }
 
 // What taking prefixes apart saves is counted in passes of the split kernel over a tile (one row block, one KV head): `tiles` of them take
-// a us of the whole GPU, one of the chunk kernel takes as long as many_cost of them. From calls of 40 to 300 requests, by head dim: 151k
-// passes 72 us and 60k 52 us, 24k 43 us, 43k 133 us; the chunk kernel's 2.1 us a tile and CU at D = 512, 1.3, 1.1, 0.5.
+// a us of the whole GPU (by head dim, 151k passes 72 us and 60k 52 us, 24k 43 us, 43k 133 us), one of the chunk kernel takes as long as many_cost
+// of them. many_cost, and what the choice has to promise, are the ones with which 1270 drawn calls, in tight tables and in wide ones, took the least time;
+// soft-capping costs the chunk kernel most at D = 64, where scores are the larger part of its work.
 struct Rate {
   float tiles, many_cost;
 };
-Rate rate_of(int D) { return D == 64 ? Rate{2100.f, 3.5f} : D == 128 ? Rate{1200.f, 5.f} : D == 256 ? Rate{570.f, 2.9f} : Rate{320.f, 2.6f}; }
-// A row block whose request is taken apart leaves sums in two parts and is joined, about as much again as 10 tiles of it; a call has one
-// kernel's latency more: it pays from 4 us on. Apart against whole, us: two answers of 5 tokens to a 2k prompt, 32:4 D = 512, 35.7 24.0;
-// 16 answers of 8 to each of eight prompts of 740 tokens, 8:4 D = 256, 66 51; two answers to each of six prompts of 8k, 8:1 D = 512,
-// 27.8 31.7; 16 of 4 drafted tokens, 3k, 8:4 D = 256, 24.2 25.7; 44 to each of four of 1352, 32:8 D = 128, 41 52; 64 to one of 16k, 47 215.
-constexpr float kApartCost = 10.f, kApartLeast = 4.f;
-float worth_of(const gfa_kv4_attn_args* a) { return kApartLeast * rate_of(a->cache.head_dim).tiles / (float)a->cache.heads_kv; }
+Rate rate_of(int D, bool cap) {
+  return D == 64 ? Rate{2100.f, cap ? 7.f : 3.5f} : D == 128 ? Rate{1200.f, 6.f} : D == 256 ? Rate{570.f, cap ? 5.f : 4.f} : Rate{320.f, 5.2f};
+}
+// A row block whose request is taken apart leaves sums in two parts and is joined, about as much again as 10 tiles of it; and a call has
+// the other kernel's start and the joins' latency more, which D = 512's one workgroup a CU makes longest. Apart against whole in the same launch, us: two
+// answers of 5 tokens to a 2k prompt, 32:4 D = 512, 35.7 24.0; 16 answers of 8 to each of eight prompts of 740 tokens, 8:4 D = 256, 66 51;
+// 44 to each of four of 1352, 32:8 D = 128, 41 52; 64 to one of 16k, 47 215.
+constexpr float kApartCost = 10.f;
+float worth_of(const gfa_kv4_attn_args* a) {
+  const int D = a->cache.head_dim;
+  return (D == 512 ? 10.f : 4.f) * rate_of(D, a->softcap > 0.f).tiles / (float)a->cache.heads_kv;
+}
+// The call without prefixes is a launch shorter, and its kernel keeps more workgroups on a CU: whole requests in the shared launch take 3 to 5 us
+// longer, at D = 512 sometimes less (26 requests of 8 tokens over 1.5k, 8:1, 29.6 against 35.2). So it is left to calls whose tables
+// can hold far more than the choice has to promise. Of the 1270 calls 138 take over a tenth longer than without prefixes then, most of
+// them short requests in wide tables (lengths are not the host's to see); from the choice's own line on, 4 us, it was 344. (300 others, geometric
+// mean: 25.7 us without prefixes, 24.3 so.)
+float least_of(const gfa_kv4_attn_args* a) {
+  const int D = a->cache.head_dim;
+  return (D == 512 ? 8.f : 20.f) * rate_of(D, a->softcap > 0.f).tiles / (float)a->cache.heads_kv;
+}
 
 // Whether prefixes may be taken apart: without a window, which bounds what a request reads, and for requests of few rows; where
 // max_new is not known, of few rows on average (those of many are the chunk kernel's then, see steps_of). Not where the tables are too narrow for it to pay.
@@ -241,7 +256,7 @@ bool takes_prefixes(const gfa_kv4_attn_args* a) {
   const int64_t rows = a->max_new > 0 ? a->max_new : (T + a->requests - 1) / a->requests;
   if (rows * G > row_limit(a, a->requests)) return false;
   const double tiles = (double)a->table_width * a->cache.block_size / 32, row_blocks = (double)(T * G + (kRows - 1) * (int64_t)a->requests) / kRows;
-  return a->shared_apart != 0 || (tiles - kApartCost) * row_blocks > worth_of(a);
+  return a->shared_apart != 0 || (tiles - kApartCost) * row_blocks > least_of(a);
 }
 
 // The parts of a call.
@@ -637,7 +652,7 @@ int gfa_kv4_attn(const gfa_kv4_attn_args* a) {
     sp.rest = sums_of(s.rest.few);
     sp.joined = reinterpret_cast<int*>(ws);
     sp.joins = reinterpret_cast<gfa::Kv4Join*>(ws + 64);
-    sp.many_cost = rate_of(D).many_cost;
+    sp.many_cost = rate_of(D, cap).many_cost;
     sp.apart_cost = kApartCost;
     const int64_t bound = s.prefix.many.nblocks + s.prefix.few.nblocks + s.rest.few.nblocks;
     sp.grid = (int)std::min<int64_t>(bound, 256 * gfa::kv4_shared_wgs(D) * 3);

@@ -13,7 +13,7 @@
 // Bound: issue of the chunk kernel's products and decoding (64 answers to a 16k prompt, 32:8 D = 128: 47.8 us against 215 without
 // sharing; the tiles' loop 31, 1.1 us a tile and CU), around it latency: 2.5 us until a workgroup has its work, 8 until its first
 // products, 2 (D = 128) to 7 us (D = 512) for sums out, 6 for the join. Eight answers to each of four prompts of 8k, 32:4 D = 512, 54 us
-// (90), 16 of 4 drafted tokens, 3k, 8:4 D = 256, 25 (21: there it does not pay yet).
+// (90), 16 of 4 drafted tokens, 3k, 8:4 D = 256, 25 (21, to which tables so narrow leave it).
 #include <algorithm>
 
 #include "gfa_kv4_chunk.h"

@@ -162,8 +162,9 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
 
     ``shared``: ``share``'s result for this table, lens and cu. The prefix of a group of requests is then read once for all
     of them, and the parts are joined: the same result, but for the order in which 32-bit sums are taken. That is done
-    where it is faster, which is found on the device from the lengths of all requests, or with ``apart`` wherever there is a
-    group. It has no effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average,
+    where the lengths of all requests promise that it is faster, which is found on the device, or with ``apart`` wherever there
+    is a group. Tables too narrow to gain by it take the call without ``shared``; in wide ones, whose requests' lengths the host does not
+    know, a call that finds little in common can take some us longer than without. It has no effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average,
     times Hq / Hkv above 64; 128 where requests times KV heads are at most four), which are bound by products; without
     ``max_new`` single requests of more rows than that are computed as without ``shared``."""
     _refuse_gradients("attention over the cache", q, q)

@@ -96,3 +96,51 @@ def test_captured_with_a_chunk(D, device):
         assert torch.equal(seen, call())
         if i == 0:
             check(seen, *a.expected())
+
+
+# (Hq, Hkv, D, bs, softcap, prompts, answers to each, tokens of a prompt, of an answer, new tokens): which way the call goes
+CHOICES = {
+    # 22 us without prefixes, 25 apart
+    "drafts": ((8, 4, 256, 64, 50.0, 1, 16, 3001, 333, 4), "plain"),
+    # short requests in tables as short
+    "short": ((16, 8, 256, 64, 0.0, 2, 32, 330, 20, 1), "plain"),
+    "few": ((32, 8, 128, 64, 0.0, 3, 2, 5800, 60, 2), "plain"),
+    # 215 us without, 47 apart
+    "long": ((32, 8, 128, 64, 0.0, 1, 64, 16384, 600, 1), "apart"),
+    "global": ((32, 4, 512, 64, 0.0, 4, 8, 8192, 1000, 1), "apart"),
+    "d64": ((16, 16, 64, 64, 0.0, 8, 3, 11000, 500, 1), "apart"),
+    # 145 us without, 152 whole, 184 apart
+    "capped": ((8, 4, 256, 64, 50.0, 10, 5, 14000, 400, 8), "whole"),
+    # 175 without, 168 whole, 156 apart; of fewer answers 49, 51 and 54
+    "capped_d64": ((16, 2, 64, 64, 30.0, 9, 23, 5700, 100, 8), "apart"),
+    "capped_d64_few": ((16, 2, 64, 64, 30.0, 4, 10, 5700, 100, 8), "whole"),
+    # 70 without, 48 whole, 60 apart
+    "d512": ((32, 4, 512, 64, 0.0, 1, 52, 2100, 60, 2), "whole"),
+}
+
+
+@pytest.mark.parametrize("name", list(CHOICES))
+def test_the_choice(name, device):
+    """Apart, whole in the same launch or the call without prefixes, told by the bits that each leaves."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    (Hq, Hkv, D, bs, cap, prompts, answers, prompt, own, new), way = CHOICES[name]
+    g = torch.Generator().manual_seed(len(name))
+    lens = [prompt + new + int(x) for x in torch.randint(0, own, (prompts * answers,), generator=g)]
+    width, whole = max(-(-n // bs) for n in lens) + 2, prompt // bs
+    table = torch.arange(len(lens) * width, dtype=torch.int32).view(-1, width)
+    for b in range(len(lens)):
+        table[b, :whole] = table[b // answers * answers, :whole]
+    ids, table = torch.unique(table, return_inverse=True)
+    cache = kv4.allocate(len(ids), Hkv, D, bs, torch.bfloat16, device)
+    cache.codes.random_(0, 256)
+    cache.scales.fill_(125)
+    table, lens = table.to(device, torch.int32), torch.tensor(lens, dtype=torch.int32, device=device)
+    cu = torch.arange(len(lens) + 1, dtype=torch.int32, device=device) * new
+    q = torch.randn(1, Hq, len(lens) * new, D, generator=g).to(device, torch.bfloat16)
+    s = kv4.share(table, lens, cu, block_size=bs)
+    call = lambda **kw: kv4.attention(q, cache, table, lens, cu, max_new=new, softcap=cap or None, **kw)  # noqa: E731
+    o, plain, apart = call(shared=s), call(), call(shared=s, apart=True)
+    # (whole requests may leave the plain call's bits, and calls without groups are whole with `apart`, too)
+    assert torch.equal(o, plain) or way != "plain"
+    assert torch.equal(o, apart) == (way == "apart" or (way == "plain" and torch.equal(plain, apart)))
