@@ -41,7 +41,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 constexpr int kRows = kSplitRows;
 constexpr int kWaves = 4;
 
-// 16 bytes of codes; ONCE: non-temporal, for tiles that no other workgroup reads.
+// 16 bytes of codes; ONCE: non-temporal, for tiles that no other workgroup reads, or few (gfa_kv4_shared.hip).
 template <bool ONCE>
 __device__ __forceinline__ uint4 load16(const uint8_t* p) {
   typedef unsigned vec __attribute__((ext_vector_type(4)));
