@@ -9,8 +9,8 @@
 // of a wave each, then the segment's entries. Only two rows of the vocabulary are read per request, whatever was
 // drafted: the first kernel finds the row (every wave for itself, one probability a lane) and sums its segments, the
 // second picks the segment and the entry.
-// Bound: memory for large batches (64 requests, 262144 entries in 32 bits: 134 MB in 21.8 us, 6.2 TB/s, then 5.8 to pick), latency of
-// dependent loads for small ones (8 requests, 32000 entries: 4.4 and 5.4 us).
+// Bound: memory for large batches (64 requests, 262144 entries in 32 bits, a drafted token not accepted in 40 of them, so 104 rows: 109 MB in
+// 21.8 us, 5.0 TB/s, then 5.8 to pick), latency of dependent loads for small ones (8 requests, 32000 entries: 4.4 and 5.4 us).
 #include "gfa_common.h"
 #include "gfa_launch.h"
 #include "gfa_verify.h"
