@@ -203,8 +203,9 @@ constexpr int kv4_chunk_rows(int D) { return D >= 128 ? 128 : 256; }
 
 // Workgroups of the chunk kernel that a CU holds (by their registers).
 constexpr int kv4_chunk_wgs(int D) { return D == 512 ? 1 : D == 128 ? 3 : 2; }
-// Of the shared prefixes' kernel (gfa_kv4_shared.hip) rows of a workgroup and workgroups of a CU. With the chunk kernel's 256 rows at D = 64 a CU
-// holds two (forty drawn calls, geometric mean 16.7 us; three, with spills, 15.8; 128 rows, three 15.5), and groups seldom have as many.
+// Of the shared prefixes' kernel (gfa_kv4_shared.hip) rows of a workgroup and workgroups of a CU that the compiler leaves registers for. With the
+// chunk kernel's 256 rows at D = 64 those are two (forty drawn calls, geometric mean 16.7 us; three, with spills, 15.8; 128 rows, at least three 15.5; the
+// kernel takes 108 registers, with which a CU holds four), and groups seldom have as many.
 constexpr int kSharedRows = 128;
 constexpr int kv4_shared_wgs(int D) { return D == 64 ? 3 : kv4_chunk_wgs(D); }
 

@@ -66,7 +66,7 @@ __device__ __forceinline__ Kv4AttnParams part_of(const Kv4SharedParams& s, const
 // ---- the split of the call ----
 // As in gfa_kv4_sched.h, of three kinds of items in this order: row blocks of groups of many rows, of groups of few, of the
 // requests behind their prefixes. A grid for any lengths would be several times the items there are, and one that finds nothing takes
-// 2 to 4 us to find that out: three times what the CUs hold are launched at most, and take the items in turn (308 requests without
+// 2 to 4 us to find that out: three times kv4_shared_wgs for every CU are launched at most, and take the items in turn (308 requests without
 // prefixes, 16:8 D = 256, 87 -> 74 us, 93 in three groups, 32:8 D = 128, 28 -> 24; as many as the CUs hold 10 to 20% slower where there
 // is more to do, ten times the same as a grid for any lengths).
 // Up to 64 requests every wave looks through all of them; more are dealt to the four waves, which trade what they found in LDS.
