@@ -48,7 +48,9 @@
 extern "C" {
 #endif
 
-#define GFA_VERSION 109 /* 1.0.8: key/value cache in 4 bits (1.0.7: segment tables from position ids and masks, 1.0.6: materialised backward, 1.0.5: run-time work distribution, 1.0.4: attention dropout, 1.0.3: soft-capping) */
+/* The argument structs grow at their ends from version to version: a caller is compiled against the header of the library that it loads
+ * (gfa_version() tells), sets every struct to zero first and then what it uses. */
+#define GFA_VERSION 109 /* 1.0.9: requests that share blocks, drafted tokens; gfa_kv4_attn_args ends with shared_skip to shared_apart (1.0.8: key/value cache in 4 bits, 1.0.7: segment tables from position ids and masks, 1.0.6: materialised backward, 1.0.5: run-time work distribution, 1.0.4: attention dropout, 1.0.3: soft-capping) */
 
 typedef enum {
   GFA_DTYPE_FP16 = 0,
