@@ -140,7 +140,8 @@ void size_part(Part& s, const gfa_kv4_attn_args* a, Kind kind, int64_t row_block
   const int D = a->cache.head_dim;
   s.join_slice = rows == kRows && D > 128 && n * (D / 128) <= 1024 ? 128 : D;
   const int groups = 1024 / s.join_slice;
-  // (Over prefixes a row has many chunks: 64 answers to a 16k prompt, 32:8 D = 128, two groups of lanes a row 46.2 us, one 50.3.)
+  // (Over prefixes a row has many chunks: 64 answers to a 16k prompt, 32:8 D = 128, two groups of lanes a row 46.2 us, one 50.3;
+  // 160 drawn calls: one within 1% of two, four 1 to 4% longer.)
   s.join_parts = n <= 2048 ? groups : kind == kRest ? 2 : 1;
   const int64_t wgs = rows == kRows ? (row_bound * s.join_parts + groups - 1) / groups : rows / 32 * (D <= 128 ? 16 : D / 8) / 4;
   const int64_t most_wgs = 4096 / std::max<int64_t>(1, row_blocks * hkv);
@@ -199,7 +200,8 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
     size_part(s.few, a, kind, few, kRows, most * G, 8, 512, spare);
   } else {
     // At D = 512 a CU holds one workgroup, and the prefixes' and the requests' share the GPU (eight answers to each of four prompts,
-    // 32:4: 160 of the chunk kernel and 128 52.8 us, 160 and 256 57-61, 256 and 256 63-71). A few answers leave it to
+    // 32:4: 160 of the chunk kernel and 128 52.8 us, 160 and 256 57-61, 256 and 256 63-71; 39 drawn calls: 64 or 256
+    // of the requests within 0.5%, 128 of the prefixes' split kernel 3% shorter, 512 1% longer). A few answers leave it to
     // chunks of one tile a wave (four answers to 700 tokens, 8:1 D = 512, taken apart: 15.8 us, of two 17.5).
     const int min_tiles = (int64_t)a->requests * a->cache.heads_kv <= 16 ? 4 : 8;
     size_part(s.few, a, kind, few, kRows, most * G, min_tiles, D < 512 ? 512 : kind == kPrefix ? 256 : 128, spare);
@@ -210,7 +212,8 @@ Split split_of(const gfa_kv4_attn_args* a, Kind kind) {
   // 1024, 33 us with chunks of 8 tiles, 57 unsplit; 1000 tokens beside seven requests 66 us with 18 tiles, 74 unsplit;
   // 512 tokens of four requests 76-84 us split, 71 unsplit.
   // Of prefixes one workgroup a CU: their sums are as much again as what they read (64 answers to a 16k prompt, D = 128: 46.2 us, two
-  // 57), chunks of 8 tiles however many the row blocks could be (31 answers to each of three prompts of 500, 32:8 D = 128: 30 us, of 32
+  // 57; 121 drawn calls: one and a half 2 to 4% shorter at D = 64 and 128, the same at 256, two 3% longer there; 39 at D = 512: 128 workgroups 5% and 256
+  // 6% longer than 160), chunks of 8 tiles however many the row blocks could be (31 answers to each of three prompts of 500, 32:8 D = 128: 30 us, of 32
   // 36), of 4 where they are few (16 answers of 4 drafted tokens, 3k, 8:4 D = 256: 24.3 us, of 8 27.8).
   const int64_t alone = many * a->cache.heads_kv;
   const int target = kind != kPrefix ? 256 * gfa::kv4_chunk_wgs(D) : D < 512 ? 256 : 160;
