@@ -161,14 +161,16 @@ def attention(q: torch.Tensor, cache: Cache, table: torch.Tensor, lens: torch.Te
     kernels. ``scale`` defaults to 1/sqrt(D); ``softcap`` as in ``flash_attn_gqa_train``. There is no gradient.
 
     ``shared``: ``share``'s result for this table, lens and cu. The prefix of a group of requests is then read once for all
-    of them, and the parts are joined: the same result within the same bound, with other roundings (weights are rounded to 16 bits
-    against a maximum of their part, which below head dim 512 is exact without ``shared`` and may be passed by 2^8 in a prefix,
-    and 32-bit sums are taken in another order). That is done
-    where the lengths of all requests promise that it is faster, which is found on the device, or with ``apart`` wherever there
-    is a group. Tables too narrow to gain by it take the call without ``shared``; in wide ones, whose requests' lengths the host does not
-    know, a call that finds little in common can take some us longer than without. It has no effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average,
-    times Hq / Hkv above 64; 128 where requests times KV heads are at most four), which are bound by products; without
-    ``max_new`` single requests of more rows than that are computed as without ``shared``."""
+    of them, and the parts are joined: the same result within the same bound, with other roundings (weights are rounded to
+    16 bits against a maximum of their part, which below head dim 512 is exact without ``shared`` and may be passed by 2^8
+    in a prefix, and 32-bit sums are taken in another order). That is done where the lengths of all requests promise that
+    it is faster, which is found on the device, or with ``apart`` wherever there is a group. Tables too narrow to gain by it
+    take the call without ``shared``; in wide ones, whose requests' lengths the host does not know, a call that finds little
+    in common can take some us longer than without.
+
+    It has no effect with ``slide_size``, nor where requests have many query rows (``max_new``, else the average, times
+    Hq / Hkv above 64; 128 where requests times KV heads are at most four), which are bound by products; without ``max_new``
+    single requests of more rows than that are computed as without ``shared``, beside the others."""
     _refuse_gradients("attention over the cache", q, q)
     if max_new is not None and max_new < 1:
         raise ValueError("max_new must be at least 1")

@@ -342,7 +342,9 @@ typedef struct {
   /* gfa_kv4_share's results for this table, lens and cu, or NULL: the groups' prefixes are attended to once for all of a
    * group's queries, where their lengths promise that it is faster (shared_apart 0) or wherever there is a group (1). Tables too narrow
    * to gain by it take the call without; in wide ones a call that finds little in common can take some us longer. The same
-   * result within the same bound: weights are rounded against other maxima, and 32-bit sums taken in another order. Without effect with a window, for requests of many rows, and where max_new times heads_q / heads_kv are many. */
+   * result within the same bound: weights are rounded against other maxima, and 32-bit sums taken in another order. Without
+   * effect with a window and where max_new (0: the average) times heads_q / heads_kv are many; with max_new 0 single requests of
+   * many rows are computed as without. */
   const int32_t* shared_skip; /* (requests) */
   const int32_t* shared_cu;   /* (requests + 1) */
   const int32_t* shared_lens; /* (requests) */
