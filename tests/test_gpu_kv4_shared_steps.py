@@ -144,3 +144,28 @@ def test_the_choice(name, device):
     # (whole requests may leave the plain call's bits, and calls without groups are whole with `apart`, too)
     assert torch.equal(o, plain) or way != "plain"
     assert torch.equal(o, apart) == (way == "apart" or (way == "plain" and torch.equal(plain, apart)))
+
+
+@pytest.mark.parametrize("n,D", [(40, 512), (70, 128), (300, 64)])
+def test_numbers_that_fit_nothing(n, D, device):
+    """Without max_new: tables, lengths and offsets that are no such things touch nothing outside the arrays, and the next call is right."""
+    from gemma_triton_flash_attn_amd import kv4
+
+    a, _ = step(D, device, "inside", (100,), n=n)
+    s, want, q = a.share(), a.expected(), a.q.to(device)
+    before = [t.clone() for t in (a.cache.codes, a.cache.scales)]
+    g = torch.Generator().manual_seed(n)
+    big = torch.tensor([-2 ** 31, -70000, -1, 0, 1, 17, n, 100, 5000, 2 ** 20, 2 ** 31 - 1])
+
+    def wild(t, p):
+        other = big[torch.randint(0, len(big), t.shape, generator=g)]
+        return torch.where(torch.rand(t.shape, generator=g) < p, other, t.cpu().long()).to(torch.int32).to(device)
+
+    for i in range(18):
+        p = [0.02, 0.3, 1.0][i % 3]
+        table, lens, cu = (wild(t, p if i >> k & 1 else 0) for k, t in enumerate((a.table, a.lens_dev, a.cu)))
+        bad = kv4.Shared(*(wild(t, p if (i + 1) >> k & 1 else 0) for k, t in enumerate(s)))
+        assert kv4.attention(q, a.cache, table, lens, cu, shared=bad, apart=i % 2 == 0).shape == q.shape
+        torch.cuda.synchronize()
+    assert torch.equal(q.cpu(), a.q) and all(torch.equal(x, y) for x, y in zip(before, (a.cache.codes, a.cache.scales)))
+    check(a.attend(shared=s, apart=True), *want)
